@@ -33,6 +33,8 @@ EXPORTS = [
     "fi_tv_loss_fwd", "fi_tv_loss_bwd", "fi_conv3d_first_fwd", "fi_conv3d_first_wgrad", "fi_conv3d_first_wgrad_workspace",
     "fi_conv3d_point_fwd", "fi_conv3d_point_dgrad", "fi_conv3d_point_wgrad", "fi_conv3d_point_wgrad_workspace",
     "fi_bn_fused_fwd_batched", "fi_bn_act_bwd_reduce_batched", "fi_bn_act_bwd_apply_batched",
+    "fi_newton_schulz", "fi_newton_schulz_workspace", "fi_linear_ce_saved", "fi_linear_ce_fwd_workspace", "fi_linear_ce_fwd",
+    "fi_linear_ce_bwd_workspace", "fi_linear_ce_bwd",
 ]
 
 
@@ -54,6 +56,15 @@ class FiBnAct(C.Structure):
                 ("seed_offset", C.c_void_p)]
 
 
+class FiNsMat(C.Structure):
+    _fields_ = [("u", C.c_void_p), ("out", C.c_void_p), ("dtype", C.c_int), ("rows", C.c_int), ("cols", C.c_int)]
+
+
+class FiLinearCe(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("wdtype", C.c_int), ("ltype", C.c_int), ("reduction", C.c_int), ("V", C.c_int), ("D", C.c_int),
+                ("T", C.c_int64), ("ldx", C.c_int64), ("ldw", C.c_int64), ("ignore_index", C.c_int64)]
+
+
 FI_ERR_UNSUPPORTED = -3                                    # include/fedicra_hip.h
 
 
@@ -64,7 +75,7 @@ class FiError(RuntimeError):
 _lib = None
 
 
-ABI_VERSION = 6             # include/fedicra_hip.h FI_ABI_VERSION
+ABI_VERSION = 7             # include/fedicra_hip.h FI_ABI_VERSION
 
 
 def source_hash():
@@ -105,6 +116,8 @@ def lib():
         _lib.fi_conv2d_stats_xcorr_workspace.restype = C.c_long
         _lib.fi_conv3d_first_wgrad_workspace.restype = C.c_long
         _lib.fi_conv3d_point_wgrad_workspace.restype = C.c_long
+        for name in ("fi_newton_schulz_workspace", "fi_linear_ce_saved", "fi_linear_ce_fwd_workspace", "fi_linear_ce_bwd_workspace"):
+            getattr(_lib, name).restype = C.c_long
     return _lib
 
 
@@ -1139,3 +1152,51 @@ def nhwc_to_nchw(src, dst):
 
 def probe_tr16(inp, offs, out):
     _chk(lib().fi_probe_tr16(ptr(_dev(inp)), ptr(offs), ptr(out), stream()), "fi_probe_tr16")
+
+
+# ------------------------------------------------------------------ the tail of a training step
+def newton_schulz(updates, outs, steps, coeffs, eps):
+    """fi_newton_schulz over dense 2-D tensors; outs[i] may be updates[i].  coeffs: `steps` triples."""
+    n = len(updates)
+    mats = (FiNsMat * n)()
+    for q, u, o in zip(mats, updates, outs):
+        q.u, q.out, q.dtype, q.rows, q.cols = _dev(u).data_ptr(), o.data_ptr(), dt(u.dtype), u.shape[0], u.shape[1]
+    flat = (C.c_float * (3 * steps))(*[float(v) for abc in coeffs for v in abc])
+    size = lib().fi_newton_schulz_workspace(mats, n)
+    if size < 0:
+        _chk(int(size), "fi_newton_schulz_workspace")
+    ws = torch.empty(size, dtype=torch.uint8, device=updates[0].device)
+    _chk(lib().fi_newton_schulz(mats, n, int(steps), flat, C.c_float(eps), ptr(ws), stream()), "fi_newton_schulz")
+
+
+LABEL_TYPES = {torch.uint8: 0, torch.int32: 1, torch.int64: 2}                 # FI_LABEL_*
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _scratch(size, what, device):
+    if size < 0:
+        _chk(int(size), what)
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def linear_ce_desc(x, w, labels, ignore_index, reduction):
+    """x [T, D], w [V, D], both with dense rows; labels [T] dense."""
+    return FiLinearCe(dt(x.dtype), dt(w.dtype), LABEL_TYPES[labels.dtype], REDUCTIONS[reduction], w.shape[0], x.shape[1], x.shape[0],
+                      max(x.stride(0), x.shape[1]), max(w.stride(0), w.shape[1]), int(ignore_index))
+
+
+def linear_ce_fwd(d, x, w, bias, labels, loss):
+    """Returns the buffer the backward pass needs."""
+    dev = _dev(x).device
+    saved = _scratch(lib().fi_linear_ce_saved(C.byref(d)), "fi_linear_ce_saved", dev)
+    ws = _scratch(lib().fi_linear_ce_fwd_workspace(C.byref(d), ptr(w)), "fi_linear_ce_fwd_workspace", dev)
+    _chk(lib().fi_linear_ce_fwd(C.byref(d), ptr(x), ptr(w), ptr(bias), ptr(labels), ptr(loss), ptr(saved), ptr(ws), stream()),
+         "fi_linear_ce_fwd")
+    return saved
+
+
+def linear_ce_bwd(d, x, w, bias, labels, saved, gloss, dx, dw, dw_accumulate, db, db_accumulate):
+    size = lib().fi_linear_ce_bwd_workspace(C.byref(d), ptr(w), int(dx is not None), int(dw is not None), int(db is not None))
+    ws = _scratch(size, "fi_linear_ce_bwd_workspace", _dev(x).device)
+    _chk(lib().fi_linear_ce_bwd(C.byref(d), ptr(x), ptr(w), ptr(bias), ptr(labels), ptr(saved), ptr(gloss), ptr(dx), ptr(dw),
+                                int(dw_accumulate), ptr(db), int(db_accumulate), ptr(ws), stream()), "fi_linear_ce_bwd")

@@ -1,0 +1,1067 @@
+// Softmax cross entropy of a linear head over many classes, without its logits:  z = x W^T + b,
+//     loss_t = log sum_v exp z_tv - z_{t, label_t},        G_tv = g_t (exp(z_tv) / sum_v exp z_tv - [v = label_t]),
+//     dx = G W,   dW = G^T x,   db = sum_t G_t            (g_t: the gradient of row t's loss; ignored rows take no part)
+//
+// Forward: one product whose epilogue turns each tile of logits into the row's maximum and sum of exponentials over the tile's
+// classes and picks the label's logit; a second pass over those (8 bytes per row and tile) joins them.  Backward: the product is made
+// again, a piece of rows x classes at a time, its epilogue writes G in 16 bits in both orientations, and two products take it from there.
+// The logits never exist in memory, G only a piece at a time.
+//
+// Only labelled rows take part: their numbers are gathered first (stable, no atomics), x is packed through that list, and every
+// kernel takes the number of rows from the device -- nine pixels of ten unlabelled cost a tenth.
+//
+// Types: 16-bit x and W go to the matrix pipe as they are; fp32 as pairs of fp16 (nt_product.h) under one power-of-two scale per tensor, which
+// keeps 22 bits of everything within 2^-17 of the tensor's largest value.  In the backward products x and W are always fp16 (bf16 ones
+// converted exactly, under such a scale), because G in fp16 keeps 11 bits where bf16 would keep 8; G is scaled so that the largest |g_t| is at
+// 2^14.  Row statistics, sums and db are fp32 (joins in fp64).
+#include "nt_product.h"
+
+namespace {
+
+typedef int64_t i64;
+constexpr float CE_LOG2E = 1.4426950408889634f;
+constexpr int CE_ROWS = 2048;                   // rows per workgroup of the gathering passes
+constexpr int CE_PARTS = 1024;                  // partial results of the max passes
+constexpr int CE_LOSS_WGS = 512;
+
+// kept from the forward to the backward pass, at the head of the caller's `saved` buffer; T = rows
+//   int count (labelled rows) | ... 64 bytes | int idx[T] | int label[T] | float2 stat[T] (row maximum, 1 / sum)
+struct CeSaved {
+  int* count;
+  int* idx;
+  int* lab;
+  float2* stat;
+};
+__host__ __device__ __forceinline__ i64 ce_up(i64 v, i64 a) { return (v + a - 1) / a * a; }
+CeSaved ce_saved(void* p, i64 T) {
+  char* c = (char*)p;
+  const i64 n = ce_up(4 * T, 64);
+  return CeSaved{(int*)c, (int*)(c + 64), (int*)(c + 64 + n), (float2*)(c + 64 + 2 * n)};
+}
+
+// scalars on the device: [0] / [1] the scale of x / W in pair or converted form, [2] / [3] their reciprocals, [4] 1 / (scale of G)
+enum { SC_X = 0, SC_W = 1, SC_RX = 2, SC_RW = 3, SC_RG = 4, SC_N = 8 };
+
+__device__ __forceinline__ float ce_load(const void* p, int dtype, i64 i) {
+  return dtype == FI_F32 ? ((const float*)p)[i] : dtype == FI_BF16 ? (float)((const bf16_t*)p)[i] : (float)((const f16_t*)p)[i];
+}
+__device__ __forceinline__ i64 ce_label(const void* p, int ltype, i64 i) {
+  return ltype == FI_LABEL_U8 ? (i64)((const uint8_t*)p)[i] : ltype == FI_LABEL_I32 ? (i64)((const int*)p)[i] : ((const i64*)p)[i];
+}
+__device__ __forceinline__ float ce_pow2_scale(float amax) {          // s with amax * s in [2^14, 2^15); 1 where there is nothing to scale
+  if (!(amax > 0.f) || !(amax < INFINITY)) return 1.f;
+  int e = (int)((__float_as_uint(amax) >> 23) & 255) - 127;
+  e = 14 - e;
+  e = e > 126 ? 126 : e < -126 ? -126 : e;
+  return __uint_as_float((unsigned)(e + 127) << 23);
+}
+
+// ---- gathering the labelled rows ----------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void ce_count_kernel(const void* labels, int ltype, i64 T, i64 ignore, int* cnt) {
+  __shared__ int sm[4];
+  const i64 r0 = (i64)blockIdx.x * CE_ROWS;
+  int n = 0;
+  for (int k = threadIdx.x; k < CE_ROWS; k += 256)
+    if (r0 + k < T && ce_label(labels, ltype, r0 + k) != ignore) ++n;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) cnt[blockIdx.x] = sm[0] + sm[1] + sm[2] + sm[3];
+}
+
+// each thread owns 8 consecutive rows; the workgroups before this one are summed again by every workgroup
+__global__ __launch_bounds__(256) void ce_gather_kernel(const void* labels, int ltype, i64 T, i64 ignore, int V, const int* cnt, CeSaved s,
+                                                        float* zt, float* rows_out) {
+  __shared__ int sm[256], base_sm[4];
+  const int tid = threadIdx.x;
+  int before = 0;
+  for (int k = tid; k < (int)blockIdx.x; k += 256) before += cnt[k];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+  if ((tid & 63) == 0) base_sm[tid >> 6] = before;
+  const i64 r0 = (i64)blockIdx.x * CE_ROWS + tid * 8;
+  i64 lab[8];
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    lab[k] = r0 + k < T ? ce_label(labels, ltype, r0 + k) : ignore;
+    n += lab[k] != ignore;
+  }
+  sm[tid] = n;
+  __syncthreads();
+  for (int o = 1; o < 256; o <<= 1) {                                  // inclusive scan
+    const int v = tid >= o ? sm[tid - o] : 0;
+    __syncthreads();
+    sm[tid] += v;
+    __syncthreads();
+  }
+  int at = base_sm[0] + base_sm[1] + base_sm[2] + base_sm[3] + sm[tid] - n;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (lab[k] != ignore) {
+      s.idx[at] = (int)(r0 + k);
+      s.lab[at] = lab[k] >= 0 && lab[k] < V ? (int)lab[k] : -1;
+      zt[at] = __uint_as_float(0x7fc00000u);                           // (a label that is no class leaves NaN behind)
+      ++at;
+    } else if (rows_out && r0 + k < T) {
+      rows_out[r0 + k] = 0.f;
+    }
+  }
+  if (blockIdx.x == gridDim.x - 1 && tid == 255) s.count[0] = at;
+}
+
+// ---- the largest finite magnitude of x's labelled rows and of W ------------------------------------------------------------------------
+// (a wave per row; 16-byte loads where the rows are aligned for them)
+template <typename T>
+__global__ __launch_bounds__(256) void ce_amax_kernel(const T* p, i64 ld, int D, int vec, const int* idx, const int* count, i64 rows, float* part) {
+  __shared__ float sm[4];
+  if (count) rows = count[0];
+  const int l = threadIdx.x & 63;
+  constexpr int VG = DT<T>::VG;
+  float m = 0.f;
+  const int dv = vec ? D / VG : 0;
+  for (i64 r = (i64)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (i64)gridDim.x * 4) {
+    const T* q = p + (idx ? (i64)idx[r] : r) * ld;
+    for (int c = l; c < dv; c += 64) {
+      float f[VG];
+      VecWords<T>::unpack(((const typename DT<T>::vec_t*)q)[c], f);
+#pragma unroll
+      for (int t = 0; t < VG; ++t) m = fabsf(f[t]) < INFINITY ? fmaxf(m, fabsf(f[t])) : m;
+    }
+    for (int c = dv * VG + l; c < D; c += 64) {
+      const float v = fabsf(to_f32(q[c]));
+      if (v < INFINITY) m = fmaxf(m, v);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if (l == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+}
+__global__ __launch_bounds__(256) void ce_scales_kernel(const float* px, const float* pw, float* scal) {
+  __shared__ float sm[2][4];
+  float x = 0.f, w = 0.f;
+  for (int k = threadIdx.x; k < CE_PARTS; k += 256) x = fmaxf(x, px[k]), w = fmaxf(w, pw[k]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64)), w = fmaxf(w, __shfl_xor(w, o, 64));
+  if ((threadIdx.x & 63) == 0) sm[0][threadIdx.x >> 6] = x, sm[1][threadIdx.x >> 6] = w;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const float sx = ce_pow2_scale(fmaxf(fmaxf(sm[0][0], sm[0][1]), fmaxf(sm[0][2], sm[0][3])));
+    const float sw = ce_pow2_scale(fmaxf(fmaxf(sm[1][0], sm[1][1]), fmaxf(sm[1][2], sm[1][3])));
+    scal[SC_X] = sx, scal[SC_W] = sw, scal[SC_RX] = 1.f / sx, scal[SC_RW] = 1.f / sw;
+  }
+}
+
+// ---- packing an operand ---------------------------------------------------------------------------------------------------------------
+struct CePack {
+  const void* src;         // [rows][D], leading dimension ld, storage `dtype`
+  int dtype, D;
+  i64 ld, rows, begin;     // rows [begin, begin + rows) of the source (of the list); same and turned start there
+  const int* idx;          // row list (x) or NULL
+  const int* count;        // rows from the device, or NULL
+  const float* scale;      // device scalar or NULL: applied to the pair form and to fp16 made of bf16
+  void* same;              // [rows][K] operand rows, or NULL
+  i64 ld_same;
+  int same_k;              // its padded width: whole stages, a multiple of 8
+  int same_kind;           // 0 bf16, 1 fp16, 2 pair
+  void* turned;            // [D][rows] operand rows (fp16 or pair), or NULL
+  i64 ld_turned;
+  int turned_pair;
+};
+// one 64 x 64 block of the source per workgroup (blockIdx.x: rows, blockIdx.y: columns); pads are written as zeros
+__global__ __launch_bounds__(256) void ce_pack_kernel(CePack a) {
+  __shared__ float tile[64][65];
+  const i64 have = a.count ? (i64)a.count[0] - a.begin : a.rows, rows = have < a.rows ? have : a.rows;
+  const i64 r0 = (i64)blockIdx.x * 64;
+  const int c0 = (int)blockIdx.y * 64, tid = threadIdx.x;
+  if (r0 >= rows) return;
+  for (int e = tid; e < 64 * 64; e += 256) {
+    const i64 r = r0 + (e >> 6);
+    const int c = c0 + (e & 63);
+    tile[e >> 6][e & 63] = r < rows && c < a.D ? ce_load(a.src, a.dtype, (a.idx ? (i64)a.idx[a.begin + r] : r) * a.ld + c) : 0.f;
+  }
+  __syncthreads();
+  const float sc = a.scale ? a.scale[0] : 1.f;
+  for (int e = tid; e < 64 * 8; e += 256) {
+    const int r = e >> 3, c = (e & 7) * 8;
+    float v[8];
+    if (a.same && r0 + r < rows && c0 + c < a.same_k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = tile[r][c + i] * (a.same_kind == 2 ? sc : 1.f);
+      char* row = (char*)a.same + (r0 + r) * a.ld_same * 2;
+      if (a.same_kind == 2)
+        nt_store_pair((f16_t*)row, c0 + c, v);
+      else if (a.same_kind == 1)
+        *(uint4*)((f16_t*)row + c0 + c) = VecWords<f16_t>::pack(v);
+      else
+        *(uint4*)((bf16_t*)row + c0 + c) = VecWords<bf16_t>::pack(v);
+    }
+    if (a.turned && c0 + r < a.D) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = tile[c + i][r] * sc;
+      f16_t* row = (f16_t*)a.turned + (i64)(c0 + r) * a.ld_turned;
+      if (a.turned_pair)
+        nt_store_pair(row, r0 + c, v);
+      else
+        *(uint4*)(row + r0 + c) = VecWords<f16_t>::pack(v);
+    }
+  }
+}
+
+// ---- the logits' product --------------------------------------------------------------------------------------------------------------
+struct CeLogits {
+  const void* x;           // packed rows
+  const void* w;           // operand rows [V]
+  i64 ldx, ldw;
+  int stages, V;
+  const float* bias;
+  const float* scal;       // NULL, or the pair form's scales
+  CeSaved s;
+  // forward
+  float2* part;            // [row][ntj]
+  float* zt;
+  int ntj;
+  // backward: rows [t0, t0 + Tc), classes [v0, v0 + Vc)
+  i64 t0, Tc;
+  int v0, Vc;
+  const float* g;          // row factors, scaled
+  f16_t *dl, *dlt;
+  i64 ld_dl, ld_dlt;
+  float* db;               // [row tile][V] partial column sums, or NULL
+};
+
+// item -> tile, groups of 8 row tiles walking the classes together so that an XCD's workgroups share both operands in its L2
+__device__ __forceinline__ bool ce_tile(int nti, int ntj, int& ti, int& tj) {
+  const unsigned total = (unsigned)nti * (unsigned)ntj, per = (total + 7) >> 3;
+  const unsigned k = blockIdx.x >> 3, t = (blockIdx.x & 7) * per + k;
+  if (k >= per || t >= total) return false;
+  const unsigned grp = t / (8u * (unsigned)ntj), in = t - grp * 8u * (unsigned)ntj;
+  const unsigned gm = (unsigned)nti - grp * 8u < 8u ? (unsigned)nti - grp * 8u : 8u;
+  ti = (int)(grp * 8u + in % gm);
+  tj = (int)(in / gm);
+  return true;
+}
+
+// exp(z - m) with m2 = m log2 e: one rounding more is spent on the parity type, whose row sums are held to fp32's error
+template <bool PAIR>
+__device__ __forceinline__ float ce_exp(float z, float m, float m2) {
+  return __builtin_amdgcn_exp2f(PAIR ? (z - m) * CE_LOG2E : __builtin_fmaf(z, CE_LOG2E, -m2));
+}
+
+// The bias of a lane's columns: 16-bit operands start from it, pairs get it behind their scales.
+template <bool PAIR, class Core>
+__device__ __forceinline__ void ce_begin(Core& c, const CeLogits& a, int c0) {
+  c.clear();
+  if (PAIR || !a.bias) return;
+  const int j0 = c0 + Core::col0() + 4 * (Core::lane() >> 4);
+#pragma unroll
+  for (int j = 0; j < Core::TJ; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float b = j0 + j * 16 + r < a.V ? a.bias[j0 + j * 16 + r] : 0.f;
+#pragma unroll
+      for (int i = 0; i < Core::TI; ++i) c.acc[i][j][r] = b;
+    }
+}
+template <bool PAIR, class Core>
+__device__ __forceinline__ void ce_finish(Core& c, const CeLogits& a, int c0) {
+  if constexpr (PAIR) {
+    const float rx = a.scal[SC_RX], rw = a.scal[SC_RW];
+    const int j0 = c0 + Core::col0() + 4 * (Core::lane() >> 4);
+#pragma unroll
+    for (int j = 0; j < Core::TJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float b = a.bias && j0 + j * 16 + r < a.V ? a.bias[j0 + j * 16 + r] : 0.f;
+#pragma unroll
+        for (int i = 0; i < Core::TI; ++i) c.acc[i][j][r] = c.acc[i][j][r] * rx * rw + b;
+      }
+  }
+}
+
+template <class Core, typename T, bool PAIR>
+__global__ __launch_bounds__(Core::THREADS) void ce_fwd_kernel(CeLogits a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int n = a.s.count[0];
+  int ti, tj;
+  if (!ce_tile((n + Core::BM - 1) / Core::BM, a.ntj, ti, tj)) return;
+  const int r0 = ti * Core::BM, c0 = tj * Core::BN;
+  Core c;
+  ce_begin<PAIR>(c, a, c0);
+  c.run((const T*)a.x + (i64)r0 * a.ldx, a.ldx, n - r0, (const T*)a.w + (i64)c0 * a.ldw, a.ldw, a.V - c0, 0, a.stages, smem);
+  ce_finish<PAIR>(c, a, c0);
+  const int l = Core::lane(), j0 = c0 + Core::col0() + 4 * (l >> 4);
+  if (c0 + Core::BN > a.V) {
+#pragma unroll
+    for (int j = 0; j < Core::TJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (j0 + j * 16 + r >= a.V) {
+#pragma unroll
+          for (int i = 0; i < Core::TI; ++i) c.acc[i][j][r] = -INFINITY;
+        }
+  }
+  // a lane's 4 TJ columns of a row first, each with its own maximum; 4 NWN such pairs per row meet in LDS
+  float2* red = (float2*)smem;                                          // [4 NWN][BM]
+  const int q0 = (Core::wave() % Core::NWN) * 4 + (l >> 4);
+#pragma unroll
+  for (int i = 0; i < Core::TI; ++i) {
+    const int row = Core::row0() + i * 16 + (l & 15);
+    const int lab = r0 + row < n ? a.s.lab[r0 + row] - (c0 + Core::col0()) : -1;
+    if ((unsigned)lab < (unsigned)Core::WN) {
+#pragma unroll
+      for (int j = 0; j < Core::TJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (lab == j * 16 + 4 * (l >> 4) + r) a.zt[r0 + row] = c.acc[i][j][r];
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < Core::TJ; ++j)
+      m = fmaxf(fmaxf(m, fmaxf(c.acc[i][j][0], c.acc[i][j][1])), fmaxf(c.acc[i][j][2], c.acc[i][j][3]));
+    const float safe = m == -INFINITY ? 0.f : m, m2 = safe * CE_LOG2E;
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < Core::TJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum += ce_exp<PAIR>(c.acc[i][j][r], safe, m2);
+    red[q0 * Core::BM + row] = make_float2(m, sum);
+  }
+  __syncthreads();
+  for (int row = threadIdx.x; row < Core::BM; row += Core::THREADS) {
+    if (r0 + row >= n) continue;
+    float m = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4 * Core::NWN; ++q) m = fmaxf(m, red[q * Core::BM + row].x);
+    const float safe = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int q = 0; q < 4 * Core::NWN; ++q) {
+      const float2 o = red[q * Core::BM + row];
+      sum += o.y * __builtin_amdgcn_exp2f((o.x - safe) * CE_LOG2E);
+    }
+    a.part[(i64)(r0 + row) * a.ntj + tj] = make_float2(m, sum);
+  }
+}
+
+// joins a row's tiles: LANES lanes per row
+template <int LANES>
+__global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ntj, const float* zt, CeSaved s, float* rows_out, double* sums) {
+  __shared__ double sm[4];
+  const int n = s.count[0], sub = threadIdx.x % LANES;
+  double acc = 0.0;
+  for (i64 r0 = (i64)blockIdx.x * (256 / LANES); r0 < n; r0 += (i64)gridDim.x * (256 / LANES)) {
+    const i64 r = r0 + threadIdx.x / LANES;
+    float m = -INFINITY;
+    double sum = 0.0;
+    if (r < n) {
+      for (int k = sub; k < ntj; k += LANES) m = fmaxf(m, part[r * ntj + k].x);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const float safe = m == -INFINITY ? 0.f : m;
+    if (r < n) {
+      for (int k = sub; k < ntj; k += LANES) {
+        const float2 p = part[r * ntj + k];
+        sum += (double)(p.y * __builtin_amdgcn_exp2f((p.x - safe) * CE_LOG2E));
+      }
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (r < n && sub == 0) {
+      const float loss = (float)((double)(safe - zt[r]) + log(sum));
+      s.stat[r] = make_float2(safe, (float)(1.0 / sum));
+      if (rows_out) rows_out[s.idx[r]] = loss;
+      acc += (double)loss;
+    }
+  }
+  acc = wave_sum(acc);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) sums[blockIdx.x] = sm[0] + sm[1] + sm[2] + sm[3];
+}
+__global__ __launch_bounds__(256) void ce_loss_kernel(const double* sums, int nsums, const int* count, int mean, float* loss) {
+  __shared__ double sm[4];
+  double acc = 0.0;
+  for (int k = threadIdx.x; k < nsums; k += 256) acc += sums[k];
+  acc = wave_sum(acc);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    acc = sm[0] + sm[1] + sm[2] + sm[3];
+    loss[0] = (float)(mean ? acc / (double)count[0] : acc);            // (no labelled row: NaN, as fi_ce_finalize)
+  }
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void ce_gmax_kernel(const float* g, const int* idx, const int* count, float* part) {
+  __shared__ float sm[4];
+  const int n = count[0];
+  float m = 0.f;
+  for (i64 r = (i64)blockIdx.x * 256 + threadIdx.x; r < n; r += (i64)gridDim.x * 256) {
+    const float v = fabsf(g[idx[r]]);
+    if (v < INFINITY) m = fmaxf(m, v);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+}
+// rows' factors g_t * scale (reduction 0: one upstream gradient per row; 1 mean, 2 sum: one for all)
+__global__ __launch_bounds__(256) void ce_factors_kernel(const float* g, int reduction, const float* part, CeSaved s, float* scal, float* out) {
+  __shared__ float sm[4], s_max;
+  const int n = s.count[0], tid = threadIdx.x;
+  const float one = reduction == 1 ? (float)((double)g[0] / (double)n) : reduction == 2 ? g[0] : 0.f;
+  float m = fabsf(one);
+  if (reduction == 0)
+    for (int k = tid; k < CE_PARTS; k += 256) m = fmaxf(m, part[k]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((tid & 63) == 0) sm[tid >> 6] = m;
+  __syncthreads();
+  if (tid == 0) s_max = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  __syncthreads();
+  const float sc = 0.5f * ce_pow2_scale(s_max);                         // largest factor in [2^13, 2^14)
+  if (blockIdx.x == 0 && tid == 0) scal[SC_RG] = 1.f / sc;
+  for (i64 r = (i64)blockIdx.x * 256 + tid; r < n; r += (i64)gridDim.x * 256) {
+    const float f = reduction == 0 ? g[s.idx[r]] : one;
+    out[r] = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : f * sc;
+  }
+}
+
+template <bool PAIR>
+__device__ __forceinline__ int ce_kpad(int n) { return PAIR ? (n + 31) & ~31 : (n + 63) & ~63; }
+
+// G of a piece, in both orientations
+template <class Core, typename T, bool PAIR>
+__global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int SB = Core::WM >= 64 && Core::WN >= 64 ? 64 : 32, EXTRA = Core::NW * NtBlock<SB, SB>::BYTES > Core::LDS ? Core::NW * NtBlock<SB, SB>::BYTES : Core::LDS;
+  const i64 left = (i64)a.s.count[0] - a.t0;
+  const int n = (int)(left < 0 ? 0 : left < a.Tc ? left : a.Tc);       // rows of this piece
+  int ti, tj;
+  if (!ce_tile((n + Core::BM - 1) / Core::BM, (a.Vc + Core::BN - 1) / Core::BN, ti, tj)) return;
+  const int r0 = ti * Core::BM, c0 = tj * Core::BN;
+  const i64 rg = a.t0 + r0;
+  const int cg = a.v0 + c0;
+  Core c;
+  ce_begin<PAIR>(c, a, cg);
+  c.run((const T*)a.x + rg * a.ldx, a.ldx, n - r0, (const T*)a.w + (i64)cg * a.ldw, a.ldw, a.V - cg, 0, a.stages, smem);
+  ce_finish<PAIR>(c, a, cg);
+  float4* meta = (float4*)(smem + EXTRA);                               // [BM]: maximum (* log2 e unless PAIR), factor / sum, factor, label
+  float* colsum = (float*)(smem + EXTRA + Core::BM * 16);              // [BM / WM][BN]
+  for (int row = threadIdx.x; row < Core::BM; row += Core::THREADS) {
+    float4 m = make_float4(INFINITY, 0.f, 0.f, __int_as_float(-1));    // (rows behind the last one: exp2(-inf) = 0)
+    if (r0 + row < n) {
+      const float2 st = a.s.stat[rg + row];
+      const float g = a.g[rg + row];
+      m = make_float4(PAIR ? st.x : st.x * CE_LOG2E, g * st.y, g, __int_as_float(a.s.lab[rg + row]));
+    }
+    meta[row] = m;
+  }
+  __syncthreads();
+  const int l = Core::lane(), j0 = cg + Core::col0() + 4 * (l >> 4);
+#pragma unroll
+  for (int i = 0; i < Core::TI; ++i) {
+    const float4 m = meta[Core::row0() + i * 16 + (l & 15)];
+#pragma unroll
+    for (int j = 0; j < Core::TJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c.acc[i][j][r] = ce_exp<PAIR>(c.acc[i][j][r], m.x, m.x) * m.y;
+    const int lab = __float_as_int(m.w) - (cg + Core::col0());
+    if ((unsigned)lab < (unsigned)Core::WN) {
+#pragma unroll
+      for (int j = 0; j < Core::TJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c.acc[i][j][r] -= lab == j * 16 + 4 * (l >> 4) + r ? m.z : 0.f;
+    }
+  }
+  if (cg + Core::BN > a.V) {
+#pragma unroll
+    for (int j = 0; j < Core::TJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (j0 + j * 16 + r >= a.V) {
+#pragma unroll
+          for (int i = 0; i < Core::TI; ++i) c.acc[i][j][r] = 0.f;
+        }
+  }
+  if (a.db) {
+#pragma unroll
+    for (int j = 0; j < Core::TJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < Core::TI; ++i) v += c.acc[i][j][r];
+        v = fi_row16_sum(v);
+        if ((l & 15) == 0) colsum[(Core::wave() / Core::NWN) * Core::BN + Core::col0() + j * 16 + 4 * (l >> 4) + r] = v;
+      }
+    __syncthreads();
+    for (int j = threadIdx.x; j < Core::BN; j += Core::THREADS) {
+      float v = 0.f;
+#pragma unroll
+      for (int q = 0; q < Core::BM / Core::WM; ++q) v += colsum[q * Core::BN + j];
+      if (cg + j < a.V) a.db[(rg / Core::BM) * a.V + cg + j] = v;
+    }
+  }
+  const NtBlock<SB, SB> blk{(float*)(smem + Core::wave() * NtBlock<SB, SB>::BYTES)};
+  const int vcols = a.V - a.v0 < a.Vc ? a.V - a.v0 : a.Vc, vpad = ce_kpad<PAIR>(vcols), npad = ce_kpad<PAIR>(n);
+#pragma unroll
+  for (int bi = 0; bi < Core::WM / SB; ++bi)
+#pragma unroll
+    for (int bj = 0; bj < Core::WN / SB; ++bj) {
+      const int gi = r0 + Core::row0() + bi * SB, gj = c0 + Core::col0() + bj * SB;
+      blk.put(c, bi, bj, 1.f);
+      if (a.dl) {
+        blk.template rows<false>([&](int i, int j0, float (&v)[8]) {
+          if (gi + i >= n || gj + j0 >= vpad) return;
+          f16_t* row = a.dl + (i64)(gi + i) * a.ld_dl;
+          if constexpr (PAIR)
+            nt_store_pair(row, gj + j0, v);
+          else
+            *(uint4*)(row + gj + j0) = VecWords<f16_t>::pack(v);
+        });
+      }
+      if (a.dlt) {
+        blk.cols([&](int j, int i0, float (&v)[8]) {
+          if (gj + j >= vcols || gi + i0 >= npad) return;
+          f16_t* row = a.dlt + (i64)(gj + j) * a.ld_dlt;
+          if constexpr (PAIR)
+            nt_store_pair(row, gi + i0, v);
+          else
+            *(uint4*)(row + gi + i0) = VecWords<f16_t>::pack(v);
+        });
+      }
+    }
+}
+
+// dx (A = G rows, B = W^T rows) or dW (A = G^T rows, B = x^T rows)
+struct CeGrad {
+  const f16_t *a, *b;
+  i64 lda, ldb;
+  int M, N;                // upper bound of the output's rows; columns (D)
+  i64 K;                   // upper bound of the contraction (values)
+  const int* count;        // labelled rows
+  i64 t0, Tc;              // the piece's rows
+  int rows_are_tokens;     // dx: M comes from the device; else K does
+  int splits, first;       // first piece of the output: store, else add
+  float* part;             // [split][M][N] fp32, or NULL: `out` is written straight away
+  // the output
+  void* out;
+  int out_dtype, accumulate, vec;
+  i64 ldo;
+  const int* idx;          // dx: where a row belongs, else NULL
+  const float* scal;
+  int rscale;              // index of the reciprocal of b's scale, -1: none
+};
+
+__device__ __forceinline__ void ce_put(const CeGrad& a, i64 row, int col, const float (&v)[8], int nv) {
+  const i64 at = row * a.ldo + col;
+  if (a.vec && !a.accumulate) {                                         // (every vector of 8 is whole and 16-byte aligned)
+    if (a.out_dtype == FI_F32) {
+      float4* p = (float4*)((float*)a.out + at);
+      p[0] = make_float4(v[0], v[1], v[2], v[3]);
+      p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *(uint4*)((uint16_t*)a.out + at) = a.out_dtype == FI_BF16 ? VecWords<bf16_t>::pack(v) : VecWords<f16_t>::pack(v);
+    }
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    if (t < nv) {
+      if (a.out_dtype == FI_F32)
+        ((float*)a.out)[at + t] = a.accumulate ? ((float*)a.out)[at + t] + v[t] : v[t];
+      else if (a.out_dtype == FI_BF16)
+        ((bf16_t*)a.out)[at + t] = (bf16_t)v[t];
+      else
+        ((f16_t*)a.out)[at + t] = (f16_t)v[t];
+    }
+  }
+}
+__device__ __forceinline__ float ce_rscale(const CeGrad& a) { return a.rscale >= 0 ? a.scal[a.rscale] : 1.f; }
+
+template <class Core, bool PAIR>
+__global__ __launch_bounds__(Core::THREADS) void ce_grad_kernel(CeGrad a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const i64 left = (i64)a.count[0] - a.t0;
+  const int n = (int)(left < 0 ? 0 : left < a.Tc ? left : a.Tc);
+  const int M = a.rows_are_tokens ? n : a.M;
+  const i64 K = a.rows_are_tokens ? a.K : n;
+  const int nti = (M + Core::BM - 1) / Core::BM, ntj = (a.N + Core::BN - 1) / Core::BN;
+  int ti, tj;
+  if (!ce_tile(nti, ntj * a.splits, ti, tj)) return;
+  const int sp = tj % a.splits;
+  tj /= a.splits;
+  const int stages = (int)((K + (PAIR ? 31 : 63)) / (PAIR ? 32 : 64)), per = (stages + a.splits - 1) / a.splits;
+  const int s0 = sp * per < stages ? sp * per : stages, s1 = s0 + per < stages ? s0 + per : stages;
+  Core c;
+  c.clear();
+  c.run(a.a + (i64)ti * Core::BM * a.lda, a.lda, M - ti * Core::BM, a.b + (i64)tj * Core::BN * a.ldb, a.ldb, a.N - tj * Core::BN, s0, s1, smem);
+  constexpr int SB = Core::WM >= 64 && Core::WN >= 64 ? 64 : 32;
+  const NtBlock<SB, SB> blk{(float*)(smem + Core::wave() * NtBlock<SB, SB>::BYTES)};
+  const float rg = a.scal[SC_RG], rb = ce_rscale(a);
+#pragma unroll
+  for (int bi = 0; bi < Core::WM / SB; ++bi)
+#pragma unroll
+    for (int bj = 0; bj < Core::WN / SB; ++bj) {
+      const int gi = ti * Core::BM + Core::row0() + bi * SB, gj = tj * Core::BN + Core::col0() + bj * SB;
+      blk.put(c, bi, bj, 1.f);
+      blk.template rows<false>([&](int i, int j0, float (&v)[8]) {
+        const int r = gi + i, k = gj + j0;
+        if (r >= M || k >= a.N) return;
+        const int nv = a.N - k < 8 ? a.N - k : 8;
+        if (a.part) {
+          float* p = a.part + ((i64)sp * a.M + r) * a.N + k;
+          if ((a.N & 7) == 0) {
+            float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
+            if (!a.first) {
+              const float4 x = ((const float4*)p)[0], y = ((const float4*)p)[1];
+              lo.x += x.x, lo.y += x.y, lo.z += x.z, lo.w += x.w, hi.x += y.x, hi.y += y.y, hi.z += y.z, hi.w += y.w;
+            }
+            ((float4*)p)[0] = lo, ((float4*)p)[1] = hi;
+            return;
+          }
+#pragma unroll
+          for (int t = 0; t < 8; ++t)
+            if (t < nv) p[t] = a.first ? v[t] : p[t] + v[t];
+        } else {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) v[t] = v[t] * rg * rb;
+          ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : (i64)r, k, v, nv);
+        }
+      });
+    }
+}
+
+// joins the split parts of an output in their order
+__global__ __launch_bounds__(256) void ce_join_kernel(CeGrad a) {
+  const i64 left = (i64)a.count[0] - a.t0;
+  const i64 M = a.rows_are_tokens ? (left < 0 ? 0 : left < a.Tc ? left : a.Tc) : a.M;
+  const i64 nv = (a.N + 7) / 8, total = M * nv;
+  const float rg = a.scal[SC_RG], rb = ce_rscale(a);
+  for (i64 e = (i64)blockIdx.x * 256 + threadIdx.x; e < total; e += (i64)gridDim.x * 256) {
+    const i64 r = e / nv;
+    const int k = (int)(e - r * nv) * 8, n = a.N - k < 8 ? a.N - k : 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+      const float* p = a.part + ((i64)s * a.M + r) * a.N + k;
+      if ((a.N & 7) == 0) {
+        const float4 x = ((const float4*)p)[0], y = ((const float4*)p)[1];
+        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+      } else {
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          if (t < n) v[t] += p[t];
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t) v[t] = v[t] * rg * rb;
+    ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : r, k, v, n);
+  }
+}
+
+// db: column sums over the row tiles, in fp64
+__global__ __launch_bounds__(256) void ce_dbias_kernel(const float* part, int tile, int V, const int* count, const float* scal, float* db, int accumulate) {
+  __shared__ double sm[4][64];
+  const int v = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+  const int nt = (count[0] + tile - 1) / tile;
+  double acc = 0.0;
+  if (v < V)
+    for (int t = q; t < nt; t += 4) acc += (double)part[(i64)t * V + v];
+  sm[q][threadIdx.x & 63] = acc;
+  __syncthreads();
+  if (q == 0 && v < V) {
+    acc = (sm[0][threadIdx.x] + sm[1][threadIdx.x] + sm[2][threadIdx.x] + sm[3][threadIdx.x]) * (double)scal[SC_RG];
+    db[v] = accumulate ? db[v] + (float)acc : (float)acc;
+  }
+}
+
+// dx of the rows that take no part
+__global__ __launch_bounds__(256) void ce_zero_rows_kernel(const void* labels, int ltype, i64 T, i64 ignore, void* dx, int esize, int D) {
+  const int per = 256;
+  const i64 r0 = (i64)blockIdx.x * per;
+  const i64 rb = (i64)D * esize;
+  for (int k = threadIdx.x >> 6; k < per; k += 4) {                     // a wave per row
+    const i64 r = r0 + k;
+    if (r >= T) break;
+    if (ce_label(labels, ltype, r) != ignore) continue;
+    char* p = (char*)dx + r * rb;
+    if (esize == 2)
+      for (int c = threadIdx.x & 63; c < D; c += 64) ((uint16_t*)p)[c] = 0;
+    else
+      for (int c = threadIdx.x & 63; c < D; c += 64) ((uint32_t*)p)[c] = 0;
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------------
+struct Carve {
+  char* base;
+  i64 at = 0;
+  template <typename P>
+  P* take(i64 n) {
+    P* p = base ? (P*)(base + at) : nullptr;
+    at += ce_up(n * (i64)sizeof(P), 256);
+    return p;
+  }
+};
+
+struct CeShape {
+  bool pair;
+  int ku;                  // values per stage
+  int kp;                  // D padded to stages
+  i64 ldx;                 // packed operand rows, elements
+  bool w_direct;           // W is used where it lies
+  i64 ldw;
+  bool scaled;             // scales are computed (pair forms, or fp16 made of bf16)
+};
+CeShape ce_shape(const FiLinearCe& d, const void* w) {
+  CeShape s;
+  s.pair = d.dtype == FI_F32;
+  s.ku = s.pair ? 32 : 64;
+  s.kp = (int)ce_up(d.D, s.ku);
+  s.ldx = s.pair ? 2L * s.kp : s.kp;
+  // 16-bit weights whose rows are whole stages and 16-byte aligned are read in place
+  s.w_direct = !s.pair && d.wdtype == d.dtype && d.D % 64 == 0 && d.ldw % 8 == 0 && ((uintptr_t)w & 15) == 0;
+  s.ldw = s.w_direct ? d.ldw : s.ldx;
+  s.scaled = d.dtype != FI_F16;
+  return s;
+}
+
+int ce_check(const FiLinearCe* d) {
+  if (!d) return FI_ERR_NULL;
+  if (d->dtype != FI_F32 && d->dtype != FI_BF16 && d->dtype != FI_F16) return FI_ERR_DTYPE;
+  if (d->wdtype != d->dtype && d->wdtype != FI_F32) return FI_ERR_DTYPE;
+  if (d->ltype != FI_LABEL_U8 && d->ltype != FI_LABEL_I32 && d->ltype != FI_LABEL_I64) return FI_ERR_DTYPE;
+  if (d->reduction < 0 || d->reduction > 2) return FI_ERR_SHAPE;
+  if (d->T < 1 || d->V < 1 || d->D < 1 || d->T >= (1LL << 30) || d->V > (1 << 20) || d->D > (1 << 16)) return FI_ERR_SHAPE;
+  if (d->ldx < d->D || d->ldw < d->D || d->ldw > (1 << 22)) return FI_ERR_SHAPE;
+  return 0;
+}
+
+// tiles of the logits' product: 256 x 256; 64 rows where there are no more (the classes are then streamed once, and three quarters of a
+// tall tile would repeat the last row); 64 classes likewise
+int ce_logits_tile(const FiLinearCe& d) { return d.T <= 64 ? 1 : d.V <= 64 ? 2 : 0; }
+constexpr int CE_BM[3] = {256, 64, 256}, CE_BN[3] = {256, 256, 64};
+
+template <typename T, bool PAIR> struct CeCores {
+  typedef NtCore<T, PAIR, 256, 256, 128, 64> C0;
+  typedef NtCore<T, PAIR, 64, 256, 64, 32> C1;
+  typedef NtCore<T, PAIR, 256, 64, 32, 64> C2;
+};
+
+template <class Core, typename T, bool PAIR>
+int ce_launch_fwd(const CeLogits& a, i64 T_rows, hipStream_t st) {
+  static const bool ok = nt_allow_lds((const void*)ce_fwd_kernel<Core, T, PAIR>);
+  if (!ok) return FI_ERR_UNSUPPORTED;
+  const i64 n = (T_rows + Core::BM - 1) / Core::BM * a.ntj;
+  if (n > (1LL << 30)) return FI_ERR_SHAPE;
+  hipLaunchKernelGGL((ce_fwd_kernel<Core, T, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), Core::LDS, st, a);
+  FI_CHECK_LAUNCH();
+  return 0;
+}
+template <class Core, typename T, bool PAIR>
+int ce_launch_dlogits(const CeLogits& a, hipStream_t st) {
+  static const bool ok = nt_allow_lds((const void*)ce_dlogits_kernel<Core, T, PAIR>);
+  if (!ok) return FI_ERR_UNSUPPORTED;
+  constexpr int SB = Core::WM >= 64 && Core::WN >= 64 ? 64 : 32, SCR = Core::NW * NtBlock<SB, SB>::BYTES;
+  constexpr int lds = (SCR > Core::LDS ? SCR : Core::LDS) + Core::BM * 16 + Core::BM / Core::WM * Core::BN * 4;
+  const i64 n = (a.Tc + Core::BM - 1) / Core::BM * ((a.Vc + Core::BN - 1) / Core::BN);
+  hipLaunchKernelGGL((ce_dlogits_kernel<Core, T, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), lds, st, a);
+  FI_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T, bool PAIR>
+int ce_logits(const CeLogits& a, const FiLinearCe& d, bool fwd, hipStream_t st) {
+  typedef CeCores<T, PAIR> C;
+  switch (ce_logits_tile(d)) {
+    case 0: return fwd ? ce_launch_fwd<typename C::C0, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C0, T, PAIR>(a, st);
+    case 1: return fwd ? ce_launch_fwd<typename C::C1, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C1, T, PAIR>(a, st);
+    default: return fwd ? ce_launch_fwd<typename C::C2, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C2, T, PAIR>(a, st);
+  }
+}
+int ce_logits_any(const CeLogits& a, const FiLinearCe& d, bool fwd, hipStream_t st) {
+  return d.dtype == FI_F32 ? ce_logits<f16_t, true>(a, d, fwd, st) : d.dtype == FI_BF16 ? ce_logits<bf16_t, false>(a, d, fwd, st) : ce_logits<f16_t, false>(a, d, fwd, st);
+}
+
+int ce_pack(const CePack& a, hipStream_t st) {
+  const i64 gx = (a.rows + 63) / 64;
+  const int cols = a.same ? a.same_k : a.D;
+  hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)gx, (unsigned)((cols + 63) / 64)), dim3(256), 0, st, a);
+  FI_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+void ce_amax(const void* p, i64 ld, int D, const CeSaved* s, i64 rows, float* part, hipStream_t st) {
+  const int vec = ((uintptr_t)p & 15) == 0 && ld % DT<T>::VG == 0;
+  hipLaunchKernelGGL(ce_amax_kernel<T>, dim3(CE_PARTS), dim3(256), 0, st, (const T*)p, ld, D, vec, s ? s->idx : nullptr, s ? s->count : nullptr, rows, part);
+}
+void ce_amax_any(const void* p, int dtype, i64 ld, int D, const CeSaved* s, i64 rows, float* part, hipStream_t st) {
+  dtype == FI_F32 ? ce_amax<float>(p, ld, D, s, rows, part, st) : dtype == FI_BF16 ? ce_amax<bf16_t>(p, ld, D, s, rows, part, st) : ce_amax<f16_t>(p, ld, D, s, rows, part, st);
+}
+int ce_scales(const FiLinearCe& d, const void* x, const void* w, const CeSaved& s, float* parts, float* scal, hipStream_t st) {
+  ce_amax_any(x, d.dtype, d.ldx, d.D, &s, d.T, parts, st);
+  FI_CHECK_LAUNCH();
+  ce_amax_any(w, d.wdtype, d.ldw, d.D, nullptr, d.V, parts + CE_PARTS, st);
+  FI_CHECK_LAUNCH();
+  hipLaunchKernelGGL(ce_scales_kernel, dim3(1), dim3(256), 0, st, parts, parts + CE_PARTS, scal);
+  FI_CHECK_LAUNCH();
+  return 0;
+}
+
+struct CeFwdWs {
+  int* cnt;
+  float *parts, *scal, *zt;
+  f16_t *xc, *wc;
+  float2* part;
+  double* sums;
+  i64 bytes;
+};
+CeFwdWs ce_fwd_ws(const FiLinearCe& d, const CeShape& s, void* p) {
+  Carve c{(char*)p};
+  CeFwdWs w;
+  w.cnt = c.take<int>((d.T + CE_ROWS - 1) / CE_ROWS);
+  w.parts = c.take<float>(2 * CE_PARTS);
+  w.scal = c.take<float>(SC_N);
+  w.zt = c.take<float>(d.T);
+  w.sums = c.take<double>(CE_LOSS_WGS);
+  w.xc = c.take<f16_t>(d.T * s.ldx);
+  w.wc = s.w_direct ? nullptr : c.take<f16_t>((i64)d.V * s.ldx);
+  w.part = c.take<float2>(d.T * ((d.V + CE_BN[ce_logits_tile(d)] - 1) / CE_BN[ce_logits_tile(d)]));
+  w.bytes = c.at;
+  return w;
+}
+
+CePack ce_pack_x(const FiLinearCe& d, const CeShape& s, const void* x, const CeSaved& sv, const float* scal, f16_t* xc) {
+  CePack k = {};
+  k.src = x, k.dtype = d.dtype, k.D = d.D, k.ld = d.ldx, k.rows = d.T, k.idx = sv.idx, k.count = sv.count;
+  k.scale = s.scaled ? scal + SC_X : nullptr;
+  k.same = xc, k.ld_same = s.ldx, k.same_k = s.kp, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
+  return k;
+}
+CePack ce_pack_w(const FiLinearCe& d, const CeShape& s, const void* w, const float* scal, f16_t* wc) {
+  CePack k = {};
+  k.src = w, k.dtype = d.wdtype, k.D = d.D, k.ld = d.ldw, k.rows = d.V;
+  k.scale = s.scaled ? scal + SC_W : nullptr;
+  k.same = wc, k.ld_same = s.ldx, k.same_k = s.kp, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
+  return k;
+}
+
+// ---- the backward pass's plan
+struct CeGradPlan {
+  int tile, splits;
+  bool part;
+};
+// Output tiles of 256 x 256, 128 x 128 or 64 x 64 (columns or rows that few); a contraction is split where the tiles do not fill the chip.
+constexpr int CE_GT[3] = {256, 128, 64};
+CeGradPlan ce_grad_plan(i64 M, i64 N, i64 K, int ku, bool pieces) {
+  CeGradPlan p;
+  const i64 least = M < N ? M : N;
+  p.tile = least > 128 && (M + 255) / 256 * ((N + 255) / 256) >= 128 ? 0 : least > 64 ? 1 : 2;
+  const int t = CE_GT[p.tile];
+  const i64 tiles = (M + t - 1) / t * ((N + t - 1) / t), stages = (K + ku - 1) / ku;
+  i64 s = 512 / tiles;
+  if (s > stages / 8) s = stages / 8;
+  if (s > 64) s = 64;
+  if (s < 1) s = 1;
+  p.splits = (int)s;
+  p.part = p.splits > 1 || pieces;
+  return p;
+}
+struct CeBwdWs {
+  float *parts, *scal, *g, *db, *pdx, *pdw;
+  f16_t *xc, *wc, *xt, *wt, *dl, *dlt;
+  i64 ld_xt, ld_wt, ld_dl, ld_dlt, Tc;
+  int Vc;
+  CeGradPlan dx, dw;
+  i64 pdw_piece, bytes;
+};
+constexpr i64 CE_PIECE = 1LL << 27;              // values of G held at a time (two orientations: 512 MiB; twice that for pairs)
+CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need_dw, bool need_db, void* p) {
+  Carve c{(char*)p};
+  CeBwdWs w;
+  const int f = s.pair ? 2 : 1;
+  const i64 Tp = ce_up(d.T, 256), Vp = ce_up(d.V, 256);
+  // a piece: all rows, if 256 classes of them fit, and as many classes as do
+  w.Tc = Tp < CE_PIECE / 256 ? Tp : CE_PIECE / 256;
+  const i64 vc = CE_PIECE / w.Tc / 256 * 256;
+  w.Vc = (int)(vc < Vp ? vc : Vp);
+  w.ld_xt = f * w.Tc, w.ld_wt = f * Vp, w.ld_dl = (i64)f * w.Vc, w.ld_dlt = f * w.Tc;
+  w.parts = c.take<float>(2 * CE_PARTS);
+  w.scal = c.take<float>(SC_N);
+  w.g = c.take<float>(d.T);
+  const int bm = CE_BM[ce_logits_tile(d)];
+  w.db = need_db ? c.take<float>((d.T + bm - 1) / bm * d.V) : nullptr;
+  w.xc = c.take<f16_t>(d.T * s.ldx);
+  w.wc = s.w_direct ? nullptr : c.take<f16_t>((i64)d.V * s.ldx);
+  w.xt = need_dw ? c.take<f16_t>(d.D * w.ld_xt) : nullptr;
+  w.wt = need_dx ? c.take<f16_t>(d.D * w.ld_wt) : nullptr;
+  w.dl = need_dx ? c.take<f16_t>(w.Tc * w.ld_dl) : nullptr;
+  w.dlt = need_dw ? c.take<f16_t>((i64)w.Vc * w.ld_dlt) : nullptr;
+  w.dx = ce_grad_plan(d.T < w.Tc ? d.T : w.Tc, d.D, d.V < w.Vc ? d.V : w.Vc, s.ku, w.Vc < d.V);
+  w.dw = ce_grad_plan(d.V < w.Vc ? d.V : w.Vc, d.D, d.T < w.Tc ? d.T : w.Tc, s.ku, w.Tc < d.T);
+  w.pdx = need_dx && w.dx.part ? c.take<float>((i64)w.dx.splits * w.Tc * d.D) : nullptr;
+  // (dW's sum over several row pieces is kept for every class piece)
+  w.pdw_piece = (i64)w.dw.splits * w.Vc * d.D;
+  w.pdw = need_dw && w.dw.part ? c.take<float>(w.pdw_piece * (w.Tc < d.T ? (d.V + w.Vc - 1) / w.Vc : 1)) : nullptr;
+  w.bytes = c.at;
+  return w;
+}
+
+template <class Core, bool PAIR>
+int ce_launch_grad(const CeGrad& a, hipStream_t st) {
+  static const bool ok = nt_allow_lds((const void*)ce_grad_kernel<Core, PAIR>);
+  if (!ok) return FI_ERR_UNSUPPORTED;
+  const i64 n = (i64)((a.M + Core::BM - 1) / Core::BM) * ((a.N + Core::BN - 1) / Core::BN) * a.splits;
+  hipLaunchKernelGGL((ce_grad_kernel<Core, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), Core::LDS, st, a);
+  FI_CHECK_LAUNCH();
+  return 0;
+}
+template <bool PAIR>
+int ce_grad(const CeGrad& a, int tile, hipStream_t st) {
+  return tile == 0 ? ce_launch_grad<NtCore<f16_t, PAIR, 256, 256, 128, 64>, PAIR>(a, st)
+         : tile == 1 ? ce_launch_grad<NtCore<f16_t, PAIR, 128, 128, 64, 64>, PAIR>(a, st)
+                     : ce_launch_grad<NtCore<f16_t, PAIR, 64, 64, 32, 32>, PAIR>(a, st);
+}
+int ce_join(const CeGrad& a, hipStream_t st) {
+  const i64 n = ((i64)a.M * ((a.N + 7) / 8) + 255) / 256;
+  hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)(n < 4096 ? n : 4096)), dim3(256), 0, st, a);
+  FI_CHECK_LAUNCH();
+  return 0;
+}
+
+}  // namespace
+
+extern "C" long fi_linear_ce_saved(const FiLinearCe* d) {
+  const int rc = ce_check(d);
+  return rc ? rc : 64 + 4 * ce_up(4 * d->T, 64);
+}
+extern "C" long fi_linear_ce_fwd_workspace(const FiLinearCe* d, const void* w) {
+  const int rc = ce_check(d);
+  return rc ? rc : ce_fwd_ws(*d, ce_shape(*d, w), nullptr).bytes;
+}
+extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* w, const float* bias, const void* labels, float* loss,
+                                void* saved, void* workspace, void* stream) {
+  int rc = ce_check(d);
+  if (rc) return rc;
+  if (!x || !w || !labels || !loss || !saved || !workspace) return FI_ERR_NULL;
+  hipStream_t st = (hipStream_t)stream;
+  const CeShape s = ce_shape(*d, w);
+  const CeFwdWs ws = ce_fwd_ws(*d, s, workspace);
+  const CeSaved sv = ce_saved(saved, d->T);
+  float* const rows_out = d->reduction == 0 ? loss : nullptr;
+  const unsigned nb = (unsigned)((d->T + CE_ROWS - 1) / CE_ROWS);
+  hipLaunchKernelGGL(ce_count_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, ws.cnt);
+  FI_CHECK_LAUNCH();
+  hipLaunchKernelGGL(ce_gather_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, d->V, ws.cnt, sv, ws.zt, rows_out);
+  FI_CHECK_LAUNCH();
+  if (s.pair && (rc = ce_scales(*d, x, w, sv, ws.parts, ws.scal, st))) return rc;
+  if ((rc = ce_pack(ce_pack_x(*d, s, x, sv, ws.scal, ws.xc), st))) return rc;
+  if (!s.w_direct && (rc = ce_pack(ce_pack_w(*d, s, w, ws.scal, ws.wc), st))) return rc;
+  CeLogits a = {};
+  const int bn = CE_BN[ce_logits_tile(*d)];
+  a.x = ws.xc, a.ldx = s.ldx, a.w = s.w_direct ? w : ws.wc, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
+  a.scal = s.pair ? ws.scal : nullptr, a.s = sv, a.part = ws.part, a.zt = ws.zt, a.ntj = (d->V + bn - 1) / bn;
+  if ((rc = ce_logits_any(a, *d, true, st))) return rc;
+  const int lanes = a.ntj > 32 ? 64 : a.ntj > 4 ? 8 : 1;
+  i64 g = (d->T * lanes + 255) / 256;
+  if (g > CE_LOSS_WGS) g = CE_LOSS_WGS;
+  if (lanes == 64)
+    hipLaunchKernelGGL(ce_rows_kernel<64>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums);
+  else if (lanes == 8)
+    hipLaunchKernelGGL(ce_rows_kernel<8>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums);
+  else
+    hipLaunchKernelGGL(ce_rows_kernel<1>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums);
+  FI_CHECK_LAUNCH();
+  if (d->reduction != 0) {
+    hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(256), 0, st, ws.sums, (int)g, sv.count, d->reduction == 1 ? 1 : 0, loss);
+    FI_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+extern "C" long fi_linear_ce_bwd_workspace(const FiLinearCe* d, const void* w, int need_dx, int need_dw, int need_db) {
+  const int rc = ce_check(d);
+  return rc ? rc : ce_bwd_ws(*d, ce_shape(*d, w), need_dx != 0, need_dw != 0, need_db != 0, nullptr).bytes;
+}
+extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* w, const float* bias, const void* labels, const void* saved,
+                                const float* gloss, void* dx, void* dw, int dw_accumulate, float* db, int db_accumulate, void* workspace,
+                                void* stream) {
+  int rc = ce_check(d);
+  if (rc) return rc;
+  if (!x || !w || !labels || !saved || !gloss || !workspace) return FI_ERR_NULL;
+  if (dw_accumulate && d->wdtype != FI_F32) return FI_ERR_DTYPE;
+  if (!dx && !dw && !db) return 0;
+  hipStream_t st = (hipStream_t)stream;
+  const CeShape s = ce_shape(*d, w);
+  const CeBwdWs ws = ce_bwd_ws(*d, s, dx != nullptr, dw != nullptr, db != nullptr, workspace);
+  const CeSaved sv = ce_saved((void*)saved, d->T);
+  if (s.scaled && (rc = ce_scales(*d, x, w, sv, ws.parts, ws.scal, st))) return rc;
+  CePack px = ce_pack_x(*d, s, x, sv, ws.scal, ws.xc);
+  const bool rows_pieces = ws.Tc < d->T;
+  if (!rows_pieces) px.turned = ws.xt, px.ld_turned = ws.ld_xt, px.turned_pair = s.pair;
+  if ((rc = ce_pack(px, st))) return rc;
+  if (!s.w_direct || ws.wt) {
+    CePack pw = ce_pack_w(*d, s, w, ws.scal, ws.wc);
+    pw.turned = ws.wt, pw.ld_turned = ws.ld_wt, pw.turned_pair = s.pair;
+    if ((rc = ce_pack(pw, st))) return rc;
+  }
+  if (d->reduction == 0) {
+    hipLaunchKernelGGL(ce_gmax_kernel, dim3(CE_PARTS), dim3(256), 0, st, gloss, sv.idx, sv.count, ws.parts);
+    FI_CHECK_LAUNCH();
+  }
+  const i64 ng = (d->T + 255) / 256;
+  hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)(ng < 1024 ? ng : 1024)), dim3(256), 0, st, gloss, d->reduction, ws.parts, sv, ws.scal, ws.g);
+  FI_CHECK_LAUNCH();
+  if (dx) {
+    hipLaunchKernelGGL(ce_zero_rows_kernel, dim3((unsigned)ng), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, dx, s.pair ? 4 : 2, d->D);
+    FI_CHECK_LAUNCH();
+  }
+  const int f = s.pair ? 2 : 1;
+  CeGrad gx = {}, gw = {};
+  gx.a = ws.dl, gx.lda = ws.ld_dl, gx.ldb = ws.ld_wt, gx.N = d->D, gx.count = sv.count, gx.rows_are_tokens = 1;
+  gx.splits = ws.dx.splits, gx.out = dx, gx.out_dtype = d->dtype, gx.ldo = d->D, gx.idx = sv.idx, gx.scal = ws.scal, gx.rscale = s.scaled ? SC_RW : -1;
+  gw.a = ws.dlt, gw.lda = ws.ld_dlt, gw.ldb = ws.ld_xt, gw.N = d->D, gw.count = sv.count;
+  gw.splits = ws.dw.splits, gw.out_dtype = d->wdtype, gw.accumulate = dw_accumulate, gw.ldo = d->D, gw.scal = ws.scal, gw.rscale = s.scaled ? SC_RX : -1;
+  gx.vec = d->D % 8 == 0 && ((uintptr_t)dx & 15) == 0, gw.vec = d->D % 8 == 0 && ((uintptr_t)dw & 15) == 0;
+  CeLogits a = {};
+  a.x = ws.xc, a.ldx = s.ldx, a.w = s.w_direct ? w : ws.wc, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
+  a.scal = s.pair ? ws.scal : nullptr, a.s = sv, a.g = ws.g, a.dl = ws.dl, a.dlt = ws.dlt, a.ld_dl = ws.ld_dl, a.ld_dlt = ws.ld_dlt, a.db = ws.db;
+  const int wsize = d->wdtype == FI_F32 ? 4 : 2;
+  // the classes innermost: dx of a row piece is complete with its last class piece, dW's parts are joined behind the last row piece
+  const i64 nt = (d->T + ws.Tc - 1) / ws.Tc, nv = (d->V + ws.Vc - 1) / ws.Vc;
+  for (i64 o = 0; o < nt * nv; ++o) {
+    const i64 it = o / nv, iv = o % nv;
+    a.t0 = it * ws.Tc, a.Tc = ws.Tc < d->T - a.t0 ? ws.Tc : d->T - a.t0;
+    a.v0 = (int)(iv * ws.Vc), a.Vc = ws.Vc < d->V - a.v0 ? ws.Vc : d->V - a.v0;
+    if (rows_pieces && dw && iv == 0) {
+      CePack pt = ce_pack_x(*d, s, x, sv, ws.scal, nullptr);
+      pt.begin = a.t0, pt.rows = a.Tc, pt.turned = ws.xt, pt.ld_turned = ws.ld_xt, pt.turned_pair = s.pair;
+      if ((rc = ce_pack(pt, st))) return rc;
+    }
+    if ((rc = ce_logits_any(a, *d, false, st))) return rc;
+    if (dx) {
+      gx.b = ws.wt + (i64)f * a.v0, gx.M = (int)a.Tc, gx.K = a.Vc, gx.t0 = a.t0, gx.Tc = a.Tc, gx.first = iv == 0;
+      gx.part = ws.pdx;
+      if ((rc = s.pair ? ce_grad<true>(gx, ws.dx.tile, st) : ce_grad<false>(gx, ws.dx.tile, st))) return rc;
+      if (gx.part && iv == nv - 1 && (rc = ce_join(gx, st))) return rc;
+    }
+    if (dw) {
+      gw.b = ws.xt, gw.M = a.Vc, gw.K = a.Tc, gw.t0 = a.t0, gw.Tc = a.Tc, gw.first = it == 0;
+      gw.out = (char*)dw + (i64)a.v0 * d->D * wsize;
+      gw.part = ws.pdw ? ws.pdw + (rows_pieces ? iv * ws.pdw_piece : 0) : nullptr;
+      if ((rc = s.pair ? ce_grad<true>(gw, ws.dw.tile, st) : ce_grad<false>(gw, ws.dw.tile, st))) return rc;
+      if (gw.part && it == nt - 1 && (rc = ce_join(gw, st))) return rc;
+    }
+  }
+  if (db) {
+    hipLaunchKernelGGL(ce_dbias_kernel, dim3((unsigned)((d->V + 63) / 64)), dim3(256), 0, st, ws.db, CE_BM[ce_logits_tile(*d)], d->V, sv.count, ws.scal, db, db_accumulate);
+    FI_CHECK_LAUNCH();
+  }
+  return 0;
+}

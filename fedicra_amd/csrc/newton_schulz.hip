@@ -1,0 +1,399 @@
+// Orthogonalising updates by Newton-Schulz products:  X <- U / (|U|_F + eps),  then `steps` times
+//     A = X X^T,   S = a I + b A + c A A,   X <- S X          (X has m rows of n >= m values; U^T where U is tall)
+// which applies the odd polynomial a s + b s^3 + c s^5 to every singular value s.
+//
+// Numerics: the smallest singular values grow 3.44-fold per step, and rounding of X, A or S to 16 bits is carried along with them
+// (2e-3 .. 3e-2 of the result's norm after five steps); operands are therefore kept as pairs of fp16 (nt_product.h), which reproduces an fp32
+// iteration's error.  Everything is scaled by 2^12 in storage: |X|, |A| and |S| stay below 16 (the entry checks the polynomial for
+// that), so nothing overflows fp16, and the low parts reach down to 2^-36.  The Frobenius norm is summed in fp64.
+//
+// Work per step: m^2 n + m^3 multiply-adds halved by symmetry + m^2 n: A and S are computed on and below the diagonal and stored twice.  Every
+// product's second operand is wanted with its contraction index contiguous, so X is kept in both orientations (X for A, X^T for S X); the
+// product that makes the next X stores both.  All matrices of a call (one model's filters) share each launch: 2 + 3 (+1) launches per step
+// whatever their number.
+#include <math.h>
+
+#include "nt_product.h"
+
+namespace {
+
+constexpr int NS_MAX = 24;                       // matrices per launch (their descriptors travel as kernel arguments)
+constexpr float NS_SCALE = 4096.f;
+constexpr int NS_CHUNK = 16384;                  // elements per partial sum of squares
+
+struct NsItem {
+  const void* u;
+  void* out;
+  f16_t *x, *xt[2], *a, *s;                      // pair rows: x [m][n], xt [n][m], a, s [m][m]
+  float* part;                                   // split contraction: raw accumulators [tile][split][TILE * TILE]
+  double* sums;                                  // partial sums of squares
+  int m, n, tall, dtype, split, nsums;
+};
+struct NsArgs {
+  NsItem it[NS_MAX];
+  int start[NS_MAX + 1];                         // first work item of each matrix in this launch
+  int count, cur, last;
+  float ca, cb, cc, eps;
+};
+
+__device__ __host__ __forceinline__ int ns_pad(int v) { return (v + 31) & ~31; }
+
+__device__ __forceinline__ int ns_find(const NsArgs& g, int w) {
+  int i = 0;
+  while (i + 1 < g.count && w >= g.start[i + 1]) ++i;
+  return i;
+}
+__device__ __forceinline__ float ns_load(const void* p, int dtype, long i) {
+  return dtype == FI_F32 ? ((const float*)p)[i] : dtype == FI_BF16 ? (float)((const bf16_t*)p)[i] : (float)((const f16_t*)p)[i];
+}
+__device__ __forceinline__ void ns_tri(int t, int& i, int& j) {               // t = i (i + 1) / 2 + j, j <= i
+  i = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+  while ((i + 1) * (i + 2) / 2 <= t) ++i;
+  while (i * (i + 1) / 2 > t) --i;
+  j = t - i * (i + 1) / 2;
+}
+
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
+  __shared__ double sm[4];
+  const int w = (int)blockIdx.x, k = ns_find(g, w);
+  const NsItem& q = g.it[k];
+  const long total = (long)q.m * q.n, lo = (long)(w - g.start[k]) * NS_CHUNK;
+  const long hi = lo + NS_CHUNK < total ? lo + NS_CHUNK : total;
+  double acc = 0.0;
+  for (long i = lo + threadIdx.x; i < hi; i += 256) {
+    const double v = (double)ns_load(q.u, q.dtype, i);
+    acc += v * v;
+  }
+  acc = wave_sum(acc);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) q.sums[w - g.start[k]] = sm[0] + sm[1] + sm[2] + sm[3];
+}
+
+// U, normalised, as pair rows in both orientations: one 64 x 64 block of U per workgroup
+__global__ __launch_bounds__(256) void ns_prep_kernel(NsArgs g) {
+  __shared__ float tile[64][65];
+  __shared__ double sm[4];
+  __shared__ float s_inv;
+  const int w = (int)blockIdx.x, k = ns_find(g, w), tid = threadIdx.x;
+  const NsItem& q = g.it[k];
+  double acc = 0.0;
+  for (int i = tid; i < q.nsums; i += 256) acc += q.sums[i];
+  acc = wave_sum(acc);
+  if ((tid & 63) == 0) sm[tid >> 6] = acc;
+  __syncthreads();
+  if (tid == 0) s_inv = (float)((double)NS_SCALE / (sqrt(sm[0] + sm[1] + sm[2] + sm[3]) + (double)g.eps));
+  __syncthreads();
+  const float inv = s_inv;
+  const int rows = q.tall ? q.n : q.m, cols = q.tall ? q.m : q.n;
+  const int nb = (cols + 63) / 64, t = w - g.start[k], r0 = (t / nb) * 64, c0 = (t % nb) * 64;
+  for (int e = tid; e < 64 * 64; e += 256) {
+    const int r = r0 + (e >> 6), c = c0 + (e & 63);
+    tile[e >> 6][e & 63] = r < rows && c < cols ? ns_load(q.u, q.dtype, (long)r * cols + c) * inv : 0.f;
+  }
+  __syncthreads();
+  f16_t* const same = q.tall ? q.xt[0] : q.x;          // U's own orientation
+  f16_t* const turned = q.tall ? q.x : q.xt[0];
+  const int cpad = ns_pad(cols), rpad = ns_pad(rows);
+  for (int e = tid; e < 64 * 8; e += 256) {
+    const int r = e >> 3, c = (e & 7) * 8;
+    float v[8];
+    if (r0 + r < rows && c0 + c < cpad) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = tile[r][c + i];
+      nt_store_pair(same + (long)(r0 + r) * 2 * cpad, c0 + c, v);
+    }
+    if (c0 + r < cols && r0 + c < rpad) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = tile[c + i][r];
+      nt_store_pair(turned + (long)(c0 + r) * 2 * rpad, r0 + c, v);
+    }
+  }
+}
+
+template <int TILE>
+struct NsTile;
+template <> struct NsTile<64> { typedef NtCore<f16_t, true, 64, 64, 32, 32> Core; };
+template <> struct NsTile<128> { typedef NtCore<f16_t, true, 128, 128, 64, 64> Core; };
+template <> struct NsTile<256> { typedef NtCore<f16_t, true, 256, 256, 128, 64> Core; };
+
+__device__ __forceinline__ void ns_put(void* out, int dtype, long at, const float (&v)[8], int n) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    if (t < n) {
+      if (dtype == FI_F32)
+        ((float*)out)[at + t] = v[t];
+      else if (dtype == FI_BF16)
+        ((bf16_t*)out)[at + t] = (bf16_t)v[t];
+      else
+        ((f16_t*)out)[at + t] = (f16_t)v[t];
+    }
+  }
+}
+
+// what becomes of a tile of PHASE 0 (A), 1 (S) or 2 (X)
+template <int PHASE, class Core>
+__device__ __forceinline__ void ns_store(const NsArgs& g, const NsItem& q, const Core& c, int ti, int tj, char* smem) {
+  constexpr int SB = Core::WM >= 64 && Core::WN >= 64 ? 64 : 32, T = Core::BM;
+  const NtBlock<SB, SB> blk{(float*)(smem + Core::wave() * NtBlock<SB, SB>::BYTES)};
+  const int m = q.m, N = PHASE == 2 ? q.n : q.m;
+  const int mpad = ns_pad(m), npad = ns_pad(N);
+  f16_t* const direct = PHASE == 0 ? q.a : PHASE == 1 ? q.s : q.x;
+  f16_t* const turned = PHASE == 2 ? q.xt[g.cur ^ 1] : direct;
+  const bool out = PHASE == 2 && g.last;
+  const bool do_rows = !out || !q.tall, do_cols = out ? q.tall != 0 : PHASE == 2 || ti != tj;      // (a diagonal tile is its own mirror image)
+#pragma unroll
+  for (int bi = 0; bi < Core::WM / SB; ++bi)
+#pragma unroll
+    for (int bj = 0; bj < Core::WN / SB; ++bj) {
+      const int gi = ti * T + Core::row0() + bi * SB, gj = tj * T + Core::col0() + bj * SB;
+      blk.put(c, bi, bj, 1.f / NS_SCALE);
+      if (do_rows || PHASE == 1) {
+        blk.template rows<PHASE == 1>([&](int i, int j0, float (&v)[8]) {
+          const int r = gi + i, k = gj + j0;
+          if (r >= m || k >= npad) return;
+          if constexpr (PHASE == 1) {
+            float a[8];
+            nt_load_pair(q.a + (long)r * 2 * mpad, k, a);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[t] = g.cc * v[t] + g.cb * a[t] + (r == k + t ? g.ca * NS_SCALE : 0.f);
+          }
+          if (out) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[t] *= 1.f / NS_SCALE;
+            ns_put(q.out, q.dtype, (long)r * N + k, v, N - k);
+          } else {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[t] = k + t < N ? v[t] : 0.f;
+            nt_store_pair(direct + (long)r * 2 * npad, k, v);
+          }
+        });
+      }
+      nt_wave_lds_fence();
+      if (do_cols) {
+        blk.cols([&](int j, int i0, float (&v)[8]) {
+          const int r = gj + j, k = gi + i0;
+          if (r >= N || k >= mpad) return;
+          if (out) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[t] *= 1.f / NS_SCALE;
+            ns_put(q.out, q.dtype, (long)r * m + k, v, m - k);
+          } else {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[t] = k + t < m ? v[t] : 0.f;
+            nt_store_pair(turned + (long)r * 2 * mpad, k, v);
+          }
+        });
+      }
+    }
+}
+
+template <int PHASE, int TILE>
+__global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_product_kernel(NsArgs g) {
+  typedef typename NsTile<TILE>::Core Core;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int w = nt_xcd_item((int)blockIdx.x, (int)gridDim.x, g.start[g.count]);
+  if (w < 0) return;
+  const int k = ns_find(g, w);
+  const NsItem& q = g.it[k];
+  const int mt = (q.m + TILE - 1) / TILE, mpad = ns_pad(q.m), npad = ns_pad(q.n);
+  int t = w - g.start[k], sp = 0, ti, tj;
+  if (PHASE == 0) sp = t % q.split, t /= q.split;
+  if (PHASE == 2)
+    ti = t % mt, tj = t / mt;
+  else
+    ns_tri(t, ti, tj);
+  const f16_t* a = PHASE == 0 ? q.x : PHASE == 1 ? q.a : q.s;
+  const f16_t* b = PHASE == 0 ? q.x : PHASE == 1 ? q.a : q.xt[g.cur];
+  const long ld = 2L * (PHASE == 0 ? npad : mpad);
+  const int stages = (PHASE == 0 ? npad : mpad) / 32;
+  const int per = PHASE == 0 ? (stages + q.split - 1) / q.split : stages;
+  const int s0 = sp * per, s1 = s0 + per < stages ? s0 + per : stages;
+  Core c;
+  c.clear();
+  c.run(a + (long)ti * TILE * ld, ld, q.m - ti * TILE, b + (long)tj * TILE * ld, ld, (PHASE == 2 ? q.n : q.m) - tj * TILE, s0, s1, smem);
+  if (PHASE == 0 && q.split > 1) {
+    f32x4* p = (f32x4*)(q.part + ((long)t * q.split + sp) * TILE * TILE) + (long)Core::wave() * Core::TI * Core::TJ * 64 + Core::lane();
+#pragma unroll
+    for (int i = 0; i < Core::TI; ++i)
+#pragma unroll
+      for (int j = 0; j < Core::TJ; ++j) p[(i * Core::TJ + j) * 64] = c.acc[i][j];
+    return;
+  }
+  ns_store<PHASE>(g, q, c, ti, tj, smem);
+}
+
+// joins the partial tiles of a split A = X X^T, in their order
+template <int TILE>
+__global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_join_kernel(NsArgs g) {
+  typedef typename NsTile<TILE>::Core Core;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int w = (int)blockIdx.x, k = ns_find(g, w);
+  const NsItem& q = g.it[k];
+  const int t = w - g.start[k];
+  int ti, tj;
+  ns_tri(t, ti, tj);
+  Core c;
+  c.clear();
+  const f32x4* p = (const f32x4*)(q.part + (long)t * q.split * TILE * TILE) + (long)Core::wave() * Core::TI * Core::TJ * 64 + Core::lane();
+  for (int s = 0; s < q.split; ++s, p += TILE * TILE / 4) {
+#pragma unroll
+    for (int i = 0; i < Core::TI; ++i)
+#pragma unroll
+      for (int j = 0; j < Core::TJ; ++j) c.acc[i][j] += p[(i * Core::TJ + j) * 64];
+  }
+  ns_store<0>(g, q, c, ti, tj, smem);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------------
+int ns_tile(const FiNsMat& q) {
+  const int m = q.rows < q.cols ? q.rows : q.cols;
+  return m <= 256 ? 64 : m <= 1024 ? 128 : 256;
+}
+
+// Carves the workspace of one launch group (matrices of one tile size); base == 0 only counts.
+long ns_layout(const FiNsMat* const* mats, int count, int tile, NsArgs& g, char* base) {
+  long at = 0;
+  auto take = [&](long bytes) {
+    char* p = base ? base + at : nullptr;
+    at += (bytes + 255) & ~255L;
+    return p;
+  };
+  long tri = 0;
+  for (int i = 0; i < count; ++i) {
+    const long t = (((mats[i]->rows < mats[i]->cols ? mats[i]->rows : mats[i]->cols) + tile - 1) / tile);
+    tri += t * (t + 1) / 2;
+  }
+  g.count = count;
+  for (int i = 0; i < count; ++i) {
+    NsItem& q = g.it[i];
+    q.u = mats[i]->u, q.out = mats[i]->out, q.dtype = mats[i]->dtype;
+    q.tall = mats[i]->rows > mats[i]->cols;
+    q.m = q.tall ? mats[i]->cols : mats[i]->rows;
+    q.n = q.tall ? mats[i]->rows : mats[i]->cols;
+    const long mp = ns_pad(q.m), np = ns_pad(q.n), mt = (q.m + tile - 1) / tile, nt = mt * (mt + 1) / 2;
+    q.x = (f16_t*)take(4L * q.m * np);
+    q.xt[0] = (f16_t*)take(4L * q.n * mp);
+    q.xt[1] = (f16_t*)take(4L * q.n * mp);
+    q.a = (f16_t*)take(4L * q.m * mp);
+    q.s = (f16_t*)take(4L * q.m * mp);
+    q.nsums = (int)(((long)q.m * q.n + NS_CHUNK - 1) / NS_CHUNK);
+    q.sums = (double*)take(8L * q.nsums);
+    // The long product A = X X^T has few tiles: with fewer than two per CU its contraction is split, down to 8 stages (256 values) a piece.
+    const long stages = np / 32;
+    long split = 512 / (tri > 0 ? tri : 1);
+    if (split > stages / 8) split = stages / 8;
+    if (split < 1) split = 1;
+    const long per = (stages + split - 1) / split;
+    q.split = (int)((stages + per - 1) / per);
+    q.part = q.split > 1 ? (float*)take(4L * nt * q.split * tile * tile) : nullptr;
+  }
+  return at;
+}
+
+int ns_check(const FiNsMat* mats, int count, int steps, const float* coeffs) {
+  if (!mats || !coeffs) return FI_ERR_NULL;
+  if (count < 1 || steps < 1) return FI_ERR_SHAPE;
+  for (int i = 0; i < count; ++i) {
+    const FiNsMat& q = mats[i];
+    if (q.dtype != FI_F32 && q.dtype != FI_BF16 && q.dtype != FI_F16) return FI_ERR_DTYPE;
+    if (q.rows < 1 || q.cols < 1 || q.rows > (1 << 20) || q.cols > (1 << 20)) return FI_ERR_SHAPE;
+    const int m = q.rows < q.cols ? q.rows : q.cols;
+    if (m > 32768) return FI_ERR_SHAPE;
+  }
+  // every singular value starts in [0, 1]: the polynomial must keep X, A and S inside the storage's range (16 / 2^-12)
+  for (int i = 0; i <= 1024; ++i) {
+    double s = i / 1024.0;
+    for (int k = 0; k < steps; ++k) {
+      const double l = s * s, f = coeffs[3 * k] + coeffs[3 * k + 1] * l + coeffs[3 * k + 2] * l * l;
+      if (!(fabs(f) < 15.0)) return FI_ERR_UNSUPPORTED;
+      s = f * s;
+      if (!(fabs(s) < 3.75)) return FI_ERR_UNSUPPORTED;
+    }
+  }
+  return 0;
+}
+
+template <int TILE>
+int ns_run(NsArgs& g, int steps, const float* coeffs, float eps, hipStream_t st) {
+  typedef typename NsTile<TILE>::Core Core;
+  static const bool lds_ok = nt_allow_lds((const void*)ns_product_kernel<0, TILE>) && nt_allow_lds((const void*)ns_product_kernel<1, TILE>) &&
+                             nt_allow_lds((const void*)ns_product_kernel<2, TILE>) && nt_allow_lds((const void*)ns_join_kernel<TILE>);
+  if (!lds_ok) return FI_ERR_UNSUPPORTED;
+  g.eps = eps;
+  auto plan = [&](int what) {                              // fills g.start for a launch, returns its work items
+    long n = 0;
+    for (int i = 0; i < g.count; ++i) {
+      g.start[i] = (int)n;
+      const NsItem& q = g.it[i];
+      const long mt = (q.m + TILE - 1) / TILE, nt = (q.n + TILE - 1) / TILE, tri = mt * (mt + 1) / 2;
+      n += what == 0 ? q.nsums : what == 1 ? (long)((q.m + 63) / 64) * ((q.n + 63) / 64) : what == 2 ? tri * q.split
+           : what == 3 ? (q.split > 1 ? tri : 0) : what == 4 ? tri : mt * nt;
+    }
+    g.start[g.count] = (int)n;
+    return (int)n;
+  };
+  const dim3 blk(Core::THREADS);
+  hipLaunchKernelGGL(ns_norm_kernel, dim3(plan(0)), dim3(256), 0, st, g);
+  FI_CHECK_LAUNCH();
+  hipLaunchKernelGGL(ns_prep_kernel, dim3(plan(1)), dim3(256), 0, st, g);
+  FI_CHECK_LAUNCH();
+  for (int k = 0; k < steps; ++k) {
+    g.ca = coeffs[3 * k], g.cb = coeffs[3 * k + 1], g.cc = coeffs[3 * k + 2];
+    g.cur = k & 1, g.last = k + 1 == steps;
+    hipLaunchKernelGGL((ns_product_kernel<0, TILE>), dim3((plan(2) + 7) & ~7), blk, Core::LDS, st, g);
+    FI_CHECK_LAUNCH();
+    if (const int n = plan(3)) {
+      hipLaunchKernelGGL((ns_join_kernel<TILE>), dim3(n), blk, Core::LDS, st, g);
+      FI_CHECK_LAUNCH();
+    }
+    hipLaunchKernelGGL((ns_product_kernel<1, TILE>), dim3((plan(4) + 7) & ~7), blk, Core::LDS, st, g);
+    FI_CHECK_LAUNCH();
+    hipLaunchKernelGGL((ns_product_kernel<2, TILE>), dim3((plan(5) + 7) & ~7), blk, Core::LDS, st, g);
+    FI_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+// f(group's arguments, tile, workspace bytes so far) for every launch group; returns the workspace's size or an error of f
+template <class F>
+long ns_groups(const FiNsMat* mats, int count, char* base, F f) {
+  long at = 0;
+  for (int tile = 64; tile <= 256; tile *= 2) {
+    const FiNsMat* pick[NS_MAX];
+    int n = 0;
+    for (int i = 0; i <= count; ++i) {
+      if (i < count && ns_tile(mats[i]) == tile) pick[n++] = &mats[i];
+      if (n == NS_MAX || (i == count && n)) {
+        NsArgs g = {};
+        at += ns_layout(pick, n, tile, g, base ? base + at : nullptr);
+        const int rc = f(g, tile);
+        if (rc) return rc < 0 ? rc : -1000 - rc;
+        n = 0;
+      }
+    }
+  }
+  return at;
+}
+
+}  // namespace
+
+extern "C" long fi_newton_schulz_workspace(const FiNsMat* mats, int count) {
+  const float c[3] = {0.f, 0.f, 0.f};
+  const int rc = ns_check(mats, count, 1, c);
+  if (rc) return rc;
+  return ns_groups(mats, count, nullptr, [](NsArgs&, int) { return 0; });
+}
+
+extern "C" int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const float* coeffs, float eps, void* workspace, void* stream) {
+  const int rc = ns_check(mats, count, steps, coeffs);
+  if (rc) return rc;
+  if (!workspace) return FI_ERR_NULL;
+  for (int i = 0; i < count; ++i)
+    if (!mats[i].u || !mats[i].out) return FI_ERR_NULL;
+  hipStream_t st = (hipStream_t)stream;
+  const long got = ns_groups(mats, count, (char*)workspace, [&](NsArgs& g, int tile) {
+    return tile == 64 ? ns_run<64>(g, steps, coeffs, eps, st) : tile == 128 ? ns_run<128>(g, steps, coeffs, eps, st) : ns_run<256>(g, steps, coeffs, eps, st);
+  });
+  return got >= 0 ? 0 : got > -1000 ? (int)got : (int)(-1000 - got);
+}

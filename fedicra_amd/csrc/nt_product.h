@@ -1,0 +1,241 @@
+// The matrix-pipe product core behind newton_schulz.hip and linear_ce.hip:  C[i][j] = sum_k A[i][k] * B[j][k], both operands with
+// their contraction index contiguous ("NT"), 16-bit storage, fp32 accumulation (v_mfma_f32_16x16x32).
+//
+// Operands come in one of two forms:
+//   plain  rows of 16-bit values, a multiple of 64 per row (the tail is zero);
+//   pair   every value as the sum of two fp16 (22 significant bits): per 32 values of a row 64 bytes of high parts, then 64 bytes of
+//          low parts.  Three products hi*hi + hi*lo + lo*hi give what an fp32 product gives up to 2^-22 per term, at a third of the
+//          16-bit matrix rate -- some five times the fp32 matrix instructions' -- and one LDS fragment serves two products.
+// Either way 128 bytes of a row are one STAGE of the contraction, so that loading, LDS layout and addressing are the same.
+//
+// A workgroup owns a BM x BN tile, a wave WM x WN of it.  Stages are brought into a two-slot LDS ring by LDS-DMA (16 bytes per lane, 8 rows
+// of 128 bytes per instruction); 16-byte piece c of row r lies at piece c ^ (r & 7), the swizzle being applied to the source address
+// because the LDS side of the instruction is linear: the eight lanes a ds_read_b128 serves per clock then touch all 32 banks once.
+#pragma once
+#include "common.h"
+
+typedef int nt_v4i __attribute__((ext_vector_type(4)));
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// lane L's 16 bytes at resource offset voff + soff go to LDS[lds_addr + 16 L]; zeros beyond the resource.  (s_nop: M0 is read by the
+// load, and an LDS-DMA needs a wait state behind a scalar write of M0.)
+__device__ __forceinline__ void nt_dma16(nt_v4i rsrc, unsigned lds_addr, unsigned voff, unsigned soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ nt_v4i nt_rsrc(const void* ptr, unsigned long long bytes) {
+  const unsigned long long p = (unsigned long long)ptr;
+  const unsigned n = bytes > 0xffffffffull ? 0xffffffffu : (unsigned)bytes;
+  return nt_v4i{__builtin_amdgcn_readfirstlane((int)(unsigned)p), __builtin_amdgcn_readfirstlane((int)((unsigned)(p >> 32) & 0xffffu)),
+                __builtin_amdgcn_readfirstlane((int)n), 0x00020000};
+}
+// more than 64 KB of dynamic LDS per workgroup has to be allowed per kernel (once; a CU has 160 KB)
+static inline bool nt_allow_lds(const void* kernel) {
+  return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
+}
+// orders this wave's LDS traffic: what other lanes of the wave wrote before is there after
+__device__ __forceinline__ void nt_wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+template <typename T, bool PAIR, int BM_, int BN_, int WM_, int WN_>
+struct NtCore {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int NWN = BN / WN, NW = (BM / WM) * NWN, THREADS = NW * 64;
+  static constexpr int TI = WM / 16, TJ = WN / 16;
+  static constexpr int STAGE = (BM + BN) * 128, LDS = 2 * STAGE;
+  static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;       // DMA instructions of a wave per stage: 8 rows of A, of B
+  static_assert(PA * NW * 8 == BM && PB * NW * 8 == BN, "whole DMA instructions for every wave");
+  typedef typename DT<T>::frag_t frag_t;
+
+  f32x4 acc[TI][TJ];
+
+  // lane's coordinates inside the tile: row of acc[ti][..] is row0() + ti * 16 + lane % 16, columns of acc[..][tj][r] are
+  // col0() + tj * 16 + 4 * (lane / 16) + r  (the fragments are handed to the matrix instruction in the order that puts four consecutive columns
+  // of one row into a lane: row statistics stay mostly inside a lane, stores go out in vectors)
+  static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+  static __device__ __forceinline__ int lane() { return (int)(threadIdx.x & 63); }
+  static __device__ __forceinline__ int row0() { return (wave() / NWN) * WM; }
+  static __device__ __forceinline__ int col0() { return (wave() % NWN) * WN; }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // Adds the product to acc.  a, b: first row of the tile (ld in elements, rowsA / rowsB >= 1 valid rows from there: the rest of the tile repeats the last one and
+  // its results mean nothing); stages [s0, s1) of the contraction.  BM * ld * sizeof(T) < 2^32 (the callers check).
+  __device__ __forceinline__ void run(const T* a, long lda, int rowsA, const T* b, long ldb, int rowsB, int s0, int s1, char* smem) {
+    typedef __attribute__((address_space(3))) char* lds_ptr_t;
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr_t)smem;
+    const int w = wave(), l = lane();
+    // (the resources end with the operands' last byte in use: nothing behind them is ever fetched)
+    const nt_v4i ra = nt_rsrc(a, ((unsigned long long)(rowsA - 1) * lda + (unsigned long long)s1 * 64) * 2);
+    const nt_v4i rb = nt_rsrc(b, ((unsigned long long)(rowsB - 1) * ldb + (unsigned long long)s1 * 64) * 2);
+    const unsigned piece = (unsigned)(((l & 7) ^ (l >> 3)) * 16);
+    unsigned va[PA], vb[PB];
+#pragma unroll
+    for (int q = 0; q < PA; ++q) {
+      int r = (w * PA + q) * 8 + (l >> 3);
+      va[q] = (unsigned)(r < rowsA ? r : rowsA - 1) * (unsigned)(lda * 2) + piece;
+    }
+#pragma unroll
+    for (int q = 0; q < PB; ++q) {
+      int r = (w * PB + q) * 8 + (l >> 3);
+      vb[q] = (unsigned)(r < rowsB ? r : rowsB - 1) * (unsigned)(ldb * 2) + piece;
+    }
+    const unsigned la = lds0 + (unsigned)(w * PA * 1024), lb = lds0 + (unsigned)(BM * 128 + w * PB * 1024);
+    auto fetch = [&](int s, int slot) {
+#pragma unroll
+      for (int q = 0; q < PA; ++q) nt_dma16(ra, la + (unsigned)(slot * STAGE + q * 1024), va[q], (unsigned)s * 128u);
+#pragma unroll
+      for (int q = 0; q < PB; ++q) nt_dma16(rb, lb + (unsigned)(slot * STAGE + q * 1024), vb[q], (unsigned)s * 128u);
+    };
+    const int sw = l & 7, g = l >> 4, lr = l & 15;
+    const int oa = (row0() + lr) * 128, ob = BM * 128 + (col0() + lr) * 128;
+    const int p0 = ((g) ^ sw) * 16, p1 = ((4 + g) ^ sw) * 16;
+
+    if (s0 < s1) fetch(s0, 0);
+    for (int s = s0; s < s1; ++s) {
+      const int cur = (s - s0) & 1;
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + 1 < s1) fetch(s + 1, cur ^ 1);
+      const char* sa = smem + cur * STAGE + oa;
+      const char* sb = smem + cur * STAGE + ob;
+      if constexpr (PAIR) {
+        frag_t bh[TJ], bl[TJ];
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+          bh[j] = *(const frag_t*)(sb + j * 2048 + p0);
+          bl[j] = *(const frag_t*)(sb + j * 2048 + p1);
+        }
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+          const frag_t ah = *(const frag_t*)(sa + i * 2048 + p0);
+          const frag_t al = *(const frag_t*)(sa + i * 2048 + p1);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bh[j], al, acc[i][j]);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bl[j], ah, acc[i][j]);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bh[j], ah, acc[i][j]);
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const int p = kk ? p1 : p0;
+          frag_t bf[TJ];
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) bf[j] = *(const frag_t*)(sb + j * 2048 + p);
+#pragma unroll
+          for (int i = 0; i < TI; ++i) {
+            const frag_t af = *(const frag_t*)(sa + i * 2048 + p);
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bf[j], af, acc[i][j]);
+          }
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // the ring is free: epilogues use it as scratch
+  }
+};
+
+// ---- storing a tile in both orientations ------------------------------------------------------------------------------------------
+// A wave takes a block of its fp32 results through its own LDS scratch (no workgroup barrier) and stores it as rows of 8-value vectors,
+// row-major and / or transposed.  Scratch word of (i, j): the 8-column group is swizzled by the row inside its 8-row group and by that group, so
+// that the accumulators' writes (ds_write_b128, lanes over 16 rows), row reads (2 x ds_read_b128) and column reads (8 x ds_read_b32, lanes over
+// 8 columns x 8 row groups) all spread over the banks.
+template <int SI, int SJ>
+struct NtBlock {
+  static constexpr int BYTES = SI * SJ * 4;
+  float* s;
+  __device__ __forceinline__ float* at(int i, int j) const { return s + i * SJ + (j ^ ((((i >> 3) ^ i) << 3) & (SJ - 1))); }
+  // the wave's accumulators of block (bi, bj), times `by`
+  template <class Core>
+  __device__ __forceinline__ void put(const Core& c, int bi, int bj, float by) const {
+    const int l = threadIdx.x & 63;
+    nt_wave_lds_fence();
+#pragma unroll
+    for (int i = 0; i < SI / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < SJ / 16; ++j) {
+        const f32x4 v = c.acc[bi * (SI / 16) + i][bj * (SJ / 16) + j];
+        *(float4*)at(i * 16 + (l & 15), j * 16 + 4 * (l >> 4)) = make_float4(v[0] * by, v[1] * by, v[2] * by, v[3] * by);
+      }
+    nt_wave_lds_fence();
+  }
+  // f(i, j0, v): 8 values of row i from column j0 on; what it leaves in v is written back if KEEP
+  template <bool KEEP, class F>
+  __device__ __forceinline__ void rows(F f) const {
+    constexpr int PL = SJ / 8, RP = 64 / PL;
+    const int l = threadIdx.x & 63, j0 = (l % PL) * 8;
+#pragma unroll
+    for (int i0 = 0; i0 < SI; i0 += RP) {
+      const int i = i0 + l / PL;
+      float v[8];
+      float4* p = (float4*)at(i, j0);
+      const float4 x = p[0], y = p[1];
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+      f(i, j0, v);
+      if constexpr (KEEP) {
+        p[0] = make_float4(v[0], v[1], v[2], v[3]);
+        p[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    }
+  }
+  // f(j, i0, v): 8 values of column j from row i0 on
+  template <class F>
+  __device__ __forceinline__ void cols(F f) const {
+    constexpr int PL = SI / 8, CP = 64 / PL;
+    const int l = threadIdx.x & 63, i0 = (l % PL) * 8;
+#pragma unroll
+    for (int jb = 0; jb < SJ; jb += CP) {
+      const int j = jb + l / PL;
+      float v[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] = *at(i0 + t, j);
+      f(j, i0, v);
+    }
+  }
+};
+
+// 8 values -> high and low fp16 parts (value = hi + lo up to 2^-22 of it)
+__device__ __forceinline__ void nt_split8(const float (&v)[8], uint4& hi, uint4& lo) {
+  unsigned h[4], q[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    f16x2_t a, b;
+    a[0] = (f16_t)v[2 * t], a[1] = (f16_t)v[2 * t + 1];
+    b[0] = (f16_t)(v[2 * t] - (float)a[0]), b[1] = (f16_t)(v[2 * t + 1] - (float)a[1]);
+    h[t] = __builtin_bit_cast(unsigned, a), q[t] = __builtin_bit_cast(unsigned, b);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(q[0], q[1], q[2], q[3]);
+}
+// element offset of value k (a multiple of 8) inside a pair row; its low part lies 32 elements further
+__device__ __forceinline__ long nt_pair_at(long k) { return ((k >> 5) << 6) + (k & 31); }
+__device__ __forceinline__ void nt_store_pair(f16_t* row, long k, const float (&v)[8]) {
+  uint4 hi, lo;
+  nt_split8(v, hi, lo);
+  f16_t* p = row + nt_pair_at(k);
+  *(uint4*)p = hi;
+  *(uint4*)(p + 32) = lo;
+}
+__device__ __forceinline__ void nt_load_pair(const f16_t* row, long k, float (&v)[8]) {
+  const f16_t* p = row + nt_pair_at(k);
+  const uint4 hi = *(const uint4*)p, lo = *(const uint4*)(p + 32);
+  float a[8], b[8];
+  VecWords<f16_t>::unpack(hi, a);
+  VecWords<f16_t>::unpack(lo, b);
+#pragma unroll
+  for (int t = 0; t < 8; ++t) v[t] = a[t] + b[t];
+}
+
+// Workgroups are handed to the eight XCDs in turn (id % 8): this maps a launch of `n` work items (grid rounded up to a multiple of 8) so that each
+// XCD's L2 sees one contiguous run of items.  Returns an item, or -1 for the rounding's surplus.
+__device__ __forceinline__ int nt_xcd_item(int bid, int grid, int n) {
+  const int per = grid >> 3, t = (bid & 7) * per + (bid >> 3);
+  return t < n ? t : -1;
+}

@@ -917,3 +917,6 @@ def to_nhwc(x_nchw, dtype):
     out = torch.empty((N, H, W, Cc), dtype=dtype, device=x.device)
     L.nchw_to_nhwc(x, out)
     return out
+
+
+from .step_ops import linear_ce_loss, newton_schulz  # noqa: E402,F401  (the tail of a training step)

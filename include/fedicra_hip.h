@@ -51,8 +51,9 @@ extern "C" {
  *      fi_pcs_gate_*, fi_lc_loss_*, fi_conv3d_wgrad_fused*, this check)
  *   3: round 4 (new entry points: fi_conv2d_stats_xcorr*, fi_bn_act_pool_groups, fi_conv1x1_up2x_fwd, fi_wgrad_tuning / fi_narrow_tuning /
  *      fi_upfuse_tuning, fi_pack_weights3d_multi; fi_wgrad_tuning's argument became a bit mask)
- *   5: round 6 (fi_conv3d_tuning; fi_conv_tuning(7, 8): the LDS-DMA forward form) */
-#define FI_ABI_VERSION 6
+ *   5: round 6 (fi_conv3d_tuning; fi_conv_tuning(7, 8): the LDS-DMA forward form)
+ *   7: fi_newton_schulz*, fi_linear_ce_* */
+#define FI_ABI_VERSION 7
 int fi_abi_version(void);
 
 /* ---------------------------------------------------------------- convolution ------------
@@ -713,6 +714,50 @@ int fi_groupnorm_fwd(int dtype, const void* x, void* z, const float* gamma, cons
                      int N, long pixels, int C, int G, float eps, int relu, void* stream);
 int fi_groupnorm_bwd(int dtype, const void* dz, const void* x, const void* z, const float* gamma, const float* mean,
                      const float* invstd, void* dx, float* dgamma, float* dbeta, int N, long pixels, int C, int G, int relu,
+                     void* stream);
+
+/* ---------------------------------------------------------------- orthogonalised updates ---
+ * The Newton-Schulz iteration of an orthogonalising optimizer step (optim.FusedMuon), for any number of matrices at once:
+ *   X <- u / (|u|_F + eps);  `steps` times  A = X X^T,  X <- (a I + b A + c A A) X;  out <- X
+ * (for rows > cols the same on u^T).  u, out: dense [rows][cols] in `dtype`, out may be u; coeffs: HOST fp32 [steps][3] = (a, b, c) per
+ * step.  Products are accurate to 22 bits whatever the storage type; nothing is rounded to `dtype` but the result.  A zero matrix
+ * gives zeros, one with an inf or NaN gives NaN.  FI_ERR_UNSUPPORTED: a polynomial that takes a singular value of [0, 1]
+ * beyond 3.75 or a factor a + b s^2 + c s^4 beyond 15.  The shorter side may have 32768 values, the longer 2^20.
+ * `mats` is a HOST array, read during the call only; workspace bytes from fi_newton_schulz_workspace (< 0: FI_ERR_*). */
+typedef struct FiNsMat {
+  const void* u;
+  void* out;
+  int dtype;
+  int rows, cols;
+} FiNsMat;
+long fi_newton_schulz_workspace(const FiNsMat* mats, int count);
+int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const float* coeffs, float eps, void* workspace, void* stream);
+
+/* ---------------------------------------------------------------- linear head + cross entropy ---
+ * Softmax cross entropy of z = x w^T + bias over V classes without storing z (ops.linear_ce_loss; beside fi_ce_*, which takes stored
+ * fp32 logits and uint8 labels).  x [T][ldx] and w [V][ldw] (D values of each row), w in x's type or fp32 (then rounded to x's 16-bit type
+ * as the operand; the gradient is fp32); bias fp32 [V] or NULL; labels [T] of `ltype`; rows with label == ignore_index take no part
+ * (whatever x holds there) and get dx = 0; a label outside [0, V) makes the loss and the gradients NaN.
+ *   fwd: reduction 0: loss[T] per row (0 where ignored); 1: loss[0] = mean over labelled rows (NaN if none); 2: their sum.  `saved`
+ *        (fi_linear_ce_saved bytes) is what bwd needs besides x, w and bias.
+ *   bwd: gloss = upstream gradient, fp32 [T] or [1]; dx in x's type, dense [T][D]; dw in w's type, dense [V][D] (dw_accumulate: fp32, +=); db fp32
+ *        [V] (db_accumulate: +=); any of the three may be NULL.
+ * Deterministic: no atomics.  T < 2^30, V <= 2^20, D <= 65536. */
+#define FI_LABEL_U8 0
+#define FI_LABEL_I32 1
+#define FI_LABEL_I64 2
+typedef struct FiLinearCe {
+  int dtype, wdtype, ltype, reduction;
+  int V, D;
+  int64_t T, ldx, ldw, ignore_index;
+} FiLinearCe;
+long fi_linear_ce_saved(const FiLinearCe* d);
+long fi_linear_ce_fwd_workspace(const FiLinearCe* d, const void* w);
+int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* w, const float* bias, const void* labels, float* loss, void* saved,
+                     void* workspace, void* stream);
+long fi_linear_ce_bwd_workspace(const FiLinearCe* d, const void* w, int need_dx, int need_dw, int need_db);
+int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* w, const float* bias, const void* labels, const void* saved,
+                     const float* gloss, void* dx, void* dw, int dw_accumulate, float* db, int db_accumulate, void* workspace,
                      void* stream);
 
 #ifdef __cplusplus
