@@ -439,7 +439,7 @@ __device__ __forceinline__ int ce_kpad(int n) { return PAIR ? (n + 31) & ~31 : (
 template <class Core, typename T, bool PAIR>
 __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int SB = Core::WM >= 64 && Core::WN >= 64 ? 64 : 32, EXTRA = Core::NW * NtBlock<SB, SB>::BYTES > Core::LDS ? Core::NW * NtBlock<SB, SB>::BYTES : Core::LDS;
+  constexpr int SB = Core::BLOCK, EXTRA = Core::NW * NtBlock<SB, SB>::BYTES;
   const i64 left = (i64)a.s.count[0] - a.t0;
   const int n = (int)(left < 0 ? 0 : left < a.Tc ? left : a.Tc);       // rows of this piece
   int ti, tj;
@@ -595,14 +595,14 @@ __global__ __launch_bounds__(Core::THREADS) void ce_grad_kernel(CeGrad a) {
   const int nti = (M + Core::BM - 1) / Core::BM, ntj = (a.N + Core::BN - 1) / Core::BN;
   int ti, tj;
   if (!ce_tile(nti, ntj * a.splits, ti, tj)) return;
-  const int sp = tj % a.splits;
-  tj /= a.splits;
+  const int sp = tj / ntj;                                              // (workgroups that run together share a part of the contraction)
+  tj -= sp * ntj;
   const int stages = (int)((K + (PAIR ? 31 : 63)) / (PAIR ? 32 : 64)), per = (stages + a.splits - 1) / a.splits;
   const int s0 = sp * per < stages ? sp * per : stages, s1 = s0 + per < stages ? s0 + per : stages;
   Core c;
   c.clear();
   c.run(a.a + (i64)ti * Core::BM * a.lda, a.lda, M - ti * Core::BM, a.b + (i64)tj * Core::BN * a.ldb, a.ldb, a.N - tj * Core::BN, s0, s1, smem);
-  constexpr int SB = Core::WM >= 64 && Core::WN >= 64 ? 64 : 32;
+  constexpr int SB = Core::BLOCK;
   const NtBlock<SB, SB> blk{(float*)(smem + Core::wave() * NtBlock<SB, SB>::BYTES)};
   const float rg = a.scal[SC_RG], rb = ce_rscale(a);
 #pragma unroll
@@ -665,36 +665,50 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeGrad a) {
   }
 }
 
-// db: column sums over the row tiles, in fp64
-__global__ __launch_bounds__(256) void ce_dbias_kernel(const float* part, int tile, int V, const int* count, const float* scal, float* db, int accumulate) {
-  __shared__ double sm[4][64];
-  const int v = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+// db: column sums over the row tiles, in fp64: 16 columns per workgroup, 64 lanes' worth of row tiles each
+__global__ __launch_bounds__(1024) void ce_dbias_kernel(const float* part, int tile, int V, const int* count, const float* scal, float* db, int accumulate) {
+  __shared__ double sm[64][17];
+  const int col = threadIdx.x & 15, q = threadIdx.x >> 4, v = blockIdx.x * 16 + col;
   const int nt = (count[0] + tile - 1) / tile;
   double acc = 0.0;
   if (v < V)
-    for (int t = q; t < nt; t += 4) acc += (double)part[(i64)t * V + v];
-  sm[q][threadIdx.x & 63] = acc;
+    for (int t = q; t < nt; t += 64) acc += (double)part[(i64)t * V + v];
+  sm[q][col] = acc;
   __syncthreads();
+  for (int o = 32; o > 0; o >>= 1) {
+    if (q < o) sm[q][col] += sm[q + o][col];
+    __syncthreads();
+  }
   if (q == 0 && v < V) {
-    acc = (sm[0][threadIdx.x] + sm[1][threadIdx.x] + sm[2][threadIdx.x] + sm[3][threadIdx.x]) * (double)scal[SC_RG];
+    acc = sm[0][col] * (double)scal[SC_RG];
     db[v] = accumulate ? db[v] + (float)acc : (float)acc;
   }
 }
 
-// dx of the rows that take no part
-__global__ __launch_bounds__(256) void ce_zero_rows_kernel(const void* labels, int ltype, i64 T, i64 ignore, void* dx, int esize, int D) {
-  const int per = 256;
-  const i64 r0 = (i64)blockIdx.x * per;
-  const i64 rb = (i64)D * esize;
-  for (int k = threadIdx.x >> 6; k < per; k += 4) {                     // a wave per row
-    const i64 r = r0 + k;
-    if (r >= T) break;
-    if (ce_label(labels, ltype, r) != ignore) continue;
-    char* p = (char*)dx + r * rb;
-    if (esize == 2)
-      for (int c = threadIdx.x & 63; c < D; c += 64) ((uint16_t*)p)[c] = 0;
+// dx of the rows that take no part: a lane looks at a label, the wave clears the rows it finds
+__global__ __launch_bounds__(256) void ce_zero_rows_kernel(const void* labels, int ltype, i64 T, i64 ignore, char* dx, i64 row_bytes) {
+  const int l = threadIdx.x & 63;
+  const i64 r0 = ((i64)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
+  const bool mine = r0 + l < T && ce_label(labels, ltype, r0 + l) == ignore;
+  unsigned long long todo = __ballot(mine);
+  const bool vec = row_bytes % 16 == 0 && ((uintptr_t)dx & 15) == 0;
+  if (vec && row_bytes <= 512) {                                        // several rows at a time
+    const int per = (int)(row_bytes / 16), rows = 64 / per;
+    if (todo)
+      for (int i = 0; i < 64; i += rows) {
+        const int r = i + l / per;
+        if (l / per < rows && r < 64 && (todo >> r & 1)) ((uint4*)(dx + (r0 + r) * row_bytes))[l % per] = make_uint4(0, 0, 0, 0);
+      }
+    return;
+  }
+  while (todo) {
+    const int r = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    char* p = dx + (r0 + r) * row_bytes;
+    if (vec)
+      for (i64 c = l; c < row_bytes / 16; c += 64) ((uint4*)p)[c] = make_uint4(0, 0, 0, 0);
     else
-      for (int c = threadIdx.x & 63; c < D; c += 64) ((uint32_t*)p)[c] = 0;
+      for (i64 c = l; c < row_bytes / 2; c += 64) ((uint16_t*)p)[c] = 0;
   }
 }
 
@@ -748,7 +762,10 @@ int ce_check(const FiLinearCe* d) {
 int ce_logits_tile(const FiLinearCe& d) { return d.T <= 64 ? 1 : d.V <= 64 ? 2 : 0; }
 constexpr int CE_BM[3] = {256, 64, 256}, CE_BN[3] = {256, 256, 64};
 
+// (the same tile by 16 waves of 64 x 64 in the forward pass -- four per SIMD hide LDS and DMA latency: 845 -> 757 us at 7370 x 50000 x 1024 -- and by
+// 8 of 128 x 64 for G, whose epilogue wants 64 x 64 blocks of scratch: 267 against 290 us a piece of 7370 x 16384)
 template <typename T, bool PAIR> struct CeCores {
+  typedef NtCore<T, PAIR, 256, 256, 64, 64> F0;
   typedef NtCore<T, PAIR, 256, 256, 128, 64> C0;
   typedef NtCore<T, PAIR, 64, 256, 64, 32> C1;
   typedef NtCore<T, PAIR, 256, 64, 32, 64> C2;
@@ -768,8 +785,8 @@ template <class Core, typename T, bool PAIR>
 int ce_launch_dlogits(const CeLogits& a, hipStream_t st) {
   static const bool ok = nt_allow_lds((const void*)ce_dlogits_kernel<Core, T, PAIR>);
   if (!ok) return FI_ERR_UNSUPPORTED;
-  constexpr int SB = Core::WM >= 64 && Core::WN >= 64 ? 64 : 32, SCR = Core::NW * NtBlock<SB, SB>::BYTES;
-  constexpr int lds = (SCR > Core::LDS ? SCR : Core::LDS) + Core::BM * 16 + Core::BM / Core::WM * Core::BN * 4;
+  constexpr int SB = Core::BLOCK, SCR = Core::NW * NtBlock<SB, SB>::BYTES;
+  constexpr int need = SCR + Core::BM * 16 + Core::BM / Core::WM * Core::BN * 4, lds = need > Core::LDS ? need : Core::LDS;
   const i64 n = (a.Tc + Core::BM - 1) / Core::BM * ((a.Vc + Core::BN - 1) / Core::BN);
   hipLaunchKernelGGL((ce_dlogits_kernel<Core, T, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), lds, st, a);
   FI_CHECK_LAUNCH();
@@ -779,7 +796,7 @@ template <typename T, bool PAIR>
 int ce_logits(const CeLogits& a, const FiLinearCe& d, bool fwd, hipStream_t st) {
   typedef CeCores<T, PAIR> C;
   switch (ce_logits_tile(d)) {
-    case 0: return fwd ? ce_launch_fwd<typename C::C0, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C0, T, PAIR>(a, st);
+    case 0: return fwd ? ce_launch_fwd<typename C::F0, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C0, T, PAIR>(a, st);
     case 1: return fwd ? ce_launch_fwd<typename C::C1, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C1, T, PAIR>(a, st);
     default: return fwd ? ce_launch_fwd<typename C::C2, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C2, T, PAIR>(a, st);
   }
@@ -924,9 +941,9 @@ int ce_launch_grad(const CeGrad& a, hipStream_t st) {
 }
 template <bool PAIR>
 int ce_grad(const CeGrad& a, int tile, hipStream_t st) {
-  return tile == 0 ? ce_launch_grad<NtCore<f16_t, PAIR, 256, 256, 128, 64>, PAIR>(a, st)
-         : tile == 1 ? ce_launch_grad<NtCore<f16_t, PAIR, 128, 128, 64, 64>, PAIR>(a, st)
-                     : ce_launch_grad<NtCore<f16_t, PAIR, 64, 64, 32, 32>, PAIR>(a, st);
+  return tile == 0 ? ce_launch_grad<NtCore<f16_t, PAIR, 256, 256, 64, 64>, PAIR>(a, st)
+         : tile == 1 ? ce_launch_grad<NtCore<f16_t, PAIR, 128, 128, 64, PAIR ? 32 : 64>, PAIR>(a, st)
+                     : ce_launch_grad<NtCore<f16_t, PAIR, 64, 64, 32, 32, 3>, PAIR>(a, st);
 }
 int ce_join(const CeGrad& a, hipStream_t st) {
   const i64 n = ((i64)a.M * ((a.N + 7) / 8) + 255) / 256;
@@ -1019,7 +1036,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)(ng < 1024 ? ng : 1024)), dim3(256), 0, st, gloss, d->reduction, ws.parts, sv, ws.scal, ws.g);
   FI_CHECK_LAUNCH();
   if (dx) {
-    hipLaunchKernelGGL(ce_zero_rows_kernel, dim3((unsigned)ng), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, dx, s.pair ? 4 : 2, d->D);
+    hipLaunchKernelGGL(ce_zero_rows_kernel, dim3((unsigned)ng), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, (char*)dx, (i64)d->D * (s.pair ? 4 : 2));
     FI_CHECK_LAUNCH();
   }
   const int f = s.pair ? 2 : 1;
@@ -1060,7 +1077,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
     }
   }
   if (db) {
-    hipLaunchKernelGGL(ce_dbias_kernel, dim3((unsigned)((d->V + 63) / 64)), dim3(256), 0, st, ws.db, CE_BM[ce_logits_tile(*d)], d->V, sv.count, ws.scal, db, db_accumulate);
+    hipLaunchKernelGGL(ce_dbias_kernel, dim3((unsigned)((d->V + 15) / 16)), dim3(1024), 0, st, ws.db, CE_BM[ce_logits_tile(*d)], d->V, sv.count, ws.scal, db, db_accumulate);
     FI_CHECK_LAUNCH();
   }
   return 0;

@@ -17,31 +17,62 @@
 
 namespace {
 
-constexpr int NS_MAX = 24;                       // matrices per launch (their descriptors travel as kernel arguments)
+constexpr int NS_MAX = 64;                       // matrices per launch (their descriptors travel as kernel arguments)
 constexpr float NS_SCALE = 4096.f;
-constexpr int NS_CHUNK = 16384;                  // elements per partial sum of squares
+constexpr int NS_CHUNK = 8192;                   // elements per partial sum of squares
 
 struct NsItem {
   const void* u;
   void* out;
-  f16_t *x, *xt[2], *a, *s;                      // pair rows: x [m][n], xt [n][m], a, s [m][m]
-  float* part;                                   // split contraction: raw accumulators [tile][split][TILE * TILE]
-  double* sums;                                  // partial sums of squares
-  int m, n, tall, dtype, split, nsums;
+  unsigned base;                                 // its place in the workspace, in 256 bytes
+  int m, n, tall, dtype, split;
 };
 struct NsArgs {
+  char* ws;
   NsItem it[NS_MAX];
   int start[NS_MAX + 1];                         // first work item of each matrix in this launch
   int count, cur, last;
   float ca, cb, cc, eps;
 };
+static_assert(sizeof(NsArgs) <= 4096, "kernel arguments");
 
 __device__ __host__ __forceinline__ int ns_pad(int v) { return (v + 31) & ~31; }
+__device__ __host__ __forceinline__ int ns_sums(const NsItem& q) { return (int)(((long)q.m * q.n + NS_CHUNK - 1) / NS_CHUNK); }
 
-__device__ __forceinline__ int ns_find(const NsArgs& g, int w) {
-  int i = 0;
-  while (i + 1 < g.count && w >= g.start[i + 1]) ++i;
-  return i;
+// a matrix's part of the workspace: pair rows x [m][n], xt [n][m] twice (S X reads one and writes the other), a, s [m][m]; partial sums of
+// squares; the partial tiles of a split A
+struct NsMem {
+  f16_t *x, *xt[2], *a, *s;
+  double* sums;
+  float* part;
+  long bytes;
+};
+__device__ __host__ __forceinline__ NsMem ns_mem(char* p, const NsItem& q) {
+  const long mp = ns_pad(q.m), np = ns_pad(q.n);
+  const long bx = (4L * q.m * np + 255) & ~255L, bt = (4L * q.n * mp + 255) & ~255L, ba = (4L * q.m * mp + 255) & ~255L, bs = (8L * ns_sums(q) + 255) & ~255L;
+  NsMem r;
+  r.x = (f16_t*)p, p += bx;
+  r.xt[0] = (f16_t*)p, p += bt;
+  r.xt[1] = (f16_t*)p, p += bt;
+  r.a = (f16_t*)p, p += ba;
+  r.s = (f16_t*)p, p += ba;
+  r.sums = (double*)p, p += bs;
+  r.part = (float*)p;
+  r.bytes = bx + 2 * bt + 2 * ba + bs;
+  return r;
+}
+__device__ __forceinline__ NsMem ns_mem(const NsArgs& g, const NsItem& q) { return ns_mem(g.ws + (long)q.base * 256, q); }
+
+__device__ __forceinline__ int ns_find(const NsArgs& g, int w) {             // the last matrix that starts at or before w
+  int lo = 0, hi = g.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (g.start[mid] <= w)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
 }
 __device__ __forceinline__ float ns_load(const void* p, int dtype, long i) {
   return dtype == FI_F32 ? ((const float*)p)[i] : dtype == FI_BF16 ? (float)((const bf16_t*)p)[i] : (float)((const f16_t*)p)[i];
@@ -53,21 +84,35 @@ __device__ __forceinline__ void ns_tri(int t, int& i, int& j) {               //
   j = t - i * (i + 1) / 2;
 }
 
+template <typename T>
+__device__ __forceinline__ double ns_squares(const T* p, long n) {
+  constexpr int VG = DT<T>::VG;
+  const long head = ((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T);            // up to the first aligned vector
+  const long h = head < n ? head : n, vecs = (n - h) / VG, tail = h + vecs * VG;
+  double acc = 0.0;
+  for (long i = threadIdx.x; i < vecs; i += 256) {
+    float f[VG];
+    VecWords<T>::unpack(((const typename DT<T>::vec_t*)(p + h))[i], f);
+#pragma unroll
+    for (int t = 0; t < VG; ++t) acc += (double)f[t] * (double)f[t];
+  }
+  if ((long)threadIdx.x < h + n - tail) {
+    const double v = (double)to_f32(p[(long)threadIdx.x < h ? (long)threadIdx.x : tail + threadIdx.x - h]);
+    acc += v * v;
+  }
+  return acc;
+}
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
   __shared__ double sm[4];
   const int w = (int)blockIdx.x, k = ns_find(g, w);
   const NsItem& q = g.it[k];
-  const long total = (long)q.m * q.n, lo = (long)(w - g.start[k]) * NS_CHUNK;
-  const long hi = lo + NS_CHUNK < total ? lo + NS_CHUNK : total;
-  double acc = 0.0;
-  for (long i = lo + threadIdx.x; i < hi; i += 256) {
-    const double v = (double)ns_load(q.u, q.dtype, i);
-    acc += v * v;
-  }
+  const long total = (long)q.m * q.n, lo = (long)(w - g.start[k]) * NS_CHUNK, n = total - lo < NS_CHUNK ? total - lo : NS_CHUNK;
+  double acc = q.dtype == FI_F32 ? ns_squares((const float*)q.u + lo, n) : q.dtype == FI_BF16 ? ns_squares((const bf16_t*)q.u + lo, n)
+                                                                                           : ns_squares((const f16_t*)q.u + lo, n);
   acc = wave_sum(acc);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = acc;
   __syncthreads();
-  if (threadIdx.x == 0) q.sums[w - g.start[k]] = sm[0] + sm[1] + sm[2] + sm[3];
+  if (threadIdx.x == 0) ns_mem(g, q).sums[w - g.start[k]] = sm[0] + sm[1] + sm[2] + sm[3];
 }
 
 // U, normalised, as pair rows in both orientations: one 64 x 64 block of U per workgroup
@@ -77,8 +122,9 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsArgs g) {
   __shared__ float s_inv;
   const int w = (int)blockIdx.x, k = ns_find(g, w), tid = threadIdx.x;
   const NsItem& q = g.it[k];
+  const NsMem mem = ns_mem(g, q);
   double acc = 0.0;
-  for (int i = tid; i < q.nsums; i += 256) acc += q.sums[i];
+  for (int i = tid, n = ns_sums(q); i < n; i += 256) acc += mem.sums[i];
   acc = wave_sum(acc);
   if ((tid & 63) == 0) sm[tid >> 6] = acc;
   __syncthreads();
@@ -92,8 +138,8 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsArgs g) {
     tile[e >> 6][e & 63] = r < rows && c < cols ? ns_load(q.u, q.dtype, (long)r * cols + c) * inv : 0.f;
   }
   __syncthreads();
-  f16_t* const same = q.tall ? q.xt[0] : q.x;          // U's own orientation
-  f16_t* const turned = q.tall ? q.x : q.xt[0];
+  f16_t* const same = q.tall ? mem.xt[0] : mem.x;          // U's own orientation
+  f16_t* const turned = q.tall ? mem.x : mem.xt[0];
   const int cpad = ns_pad(cols), rpad = ns_pad(rows);
   for (int e = tid; e < 64 * 8; e += 256) {
     const int r = e >> 3, c = (e & 7) * 8;
@@ -113,9 +159,9 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsArgs g) {
 
 template <int TILE>
 struct NsTile;
-template <> struct NsTile<64> { typedef NtCore<f16_t, true, 64, 64, 32, 32> Core; };
-template <> struct NsTile<128> { typedef NtCore<f16_t, true, 128, 128, 64, 64> Core; };
-template <> struct NsTile<256> { typedef NtCore<f16_t, true, 256, 256, 128, 64> Core; };
+template <> struct NsTile<64> { typedef NtCore<f16_t, true, 64, 64, 32, 32, 3> Core; };
+template <> struct NsTile<128> { typedef NtCore<f16_t, true, 128, 128, 64, 32, 2> Core; };
+template <> struct NsTile<256> { typedef NtCore<f16_t, true, 256, 256, 64, 64> Core; };
 
 __device__ __forceinline__ void ns_put(void* out, int dtype, long at, const float (&v)[8], int n) {
 #pragma unroll
@@ -133,20 +179,20 @@ __device__ __forceinline__ void ns_put(void* out, int dtype, long at, const floa
 
 // what becomes of a tile of PHASE 0 (A), 1 (S) or 2 (X)
 template <int PHASE, class Core>
-__device__ __forceinline__ void ns_store(const NsArgs& g, const NsItem& q, const Core& c, int ti, int tj, char* smem) {
-  constexpr int SB = Core::WM >= 64 && Core::WN >= 64 ? 64 : 32, T = Core::BM;
-  const NtBlock<SB, SB> blk{(float*)(smem + Core::wave() * NtBlock<SB, SB>::BYTES)};
+__device__ __forceinline__ void ns_store(const NsArgs& g, const NsItem& q, const NsMem& mem, const Core& c, int ti, int tj, int wave, char* scratch) {
+  constexpr int SB = Core::BLOCK, T = Core::BM;
+  const NtBlock<SB, SB> blk{(float*)scratch};
   const int m = q.m, N = PHASE == 2 ? q.n : q.m;
   const int mpad = ns_pad(m), npad = ns_pad(N);
-  f16_t* const direct = PHASE == 0 ? q.a : PHASE == 1 ? q.s : q.x;
-  f16_t* const turned = PHASE == 2 ? q.xt[g.cur ^ 1] : direct;
+  f16_t* const direct = PHASE == 0 ? mem.a : PHASE == 1 ? mem.s : mem.x;
+  f16_t* const turned = PHASE == 2 ? mem.xt[g.cur ^ 1] : direct;
   const bool out = PHASE == 2 && g.last;
   const bool do_rows = !out || !q.tall, do_cols = out ? q.tall != 0 : PHASE == 2 || ti != tj;      // (a diagonal tile is its own mirror image)
 #pragma unroll
   for (int bi = 0; bi < Core::WM / SB; ++bi)
 #pragma unroll
     for (int bj = 0; bj < Core::WN / SB; ++bj) {
-      const int gi = ti * T + Core::row0() + bi * SB, gj = tj * T + Core::col0() + bj * SB;
+      const int gi = ti * T + Core::row0(wave) + bi * SB, gj = tj * T + Core::col0(wave) + bj * SB;
       blk.put(c, bi, bj, 1.f / NS_SCALE);
       if (do_rows || PHASE == 1) {
         blk.template rows<PHASE == 1>([&](int i, int j0, float (&v)[8]) {
@@ -154,7 +200,7 @@ __device__ __forceinline__ void ns_store(const NsArgs& g, const NsItem& q, const
           if (r >= m || k >= npad) return;
           if constexpr (PHASE == 1) {
             float a[8];
-            nt_load_pair(q.a + (long)r * 2 * mpad, k, a);
+            nt_load_pair(mem.a + (long)r * 2 * mpad, k, a);
 #pragma unroll
             for (int t = 0; t < 8; ++t) v[t] = g.cc * v[t] + g.cb * a[t] + (r == k + t ? g.ca * NS_SCALE : 0.f);
           }
@@ -196,15 +242,20 @@ __global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_product_kernel
   if (w < 0) return;
   const int k = ns_find(g, w);
   const NsItem& q = g.it[k];
+  const NsMem mem = ns_mem(g, q);
   const int mt = (q.m + TILE - 1) / TILE, mpad = ns_pad(q.m), npad = ns_pad(q.n);
   int t = w - g.start[k], sp = 0, ti, tj;
-  if (PHASE == 0) sp = t % q.split, t /= q.split;
+  if (PHASE == 0) {                               // (workgroups that run together share a part of the contraction)
+    const int tri = mt * (mt + 1) / 2;
+    sp = t / tri;
+    t -= sp * tri;
+  }
   if (PHASE == 2)
     ti = t % mt, tj = t / mt;
   else
     ns_tri(t, ti, tj);
-  const f16_t* a = PHASE == 0 ? q.x : PHASE == 1 ? q.a : q.s;
-  const f16_t* b = PHASE == 0 ? q.x : PHASE == 1 ? q.a : q.xt[g.cur];
+  const f16_t* a = PHASE == 0 ? mem.x : PHASE == 1 ? mem.a : mem.s;
+  const f16_t* b = PHASE == 0 ? mem.x : PHASE == 1 ? mem.a : mem.xt[g.cur];
   const long ld = 2L * (PHASE == 0 ? npad : mpad);
   const int stages = (PHASE == 0 ? npad : mpad) / 32;
   const int per = PHASE == 0 ? (stages + q.split - 1) / q.split : stages;
@@ -213,57 +264,77 @@ __global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_product_kernel
   c.clear();
   c.run(a + (long)ti * TILE * ld, ld, q.m - ti * TILE, b + (long)tj * TILE * ld, ld, (PHASE == 2 ? q.n : q.m) - tj * TILE, s0, s1, smem);
   if (PHASE == 0 && q.split > 1) {
-    f32x4* p = (f32x4*)(q.part + ((long)t * q.split + sp) * TILE * TILE) + (long)Core::wave() * Core::TI * Core::TJ * 64 + Core::lane();
+    f32x4* p = (f32x4*)(mem.part + ((long)t * q.split + sp) * TILE * TILE) + (long)Core::wave() * Core::TI * Core::TJ * 64 + Core::lane();
 #pragma unroll
     for (int i = 0; i < Core::TI; ++i)
 #pragma unroll
       for (int j = 0; j < Core::TJ; ++j) p[(i * Core::TJ + j) * 64] = c.acc[i][j];
     return;
   }
-  ns_store<PHASE>(g, q, c, ti, tj, smem);
+  constexpr int SB = Core::BLOCK;
+  ns_store<PHASE>(g, q, mem, c, ti, tj, Core::wave(), smem + Core::wave() * NtBlock<SB, SB>::BYTES);
 }
 
-// joins the partial tiles of a split A = X X^T, in their order
+// joins the partial tiles of a split A = X X^T, in their order: one wave per workgroup, for one wave's share of a tile
 template <int TILE>
-__global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_join_kernel(NsArgs g) {
+__global__ __launch_bounds__(64) void ns_join_kernel(NsArgs g) {
   typedef typename NsTile<TILE>::Core Core;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int w = (int)blockIdx.x, k = ns_find(g, w);
+  constexpr int SB = Core::BLOCK;
+  __shared__ __attribute__((aligned(16))) char scratch[NtBlock<SB, SB>::BYTES];
+  const int w = (int)blockIdx.x / Core::NW, wave = (int)blockIdx.x % Core::NW, k = ns_find(g, w);
   const NsItem& q = g.it[k];
+  const NsMem mem = ns_mem(g, q);
   const int t = w - g.start[k];
   int ti, tj;
   ns_tri(t, ti, tj);
   Core c;
   c.clear();
-  const f32x4* p = (const f32x4*)(q.part + (long)t * q.split * TILE * TILE) + (long)Core::wave() * Core::TI * Core::TJ * 64 + Core::lane();
+  const f32x4* p = (const f32x4*)(mem.part + (long)t * q.split * TILE * TILE) + (long)wave * Core::TI * Core::TJ * 64 + Core::lane();
   for (int s = 0; s < q.split; ++s, p += TILE * TILE / 4) {
 #pragma unroll
     for (int i = 0; i < Core::TI; ++i)
 #pragma unroll
       for (int j = 0; j < Core::TJ; ++j) c.acc[i][j] += p[(i * Core::TJ + j) * 64];
   }
-  ns_store<0>(g, q, c, ti, tj, smem);
+  ns_store<0>(g, q, mem, c, ti, tj, wave, scratch);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------
-int ns_tile(const FiNsMat& q) {
-  const int m = q.rows < q.cols ? q.rows : q.cols;
-  return m <= 256 ? 64 : m <= 1024 ? 128 : 256;
+// One tile size serves all matrices of a launch.  A workgroup's stage takes about CYC cycles where it shares a CU with others (the matrix pipe and
+// LDS are then busy) and at least LAT where it is alone; 256-wide tiles move the fewest bytes per product, smaller ones reach more CUs.
+struct NsPlan {
+  int tile[3], split;                            // per phase; parts of A's contraction
+};
+constexpr int NS_TILES[3] = {256, 128, 64};
+constexpr double NS_CYC[3] = {5200, 1500, 480}, NS_LAT[3] = {5200, 1900, 700}, NS_LAUNCH = 9000;
+
+NsPlan ns_plan(const FiNsMat* const* mats, int count) {
+  NsPlan p = {};
+  for (int phase = 0; phase < 3; ++phase) {
+    double best = 0;
+    for (int k = 0; k < 3; ++k) {
+      const int T = NS_TILES[k];
+      for (int split = 1; split <= (phase == 0 ? 32 : 1); split *= 2) {
+        double wgs = 0, longest = 0;
+        for (int i = 0; i < count; ++i) {
+          const int m = mats[i]->rows < mats[i]->cols ? mats[i]->rows : mats[i]->cols, n = mats[i]->rows < mats[i]->cols ? mats[i]->cols : mats[i]->rows;
+          const double mt = (m + T - 1) / T, nt = (n + T - 1) / T, stages = (ns_pad(phase == 0 ? n : m) / 32 + split - 1) / split;
+          wgs += phase == 2 ? mt * nt : mt * (mt + 1) / 2 * split;
+          if (stages > longest) longest = stages;
+        }
+        const double rounds = (double)((long)(wgs + 255) / 256);
+        double cost = longest * (rounds * NS_CYC[k] > NS_LAT[k] ? rounds * NS_CYC[k] : NS_LAT[k]);
+        if (split > 1) cost += NS_LAUNCH + split * T * T / 12.0;       // the joining launch, its partial tiles read by one workgroup each
+        if (best == 0 || cost < best) best = cost, p.tile[phase] = T, p.split = phase == 0 ? split : p.split;
+      }
+    }
+  }
+  return p;
 }
 
-// Carves the workspace of one launch group (matrices of one tile size); base == 0 only counts.
-long ns_layout(const FiNsMat* const* mats, int count, int tile, NsArgs& g, char* base) {
+// Fills in the matrices of a launch group; returns their workspace's size.
+long ns_layout(const FiNsMat* const* mats, int count, const NsPlan& plan, NsArgs& g) {
   long at = 0;
-  auto take = [&](long bytes) {
-    char* p = base ? base + at : nullptr;
-    at += (bytes + 255) & ~255L;
-    return p;
-  };
-  long tri = 0;
-  for (int i = 0; i < count; ++i) {
-    const long t = (((mats[i]->rows < mats[i]->cols ? mats[i]->rows : mats[i]->cols) + tile - 1) / tile);
-    tri += t * (t + 1) / 2;
-  }
   g.count = count;
   for (int i = 0; i < count; ++i) {
     NsItem& q = g.it[i];
@@ -271,22 +342,12 @@ long ns_layout(const FiNsMat* const* mats, int count, int tile, NsArgs& g, char*
     q.tall = mats[i]->rows > mats[i]->cols;
     q.m = q.tall ? mats[i]->cols : mats[i]->rows;
     q.n = q.tall ? mats[i]->rows : mats[i]->cols;
-    const long mp = ns_pad(q.m), np = ns_pad(q.n), mt = (q.m + tile - 1) / tile, nt = mt * (mt + 1) / 2;
-    q.x = (f16_t*)take(4L * q.m * np);
-    q.xt[0] = (f16_t*)take(4L * q.n * mp);
-    q.xt[1] = (f16_t*)take(4L * q.n * mp);
-    q.a = (f16_t*)take(4L * q.m * mp);
-    q.s = (f16_t*)take(4L * q.m * mp);
-    q.nsums = (int)(((long)q.m * q.n + NS_CHUNK - 1) / NS_CHUNK);
-    q.sums = (double*)take(8L * q.nsums);
-    // The long product A = X X^T has few tiles: with fewer than two per CU its contraction is split, down to 8 stages (256 values) a piece.
-    const long stages = np / 32;
-    long split = 512 / (tri > 0 ? tri : 1);
-    if (split > stages / 8) split = stages / 8;
-    if (split < 1) split = 1;
-    const long per = (stages + split - 1) / split;
-    q.split = (int)((stages + per - 1) / per);
-    q.part = q.split > 1 ? (float*)take(4L * nt * q.split * tile * tile) : nullptr;
+    const int stages = ns_pad(q.n) / 32, per = (stages + plan.split - 1) / plan.split;
+    q.split = (stages + per - 1) / per;          // (no part is empty)
+    q.base = (unsigned)(at >> 8);
+    const long mt = (q.m + plan.tile[0] - 1) / plan.tile[0];
+    at += ns_mem(nullptr, q).bytes;
+    if (q.split > 1) at += 4L * (mt * (mt + 1) / 2) * q.split * plan.tile[0] * plan.tile[0];
   }
   return at;
 }
@@ -314,66 +375,77 @@ int ns_check(const FiNsMat* mats, int count, int steps, const float* coeffs) {
   return 0;
 }
 
-template <int TILE>
-int ns_run(NsArgs& g, int steps, const float* coeffs, float eps, hipStream_t st) {
+// work items of a launch: 0 sums of squares, 1 normalising, 2 A, 3 joining A, 4 S, 5 X
+int ns_items(NsArgs& g, int what, int T) {
+  long n = 0;
+  for (int i = 0; i < g.count; ++i) {
+    g.start[i] = (int)n;
+    const NsItem& q = g.it[i];
+    const long mt = (q.m + T - 1) / T, nt = (q.n + T - 1) / T, tri = mt * (mt + 1) / 2;
+    n += what == 0 ? ns_sums(q) : what == 2 ? tri * q.split : what == 3 ? (q.split > 1 ? tri : 0) : what == 4 ? tri : mt * nt;
+  }
+  g.start[g.count] = (int)n;
+  return n < (1L << 30) ? (int)n : -1;
+}
+template <int PHASE, int TILE>
+int ns_product(NsArgs& g, hipStream_t st) {
   typedef typename NsTile<TILE>::Core Core;
-  static const bool lds_ok = nt_allow_lds((const void*)ns_product_kernel<0, TILE>) && nt_allow_lds((const void*)ns_product_kernel<1, TILE>) &&
-                             nt_allow_lds((const void*)ns_product_kernel<2, TILE>) && nt_allow_lds((const void*)ns_join_kernel<TILE>);
+  static const bool lds_ok = nt_allow_lds((const void*)ns_product_kernel<PHASE, TILE>);
   if (!lds_ok) return FI_ERR_UNSUPPORTED;
-  g.eps = eps;
-  auto plan = [&](int what) {                              // fills g.start for a launch, returns its work items
-    long n = 0;
-    for (int i = 0; i < g.count; ++i) {
-      g.start[i] = (int)n;
-      const NsItem& q = g.it[i];
-      const long mt = (q.m + TILE - 1) / TILE, nt = (q.n + TILE - 1) / TILE, tri = mt * (mt + 1) / 2;
-      n += what == 0 ? q.nsums : what == 1 ? (long)((q.m + 63) / 64) * ((q.n + 63) / 64) : what == 2 ? tri * q.split
-           : what == 3 ? (q.split > 1 ? tri : 0) : what == 4 ? tri : mt * nt;
-    }
-    g.start[g.count] = (int)n;
-    return (int)n;
-  };
-  const dim3 blk(Core::THREADS);
-  hipLaunchKernelGGL(ns_norm_kernel, dim3(plan(0)), dim3(256), 0, st, g);
+  int n = ns_items(g, PHASE == 0 ? 2 : PHASE == 1 ? 4 : 5, TILE);
+  if (n < 0) return FI_ERR_SHAPE;
+  hipLaunchKernelGGL((ns_product_kernel<PHASE, TILE>), dim3((n + 7) & ~7), dim3(Core::THREADS), Core::LDS, st, g);
   FI_CHECK_LAUNCH();
-  hipLaunchKernelGGL(ns_prep_kernel, dim3(plan(1)), dim3(256), 0, st, g);
-  FI_CHECK_LAUNCH();
-  for (int k = 0; k < steps; ++k) {
-    g.ca = coeffs[3 * k], g.cb = coeffs[3 * k + 1], g.cc = coeffs[3 * k + 2];
-    g.cur = k & 1, g.last = k + 1 == steps;
-    hipLaunchKernelGGL((ns_product_kernel<0, TILE>), dim3((plan(2) + 7) & ~7), blk, Core::LDS, st, g);
-    FI_CHECK_LAUNCH();
-    if (const int n = plan(3)) {
-      hipLaunchKernelGGL((ns_join_kernel<TILE>), dim3(n), blk, Core::LDS, st, g);
-      FI_CHECK_LAUNCH();
-    }
-    hipLaunchKernelGGL((ns_product_kernel<1, TILE>), dim3((plan(4) + 7) & ~7), blk, Core::LDS, st, g);
-    FI_CHECK_LAUNCH();
-    hipLaunchKernelGGL((ns_product_kernel<2, TILE>), dim3((plan(5) + 7) & ~7), blk, Core::LDS, st, g);
+  if (PHASE == 0 && (n = ns_items(g, 3, TILE)) != 0) {
+    hipLaunchKernelGGL((ns_join_kernel<TILE>), dim3(n * Core::NW), dim3(64), 0, st, g);
     FI_CHECK_LAUNCH();
   }
   return 0;
 }
+template <int PHASE>
+int ns_product(NsArgs& g, int tile, hipStream_t st) {
+  return tile == 64 ? ns_product<PHASE, 64>(g, st) : tile == 128 ? ns_product<PHASE, 128>(g, st) : ns_product<PHASE, 256>(g, st);
+}
 
-// f(group's arguments, tile, workspace bytes so far) for every launch group; returns the workspace's size or an error of f
-template <class F>
-long ns_groups(const FiNsMat* mats, int count, char* base, F f) {
-  long at = 0;
-  for (int tile = 64; tile <= 256; tile *= 2) {
-    const FiNsMat* pick[NS_MAX];
-    int n = 0;
-    for (int i = 0; i <= count; ++i) {
-      if (i < count && ns_tile(mats[i]) == tile) pick[n++] = &mats[i];
-      if (n == NS_MAX || (i == count && n)) {
-        NsArgs g = {};
-        at += ns_layout(pick, n, tile, g, base ? base + at : nullptr);
-        const int rc = f(g, tile);
-        if (rc) return rc < 0 ? rc : -1000 - rc;
-        n = 0;
-      }
-    }
+int ns_run(NsArgs& g, const NsPlan& plan, int steps, const float* coeffs, float eps, hipStream_t st) {
+  g.eps = eps;
+  const int nsum = ns_items(g, 0, 64);
+  if (nsum < 0) return FI_ERR_SHAPE;
+  hipLaunchKernelGGL(ns_norm_kernel, dim3(nsum), dim3(256), 0, st, g);
+  FI_CHECK_LAUNCH();
+  const int nprep = ns_items(g, 1, 64);
+  if (nprep < 0) return FI_ERR_SHAPE;
+  hipLaunchKernelGGL(ns_prep_kernel, dim3(nprep), dim3(256), 0, st, g);
+  FI_CHECK_LAUNCH();
+  for (int k = 0; k < steps; ++k) {
+    g.ca = coeffs[3 * k], g.cb = coeffs[3 * k + 1], g.cc = coeffs[3 * k + 2];
+    g.cur = k & 1, g.last = k + 1 == steps;
+    int rc = ns_product<0>(g, plan.tile[0], st);
+    if (!rc) rc = ns_product<1>(g, plan.tile[1], st);
+    if (!rc) rc = ns_product<2>(g, plan.tile[2], st);
+    if (rc) return rc;
   }
-  return at;
+  return 0;
+}
+
+// f(arguments, plan) for every launch group; the workspace is used again by each.  Returns its size, or an error (positive ones as -1000 - error).
+template <class F>
+long ns_groups(const FiNsMat* mats, int count, char* ws, F f) {
+  long most = 0;
+  for (int lo = 0; lo < count; lo += NS_MAX) {
+    const FiNsMat* pick[NS_MAX];
+    const int n = count - lo < NS_MAX ? count - lo : NS_MAX;
+    for (int i = 0; i < n; ++i) pick[i] = &mats[lo + i];
+    const NsPlan plan = ns_plan(pick, n);
+    NsArgs g = {};
+    g.ws = ws;
+    const long bytes = ns_layout(pick, n, plan, g);
+    if (bytes >> 40) return FI_ERR_SHAPE;
+    if (bytes > most) most = bytes;
+    const int rc = f(g, plan);
+    if (rc) return rc < 0 ? rc : -1000 - rc;
+  }
+  return most;
 }
 
 }  // namespace
@@ -382,7 +454,7 @@ extern "C" long fi_newton_schulz_workspace(const FiNsMat* mats, int count) {
   const float c[3] = {0.f, 0.f, 0.f};
   const int rc = ns_check(mats, count, 1, c);
   if (rc) return rc;
-  return ns_groups(mats, count, nullptr, [](NsArgs&, int) { return 0; });
+  return ns_groups(mats, count, nullptr, [](NsArgs&, const NsPlan&) { return 0; });
 }
 
 extern "C" int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const float* coeffs, float eps, void* workspace, void* stream) {
@@ -392,8 +464,6 @@ extern "C" int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const
   for (int i = 0; i < count; ++i)
     if (!mats[i].u || !mats[i].out) return FI_ERR_NULL;
   hipStream_t st = (hipStream_t)stream;
-  const long got = ns_groups(mats, count, (char*)workspace, [&](NsArgs& g, int tile) {
-    return tile == 64 ? ns_run<64>(g, steps, coeffs, eps, st) : tile == 128 ? ns_run<128>(g, steps, coeffs, eps, st) : ns_run<256>(g, steps, coeffs, eps, st);
-  });
+  const long got = ns_groups(mats, count, (char*)workspace, [&](NsArgs& g, const NsPlan& plan) { return ns_run(g, plan, steps, coeffs, eps, st); });
   return got >= 0 ? 0 : got > -1000 ? (int)got : (int)(-1000 - got);
 }

@@ -8,7 +8,7 @@
 //          16-bit matrix rate -- some five times the fp32 matrix instructions' -- and one LDS fragment serves two products.
 // Either way 128 bytes of a row are one STAGE of the contraction, so that loading, LDS layout and addressing are the same.
 //
-// A workgroup owns a BM x BN tile, a wave WM x WN of it.  Stages are brought into a two-slot LDS ring by LDS-DMA (16 bytes per lane, 8 rows
+// A workgroup owns a BM x BN tile, a wave WM x WN of it.  Stages are brought into an LDS ring of SLOTS by LDS-DMA (16 bytes per lane, 8 rows
 // of 128 bytes per instruction); 16-byte piece c of row r lies at piece c ^ (r & 7), the swizzle being applied to the source address
 // because the LDS side of the instruction is linear: the eight lanes a ds_read_b128 serves per clock then touch all 32 banks once.
 #pragma once
@@ -38,12 +38,16 @@ static inline bool nt_allow_lds(const void* kernel) {
 // orders this wave's LDS traffic: what other lanes of the wave wrote before is there after
 __device__ __forceinline__ void nt_wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-template <typename T, bool PAIR, int BM_, int BN_, int WM_, int WN_>
+// SLOTS: two where two stages fill the LDS or several workgroups share a CU; more where a lone workgroup would wait for each stage's latency.
+template <typename T, bool PAIR, int BM_, int BN_, int WM_, int WN_, int SLOTS_ = 2>
 struct NtCore {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, SLOTS = SLOTS_;
   static constexpr int NWN = BN / WN, NW = (BM / WM) * NWN, THREADS = NW * 64;
   static constexpr int TI = WM / 16, TJ = WN / 16;
-  static constexpr int STAGE = (BM + BN) * 128, LDS = 2 * STAGE;
+  static constexpr int STAGE = (BM + BN) * 128, LDS = SLOTS * STAGE;
+  // side of the blocks a wave stores its results by (NtBlock): its scratch lies in the ring
+  static constexpr int BLOCK = WM >= 64 && WN >= 64 && NW * 64 * 64 * 4 <= LDS ? 64 : 32;
+  static_assert(WM % BLOCK == 0 && WN % BLOCK == 0 && NW * BLOCK * BLOCK * 4 <= LDS, "scratch");
   static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;       // DMA instructions of a wave per stage: 8 rows of A, of B
   static_assert(PA * NW * 8 == BM && PB * NW * 8 == BN, "whole DMA instructions for every wave");
   typedef typename DT<T>::frag_t frag_t;
@@ -55,8 +59,10 @@ struct NtCore {
   // of one row into a lane: row statistics stay mostly inside a lane, stores go out in vectors)
   static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
   static __device__ __forceinline__ int lane() { return (int)(threadIdx.x & 63); }
-  static __device__ __forceinline__ int row0() { return (wave() / NWN) * WM; }
-  static __device__ __forceinline__ int col0() { return (wave() % NWN) * WN; }
+  static __device__ __forceinline__ int row0(int w) { return (w / NWN) * WM; }
+  static __device__ __forceinline__ int col0(int w) { return (w % NWN) * WN; }
+  static __device__ __forceinline__ int row0() { return row0(wave()); }
+  static __device__ __forceinline__ int col0() { return col0(wave()); }
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -87,21 +93,30 @@ struct NtCore {
       vb[q] = (unsigned)(r < rowsB ? r : rowsB - 1) * (unsigned)(ldb * 2) + piece;
     }
     const unsigned la = lds0 + (unsigned)(w * PA * 1024), lb = lds0 + (unsigned)(BM * 128 + w * PB * 1024);
+    // (a stage behind the last one is asked for through an empty resource: zeros, no traffic, and every step counts the same loads)
+    const int endA = ra[2], endB = rb[2];
     auto fetch = [&](int s, int slot) {
+      nt_v4i xa = ra, xb = rb;
+      xa[2] = s < s1 ? endA : 0;
+      xb[2] = s < s1 ? endB : 0;
 #pragma unroll
-      for (int q = 0; q < PA; ++q) nt_dma16(ra, la + (unsigned)(slot * STAGE + q * 1024), va[q], (unsigned)s * 128u);
+      for (int q = 0; q < PA; ++q) nt_dma16(xa, la + (unsigned)(slot * STAGE + q * 1024), va[q], (unsigned)s * 128u);
 #pragma unroll
-      for (int q = 0; q < PB; ++q) nt_dma16(rb, lb + (unsigned)(slot * STAGE + q * 1024), vb[q], (unsigned)s * 128u);
+      for (int q = 0; q < PB; ++q) nt_dma16(xb, lb + (unsigned)(slot * STAGE + q * 1024), vb[q], (unsigned)s * 128u);
     };
     const int sw = l & 7, g = l >> 4, lr = l & 15;
     const int oa = (row0() + lr) * 128, ob = BM * 128 + (col0() + lr) * 128;
     const int p0 = ((g) ^ sw) * 16, p1 = ((4 + g) ^ sw) * 16;
 
-    if (s0 < s1) fetch(s0, 0);
+    if (s0 < s1) {
+#pragma unroll
+      for (int k = 0; k < SLOTS - 1; ++k) fetch(s0 + k, k);
+    }
+    int cur = 0, free = SLOTS - 1;                                      // slots of stage s and of the one before it
     for (int s = s0; s < s1; ++s) {
-      const int cur = (s - s0) & 1;
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + 1 < s1) fetch(s + 1, cur ^ 1);
+      // stage s is there for every wave, and every wave has read the one before it
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((SLOTS - 2) * (PA + PB)) : "memory");
+      fetch(s + SLOTS - 1, free);
       const char* sa = smem + cur * STAGE + oa;
       const char* sb = smem + cur * STAGE + ob;
       if constexpr (PAIR) {
@@ -111,16 +126,25 @@ struct NtCore {
           bh[j] = *(const frag_t*)(sb + j * 2048 + p0);
           bl[j] = *(const frag_t*)(sb + j * 2048 + p1);
         }
+        // (the next 16 rows' fragments are under way while these are multiplied)
+        frag_t ah[2], al[2];
+        ah[0] = *(const frag_t*)(sa + p0);
+        al[0] = *(const frag_t*)(sa + p1);
 #pragma unroll
         for (int i = 0; i < TI; ++i) {
-          const frag_t ah = *(const frag_t*)(sa + i * 2048 + p0);
-          const frag_t al = *(const frag_t*)(sa + i * 2048 + p1);
+          const int u = i & 1;
+          if (i + 1 < TI) {
+            ah[u ^ 1] = *(const frag_t*)(sa + (i + 1) * 2048 + p0);
+            al[u ^ 1] = *(const frag_t*)(sa + (i + 1) * 2048 + p1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bh[j], al, acc[i][j]);
+          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bh[j], al[u], acc[i][j]);
 #pragma unroll
-          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bl[j], ah, acc[i][j]);
+          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bl[j], ah[u], acc[i][j]);
 #pragma unroll
-          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bh[j], ah, acc[i][j]);
+          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bh[j], ah[u], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
         }
       } else {
 #pragma unroll
@@ -137,8 +161,10 @@ struct NtCore {
           }
         }
       }
+      free = cur;
+      cur = cur + 1 < SLOTS ? cur + 1 : 0;
     }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // the ring is free: epilogues use it as scratch
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // the ring is free: epilogues use it as scratch
   }
 };
 
