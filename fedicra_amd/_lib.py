@@ -34,7 +34,7 @@ EXPORTS = [
     "fi_conv3d_point_fwd", "fi_conv3d_point_dgrad", "fi_conv3d_point_wgrad", "fi_conv3d_point_wgrad_workspace",
     "fi_bn_fused_fwd_batched", "fi_bn_act_bwd_reduce_batched", "fi_bn_act_bwd_apply_batched",
     "fi_newton_schulz", "fi_newton_schulz_workspace", "fi_linear_ce_saved", "fi_linear_ce_fwd_workspace", "fi_linear_ce_fwd",
-    "fi_linear_ce_bwd_workspace", "fi_linear_ce_bwd",
+    "fi_linear_ce_bwd_workspace", "fi_linear_ce_bwd", "fi_muon_step", "fi_muon_step_workspace",
 ]
 
 
@@ -58,6 +58,10 @@ class FiBnAct(C.Structure):
 
 class FiNsMat(C.Structure):
     _fields_ = [("u", C.c_void_p), ("out", C.c_void_p), ("dtype", C.c_int), ("rows", C.c_int), ("cols", C.c_int)]
+
+
+class FiMuonMat(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("buf", C.c_void_p), ("rows", C.c_int), ("cols", C.c_int), ("scale", C.c_float)]
 
 
 class FiLinearCe(C.Structure):
@@ -116,7 +120,8 @@ def lib():
         _lib.fi_conv2d_stats_xcorr_workspace.restype = C.c_long
         _lib.fi_conv3d_first_wgrad_workspace.restype = C.c_long
         _lib.fi_conv3d_point_wgrad_workspace.restype = C.c_long
-        for name in ("fi_newton_schulz_workspace", "fi_linear_ce_saved", "fi_linear_ce_fwd_workspace", "fi_linear_ce_bwd_workspace"):
+        for name in ("fi_newton_schulz_workspace", "fi_linear_ce_saved", "fi_linear_ce_fwd_workspace", "fi_linear_ce_bwd_workspace",
+                     "fi_muon_step_workspace"):
             getattr(_lib, name).restype = C.c_long
     return _lib
 
@@ -1162,11 +1167,18 @@ def newton_schulz(updates, outs, steps, coeffs, eps):
     for q, u, o in zip(mats, updates, outs):
         q.u, q.out, q.dtype, q.rows, q.cols = _dev(u).data_ptr(), o.data_ptr(), dt(u.dtype), u.shape[0], u.shape[1]
     flat = (C.c_float * (3 * steps))(*[float(v) for abc in coeffs for v in abc])
-    size = lib().fi_newton_schulz_workspace(mats, n)
-    if size < 0:
-        _chk(int(size), "fi_newton_schulz_workspace")
-    ws = torch.empty(size, dtype=torch.uint8, device=updates[0].device)
+    ws = _scratch(lib().fi_newton_schulz_workspace(mats, n), "fi_newton_schulz_workspace", updates[0].device)
     _chk(lib().fi_newton_schulz(mats, n, int(steps), flat, C.c_float(eps), ptr(ws), stream()), "fi_newton_schulz")
+
+
+def muon_step(items, lr_state, momentum, nesterov, weight_decay, steps, coeffs, eps, skip=None):
+    """items: (param, grad, buf, rows, cols, scale) with dense fp32 tensors of rows * cols values."""
+    n = len(items)
+    mats = (FiMuonMat * n)(*[FiMuonMat(_dev(p).data_ptr(), g.data_ptr(), b.data_ptr(), r, c, s) for p, g, b, r, c, s in items])
+    flat = (C.c_float * (3 * steps))(*[float(v) for abc in coeffs for v in abc])
+    ws = _scratch(lib().fi_muon_step_workspace(mats, n), "fi_muon_step_workspace", items[0][0].device)
+    _chk(lib().fi_muon_step(mats, n, ptr(lr_state), C.c_float(momentum), int(nesterov), C.c_float(weight_decay), int(steps), flat,
+                            C.c_float(eps), ptr(skip), ptr(ws), stream()), "fi_muon_step")
 
 
 LABEL_TYPES = {torch.uint8: 0, torch.int32: 1, torch.int64: 2}                 # FI_LABEL_*

@@ -467,3 +467,119 @@ extern "C" int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const
   const long got = ns_groups(mats, count, (char*)workspace, [&](NsArgs& g, const NsPlan& plan) { return ns_run(g, plan, steps, coeffs, eps, st); });
   return got >= 0 ? 0 : got > -1000 ? (int)got : (int)(-1000 - got);
 }
+
+// ---- the optimizer step around it ---------------------------------------------------------------------------------------------------------
+namespace {
+
+struct MuonArgs {
+  FiMuonMat it[NS_MAX];
+  int start[NS_MAX + 1];                         // first block of NS_CHUNK values of each matrix
+  int count, nesterov;
+  float momentum, wd;
+  const double* lr;
+  const float* skip;
+  float* u;                                      // the updates, each from a multiple of NS_CHUNK values on
+};
+static_assert(sizeof(MuonArgs) <= 4096, "kernel arguments");
+
+__device__ __forceinline__ int muon_find(const MuonArgs& a, int w) {
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.start[mid] <= w)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+__host__ __device__ __forceinline__ long muon_size(const FiMuonMat& q) { return (long)q.rows * q.cols; }
+
+// buf <- momentum buf + (1 - momentum) g;  u = (1 - momentum) g + momentum buf (Nesterov) or buf
+__global__ __launch_bounds__(256) void muon_momentum_kernel(MuonArgs a) {
+  const int k = muon_find(a, (int)blockIdx.x);
+  const FiMuonMat& q = a.it[k];
+  const long n = muon_size(q), lo = (long)((int)blockIdx.x - a.start[k]) * NS_CHUNK, hi = lo + NS_CHUNK < n ? lo + NS_CHUNK : n;
+  const bool skip = a.skip && a.skip[0] != 0.f;
+  float* const u = a.u + (long)a.start[k] * NS_CHUNK;
+  for (long i = lo + threadIdx.x; i < hi; i += 256) {
+    const float g = q.grad[i], b = __builtin_fmaf(a.momentum, q.buf[i] - g, g);
+    u[i] = a.nesterov ? __builtin_fmaf(a.momentum, b - g, g) : b;
+    if (!skip) q.buf[i] = b;
+  }
+}
+// p <- (1 - lr wd) p - lr scale u
+__global__ __launch_bounds__(256) void muon_apply_kernel(MuonArgs a) {
+  if (a.skip && a.skip[0] != 0.f) return;
+  const int k = muon_find(a, (int)blockIdx.x);
+  const FiMuonMat& q = a.it[k];
+  const long n = muon_size(q), lo = (long)((int)blockIdx.x - a.start[k]) * NS_CHUNK, hi = lo + NS_CHUNK < n ? lo + NS_CHUNK : n;
+  const double lr = a.lr[0];
+  const float keep = (float)(1.0 - lr * (double)a.wd), step = (float)(lr * (double)q.scale);
+  const float* const u = a.u + (long)a.start[k] * NS_CHUNK;
+  for (long i = lo + threadIdx.x; i < hi; i += 256) q.param[i] = q.param[i] * keep - step * u[i];
+}
+
+// the step's groups of at most NS_MAX matrices: f(arguments, their matrices as the iteration takes them, count, blocks)
+template <class F>
+long muon_groups(const FiMuonMat* mats, int count, float* u, F f) {
+  long most = 0;
+  for (int lo = 0; lo < count; lo += NS_MAX) {
+    MuonArgs a = {};
+    FiNsMat ns[NS_MAX];
+    a.count = count - lo < NS_MAX ? count - lo : NS_MAX;
+    a.u = u;
+    long n = 0;
+    for (int i = 0; i < a.count; ++i) {
+      a.it[i] = mats[lo + i];
+      a.start[i] = (int)n;
+      float* const at = u + n * NS_CHUNK;
+      ns[i] = FiNsMat{at, at, FI_F32, mats[lo + i].rows, mats[lo + i].cols};
+      n += (muon_size(mats[lo + i]) + NS_CHUNK - 1) / NS_CHUNK;
+    }
+    a.start[a.count] = (int)n;
+    if (n >= (1L << 30)) return FI_ERR_SHAPE;
+    if (n * NS_CHUNK * 4 > most) most = n * NS_CHUNK * 4;
+    const long rc = f(a, ns, (int)n);
+    if (rc) return rc;
+  }
+  return most;
+}
+
+}  // namespace
+
+extern "C" long fi_muon_step_workspace(const FiMuonMat* mats, int count) {
+  if (!mats) return FI_ERR_NULL;
+  if (count < 1) return FI_ERR_SHAPE;
+  long most = 0;
+  const long u = muon_groups(mats, count, (float*)256, [&](MuonArgs& a, const FiNsMat* ns, int) {
+    const long b = fi_newton_schulz_workspace(ns, a.count);
+    if (b < 0) return b;
+    if (b > most) most = b;
+    return 0L;
+  });
+  return u < 0 ? u : u + most;
+}
+
+extern "C" int fi_muon_step(const FiMuonMat* mats, int count, const double* lr, float momentum, int nesterov, float weight_decay, int steps,
+                            const float* coeffs, float eps, const float* skip, void* workspace, void* stream) {
+  const long total = fi_muon_step_workspace(mats, count);
+  if (total < 0) return (int)total;
+  if (!lr || !coeffs || !workspace) return FI_ERR_NULL;
+  for (int i = 0; i < count; ++i)
+    if (!mats[i].param || !mats[i].grad || !mats[i].buf) return FI_ERR_NULL;
+  hipStream_t st = (hipStream_t)stream;
+  const long u = muon_groups(mats, count, (float*)workspace, [](MuonArgs&, const FiNsMat*, int) { return 0L; });
+  const long rc = muon_groups(mats, count, (float*)workspace, [&](MuonArgs& a, const FiNsMat* ns, int blocks) -> long {
+    a.lr = lr, a.momentum = momentum, a.nesterov = nesterov, a.wd = weight_decay, a.skip = skip;
+    hipLaunchKernelGGL(muon_momentum_kernel, dim3(blocks), dim3(256), 0, st, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return -1000 - (long)e;
+    const int r = fi_newton_schulz(ns, a.count, steps, coeffs, eps, (char*)workspace + u, stream);
+    if (r) return r < 0 ? r : -1000 - (long)r;
+    hipLaunchKernelGGL(muon_apply_kernel, dim3(blocks), dim3(256), 0, st, a);
+    e = hipGetLastError();
+    return e != hipSuccess ? -1000 - (long)e : 0;
+  });
+  return rc >= 0 ? 0 : rc > -1000 ? (int)rc : (int)(-1000 - rc);
+}

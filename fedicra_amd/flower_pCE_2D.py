@@ -24,7 +24,7 @@ import torch
 
 from . import fl, ops, streams
 from .flower_common import BaseClient
-from .optim import FusedAdamW
+from .optim import OPTIMIZERS
 
 
 import os
@@ -76,9 +76,10 @@ class MyClient(BaseClient):
 
     def _ensure_optimizer(self):
         if self.optimizer is None:
-            self.optimizer = FusedAdamW(self._net(), lr=self.current_lr, base_lr=self.args.base_lr,
-                                        max_iterations=self.args.max_iterations,
-                                        frozen=getattr(self.args, "adamw_frozen", "torch2"))
+            # args.optimizer (not the reference's, whose clients only know AdamW): "muon" orthogonalises the filters' updates
+            make = OPTIMIZERS[getattr(self.args, "optimizer", "adamw")]
+            self.optimizer = make(self._net(), lr=self.current_lr, base_lr=self.args.base_lr, max_iterations=self.args.max_iterations,
+                                  frozen=getattr(self.args, "adamw_frozen", "torch2"))
             self.ctx.seed_offset = self.optimizer.iter       # ops.set_dropout_seed_offset, for this client's context
         return self.optimizer
 

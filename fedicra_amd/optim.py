@@ -197,3 +197,65 @@ class FusedSGD:
 
     def advance_lr(self):
         L.lr_poly_advance(self.iter, self.lr_state, self.base_lr, float(self.max_iterations))
+
+
+class FusedMuon(FusedAdamW):
+    """Muon over the flat parameter buffer: every weight matrix -- a convolution's filter as [Cout, Cin * k * k], a linear layer's weight -- moves
+    along the orthogonalised form of its momentum (ops.newton_schulz), everything else (biases, normalisation) by AdamW:
+
+        buf <- momentum * buf + (1 - momentum) * grad
+        u    = (1 - momentum) * grad + momentum * buf        (nesterov; else buf)
+        w   <- (1 - lr * weight_decay) * w - lr * sqrt(max(1, rows / cols)) * NewtonSchulz(u)
+
+    All of a step's matrices share each launch (fi_muon_step); learning rate, schedule, freeze patterns, gradient scaling and hipGraph capture
+    are FusedAdamW's: the momentum buffers live in its first-moment buffer and restart with ``reset_round``; a parameter without a gradient
+    is left alone, momentum included.  Only the ``frozen="torch2"`` semantics exist."""
+
+    def __init__(self, model, lr, base_lr=None, max_iterations=None, momentum=0.95, nesterov=True, betas=(0.9, 0.999), eps=1e-8,
+                 weight_decay=1e-2, ns_steps=5, ns_coeffs=None, frozen="torch2"):
+        if frozen != "torch2":
+            raise ValueError("FusedMuon: frozen must be 'torch2' (a parameter without a gradient does not step)")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("FusedMuon: momentum must lie in [0, 1)")
+        if int(ns_steps) < 1:
+            raise ValueError("FusedMuon: ns_steps must be at least 1")
+        super().__init__(model, lr, base_lr, max_iterations, betas, eps, weight_decay)
+        from .step_ops import NS_COEFFS
+        self.momentum, self.nesterov = float(momentum), bool(nesterov)
+        self.ns_coeffs = [tuple(ns_coeffs or NS_COEFFS)] * int(ns_steps)
+        self._matrices = {n: p for n, p in model.named_parameters() if p.dim() >= 2}
+
+    def step_scaled(self, scale, found_inf):
+        from . import ops
+        ops.flush_wgrad()
+        params = dict(self.model.named_parameters())
+        active = [n for n in self._names if params[n].grad is not None]
+        if not active:
+            return
+        _adopt_foreign_grads(params, active)
+        P, G = self.model.flat_params, self.model.flat_grads
+        if scale is not None:                 # an overflow anywhere skips the whole step
+            for s, e in self.model.param_ranges(active):
+                L.amp_unscale(G[s:e], scale, found_inf)
+        rest = [n for n in active if n not in self._matrices]
+        if rest:
+            gi, ranges = self._group_for(rest)
+            L.adamw_hyper(self.steps[gi:gi + 1], self.hyper[gi], self.lr_state, self.betas[0], self.betas[1], self.wd)
+            if scale is not None:
+                L.amp_guard(self.steps[gi:gi + 1], self.hyper[gi], found_inf)
+            for s, e in ranges:
+                L.adamw_step(P[s:e], G[s:e], self.m[s:e], self.v[s:e], self.hyper[gi], self.betas[0], self.betas[1], self.eps)
+        items = []
+        for n in active:
+            if n in self._matrices:
+                p = params[n]
+                s, e = p._fi_off, p._fi_off + p.numel()
+                rows, cols = p.shape[0], p.numel() // p.shape[0]          # (the order of a row's values does not matter to the iteration)
+                items.append((P[s:e], G[s:e], self.m[s:e], rows, cols, max(1.0, rows / cols) ** 0.5))
+        if items:
+            L.muon_step(items, self.lr_state, self.momentum, self.nesterov, self.wd, len(self.ns_coeffs), self.ns_coeffs, 1e-7,
+                        None if scale is None else found_inf)
+        ops.bump_weights_epoch()
+
+
+OPTIMIZERS = {"adamw": FusedAdamW, "muon": FusedMuon}

@@ -73,6 +73,8 @@ def build_parser():
     p.add_argument("--synthetic", type=int, default=0, help="N > 0: N synthetic training slices per client instead of HDF5")
     p.add_argument("--dtype", type=str, default=None, help="compute dtype of the HIP kernels (fp32 | bf16 | fp16)")
     p.add_argument("--graph", type=int, default=1, help="capture the training / ALA iteration into a hipGraph")
+    p.add_argument("--optimizer", type=str, default="adamw", choices=["adamw", "muon"],
+                   help="muon: the filters step along their orthogonalised momentum, everything else by AdamW")
     p.add_argument("--adamw_frozen", type=str, default="torch2", choices=["torch2", "torch1"],
                    help="AdamW on parameters the FedICRA freeze schedule has switched off: torch2 = skipped (grad None), "
                         "torch1 = the reference's pinned PyTorch 1.10.2 (zeroed gradients: weight decay keeps acting)")
@@ -85,6 +87,8 @@ def check_args(args, world):
     # flower_common.get_strategy asserts the name (flower_common.py:431-433); a typo must not silently train FedAvg
     assert args.strategy in CENTRALIZED_FL + PERSONALIZED_FL, \
         "unknown --strategy {!r}: one of {}".format(args.strategy, CENTRALIZED_FL + PERSONALIZED_FL)
+    assert getattr(args, "optimizer", "adamw") == "adamw" or getattr(args, "adamw_frozen", "torch2") == "torch2", \
+        "--adamw_frozen torch1 is a semantics of AdamW alone"
     assert args.iters > 0
     assert args.eval_iters > 0 and args.eval_iters % args.iters == 0
     assert args.max_iterations > 0 and args.max_iterations % args.eval_iters == 0

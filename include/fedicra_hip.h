@@ -52,7 +52,7 @@ extern "C" {
  *   3: round 4 (new entry points: fi_conv2d_stats_xcorr*, fi_bn_act_pool_groups, fi_conv1x1_up2x_fwd, fi_wgrad_tuning / fi_narrow_tuning /
  *      fi_upfuse_tuning, fi_pack_weights3d_multi; fi_wgrad_tuning's argument became a bit mask)
  *   5: round 6 (fi_conv3d_tuning; fi_conv_tuning(7, 8): the LDS-DMA forward form)
- *   7: fi_newton_schulz*, fi_linear_ce_* */
+ *   7: fi_newton_schulz*, fi_linear_ce_*, fi_muon_step* */
 #define FI_ABI_VERSION 7
 int fi_abi_version(void);
 
@@ -732,6 +732,21 @@ typedef struct FiNsMat {
 } FiNsMat;
 long fi_newton_schulz_workspace(const FiNsMat* mats, int count);
 int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const float* coeffs, float eps, void* workspace, void* stream);
+/* One optimizer step of any number of fp32 matrices (dense [rows][cols]) around it:
+ *   buf <- momentum buf + (1 - momentum) grad;  u = nesterov ? (1 - momentum) grad + momentum buf : buf;
+ *   param <- (1 - lr weight_decay) param - lr scale NewtonSchulz(u)
+ * lr: device fp64 scalar (the schedule's lr_state); skip: device fp32 flag or NULL -- not zero: neither buf nor param changes (an overflow found
+ * by fi_amp_unscale).  `mats` and `coeffs` are HOST arrays. */
+typedef struct FiMuonMat {
+  float* param;
+  const float* grad;
+  float* buf;
+  int rows, cols;
+  float scale;
+} FiMuonMat;
+long fi_muon_step_workspace(const FiMuonMat* mats, int count);
+int fi_muon_step(const FiMuonMat* mats, int count, const double* lr, float momentum, int nesterov, float weight_decay, int steps,
+                 const float* coeffs, float eps, const float* skip, void* workspace, void* stream);
 
 /* ---------------------------------------------------------------- linear head + cross entropy ---
  * Softmax cross entropy of z = x w^T + bias over V classes without storing z (ops.linear_ce_loss; beside fi_ce_*, which takes stored
