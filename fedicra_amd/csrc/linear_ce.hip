@@ -25,18 +25,19 @@ constexpr int CE_PARTS = 1024;                  // partial results of the max pa
 constexpr int CE_LOSS_WGS = 512;
 
 // kept from the forward to the backward pass, at the head of the caller's `saved` buffer; T = rows
-//   int count (labelled rows) | ... 64 bytes | int idx[T] | int label[T] | float2 stat[T] (row maximum, 1 / sum)
+//   int count (labelled rows), float scales[4] at byte 16 (pair form) | ... 64 bytes | int idx[T] | int label[T] | float2 stat[T] (row maximum, 1 / sum)
 struct CeSaved {
   int* count;
   int* idx;
   int* lab;
   float2* stat;
+  float* scal;
 };
 __host__ __device__ __forceinline__ i64 ce_up(i64 v, i64 a) { return (v + a - 1) / a * a; }
 CeSaved ce_saved(void* p, i64 T) {
   char* c = (char*)p;
   const i64 n = ce_up(4 * T, 64);
-  return CeSaved{(int*)c, (int*)(c + 64), (int*)(c + 64 + n), (float2*)(c + 64 + 2 * n)};
+  return CeSaved{(int*)c, (int*)(c + 64), (int*)(c + 64 + n), (float2*)(c + 64 + 2 * n), (float*)(c + 16)};
 }
 
 // scalars on the device: [0] / [1] the scale of x / W in pair or converted form, [2] / [3] their reciprocals, [4] 1 / (scale of G)
@@ -112,57 +113,61 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const void* labels, int 
 }
 
 // ---- the largest finite magnitude of x's labelled rows and of W ------------------------------------------------------------------------
-// (a wave per row; 16-byte loads where the rows are aligned for them)
+struct CeAmax {
+  const void* p;
+  int dtype, D, vec;       // vec: rows are aligned for 16-byte loads
+  i64 ld, rows;
+  const int *idx, *count;  // row list and its length, or NULL
+  float* part;             // [CE_PARTS]
+};
 template <typename T>
-__global__ __launch_bounds__(256) void ce_amax_kernel(const T* p, i64 ld, int D, int vec, const int* idx, const int* count, i64 rows, float* part) {
-  __shared__ float sm[4];
-  if (count) rows = count[0];
-  const int l = threadIdx.x & 63;
+__device__ __forceinline__ float ce_amax_rows(const CeAmax& a, i64 rows) {
   constexpr int VG = DT<T>::VG;
+  const int l = threadIdx.x & 63, per = a.vec ? (a.D + VG - 1) / VG : a.D;
+  int lanes = 64;                                                       // per row
+  while (lanes > 1 && lanes / 2 >= per) lanes >>= 1;
+  const int sub = l & (lanes - 1), nr = 64 / lanes, dv = a.vec ? a.D / VG : 0;
   float m = 0.f;
-  const int dv = vec ? D / VG : 0;
-  for (i64 r = (i64)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (i64)gridDim.x * 4) {
-    const T* q = p + (idx ? (i64)idx[r] : r) * ld;
-    for (int c = l; c < dv; c += 64) {
+  for (i64 r = ((i64)blockIdx.x * 4 + (threadIdx.x >> 6)) * nr + l / lanes; r < rows; r += (i64)gridDim.x * 4 * nr) {
+    const T* q = (const T*)a.p + (a.idx ? (i64)a.idx[r] : r) * a.ld;
+    for (int c = sub; c < dv; c += lanes) {
       float f[VG];
       VecWords<T>::unpack(((const typename DT<T>::vec_t*)q)[c], f);
 #pragma unroll
       for (int t = 0; t < VG; ++t) m = fabsf(f[t]) < INFINITY ? fmaxf(m, fabsf(f[t])) : m;
     }
-    for (int c = dv * VG + l; c < D; c += 64) {
+    for (int c = dv * VG + sub; c < a.D; c += lanes) {
       const float v = fabsf(to_f32(q[c]));
       if (v < INFINITY) m = fmaxf(m, v);
     }
   }
+  return m;
+}
+__device__ __forceinline__ float ce_block_max(float m, float* sm) {       // 256 threads; the result in all of them
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if (l == 0) sm[threadIdx.x >> 6] = m;
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  return fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
 }
-__global__ __launch_bounds__(256) void ce_scales_kernel(const float* px, const float* pw, float* scal) {
-  __shared__ float sm[2][4];
-  float x = 0.f, w = 0.f;
-  for (int k = threadIdx.x; k < CE_PARTS; k += 256) x = fmaxf(x, px[k]), w = fmaxf(w, pw[k]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64)), w = fmaxf(w, __shfl_xor(w, o, 64));
-  if ((threadIdx.x & 63) == 0) sm[0][threadIdx.x >> 6] = x, sm[1][threadIdx.x >> 6] = w;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const float sx = ce_pow2_scale(fmaxf(fmaxf(sm[0][0], sm[0][1]), fmaxf(sm[0][2], sm[0][3])));
-    const float sw = ce_pow2_scale(fmaxf(fmaxf(sm[1][0], sm[1][1]), fmaxf(sm[1][2], sm[1][3])));
-    scal[SC_X] = sx, scal[SC_W] = sw, scal[SC_RX] = 1.f / sx, scal[SC_RW] = 1.f / sw;
-  }
+__global__ __launch_bounds__(256) void ce_amax_kernel(CeAmax x, CeAmax w) {
+  __shared__ float sm[4];
+  const CeAmax& a = blockIdx.y ? w : x;
+  const i64 rows = a.count ? (i64)a.count[0] : a.rows;
+  const float m = ce_block_max(a.dtype == FI_F32 ? ce_amax_rows<float>(a, rows) : a.dtype == FI_BF16 ? ce_amax_rows<bf16_t>(a, rows) : ce_amax_rows<f16_t>(a, rows), sm);
+  if (threadIdx.x == 0) a.part[blockIdx.x] = m;
 }
 
 // ---- packing an operand ---------------------------------------------------------------------------------------------------------------
 struct CePack {
   const void* src;         // [rows][D], leading dimension ld, storage `dtype`
-  int dtype, D;
+  int dtype, D, vec;       // vec: rows are aligned for 16-byte loads
   i64 ld, rows, begin;     // rows [begin, begin + rows) of the source (of the list); same and turned start there
   const int* idx;          // row list (x) or NULL
   const int* count;        // rows from the device, or NULL
-  const float* scale;      // device scalar or NULL: applied to the pair form and to fp16 made of bf16
+  const float* part;       // CE_PARTS maxima the scale comes from, or NULL
+  const float* scale;      // or the scale itself, or NULL: 1.  Applied to the pair form and to fp16 made of bf16
+  float *put, *rput;       // where the scale and its reciprocal go (with part)
   void* same;              // [rows][K] operand rows, or NULL
   i64 ld_same;
   int same_k;              // its padded width: whole stages, a multiple of 8
@@ -171,43 +176,80 @@ struct CePack {
   i64 ld_turned;
   int turned_pair;
 };
-// one 64 x 64 block of the source per workgroup (blockIdx.x: rows, blockIdx.y: columns); pads are written as zeros
-__global__ __launch_bounds__(256) void ce_pack_kernel(CePack a) {
+template <typename T>
+__device__ __forceinline__ void ce_load8(const T* q, int left, int vec, float (&v)[8]) {
+  if (vec && left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 x = ((const float4*)q)[0], y = ((const float4*)q)[1];
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    } else {
+      VecWords<T>::unpack(*(const uint4*)q, v);
+    }
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < 8; ++t) v[t] = t < left ? to_f32(q[t]) : 0.f;
+}
+// one 64 x 64 block of the source per workgroup (blockIdx.x: rows, .y: columns, .z: which operand); pads are written as zeros
+__global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw) {
   __shared__ float tile[64][65];
+  __shared__ float sm[4];
+  const CePack& a = blockIdx.z ? pw : px;
   const i64 have = a.count ? (i64)a.count[0] - a.begin : a.rows, rows = have < a.rows ? have : a.rows;
   const i64 r0 = (i64)blockIdx.x * 64;
   const int c0 = (int)blockIdx.y * 64, tid = threadIdx.x;
-  if (r0 >= rows) return;
-  for (int e = tid; e < 64 * 64; e += 256) {
-    const i64 r = r0 + (e >> 6);
-    const int c = c0 + (e & 63);
-    tile[e >> 6][e & 63] = r < rows && c < a.D ? ce_load(a.src, a.dtype, (a.idx ? (i64)a.idx[a.begin + r] : r) * a.ld + c) : 0.f;
+  float sc = a.scale ? a.scale[0] : 1.f;
+  if (a.part && (r0 < rows || blockIdx.x == 0)) {
+    float m = 0.f;
+    for (int k = tid; k < CE_PARTS; k += 256) m = fmaxf(m, a.part[k]);
+    sc = ce_pow2_scale(ce_block_max(m, sm));
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) a.put[0] = sc, a.rput[0] = 1.f / sc;
   }
+  if (r0 >= rows || c0 >= (a.same && a.same_k > a.D ? a.same_k : a.D)) return;
+  for (int e = tid; e < 64 * 8; e += 256) {
+    const i64 r = r0 + (e >> 3);
+    const int c = c0 + (e & 7) * 8, left = r < rows ? a.D - c : 0;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (left > 0) {
+      const i64 at = (a.idx ? (i64)a.idx[a.begin + r] : r) * a.ld + c;
+      if (a.dtype == FI_F32)
+        ce_load8((const float*)a.src + at, left, a.vec, v);
+      else if (a.dtype == FI_BF16)
+        ce_load8((const bf16_t*)a.src + at, left, a.vec, v);
+      else
+        ce_load8((const f16_t*)a.src + at, left, a.vec, v);
+    }
+    if (a.same && r < rows && c < a.same_k) {
+      char* row = (char*)a.same + r * a.ld_same * 2;
+      if (a.same_kind == 2) {
+        float q[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) q[t] = v[t] * sc;
+        nt_store_pair((f16_t*)row, c, q);
+      } else if (a.same_kind == 1) {
+        *(uint4*)((f16_t*)row + c) = VecWords<f16_t>::pack(v);
+      } else {
+        *(uint4*)((bf16_t*)row + c) = VecWords<bf16_t>::pack(v);
+      }
+    }
+    if (a.turned) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) tile[e >> 3][(e & 7) * 8 + t] = v[t] * sc;
+    }
+  }
+  if (!a.turned) return;
   __syncthreads();
-  const float sc = a.scale ? a.scale[0] : 1.f;
   for (int e = tid; e < 64 * 8; e += 256) {
     const int r = e >> 3, c = (e & 7) * 8;
+    if (c0 + r >= a.D) continue;
     float v[8];
-    if (a.same && r0 + r < rows && c0 + c < a.same_k) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = tile[r][c + i] * (a.same_kind == 2 ? sc : 1.f);
-      char* row = (char*)a.same + (r0 + r) * a.ld_same * 2;
-      if (a.same_kind == 2)
-        nt_store_pair((f16_t*)row, c0 + c, v);
-      else if (a.same_kind == 1)
-        *(uint4*)((f16_t*)row + c0 + c) = VecWords<f16_t>::pack(v);
-      else
-        *(uint4*)((bf16_t*)row + c0 + c) = VecWords<bf16_t>::pack(v);
-    }
-    if (a.turned && c0 + r < a.D) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = tile[c + i][r] * sc;
-      f16_t* row = (f16_t*)a.turned + (i64)(c0 + r) * a.ld_turned;
-      if (a.turned_pair)
-        nt_store_pair(row, r0 + c, v);
-      else
-        *(uint4*)(row + r0 + c) = VecWords<f16_t>::pack(v);
-    }
+    for (int i = 0; i < 8; ++i) v[i] = tile[c + i][r];
+    f16_t* row = (f16_t*)a.turned + (i64)(c0 + r) * a.ld_turned;
+    if (a.turned_pair)
+      nt_store_pair(row, r0 + c, v);
+    else
+      *(uint4*)(row + r0 + c) = VecWords<f16_t>::pack(v);
   }
 }
 
@@ -348,7 +390,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_fwd_kernel(CeLogits a) {
 
 // joins a row's tiles: LANES lanes per row
 template <int LANES>
-__global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ntj, const float* zt, CeSaved s, float* rows_out, double* sums) {
+__global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ntj, const float* zt, CeSaved s, float* rows_out, double* sums, int mean, float* loss) {
   __shared__ double sm[4];
   const int n = s.count[0], sub = threadIdx.x % LANES;
   double acc = 0.0;
@@ -380,7 +422,11 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int nt
   acc = wave_sum(acc);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = acc;
   __syncthreads();
-  if (threadIdx.x == 0) sums[blockIdx.x] = sm[0] + sm[1] + sm[2] + sm[3];
+  if (threadIdx.x == 0) {
+    acc = sm[0] + sm[1] + sm[2] + sm[3];
+    sums[blockIdx.x] = acc;
+    if (loss) loss[0] = (float)(mean ? acc / (double)n : acc);          // (a lone workgroup)
+  }
 }
 __global__ __launch_bounds__(256) void ce_loss_kernel(const double* sums, int nsums, const int* count, int mean, float* loss) {
   __shared__ double sm[4];
@@ -410,22 +456,51 @@ __global__ __launch_bounds__(256) void ce_gmax_kernel(const float* g, const int*
   __syncthreads();
   if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
 }
-// rows' factors g_t * scale (reduction 0: one upstream gradient per row; 1 mean, 2 sum: one for all)
-__global__ __launch_bounds__(256) void ce_factors_kernel(const float* g, int reduction, const float* part, CeSaved s, float* scal, float* out) {
-  __shared__ float sm[4], s_max;
+// dx of the rows that take no part: a lane looks at a label, the wave clears the rows it finds
+__device__ __forceinline__ void ce_zero_rows(const void* labels, int ltype, i64 T, i64 ignore, char* dx, i64 row_bytes) {
+  const int l = threadIdx.x & 63;
+  const i64 r0 = ((i64)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
+  const bool mine = r0 + l < T && ce_label(labels, ltype, r0 + l) == ignore;
+  unsigned long long todo = __ballot(mine);
+  const bool vec = row_bytes % 16 == 0 && ((uintptr_t)dx & 15) == 0;
+  if (vec && row_bytes <= 512) {                                        // several rows at a time
+    const int per = (int)(row_bytes / 16), rows = 64 / per;
+    if (todo)
+      for (int i = 0; i < 64; i += rows) {
+        const int r = i + l / per;
+        if (l / per < rows && r < 64 && (todo >> r & 1)) ((uint4*)(dx + (r0 + r) * row_bytes))[l % per] = make_uint4(0, 0, 0, 0);
+      }
+    return;
+  }
+  while (todo) {
+    const int r = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    char* p = dx + (r0 + r) * row_bytes;
+    if (vec)
+      for (i64 c = l; c < row_bytes / 16; c += 64) ((uint4*)p)[c] = make_uint4(0, 0, 0, 0);
+    else
+      for (i64 c = l; c < row_bytes / 2; c += 64) ((uint16_t*)p)[c] = 0;
+  }
+}
+
+// rows' factors g_t * scale (reduction 0: one upstream gradient per row; 1 mean, 2 sum: one for all); zeros for dx's other rows
+__global__ __launch_bounds__(256) void ce_factors_kernel(const float* g, int reduction, const float* part, CeSaved s, int pair, float* scal, float* out,
+                                                         const void* labels, int ltype, i64 T, i64 ignore, char* dx, i64 row_bytes) {
+  __shared__ float sm[4];
   const int n = s.count[0], tid = threadIdx.x;
+  if (dx) ce_zero_rows(labels, ltype, T, ignore, dx, row_bytes);
   const float one = reduction == 1 ? (float)((double)g[0] / (double)n) : reduction == 2 ? g[0] : 0.f;
   float m = fabsf(one);
   if (reduction == 0)
     for (int k = tid; k < CE_PARTS; k += 256) m = fmaxf(m, part[k]);
+  const float sc = 0.5f * ce_pow2_scale(ce_block_max(m, sm));           // largest factor in [2^13, 2^14)
+  if (blockIdx.x == 0 && tid == 0) {
+    scal[SC_RG] = 1.f / sc;
+    if (pair) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if ((tid & 63) == 0) sm[tid >> 6] = m;
-  __syncthreads();
-  if (tid == 0) s_max = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  __syncthreads();
-  const float sc = 0.5f * ce_pow2_scale(s_max);                         // largest factor in [2^13, 2^14)
-  if (blockIdx.x == 0 && tid == 0) scal[SC_RG] = 1.f / sc;
+      for (int k = 0; k < 4; ++k) scal[k] = s.scal[k];
+    }
+  }
   for (i64 r = (i64)blockIdx.x * 256 + tid; r < n; r += (i64)gridDim.x * 256) {
     const float f = reduction == 0 ? g[s.idx[r]] : one;
     out[r] = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : f * sc;
@@ -685,33 +760,6 @@ __global__ __launch_bounds__(1024) void ce_dbias_kernel(const float* part, int t
   }
 }
 
-// dx of the rows that take no part: a lane looks at a label, the wave clears the rows it finds
-__global__ __launch_bounds__(256) void ce_zero_rows_kernel(const void* labels, int ltype, i64 T, i64 ignore, char* dx, i64 row_bytes) {
-  const int l = threadIdx.x & 63;
-  const i64 r0 = ((i64)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
-  const bool mine = r0 + l < T && ce_label(labels, ltype, r0 + l) == ignore;
-  unsigned long long todo = __ballot(mine);
-  const bool vec = row_bytes % 16 == 0 && ((uintptr_t)dx & 15) == 0;
-  if (vec && row_bytes <= 512) {                                        // several rows at a time
-    const int per = (int)(row_bytes / 16), rows = 64 / per;
-    if (todo)
-      for (int i = 0; i < 64; i += rows) {
-        const int r = i + l / per;
-        if (l / per < rows && r < 64 && (todo >> r & 1)) ((uint4*)(dx + (r0 + r) * row_bytes))[l % per] = make_uint4(0, 0, 0, 0);
-      }
-    return;
-  }
-  while (todo) {
-    const int r = __builtin_ctzll(todo);
-    todo &= todo - 1;
-    char* p = dx + (r0 + r) * row_bytes;
-    if (vec)
-      for (i64 c = l; c < row_bytes / 16; c += 64) ((uint4*)p)[c] = make_uint4(0, 0, 0, 0);
-    else
-      for (i64 c = l; c < row_bytes / 2; c += 64) ((uint16_t*)p)[c] = 0;
-  }
-}
-
 // ---- host side ------------------------------------------------------------------------------------------------------------------
 struct Carve {
   char* base;
@@ -758,9 +806,9 @@ int ce_check(const FiLinearCe* d) {
 }
 
 // tiles of the logits' product: 256 x 256; 64 rows where there are no more (the classes are then streamed once, and three quarters of a
-// tall tile would repeat the last row); 64 classes likewise
-int ce_logits_tile(const FiLinearCe& d) { return d.T <= 64 ? 1 : d.V <= 64 ? 2 : 0; }
-constexpr int CE_BM[3] = {256, 64, 256}, CE_BN[3] = {256, 256, 64};
+// tall tile would repeat the last row); 64 or 128 classes likewise
+int ce_logits_tile(const FiLinearCe& d) { return d.T <= 64 ? 1 : d.V <= 64 ? 2 : d.V <= 128 ? 3 : 0; }
+constexpr int CE_BM[4] = {256, 64, 256, 256}, CE_BN[4] = {256, 256, 64, 128};
 
 // (the same tile by 16 waves of 64 x 64 in the forward pass -- four per SIMD hide LDS and DMA latency: 845 -> 757 us at 7370 x 50000 x 1024 -- and by
 // 8 of 128 x 64 for G, whose epilogue wants 64 x 64 blocks of scratch: 267 against 290 us a piece of 7370 x 16384)
@@ -769,6 +817,7 @@ template <typename T, bool PAIR> struct CeCores {
   typedef NtCore<T, PAIR, 256, 256, 128, 64> C0;
   typedef NtCore<T, PAIR, 64, 256, 64, 32> C1;
   typedef NtCore<T, PAIR, 256, 64, 32, 64> C2;
+  typedef NtCore<T, PAIR, 256, 128, 64, 64> C3;
 };
 
 template <class Core, typename T, bool PAIR>
@@ -798,42 +847,42 @@ int ce_logits(const CeLogits& a, const FiLinearCe& d, bool fwd, hipStream_t st) 
   switch (ce_logits_tile(d)) {
     case 0: return fwd ? ce_launch_fwd<typename C::F0, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C0, T, PAIR>(a, st);
     case 1: return fwd ? ce_launch_fwd<typename C::C1, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C1, T, PAIR>(a, st);
-    default: return fwd ? ce_launch_fwd<typename C::C2, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C2, T, PAIR>(a, st);
+    case 2: return fwd ? ce_launch_fwd<typename C::C2, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C2, T, PAIR>(a, st);
+    default: return fwd ? ce_launch_fwd<typename C::C3, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C3, T, PAIR>(a, st);
   }
 }
 int ce_logits_any(const CeLogits& a, const FiLinearCe& d, bool fwd, hipStream_t st) {
   return d.dtype == FI_F32 ? ce_logits<f16_t, true>(a, d, fwd, st) : d.dtype == FI_BF16 ? ce_logits<bf16_t, false>(a, d, fwd, st) : ce_logits<f16_t, false>(a, d, fwd, st);
 }
 
-int ce_pack(const CePack& a, hipStream_t st) {
-  const i64 gx = (a.rows + 63) / 64;
-  const int cols = a.same ? a.same_k : a.D;
-  hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)gx, (unsigned)((cols + 63) / 64)), dim3(256), 0, st, a);
+// one or two operands in a launch (src == NULL: none)
+int ce_pack(const CePack& x, const CePack& w, hipStream_t st) {
+  i64 gx = 0;
+  int gy = 0;
+  for (const CePack* p : {&x, &w}) {
+    if (!p->src) continue;
+    const int cols = p->same && p->same_k > p->D ? p->same_k : p->D;
+    if ((p->rows + 63) / 64 > gx) gx = (p->rows + 63) / 64;
+    if ((cols + 63) / 64 > gy) gy = (cols + 63) / 64;
+  }
+  if (!x.src && !w.src) return 0;
+  hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)gx, (unsigned)gy, x.src && w.src ? 2 : 1), dim3(256), 0, st, x.src ? x : w, w);
   FI_CHECK_LAUNCH();
   return 0;
 }
+int ce_vec(const void* p, int dtype, i64 ld) { return ((uintptr_t)p & 15) == 0 && ld % (dtype == FI_F32 ? 4 : 8) == 0; }
 
-template <typename T>
-void ce_amax(const void* p, i64 ld, int D, const CeSaved* s, i64 rows, float* part, hipStream_t st) {
-  const int vec = ((uintptr_t)p & 15) == 0 && ld % DT<T>::VG == 0;
-  hipLaunchKernelGGL(ce_amax_kernel<T>, dim3(CE_PARTS), dim3(256), 0, st, (const T*)p, ld, D, vec, s ? s->idx : nullptr, s ? s->count : nullptr, rows, part);
-}
-void ce_amax_any(const void* p, int dtype, i64 ld, int D, const CeSaved* s, i64 rows, float* part, hipStream_t st) {
-  dtype == FI_F32 ? ce_amax<float>(p, ld, D, s, rows, part, st) : dtype == FI_BF16 ? ce_amax<bf16_t>(p, ld, D, s, rows, part, st) : ce_amax<f16_t>(p, ld, D, s, rows, part, st);
-}
-int ce_scales(const FiLinearCe& d, const void* x, const void* w, const CeSaved& s, float* parts, float* scal, hipStream_t st) {
-  ce_amax_any(x, d.dtype, d.ldx, d.D, &s, d.T, parts, st);
-  FI_CHECK_LAUNCH();
-  ce_amax_any(w, d.wdtype, d.ldw, d.D, nullptr, d.V, parts + CE_PARTS, st);
-  FI_CHECK_LAUNCH();
-  hipLaunchKernelGGL(ce_scales_kernel, dim3(1), dim3(256), 0, st, parts, parts + CE_PARTS, scal);
+int ce_amax(const FiLinearCe& d, const void* x, const void* w, const CeSaved& s, float* parts, hipStream_t st) {
+  const CeAmax ax = {x, d.dtype, d.D, ce_vec(x, d.dtype, d.ldx), d.ldx, d.T, s.idx, s.count, parts};
+  const CeAmax aw = {w, d.wdtype, d.D, ce_vec(w, d.wdtype, d.ldw), d.ldw, d.V, nullptr, nullptr, parts + CE_PARTS};
+  hipLaunchKernelGGL(ce_amax_kernel, dim3(CE_PARTS, 2), dim3(256), 0, st, ax, aw);
   FI_CHECK_LAUNCH();
   return 0;
 }
 
 struct CeFwdWs {
   int* cnt;
-  float *parts, *scal, *zt;
+  float *parts, *zt;
   f16_t *xc, *wc;
   float2* part;
   double* sums;
@@ -844,7 +893,6 @@ CeFwdWs ce_fwd_ws(const FiLinearCe& d, const CeShape& s, void* p) {
   CeFwdWs w;
   w.cnt = c.take<int>((d.T + CE_ROWS - 1) / CE_ROWS);
   w.parts = c.take<float>(2 * CE_PARTS);
-  w.scal = c.take<float>(SC_N);
   w.zt = c.take<float>(d.T);
   w.sums = c.take<double>(CE_LOSS_WGS);
   w.xc = c.take<f16_t>(d.T * s.ldx);
@@ -854,17 +902,18 @@ CeFwdWs ce_fwd_ws(const FiLinearCe& d, const CeShape& s, void* p) {
   return w;
 }
 
-CePack ce_pack_x(const FiLinearCe& d, const CeShape& s, const void* x, const CeSaved& sv, const float* scal, f16_t* xc) {
+// scal: where the scales are (parts == NULL) or go
+CePack ce_pack_x(const FiLinearCe& d, const CeShape& s, const void* x, const CeSaved& sv, const float* parts, float* scal, f16_t* xc) {
   CePack k = {};
-  k.src = x, k.dtype = d.dtype, k.D = d.D, k.ld = d.ldx, k.rows = d.T, k.idx = sv.idx, k.count = sv.count;
-  k.scale = s.scaled ? scal + SC_X : nullptr;
+  k.src = x, k.dtype = d.dtype, k.D = d.D, k.vec = ce_vec(x, d.dtype, d.ldx), k.ld = d.ldx, k.rows = d.T, k.idx = sv.idx, k.count = sv.count;
+  if (scal) k.part = parts, k.scale = parts ? nullptr : scal + SC_X, k.put = scal + SC_X, k.rput = scal + SC_RX;
   k.same = xc, k.ld_same = s.ldx, k.same_k = s.kp, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
   return k;
 }
-CePack ce_pack_w(const FiLinearCe& d, const CeShape& s, const void* w, const float* scal, f16_t* wc) {
+CePack ce_pack_w(const FiLinearCe& d, const CeShape& s, const void* w, const float* parts, float* scal, f16_t* wc) {
   CePack k = {};
-  k.src = w, k.dtype = d.wdtype, k.D = d.D, k.ld = d.ldw, k.rows = d.V;
-  k.scale = s.scaled ? scal + SC_W : nullptr;
+  k.src = w, k.dtype = d.wdtype, k.D = d.D, k.vec = ce_vec(w, d.wdtype, d.ldw), k.ld = d.ldw, k.rows = d.V;
+  if (scal) k.part = parts ? parts + CE_PARTS : nullptr, k.scale = parts ? nullptr : scal + SC_W, k.put = scal + SC_W, k.rput = scal + SC_RW;
   k.same = wc, k.ld_same = s.ldx, k.same_k = s.kp, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
   return k;
 }
@@ -973,30 +1022,35 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
   const CeSaved sv = ce_saved(saved, d->T);
   float* const rows_out = d->reduction == 0 ? loss : nullptr;
   const unsigned nb = (unsigned)((d->T + CE_ROWS - 1) / CE_ROWS);
-  hipLaunchKernelGGL(ce_count_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, ws.cnt);
-  FI_CHECK_LAUNCH();
+  if (nb > 1) {
+    hipLaunchKernelGGL(ce_count_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, ws.cnt);
+    FI_CHECK_LAUNCH();
+  }
   hipLaunchKernelGGL(ce_gather_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, d->V, ws.cnt, sv, ws.zt, rows_out);
   FI_CHECK_LAUNCH();
-  if (s.pair && (rc = ce_scales(*d, x, w, sv, ws.parts, ws.scal, st))) return rc;
-  if ((rc = ce_pack(ce_pack_x(*d, s, x, sv, ws.scal, ws.xc), st))) return rc;
-  if (!s.w_direct && (rc = ce_pack(ce_pack_w(*d, s, w, ws.scal, ws.wc), st))) return rc;
+  if (s.pair && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
+  float* const scal = s.pair ? sv.scal : nullptr;
+  if ((rc = ce_pack(ce_pack_x(*d, s, x, sv, ws.parts, scal, ws.xc), s.w_direct ? CePack{} : ce_pack_w(*d, s, w, ws.parts, scal, ws.wc), st))) return rc;
   CeLogits a = {};
   const int bn = CE_BN[ce_logits_tile(*d)];
   a.x = ws.xc, a.ldx = s.ldx, a.w = s.w_direct ? w : ws.wc, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
-  a.scal = s.pair ? ws.scal : nullptr, a.s = sv, a.part = ws.part, a.zt = ws.zt, a.ntj = (d->V + bn - 1) / bn;
+  a.scal = scal, a.s = sv, a.part = ws.part, a.zt = ws.zt, a.ntj = (d->V + bn - 1) / bn;
   if ((rc = ce_logits_any(a, *d, true, st))) return rc;
   const int lanes = a.ntj > 32 ? 64 : a.ntj > 4 ? 8 : 1;
   i64 g = (d->T * lanes + 255) / 256;
   if (g > CE_LOSS_WGS) g = CE_LOSS_WGS;
+  if (g <= 16) g = 1;                                                   // (short: one workgroup also writes the loss)
+  float* const alone = g == 1 && d->reduction != 0 ? loss : nullptr;
+  const int mean = d->reduction == 1;
   if (lanes == 64)
-    hipLaunchKernelGGL(ce_rows_kernel<64>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums);
+    hipLaunchKernelGGL(ce_rows_kernel<64>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums, mean, alone);
   else if (lanes == 8)
-    hipLaunchKernelGGL(ce_rows_kernel<8>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums);
+    hipLaunchKernelGGL(ce_rows_kernel<8>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums, mean, alone);
   else
-    hipLaunchKernelGGL(ce_rows_kernel<1>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums);
+    hipLaunchKernelGGL(ce_rows_kernel<1>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums, mean, alone);
   FI_CHECK_LAUNCH();
-  if (d->reduction != 0) {
-    hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(256), 0, st, ws.sums, (int)g, sv.count, d->reduction == 1 ? 1 : 0, loss);
+  if (d->reduction != 0 && !alone) {
+    hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(256), 0, st, ws.sums, (int)g, sv.count, mean, loss);
     FI_CHECK_LAUNCH();
   }
   return 0;
@@ -1018,27 +1072,24 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   const CeShape s = ce_shape(*d, w);
   const CeBwdWs ws = ce_bwd_ws(*d, s, dx != nullptr, dw != nullptr, db != nullptr, workspace);
   const CeSaved sv = ce_saved((void*)saved, d->T);
-  if (s.scaled && (rc = ce_scales(*d, x, w, sv, ws.parts, ws.scal, st))) return rc;
-  CePack px = ce_pack_x(*d, s, x, sv, ws.scal, ws.xc);
+  // (the pair form's scales were made by the forward pass)
+  const float* const parts = s.scaled && !s.pair ? ws.parts : nullptr;
+  float* const scal = s.pair ? sv.scal : s.scaled ? ws.scal : nullptr;
+  if (parts && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
+  CePack px = ce_pack_x(*d, s, x, sv, parts, scal, ws.xc), pw = ce_pack_w(*d, s, w, parts, scal, ws.wc);
   const bool rows_pieces = ws.Tc < d->T;
   if (!rows_pieces) px.turned = ws.xt, px.ld_turned = ws.ld_xt, px.turned_pair = s.pair;
-  if ((rc = ce_pack(px, st))) return rc;
-  if (!s.w_direct || ws.wt) {
-    CePack pw = ce_pack_w(*d, s, w, ws.scal, ws.wc);
-    pw.turned = ws.wt, pw.ld_turned = ws.ld_wt, pw.turned_pair = s.pair;
-    if ((rc = ce_pack(pw, st))) return rc;
-  }
+  pw.turned = ws.wt, pw.ld_turned = ws.ld_wt, pw.turned_pair = s.pair;
+  if (s.w_direct && !ws.wt) pw.src = nullptr;                           // (its scale is dx's alone)
+  if ((rc = ce_pack(px, pw, st))) return rc;
   if (d->reduction == 0) {
     hipLaunchKernelGGL(ce_gmax_kernel, dim3(CE_PARTS), dim3(256), 0, st, gloss, sv.idx, sv.count, ws.parts);
     FI_CHECK_LAUNCH();
   }
   const i64 ng = (d->T + 255) / 256;
-  hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)(ng < 1024 ? ng : 1024)), dim3(256), 0, st, gloss, d->reduction, ws.parts, sv, ws.scal, ws.g);
+  hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)ng), dim3(256), 0, st, gloss, d->reduction, ws.parts, sv, (int)s.pair, ws.scal, ws.g, labels,
+                     d->ltype, (i64)d->T, (i64)d->ignore_index, (char*)dx, (i64)d->D * (s.pair ? 4 : 2));
   FI_CHECK_LAUNCH();
-  if (dx) {
-    hipLaunchKernelGGL(ce_zero_rows_kernel, dim3((unsigned)ng), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, (char*)dx, (i64)d->D * (s.pair ? 4 : 2));
-    FI_CHECK_LAUNCH();
-  }
   const int f = s.pair ? 2 : 1;
   CeGrad gx = {}, gw = {};
   gx.a = ws.dl, gx.lda = ws.ld_dl, gx.ldb = ws.ld_wt, gx.N = d->D, gx.count = sv.count, gx.rows_are_tokens = 1;
@@ -1057,9 +1108,9 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
     a.t0 = it * ws.Tc, a.Tc = ws.Tc < d->T - a.t0 ? ws.Tc : d->T - a.t0;
     a.v0 = (int)(iv * ws.Vc), a.Vc = ws.Vc < d->V - a.v0 ? ws.Vc : d->V - a.v0;
     if (rows_pieces && dw && iv == 0) {
-      CePack pt = ce_pack_x(*d, s, x, sv, ws.scal, nullptr);
+      CePack pt = ce_pack_x(*d, s, x, sv, nullptr, scal, nullptr);
       pt.begin = a.t0, pt.rows = a.Tc, pt.turned = ws.xt, pt.ld_turned = ws.ld_xt, pt.turned_pair = s.pair;
-      if ((rc = ce_pack(pt, st))) return rc;
+      if ((rc = ce_pack(pt, CePack{}, st))) return rc;
     }
     if ((rc = ce_logits_any(a, *d, false, st))) return rc;
     if (dx) {

@@ -5,6 +5,8 @@ matrix pipe through one core (csrc/nt_product.h).  ``fedicra_amd.ops`` re-export
 No CPU fallback: everything routes through fedicra_amd._lib."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
@@ -12,6 +14,11 @@ from torch.autograd.function import once_differentiable
 from . import _lib as L
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def _on(device):
+    """The device's context where it is not the current one (entering it costs as much as a launch)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def newton_schulz(updates, steps=5, coeffs=NS_COEFFS, eps=1e-7):
@@ -58,7 +65,7 @@ def _newton_schulz_into(updates, outs, steps, coeffs, eps):
         raise ValueError("newton_schulz: empty matrix")
     L._dev(updates[0])
     updates = [u.detach().contiguous() for u in updates]
-    with torch.cuda.device(dev):
+    with _on(dev):
         L.newton_schulz(updates, outs, steps, coeffs, eps)
 
 
@@ -77,40 +84,39 @@ def _grad_slot(param, shape):
     return g, False, g.reshape(param.shape)
 
 
+def _dense_rows(t, rows, cols):
+    """[rows, cols] view with dense rows (a copy only where there is none)."""
+    t = t.detach()
+    if t.dim() != 2:
+        t = t.reshape(rows, cols)
+    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
+
+
 class _LinearCE(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, labels, ignore_index, reduction):
-        D = x.shape[-1]
-        x2 = x.detach().reshape(-1, D)
-        if x2.stride(1) != 1:
-            x2 = x2.contiguous()
-        w2 = weight.detach().reshape(weight.shape[0], D)
-        if w2.stride(1) != 1:
-            w2 = w2.contiguous()
+        V, D = weight.shape[:2]
+        T = labels.numel()
+        x2, w2 = _dense_rows(x, T, D), _dense_rows(weight, V, D)
         b2 = None if bias is None else bias.detach().float().contiguous()
-        l2 = labels.reshape(-1).contiguous()
-        loss = torch.empty(x2.shape[0] if reduction == "none" else 1, dtype=torch.float32, device=x.device)
-        with torch.cuda.device(x.device):
+        l2 = labels.contiguous()
+        loss = torch.empty(labels.shape if reduction == "none" else (), dtype=torch.float32, device=x.device)
+        with _on(x.device):
             desc = L.linear_ce_desc(x2, w2, l2, ignore_index, reduction)
             saved = L.linear_ce_fwd(desc, x2, w2, b2, l2, loss)
         ctx.save_for_backward(x, weight, bias, labels, saved)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        return loss.reshape(labels.shape) if reduction == "none" else loss[0]
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         x, weight, bias, labels, saved = ctx.saved_tensors
-        D, V = x.shape[-1], weight.shape[0]
-        x2 = x.detach().reshape(-1, D)
-        if x2.stride(1) != 1:
-            x2 = x2.contiguous()
-        w2 = weight.detach().reshape(V, D)
-        if w2.stride(1) != 1:
-            w2 = w2.contiguous()
+        V, D = weight.shape[:2]
+        x2, w2 = _dense_rows(x, labels.numel(), D), _dense_rows(weight, V, D)
         b2 = None if bias is None else bias.detach().float().contiguous()
-        l2 = labels.reshape(-1).contiguous()
-        gl = g.reshape(-1).to(torch.float32).contiguous()
+        l2 = labels.contiguous()
+        gl = g.to(torch.float32).contiguous()
         dx = dw = db = gw = gb = None
         dw_add = db_add = False
         if ctx.needs_input_grad[0]:
@@ -122,7 +128,7 @@ class _LinearCE(Function):
                 db, db_add, gb = _grad_slot(bias, (V,))
             else:
                 db = torch.empty(V, dtype=torch.float32, device=x.device)
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             desc = L.linear_ce_desc(x2, w2, l2, ctx.ignore_index, ctx.reduction)
             L.linear_ce_bwd(desc, x2, w2, b2, l2, saved, gl, dx, dw, dw_add, db, db_add)
         if db is not None and bias.dtype != torch.float32:
