@@ -1039,7 +1039,7 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
   const int lanes = a.ntj > 32 ? 64 : a.ntj > 4 ? 8 : 1;
   i64 g = (d->T * lanes + 255) / 256;
   if (g > CE_LOSS_WGS) g = CE_LOSS_WGS;
-  if (g <= 16) g = 1;                                                   // (short: one workgroup also writes the loss)
+  if (g <= (lanes == 1 ? 16 : 2)) g = 1;                                // (short: one workgroup also writes the loss)
   float* const alone = g == 1 && d->reduction != 0 ? loss : nullptr;
   const int mean = d->reduction == 1;
   if (lanes == 64)

@@ -9,8 +9,8 @@
 //
 // Work per step: m^2 n + m^3 multiply-adds halved by symmetry + m^2 n: A and S are computed on and below the diagonal and stored twice.  Every
 // product's second operand is wanted with its contraction index contiguous, so X is kept in both orientations (X for A, X^T for S X); the
-// product that makes the next X stores both.  All matrices of a call (one model's filters) share each launch: 2 + 3 (+1) launches per step
-// whatever their number.
+// product that makes the next X stores both.  All matrices of a call (one model's filters) share each launch: 2, and 3 (4 where A's contraction is
+// split) per step, whatever their number; where none has more than 64 rows, one per step (ns_narrow_step_kernel).
 #include <math.h>
 
 #include "nt_product.h"
@@ -27,14 +27,26 @@ struct NsItem {
   unsigned base;                                 // its place in the workspace, in 256 bytes
   int m, n, tall, dtype, split;
 };
+// Work items of a launch, by kind
+enum { NS_SUMS, NS_PREP, NS_A, NS_JOIN, NS_S, NS_X, NS_NARROW, NS_KINDS };
+// The call's matrices on the device, at the head of the workspace.  They travel once, as the first kernel's arguments; that kernel leaves them here
+// and the others get a pointer: arguments of kilobytes cost the host some microseconds per launch.
+struct NsTable {
+  NsItem it[NS_MAX];
+  int start[NS_KINDS][NS_MAX];                   // first work item of each matrix
+};
 struct NsArgs {
   char* ws;
   NsItem it[NS_MAX];
-  int start[NS_MAX + 1];                         // first work item of each matrix in this launch
+  int count, narrow, tile[3];
+  float eps;
+};
+static_assert(sizeof(NsArgs) <= 4096, "kernel arguments");
+struct NsCtl {
+  char* ws;
   int count, cur, last;
   float ca, cb, cc, eps;
 };
-static_assert(sizeof(NsArgs) <= 4096, "kernel arguments");
 
 __device__ __host__ __forceinline__ int ns_pad(int v) { return (v + 31) & ~31; }
 __device__ __host__ __forceinline__ int ns_sums(const NsItem& q) { return (int)(((long)q.m * q.n + NS_CHUNK - 1) / NS_CHUNK); }
@@ -61,18 +73,51 @@ __device__ __host__ __forceinline__ NsMem ns_mem(char* p, const NsItem& q) {
   r.bytes = bx + 2 * bt + 2 * ba + bs;
   return r;
 }
-__device__ __forceinline__ NsMem ns_mem(const NsArgs& g, const NsItem& q) { return ns_mem(g.ws + (long)q.base * 256, q); }
+__device__ __forceinline__ NsMem ns_mem(const NsCtl& g, const NsItem& q) { return ns_mem(g.ws + (long)q.base * 256, q); }
 
-__device__ __forceinline__ int ns_find(const NsArgs& g, int w) {             // the last matrix that starts at or before w
-  int lo = 0, hi = g.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (g.start[mid] <= w)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
+// the same for matrices of at most 64 rows, see further down
+__device__ __host__ __forceinline__ int ns_chunks(int n) {
+  const int tiles = (n + 63) / 64;
+  int p = 1;
+  while (p < tiles && p * p < 8 * tiles) ++p;
+  const int ch = (tiles + p - 1) / p;
+  return (tiles + ch - 1) / ch;
+}
+constexpr long NS_PART64 = 64 * 64;
+// the workspace: xt pair rows [n][64], partial A's twice, partial sums of squares
+struct NsNarrow {
+  f16_t* xt;
+  float* part[2];
+  double* sums;
+  long bytes;
+};
+__device__ __host__ __forceinline__ NsNarrow ns_narrow_mem(char* p, const NsItem& q) {
+  const long bt = 256L * q.n, bp = 4 * NS_PART64 * ns_chunks(q.n), bs = (8L * ns_sums(q) + 255) & ~255L;
+  NsNarrow r;
+  r.sums = (double*)p, p += bs;
+  r.xt = (f16_t*)p, p += bt;
+  r.part[0] = (float*)p, p += bp;
+  r.part[1] = (float*)p;
+  r.bytes = bs + bt + 2 * bp;
+  return r;
+}
+
+// how many work items of a kind a matrix has (T: the launch's tile)
+__device__ __host__ __forceinline__ long ns_items(const NsItem& q, int kind, int T) {
+  const long mt = (q.m + T - 1) / T, nt = (q.n + T - 1) / T, tri = mt * (mt + 1) / 2;
+  return kind == NS_SUMS ? ns_sums(q) : kind == NS_A ? tri * q.split : kind == NS_JOIN ? (q.split > 1 ? tri : 0)
+         : kind == NS_S ? tri : kind == NS_NARROW ? ns_chunks(q.n) : mt * nt;
+}
+__device__ __host__ __forceinline__ int ns_tile_of(const NsArgs& g, int kind) {
+  return kind == NS_A || kind == NS_JOIN ? g.tile[0] : kind == NS_S ? g.tile[1] : kind == NS_X ? g.tile[2] : 64;
+}
+__device__ __forceinline__ const NsTable* ns_table(const char* ws) { return (const NsTable*)ws; }
+// the last matrix that starts at or before work item w: a lane each (64 matrices at most)
+__device__ __forceinline__ int ns_find(const NsCtl& g, int kind, int w, int& first) {
+  const int l = threadIdx.x & 63, v = l < g.count ? ns_table(g.ws)->start[kind][l] : 0x7fffffff;
+  const int k = 63 - __builtin_clzll(__ballot(v <= w));
+  first = __builtin_amdgcn_readlane(v, k);
+  return __builtin_amdgcn_readfirstlane(k);
 }
 __device__ __forceinline__ float ns_load(const void* p, int dtype, long i) {
   return dtype == FI_F32 ? ((const float*)p)[i] : dtype == FI_BF16 ? (float)((const bf16_t*)p)[i] : (float)((const f16_t*)p)[i];
@@ -102,26 +147,45 @@ __device__ __forceinline__ double ns_squares(const T* p, long n) {
   }
   return acc;
 }
+// the sums of squares; the first workgroup also leaves the table for the kernels behind
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
   __shared__ double sm[4];
-  const int w = (int)blockIdx.x, k = ns_find(g, w);
+  int k = 0, w = (int)blockIdx.x;
+  while (k + 1 < g.count && w >= ns_sums(g.it[k])) w -= ns_sums(g.it[k++]);
   const NsItem& q = g.it[k];
-  const long total = (long)q.m * q.n, lo = (long)(w - g.start[k]) * NS_CHUNK, n = total - lo < NS_CHUNK ? total - lo : NS_CHUNK;
+  if (blockIdx.x == 0 && threadIdx.x < 64) {
+    NsTable* const t = (NsTable*)g.ws;
+    const int l = threadIdx.x;
+    if (l < g.count) t->it[l] = g.it[l];
+    for (int kind = 0; kind < NS_KINDS; ++kind) {
+      int n = l < g.count ? (int)ns_items(g.it[l], kind, ns_tile_of(g, kind)) : 0, sum = n;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(sum, o, 64);
+        sum += l >= o ? up : 0;
+      }
+      t->start[kind][l] = sum - n;
+    }
+  }
+  const long total = (long)q.m * q.n, lo = (long)w * NS_CHUNK, n = total - lo < NS_CHUNK ? total - lo : NS_CHUNK;
   double acc = q.dtype == FI_F32 ? ns_squares((const float*)q.u + lo, n) : q.dtype == FI_BF16 ? ns_squares((const bf16_t*)q.u + lo, n)
                                                                                            : ns_squares((const f16_t*)q.u + lo, n);
   acc = wave_sum(acc);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = acc;
   __syncthreads();
-  if (threadIdx.x == 0) ns_mem(g, q).sums[w - g.start[k]] = sm[0] + sm[1] + sm[2] + sm[3];
+  char* const p = g.ws + (long)q.base * 256;
+  double* const sums = g.narrow ? ns_narrow_mem(p, q).sums : ns_mem(p, q).sums;
+  if (threadIdx.x == 0) sums[w] = sm[0] + sm[1] + sm[2] + sm[3];
 }
 
 // U, normalised, as pair rows in both orientations: one 64 x 64 block of U per workgroup
-__global__ __launch_bounds__(256) void ns_prep_kernel(NsArgs g) {
+__global__ __launch_bounds__(256) void ns_prep_kernel(NsCtl g) {
   __shared__ float tile[64][65];
   __shared__ double sm[4];
   __shared__ float s_inv;
-  const int w = (int)blockIdx.x, k = ns_find(g, w), tid = threadIdx.x;
-  const NsItem& q = g.it[k];
+  int first;
+  const int w = (int)blockIdx.x, k = ns_find(g, NS_PREP, w, first), tid = threadIdx.x;
+  const NsItem q = ns_table(g.ws)->it[k];
   const NsMem mem = ns_mem(g, q);
   double acc = 0.0;
   for (int i = tid, n = ns_sums(q); i < n; i += 256) acc += mem.sums[i];
@@ -132,7 +196,7 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsArgs g) {
   __syncthreads();
   const float inv = s_inv;
   const int rows = q.tall ? q.n : q.m, cols = q.tall ? q.m : q.n;
-  const int nb = (cols + 63) / 64, t = w - g.start[k], r0 = (t / nb) * 64, c0 = (t % nb) * 64;
+  const int nb = (cols + 63) / 64, t = w - first, r0 = (t / nb) * 64, c0 = (t % nb) * 64;
   for (int e = tid; e < 64 * 64; e += 256) {
     const int r = r0 + (e >> 6), c = c0 + (e & 63);
     tile[e >> 6][e & 63] = r < rows && c < cols ? ns_load(q.u, q.dtype, (long)r * cols + c) * inv : 0.f;
@@ -179,7 +243,7 @@ __device__ __forceinline__ void ns_put(void* out, int dtype, long at, const floa
 
 // what becomes of a tile of PHASE 0 (A), 1 (S) or 2 (X)
 template <int PHASE, class Core>
-__device__ __forceinline__ void ns_store(const NsArgs& g, const NsItem& q, const NsMem& mem, const Core& c, int ti, int tj, int wave, char* scratch) {
+__device__ __forceinline__ void ns_store(const NsCtl& g, const NsItem& q, const NsMem& mem, const Core& c, int ti, int tj, int wave, char* scratch) {
   constexpr int SB = Core::BLOCK, T = Core::BM;
   const NtBlock<SB, SB> blk{(float*)scratch};
   const int m = q.m, N = PHASE == 2 ? q.n : q.m;
@@ -235,16 +299,17 @@ __device__ __forceinline__ void ns_store(const NsArgs& g, const NsItem& q, const
 }
 
 template <int PHASE, int TILE>
-__global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_product_kernel(NsArgs g) {
+__global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_product_kernel(NsCtl g, int items) {
   typedef typename NsTile<TILE>::Core Core;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int w = nt_xcd_item((int)blockIdx.x, (int)gridDim.x, g.start[g.count]);
+  const int w = nt_xcd_item((int)blockIdx.x, (int)gridDim.x, items);
   if (w < 0) return;
-  const int k = ns_find(g, w);
-  const NsItem& q = g.it[k];
+  int first;
+  const int k = ns_find(g, PHASE == 0 ? NS_A : PHASE == 1 ? NS_S : NS_X, w, first);
+  const NsItem q = ns_table(g.ws)->it[k];
   const NsMem mem = ns_mem(g, q);
   const int mt = (q.m + TILE - 1) / TILE, mpad = ns_pad(q.m), npad = ns_pad(q.n);
-  int t = w - g.start[k], sp = 0, ti, tj;
+  int t = w - first, sp = 0, ti, tj;
   if (PHASE == 0) {                               // (workgroups that run together share a part of the contraction)
     const int tri = mt * (mt + 1) / 2;
     sp = t / tri;
@@ -277,14 +342,15 @@ __global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_product_kernel
 
 // joins the partial tiles of a split A = X X^T, in their order: one wave per workgroup, for one wave's share of a tile
 template <int TILE>
-__global__ __launch_bounds__(64) void ns_join_kernel(NsArgs g) {
+__global__ __launch_bounds__(64) void ns_join_kernel(NsCtl g) {
   typedef typename NsTile<TILE>::Core Core;
   constexpr int SB = Core::BLOCK;
   __shared__ __attribute__((aligned(16))) char scratch[NtBlock<SB, SB>::BYTES];
-  const int w = (int)blockIdx.x / Core::NW, wave = (int)blockIdx.x % Core::NW, k = ns_find(g, w);
-  const NsItem& q = g.it[k];
+  int first;
+  const int w = (int)blockIdx.x / Core::NW, wave = (int)blockIdx.x % Core::NW, k = ns_find(g, NS_JOIN, w, first);
+  const NsItem q = ns_table(g.ws)->it[k];
   const NsMem mem = ns_mem(g, q);
-  const int t = w - g.start[k];
+  const int t = w - first;
   int ti, tj;
   ns_tri(t, ti, tj);
   Core c;
@@ -299,17 +365,221 @@ __global__ __launch_bounds__(64) void ns_join_kernel(NsArgs g) {
   ns_store<0>(g, q, mem, c, ti, tj, wave, scratch);
 }
 
+// ---- matrices of at most 64 rows -------------------------------------------------------------------------------------------------------
+// A and S fit a workgroup, so a step is one launch: every workgroup sums the partial A's, makes S for itself, takes its columns of X through
+// S X -- in place, in the X^T orientation alone -- and leaves the partial A of what it made.  A chunk is CH tiles of 64 columns; with about
+// sqrt(8 tiles) chunks the reading of all partial A's (16 KB each) and a chunk's own tiles take about as long.  Launches, not work, are what
+// such a call costs: 2 + one per step.
+// a 64 x 64 pair operand in LDS: [2 stages][64 rows][128 bytes], pieces swizzled as in the ring
+struct NsPair64 {
+  static constexpr int BYTES = 2 * 64 * 128;
+  char* s;
+  __device__ __forceinline__ char* at(int row, int k, int lo) const {    // k: a multiple of 8
+    return s + (k >> 5) * 8192 + row * 128 + (((lo * 4 + ((k & 31) >> 3)) ^ (row & 7)) * 16);
+  }
+  __device__ __forceinline__ void put(int row, int k, const float (&v)[8]) const {
+    uint4 hi, lo;
+    nt_split8(v, hi, lo);
+    *(uint4*)at(row, k, 0) = hi;
+    *(uint4*)at(row, k, 1) = lo;
+  }
+};
+// wave w's 32 x 32 quarter of a b^T, added to acc (coordinates as NtCore's)
+__device__ __forceinline__ void ns_mul64(const NsPair64& a, const NsPair64& b, f32x4 (&acc)[2][2]) {
+  const int w = (int)(threadIdx.x >> 6), l = threadIdx.x & 63, r0 = (w >> 1) * 32 + (l & 15), c0 = (w & 1) * 32 + (l & 15), g = (l >> 4) * 8;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    f16x8 bh[2], bl[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) bh[j] = *(const f16x8*)b.at(c0 + j * 16, s * 32 + g, 0), bl[j] = *(const f16x8*)b.at(c0 + j * 16, s * 32 + g, 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f16x8 ah = *(const f16x8*)a.at(r0 + i * 16, s * 32 + g, 0), al = *(const f16x8*)a.at(r0 + i * 16, s * 32 + g, 1);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        acc[i][j] = mfma16(bh[j], al, acc[i][j]);
+        acc[i][j] = mfma16(bl[j], ah, acc[i][j]);
+        acc[i][j] = mfma16(bh[j], ah, acc[i][j]);
+      }
+    }
+  }
+}
+// fp32 64 x 64 in LDS, in NtBlock's arrangement, for the whole workgroup
+typedef NtBlock<64, 64> NsF64;
+__device__ __forceinline__ void ns_f64_put(const NsF64& f, const f32x4 (&acc)[2][2]) {
+  const int w = (int)(threadIdx.x >> 6), l = threadIdx.x & 63, r0 = (w >> 1) * 32 + (l & 15), c0 = (w & 1) * 32 + 4 * (l >> 4);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) *(float4*)f.at(r0 + i * 16, c0 + j * 16) = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+}
+__device__ __forceinline__ void ns_f64_row8(const NsF64& f, int i, int j, float (&v)[8]) {     // j: a multiple of 8
+  const float4 x = ((const float4*)f.at(i, j))[0], y = ((const float4*)f.at(i, j))[1];
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+}
+__device__ __forceinline__ void ns_part_put(float* part, const f32x4 (&acc)[2][2]) {
+  f32x4* p = (f32x4*)part + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) p[(i * 2 + j) * 256] = acc[i][j];
+}
+
+// normalises U into xt and makes the first partial A
+__global__ __launch_bounds__(256) void ns_narrow_prep_kernel(NsCtl g) {
+  __shared__ __attribute__((aligned(16))) char pool[64 * 65 * 4 + NsPair64::BYTES];
+  __shared__ double sm[4];
+  __shared__ float s_inv;
+  float* const tile = (float*)pool;                                     // [row of X][65]
+  const NsPair64 xa{pool + ((64 * 65 * 4 + 127) & ~127)};
+  int first;
+  const int w = (int)blockIdx.x, k = ns_find(g, NS_NARROW, w, first), tid = threadIdx.x, chunk = w - first;
+  const NsItem q = ns_table(g.ws)->it[k];
+  const NsNarrow mem = ns_narrow_mem(g.ws + (long)q.base * 256, q);
+  double sum = 0.0;
+  for (int i = tid, n = ns_sums(q); i < n; i += 256) sum += mem.sums[i];
+  sum = wave_sum(sum);
+  if ((tid & 63) == 0) sm[tid >> 6] = sum;
+  __syncthreads();
+  if (tid == 0) s_inv = (float)((double)NS_SCALE / (sqrt(sm[0] + sm[1] + sm[2] + sm[3]) + (double)g.eps));
+  __syncthreads();
+  const float inv = s_inv;
+  const int tiles = (q.n + 63) / 64, P = ns_chunks(q.n), ch = (tiles + P - 1) / P;
+  f32x4 acc[2][2] = {};
+  for (int t = chunk * ch; t < tiles && t < chunk * ch + ch; ++t) {
+    const int c0 = t * 64;
+    __syncthreads();
+    for (int e = tid; e < 64 * 64; e += 256) {
+      const int i = q.tall ? e & 63 : e >> 6, j = q.tall ? e >> 6 : e & 63;                    // X's row and column; along U's rows either way
+      tile[i * 65 + j] = i < q.m && c0 + j < q.n ? ns_load(q.u, q.dtype, q.tall ? (long)(c0 + j) * q.m + i : (long)i * q.n + c0 + j) * inv : 0.f;
+    }
+    __syncthreads();
+    for (int e = tid; e < 64 * 8; e += 256) {
+      const int r = e >> 3, c = (e & 7) * 8;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = tile[r * 65 + c + i];
+      xa.put(r, c, v);
+      if (c0 + r < q.n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = tile[(c + i) * 65 + r];
+        nt_store_pair(mem.xt + (long)(c0 + r) * 128, c, v);
+      }
+    }
+    __syncthreads();
+    ns_mul64(xa, xa, acc);
+  }
+  ns_part_put(mem.part[0] + NS_PART64 * chunk, acc);
+}
+
+__global__ __launch_bounds__(256) void ns_narrow_step_kernel(NsCtl g) {
+  __shared__ __attribute__((aligned(128))) char pool[NsF64::BYTES + 2 * NsPair64::BYTES];
+  const NsF64 f{(float*)pool};
+  const NsPair64 sp{pool + NsF64::BYTES}, xp{pool + NsF64::BYTES + NsPair64::BYTES};           // S; X^T's rows, then X's
+  int first;
+  const int w = (int)blockIdx.x, k = ns_find(g, NS_NARROW, w, first), tid = threadIdx.x, chunk = w - first;
+  const NsItem q = ns_table(g.ws)->it[k];
+  const NsNarrow mem = ns_narrow_mem(g.ws + (long)q.base * 256, q);
+  const int tiles = (q.n + 63) / 64, P = ns_chunks(q.n), ch = (tiles + P - 1) / P;
+  // A: the parts in their order, in the accumulators' own arrangement
+  f32x4 a[2][2] = {}, acc[2][2] = {};
+  {
+    const f32x4* p = (const f32x4*)mem.part[g.cur] + tid;
+#pragma unroll 4
+    for (int s = 0; s < P; ++s, p += NS_PART64 / 4)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i >> 1][i & 1] += p[i * 256];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i >> 1][i & 1] *= 1.f / NS_SCALE;
+  ns_f64_put(f, a);
+  __syncthreads();
+  for (int e = tid; e < 64 * 8; e += 256) {
+    float v[8];
+    ns_f64_row8(f, e >> 3, (e & 7) * 8, v);
+    xp.put(e >> 3, (e & 7) * 8, v);
+  }
+  __syncthreads();
+  ns_mul64(xp, xp, acc);
+  {
+    const int l = tid & 63, r0 = (tid >> 7) * 32 + (l & 15), c0 = ((tid >> 6) & 1) * 32 + 4 * (l >> 4);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[i][j][r] = g.cc * (acc[i][j][r] * (1.f / NS_SCALE)) + g.cb * a[i][j][r] + (r0 + i * 16 == c0 + j * 16 + r ? g.ca * NS_SCALE : 0.f);
+  }
+  ns_f64_put(f, acc);                                                   // (every wave has read A's copy: the barrier above)
+  __syncthreads();
+  for (int e = tid; e < 64 * 8; e += 256) {
+    float v[8];
+    ns_f64_row8(f, e >> 3, (e & 7) * 8, v);
+    sp.put(e >> 3, (e & 7) * 8, v);
+  }
+  f32x4 next[2][2] = {};
+  for (int t = chunk * ch; t < tiles && t < chunk * ch + ch; ++t) {
+    const int c0 = t * 64;
+    __syncthreads();
+    for (int e = tid; e < 64 * 16; e += 256) {                          // X^T's 64 rows of 256 bytes
+      const int r = e >> 4, piece = e & 15;
+      const uint4 v = c0 + r < q.n ? *(const uint4*)(mem.xt + (long)(c0 + r) * 128 + piece * 8) : make_uint4(0, 0, 0, 0);
+      *(uint4*)(xp.s + (piece >> 3) * 8192 + r * 128 + (((piece & 7) ^ (r & 7)) * 16)) = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    ns_mul64(sp, xp, acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] *= 1.f / NS_SCALE;
+    ns_f64_put(f, acc);
+    __syncthreads();
+    for (int e = tid; e < 64 * 8; e += 256) {
+      const int r = e >> 3, c = (e & 7) * 8;
+      float v[8];
+      if (g.last) {
+        if (!q.tall) {
+          ns_f64_row8(f, r, c, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] *= 1.f / NS_SCALE;
+          if (r < q.m && c0 + c < q.n) ns_put(q.out, q.dtype, (long)r * q.n + c0 + c, v, q.n - c0 - c);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = *f.at(c + i, r) * (1.f / NS_SCALE);
+          if (c0 + r < q.n && c < q.m) ns_put(q.out, q.dtype, (long)(c0 + r) * q.m + c, v, q.m - c);
+        }
+      } else {
+        ns_f64_row8(f, r, c, v);
+        xp.put(r, c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = *f.at(c + i, r);
+        if (c0 + r < q.n) nt_store_pair(mem.xt + (long)(c0 + r) * 128, c, v);
+      }
+    }
+    if (!g.last) {
+      __syncthreads();
+      ns_mul64(xp, xp, next);
+    }
+  }
+  if (!g.last) ns_part_put(mem.part[g.cur ^ 1] + NS_PART64 * chunk, next);
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------------------
 // One tile size serves all matrices of a launch.  A workgroup's stage takes about CYC cycles where it shares a CU with others (the matrix pipe and
 // LDS are then busy) and at least LAT where it is alone; 256-wide tiles move the fewest bytes per product, smaller ones reach more CUs.
 struct NsPlan {
   int tile[3], split;                            // per phase; parts of A's contraction
+  bool narrow;                                   // no matrix has more than 64 rows
 };
 constexpr int NS_TILES[3] = {256, 128, 64};
 constexpr double NS_CYC[3] = {5200, 1500, 480}, NS_LAT[3] = {5200, 1900, 700}, NS_LAUNCH = 9000;
 
 NsPlan ns_plan(const FiNsMat* const* mats, int count) {
   NsPlan p = {};
+  p.split = 1, p.narrow = true;
+  for (int i = 0; i < count; ++i) p.narrow = p.narrow && (mats[i]->rows <= 64 || mats[i]->cols <= 64);
+  if (p.narrow) return p;
   for (int phase = 0; phase < 3; ++phase) {
     double best = 0;
     for (int k = 0; k < 3; ++k) {
@@ -334,8 +604,9 @@ NsPlan ns_plan(const FiNsMat* const* mats, int count) {
 
 // Fills in the matrices of a launch group; returns their workspace's size.
 long ns_layout(const FiNsMat* const* mats, int count, const NsPlan& plan, NsArgs& g) {
-  long at = 0;
-  g.count = count;
+  long at = (sizeof(NsTable) + 255) & ~255L;
+  g.count = count, g.narrow = plan.narrow;
+  for (int k = 0; k < 3; ++k) g.tile[k] = plan.narrow ? 64 : plan.tile[k];
   for (int i = 0; i < count; ++i) {
     NsItem& q = g.it[i];
     q.u = mats[i]->u, q.out = mats[i]->out, q.dtype = mats[i]->dtype;
@@ -345,6 +616,10 @@ long ns_layout(const FiNsMat* const* mats, int count, const NsPlan& plan, NsArgs
     const int stages = ns_pad(q.n) / 32, per = (stages + plan.split - 1) / plan.split;
     q.split = (stages + per - 1) / per;          // (no part is empty)
     q.base = (unsigned)(at >> 8);
+    if (plan.narrow) {
+      at += ns_narrow_mem(nullptr, q).bytes;
+      continue;
+    }
     const long mt = (q.m + plan.tile[0] - 1) / plan.tile[0];
     at += ns_mem(nullptr, q).bytes;
     if (q.split > 1) at += 4L * (mt * (mt + 1) / 2) * q.split * plan.tile[0] * plan.tile[0];
@@ -375,60 +650,60 @@ int ns_check(const FiNsMat* mats, int count, int steps, const float* coeffs) {
   return 0;
 }
 
-// work items of a launch: 0 sums of squares, 1 normalising, 2 A, 3 joining A, 4 S, 5 X
-int ns_items(NsArgs& g, int what, int T) {
+int ns_total(const NsArgs& g, int kind) {
   long n = 0;
-  for (int i = 0; i < g.count; ++i) {
-    g.start[i] = (int)n;
-    const NsItem& q = g.it[i];
-    const long mt = (q.m + T - 1) / T, nt = (q.n + T - 1) / T, tri = mt * (mt + 1) / 2;
-    n += what == 0 ? ns_sums(q) : what == 2 ? tri * q.split : what == 3 ? (q.split > 1 ? tri : 0) : what == 4 ? tri : mt * nt;
-  }
-  g.start[g.count] = (int)n;
+  for (int i = 0; i < g.count; ++i) n += ns_items(g.it[i], kind, ns_tile_of(g, kind));
   return n < (1L << 30) ? (int)n : -1;
 }
 template <int PHASE, int TILE>
-int ns_product(NsArgs& g, hipStream_t st) {
+int ns_product(const NsCtl& c, int items, int joins, hipStream_t st) {
   typedef typename NsTile<TILE>::Core Core;
   static const bool lds_ok = nt_allow_lds((const void*)ns_product_kernel<PHASE, TILE>);
   if (!lds_ok) return FI_ERR_UNSUPPORTED;
-  int n = ns_items(g, PHASE == 0 ? 2 : PHASE == 1 ? 4 : 5, TILE);
-  if (n < 0) return FI_ERR_SHAPE;
-  hipLaunchKernelGGL((ns_product_kernel<PHASE, TILE>), dim3((n + 7) & ~7), dim3(Core::THREADS), Core::LDS, st, g);
+  hipLaunchKernelGGL((ns_product_kernel<PHASE, TILE>), dim3((items + 7) & ~7), dim3(Core::THREADS), Core::LDS, st, c, items);
   FI_CHECK_LAUNCH();
-  if (PHASE == 0 && (n = ns_items(g, 3, TILE)) != 0) {
-    hipLaunchKernelGGL((ns_join_kernel<TILE>), dim3(n * Core::NW), dim3(64), 0, st, g);
+  if (PHASE == 0 && joins) {
+    hipLaunchKernelGGL((ns_join_kernel<TILE>), dim3(joins * Core::NW), dim3(64), 0, st, c);
     FI_CHECK_LAUNCH();
   }
   return 0;
 }
 template <int PHASE>
-int ns_product(NsArgs& g, int tile, hipStream_t st) {
-  return tile == 64 ? ns_product<PHASE, 64>(g, st) : tile == 128 ? ns_product<PHASE, 128>(g, st) : ns_product<PHASE, 256>(g, st);
+int ns_product(const NsCtl& c, int tile, int items, int joins, hipStream_t st) {
+  return tile == 64 ? ns_product<PHASE, 64>(c, items, joins, st) : tile == 128 ? ns_product<PHASE, 128>(c, items, joins, st)
+                                                                               : ns_product<PHASE, 256>(c, items, joins, st);
 }
 
-int ns_run(NsArgs& g, const NsPlan& plan, int steps, const float* coeffs, float eps, hipStream_t st) {
+int ns_run(NsArgs& g, int steps, const float* coeffs, float eps, hipStream_t st) {
+  int n[NS_KINDS];
+  for (int k = 0; k < NS_KINDS; ++k)
+    if ((n[k] = ns_total(g, k)) < 0) return FI_ERR_SHAPE;
   g.eps = eps;
-  const int nsum = ns_items(g, 0, 64);
-  if (nsum < 0) return FI_ERR_SHAPE;
-  hipLaunchKernelGGL(ns_norm_kernel, dim3(nsum), dim3(256), 0, st, g);
+  NsCtl c = {g.ws, g.count, 0, 0, 0.f, 0.f, 0.f, eps};
+  hipLaunchKernelGGL(ns_norm_kernel, dim3(n[NS_SUMS]), dim3(256), 0, st, g);
   FI_CHECK_LAUNCH();
-  const int nprep = ns_items(g, 1, 64);
-  if (nprep < 0) return FI_ERR_SHAPE;
-  hipLaunchKernelGGL(ns_prep_kernel, dim3(nprep), dim3(256), 0, st, g);
+  if (g.narrow)
+    hipLaunchKernelGGL(ns_narrow_prep_kernel, dim3(n[NS_NARROW]), dim3(256), 0, st, c);
+  else
+    hipLaunchKernelGGL(ns_prep_kernel, dim3(n[NS_PREP]), dim3(256), 0, st, c);
   FI_CHECK_LAUNCH();
   for (int k = 0; k < steps; ++k) {
-    g.ca = coeffs[3 * k], g.cb = coeffs[3 * k + 1], g.cc = coeffs[3 * k + 2];
-    g.cur = k & 1, g.last = k + 1 == steps;
-    int rc = ns_product<0>(g, plan.tile[0], st);
-    if (!rc) rc = ns_product<1>(g, plan.tile[1], st);
-    if (!rc) rc = ns_product<2>(g, plan.tile[2], st);
+    c.ca = coeffs[3 * k], c.cb = coeffs[3 * k + 1], c.cc = coeffs[3 * k + 2];
+    c.cur = k & 1, c.last = k + 1 == steps;
+    if (g.narrow) {
+      hipLaunchKernelGGL(ns_narrow_step_kernel, dim3(n[NS_NARROW]), dim3(256), 0, st, c);
+      FI_CHECK_LAUNCH();
+      continue;
+    }
+    int rc = ns_product<0>(c, g.tile[0], n[NS_A], n[NS_JOIN], st);
+    if (!rc) rc = ns_product<1>(c, g.tile[1], n[NS_S], 0, st);
+    if (!rc) rc = ns_product<2>(c, g.tile[2], n[NS_X], 0, st);
     if (rc) return rc;
   }
   return 0;
 }
 
-// f(arguments, plan) for every launch group; the workspace is used again by each.  Returns its size, or an error (positive ones as -1000 - error).
+// f(arguments) for every launch group; the workspace is used again by each.  Returns its size, or an error (positive ones as -1000 - error).
 template <class F>
 long ns_groups(const FiNsMat* mats, int count, char* ws, F f) {
   long most = 0;
@@ -442,7 +717,7 @@ long ns_groups(const FiNsMat* mats, int count, char* ws, F f) {
     const long bytes = ns_layout(pick, n, plan, g);
     if (bytes >> 40) return FI_ERR_SHAPE;
     if (bytes > most) most = bytes;
-    const int rc = f(g, plan);
+    const int rc = f(g);
     if (rc) return rc < 0 ? rc : -1000 - rc;
   }
   return most;
@@ -454,7 +729,7 @@ extern "C" long fi_newton_schulz_workspace(const FiNsMat* mats, int count) {
   const float c[3] = {0.f, 0.f, 0.f};
   const int rc = ns_check(mats, count, 1, c);
   if (rc) return rc;
-  return ns_groups(mats, count, nullptr, [](NsArgs&, const NsPlan&) { return 0; });
+  return ns_groups(mats, count, nullptr, [](NsArgs&) { return 0; });
 }
 
 extern "C" int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const float* coeffs, float eps, void* workspace, void* stream) {
@@ -464,7 +739,7 @@ extern "C" int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const
   for (int i = 0; i < count; ++i)
     if (!mats[i].u || !mats[i].out) return FI_ERR_NULL;
   hipStream_t st = (hipStream_t)stream;
-  const long got = ns_groups(mats, count, (char*)workspace, [&](NsArgs& g, const NsPlan& plan) { return ns_run(g, plan, steps, coeffs, eps, st); });
+  const long got = ns_groups(mats, count, (char*)workspace, [&](NsArgs& g) { return ns_run(g, steps, coeffs, eps, st); });
   return got >= 0 ? 0 : got > -1000 ? (int)got : (int)(-1000 - got);
 }
 
