@@ -484,8 +484,8 @@ __device__ __forceinline__ void ce_zero_rows(const void* labels, int ltype, i64 
 }
 
 // rows' factors g_t * scale (reduction 0: one upstream gradient per row; 1 mean, 2 sum: one for all); zeros for dx's other rows
-__global__ __launch_bounds__(256) void ce_factors_kernel(const float* g, int reduction, const float* part, CeSaved s, int pair, float* scal, float* out,
-                                                         const void* labels, int ltype, i64 T, i64 ignore, char* dx, i64 row_bytes) {
+__global__ __launch_bounds__(256) void ce_factors_kernel(const float* g, int reduction, const float* part, CeSaved s, int pair, float* scal, float* out, float4* meta,
+                                                         const float* bias, int V, float* bias_pad, const void* labels, int ltype, i64 T, i64 ignore, char* dx, i64 row_bytes) {
   __shared__ float sm[4];
   const int n = s.count[0], tid = threadIdx.x;
   if (dx) ce_zero_rows(labels, ltype, T, ignore, dx, row_bytes);
@@ -505,6 +505,18 @@ __global__ __launch_bounds__(256) void ce_factors_kernel(const float* g, int red
     const float f = reduction == 0 ? g[s.idx[r]] : one;
     out[r] = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : f * sc;
   }
+  if (!meta) return;
+  // the fused form's row table, whole tiles of 64 rows long (a row behind the last one: exp2(-inf) * 0), and its bias likewise
+  for (i64 r = (i64)blockIdx.x * 256 + tid; r < ((n + 63) & ~63); r += (i64)gridDim.x * 256) {
+    float4 m = make_float4(INFINITY, 0.f, 0.f, __int_as_float(-1));
+    if (r < n) {
+      const float2 st = s.stat[r];
+      const float f = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : (reduction == 0 ? g[s.idx[r]] : one) * sc;
+      m = make_float4(st.x * CE_LOG2E, f * st.y, f, __int_as_float(s.lab[r]));
+    }
+    meta[r] = m;
+  }
+  for (i64 v = (i64)blockIdx.x * 256 + tid; v < ((V + 63) & ~63); v += (i64)gridDim.x * 256) bias_pad[v] = bias && v < V ? bias[v] : 0.f;
 }
 
 template <bool PAIR>
@@ -740,11 +752,11 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeGrad a) {
   }
 }
 
-// db: column sums over the row tiles, in fp64: 16 columns per workgroup, 64 lanes' worth of row tiles each
-__global__ __launch_bounds__(1024) void ce_dbias_kernel(const float* part, int tile, int V, const int* count, const float* scal, float* db, int accumulate) {
+// db: column sums over the row tiles (or over `parts` partial sums), in fp64: 16 columns per workgroup, 64 lanes' worth of row tiles each
+__global__ __launch_bounds__(1024) void ce_dbias_kernel(const float* part, int tile, int parts, int V, const int* count, const float* scal, float* db, int accumulate) {
   __shared__ double sm[64][17];
   const int col = threadIdx.x & 15, q = threadIdx.x >> 4, v = blockIdx.x * 16 + col;
-  const int nt = (count[0] + tile - 1) / tile;
+  const int nt = parts ? parts : (count[0] + tile - 1) / tile;
   double acc = 0.0;
   if (v < V)
     for (int t = q; t < nt; t += 64) acc += (double)part[(i64)t * V + v];
@@ -757,6 +769,235 @@ __global__ __launch_bounds__(1024) void ce_dbias_kernel(const float* part, int t
   if (q == 0 && v < V) {
     acc = sm[0][col] * (double)scal[SC_RG];
     db[v] = accumulate ? db[v] + (float)acc : (float)acc;
+  }
+}
+
+// ---- the backward pass of narrow operands: G stays in registers ------------------------------------------------------------------------
+// With up to 128 features the two gradient products do less work per value of G than writing and reading it costs (2 x 4 bytes against 4 D
+// operations), so each makes its own G.  A wave owns 32 rows -- tokens for dx, classes for dW (DW) -- whose operand fragments stay in registers; the
+// other side is streamed through LDS in tiles of 64, once as rows [64][K] for the logits and once turned, [D][64], for the product with G.
+// G never leaves the lane that made it: the matrix instruction returns 4 consecutive rows of its first operand per lane, so if fragment row i of
+// tile j is taken from streamed row 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4, a lane's results of two tiles are 8 consecutive streamed rows
+// -- exactly the fragment that the next product wants from it.  (Pieces of a row are swizzled by (row & 3) | (row / 8 & 1) * 4, which is free of
+// bank conflicts under that order.)
+struct CeFused {
+  CeGrad out;
+  CeSaved s;
+  const void *own, *tile;  // rows in registers, streamed rows: packed operands
+  i64 ld_own, ld_tile;
+  const f16_t* turned;     // the streamed side turned, [D][..]
+  i64 ld_turned;
+  const float4* meta;      // per token: maximum * log2 e, factor / sum, factor, label
+  const float* bias;       // padded to 64 classes (zeros without a bias)
+  float* db;               // DW: [split][V] partial sums, or NULL
+  int V;
+};
+
+__device__ __forceinline__ void ce_put4(const CeGrad& a, i64 row, int col, const float (&v)[4], int nv) {
+  const i64 at = row * a.ldo + col;
+  if (a.vec && !a.accumulate) {
+    if (a.out_dtype == FI_F32)
+      *(float4*)((float*)a.out + at) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+      *(uint2*)((uint16_t*)a.out + at) = a.out_dtype == FI_BF16 ? make_uint2(__builtin_bit_cast(unsigned, bf16x2_t{(bf16_t)v[0], (bf16_t)v[1]}), __builtin_bit_cast(unsigned, bf16x2_t{(bf16_t)v[2], (bf16_t)v[3]}))
+                                                                : make_uint2(__builtin_bit_cast(unsigned, f16x2_t{(f16_t)v[0], (f16_t)v[1]}), __builtin_bit_cast(unsigned, f16x2_t{(f16_t)v[2], (f16_t)v[3]}));
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (t < nv) {
+      if (a.out_dtype == FI_F32)
+        ((float*)a.out)[at + t] = a.accumulate ? ((float*)a.out)[at + t] + v[t] : v[t];
+      else if (a.out_dtype == FI_BF16)
+        ((bf16_t*)a.out)[at + t] = (bf16_t)v[t];
+      else
+        ((f16_t*)a.out)[at + t] = (f16_t)v[t];
+    }
+  }
+}
+
+template <typename T, int KD, bool DW>                                  // KD: 32 features each
+__global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
+  constexpr int S_BYTES = KD * 4096, T_BYTES = KD * 4096, X_BYTES = 1024, SLOT = S_BYTES + T_BYTES + X_BYTES;   // rows, turned, table or bias
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef __attribute__((address_space(3))) char* lds_ptr_t;
+  typedef typename DT<T>::frag_t frag_t;
+  const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr_t)smem;
+  const int n = a.s.count[0], M = DW ? a.V : n, S = DW ? n : a.V, D = a.out.N;
+  int ti, sp;
+  if (!ce_tile((M + 255) / 256, a.out.splits, ti, sp)) return;
+  const int tiles = (S + 63) / 64, per = (tiles + a.out.splits - 1) / a.out.splits, t0 = sp * per < tiles ? sp * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), l = threadIdx.x & 63, lr = l & 15, g = l >> 4;
+  const int o0 = ti * 256 + w * 32;
+
+  // DMA: waves 0 .. 3 fetch the rows (8 rows of 128 bytes per instruction), 4 .. 7 the turned ones, wave 0 also the table's 1 KB (the bias' 256 bytes)
+  const bool isT = w >= 4;
+  unsigned voff[KD];
+#pragma unroll
+  for (int q = 0; q < KD; ++q) {
+    const int id = (w & 3) * KD + q;
+    if (isT) {
+      const int r = id * 8 + (l >> 3);
+      voff[q] = (unsigned)(r < D ? r : D - 1) * (unsigned)(a.ld_turned * 2) + (unsigned)(((l & 7) ^ (l >> 3)) * 16);
+    } else {
+      const int r = (id & 7) * 8 + (l >> 3);
+      voff[q] = (unsigned)r * (unsigned)(a.ld_tile * 2) + (unsigned)((id >> 3) * 128 + (((l & 7) ^ (((l >> 3) & 3) | ((id & 1) << 2))) * 16));
+    }
+  }
+  auto fetch = [&](int t, int slot) {
+    const unsigned base = lds0 + (unsigned)(slot * SLOT);
+    if (isT) {
+      const nt_v4i rs = nt_rsrc(a.turned + (i64)t * 64, ((unsigned long long)(D - 1) * a.ld_turned + 64) * 2);
+#pragma unroll
+      for (int q = 0; q < KD; ++q) nt_dma16(rs, base + (unsigned)(S_BYTES + ((w & 3) * KD + q) * 1024), voff[q], 0u);
+    } else {
+      // (rows behind the last one lie beyond the resource: zeros)
+      const nt_v4i rs = nt_rsrc((const T*)a.tile + (i64)t * 64 * a.ld_tile, ((unsigned long long)(S - t * 64 - 1) * a.ld_tile + KD * 32) * 2);
+#pragma unroll
+      for (int q = 0; q < KD; ++q) nt_dma16(rs, base + (unsigned)(((w & 3) * KD + q) * 1024), voff[q], 0u);
+      if (w == 0) {
+        const nt_v4i rx = DW ? nt_rsrc(a.meta + (i64)t * 64, 1024) : nt_rsrc(a.bias + (i64)t * 64, 256);
+        nt_dma16(rx, base + (unsigned)(S_BYTES + T_BYTES), (unsigned)(l * 16), 0u);
+      }
+    }
+  };
+  if (t0 < t1) fetch(t0, 0);
+
+  // own rows
+  frag_t own[2][KD];
+  float m2[2], y[2], gg[2], b[2], cs[2] = {0.f, 0.f};
+  int lab[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int o = o0 + i * 16 + lr, oc = o < M ? o : M - 1;
+#pragma unroll
+    for (int k = 0; k < KD; ++k) own[i][k] = *(const frag_t*)((const T*)a.own + (i64)oc * a.ld_own + k * 32 + g * 8);
+    m2[i] = y[i] = gg[i] = b[i] = 0.f, lab[i] = -1;
+    if constexpr (DW) {
+      b[i] = a.bias[oc];
+    } else {
+      const float4 m = a.meta[oc];
+      m2[i] = m.x, y[i] = m.y, gg[i] = m.z, lab[i] = __float_as_int(m.w);
+    }
+  }
+  f32x4 acc[2][2 * KD];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int d = 0; d < 2 * KD; ++d) acc[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int t = t0; t < t1; ++t) {
+    const int slot = (t - t0) & 1;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 1 < t1) fetch(t + 1, slot ^ 1);
+    const char* const sm = smem + slot * SLOT;
+    const float4* const xm = (const float4*)(sm + S_BYTES + T_BYTES);
+    f32x4 z[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DW) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) z[i][j] = f32x4{b[i], b[i], b[i], b[i]};
+      } else {
+        const float4 c = xm[8 * (j >> 1) + 2 * g + (j & 1)];              // classes 32 (j / 2) + 8 g + 4 (j % 2) ..
+#pragma unroll
+        for (int i = 0; i < 2; ++i) z[i][j] = f32x4{c.x, c.y, c.z, c.w};
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KD; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 32 * (j >> 1) + 8 * (lr >> 2) + 4 * (j & 1) + (lr & 3), c = (k & 1) * 4 + g;
+        const frag_t f = *(const frag_t*)(sm + (k >> 1) * 8192 + r * 128 + ((c ^ ((r & 3) | ((r >> 1) & 4))) * 16));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) z[i][j] = mfma16(f, own[i][k], z[i][j]);
+      }
+    if constexpr (DW) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float4 m = xm[32 * (j >> 1) + 8 * g + 4 * (j & 1) + r];
+          const int cls = __float_as_int(m.w) - o0 - lr;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float v = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j][r], CE_LOG2E, -m.x)) * m.y;
+            v -= cls == i * 16 ? m.z : 0.f;
+            cs[i] += v;
+            z[i][j][r] = v;
+          }
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) z[i][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j][r], CE_LOG2E, -m2[i])) * y[i];
+        const int c = lab[i] - t * 64;
+        if ((unsigned)c < 64u) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[i][j][r] -= c == 32 * (j >> 1) + 8 * g + 4 * (j & 1) + r ? gg[i] : 0.f;
+        }
+      }
+      if (t * 64 + 64 > S) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (t * 64 + 32 * (j >> 1) + 8 * g + 4 * (j & 1) + r >= S) z[0][j][r] = z[1][j][r] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      f16x8 gf[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) gf[i][e] = (f16_t)z[i][2 * q][e], gf[i][4 + e] = (f16_t)z[i][2 * q + 1][e];
+#pragma unroll
+      for (int d = 0; d < 2 * KD; ++d) {
+        const int r = d * 16 + lr;
+        const f16x8 f = *(const f16x8*)(sm + S_BYTES + r * 128 + (((q * 4 + g) ^ (r & 7)) * 16));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][d] = mfma16(f, gf[i], acc[i][d]);
+      }
+    }
+  }
+
+  const float rg = a.out.scal[SC_RG], rb = ce_rscale(a.out);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int o = o0 + i * 16 + lr;
+    if constexpr (DW) {
+      cs[i] += __shfl_xor(cs[i], 16, 64);
+      cs[i] += __shfl_xor(cs[i], 32, 64);
+      if (a.db && g == 0 && o < M) a.db[(i64)sp * a.V + o] = cs[i];
+      if (!a.out.out) continue;
+    }
+    if (o >= M) continue;
+    const i64 row = a.out.idx ? (i64)a.out.idx[o] : (i64)o;
+#pragma unroll
+    for (int d = 0; d < 2 * KD; ++d) {
+      const int c = d * 16 + 4 * g, nv = D - c < 4 ? D - c : 4;
+      if (nv <= 0) continue;
+      if (a.out.part) {
+        float* p = a.out.part + ((i64)sp * a.out.M + o) * D + c;
+        if ((D & 3) == 0) {
+          *(float4*)p = make_float4(acc[i][d][0], acc[i][d][1], acc[i][d][2], acc[i][d][3]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r < nv) p[r] = acc[i][d][r];
+        }
+      } else {
+        const float v[4] = {acc[i][d][0] * rg * rb, acc[i][d][1] * rg * rb, acc[i][d][2] * rg * rb, acc[i][d][3] * rg * rb};
+        ce_put4(a.out, row, c, v, nv);
+      }
+    }
   }
 }
 
@@ -940,13 +1181,26 @@ CeGradPlan ce_grad_plan(i64 M, i64 N, i64 K, int ku, bool pieces) {
   return p;
 }
 struct CeBwdWs {
-  float *parts, *scal, *g, *db, *pdx, *pdw;
+  float *parts, *scal, *g, *db, *pdx, *pdw, *bias_pad;
+  float4* meta;
+  bool fused;
+  int sdx, sdw;
   f16_t *xc, *wc, *xt, *wt, *dl, *dlt;
   i64 ld_xt, ld_wt, ld_dl, ld_dlt, Tc;
   int Vc;
   CeGradPlan dx, dw;
   i64 pdw_piece, bytes;
 };
+// G stays in registers (ce_fused_kernel) for 16-bit operands of up to 128 features; rows up to where a turned operand's offsets fit 32 bits
+bool ce_fused_ok(const FiLinearCe& d, const CeShape& s) { return !s.pair && s.kp <= 128 && d.T <= (1 << 23); }
+// parts of the streamed side: enough workgroups (of 256 own rows) to fill the chip twice, no fewer than 8 tiles of 64 each
+int ce_fused_splits(i64 own, i64 streamed) {
+  const i64 wgs = (own + 255) / 256, tiles = (streamed + 63) / 64;
+  i64 s = 512 / wgs;
+  if (s > tiles / 8) s = tiles / 8;
+  if (s > 256) s = 256;
+  return s < 1 ? 1 : (int)s;
+}
 constexpr i64 CE_PIECE = 1LL << 27;              // values of G held at a time (two orientations: 512 MiB; twice that for pairs)
 CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need_dw, bool need_db, void* p) {
   Carve c{(char*)p};
@@ -961,6 +1215,23 @@ CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need
   w.parts = c.take<float>(2 * CE_PARTS);
   w.scal = c.take<float>(SC_N);
   w.g = c.take<float>(d.T);
+  w.meta = nullptr, w.bias_pad = nullptr;
+  w.fused = ce_fused_ok(d, s);
+  if (w.fused) {
+    w.sdx = ce_fused_splits(d.T, d.V), w.sdw = ce_fused_splits(d.V, d.T);
+    w.ld_xt = Tp, w.ld_wt = Vp, w.Tc = Tp;
+    w.meta = c.take<float4>(ce_up(d.T, 64));
+    w.bias_pad = c.take<float>(ce_up(d.V, 64));
+    w.db = need_db ? c.take<float>((i64)w.sdw * d.V) : nullptr;
+    w.xc = c.take<f16_t>(d.T * s.ldx);
+    w.wc = s.w_direct ? nullptr : c.take<f16_t>((i64)d.V * s.ldx);
+    w.xt = need_dw || need_db ? c.take<f16_t>(d.D * w.ld_xt) : nullptr;
+    w.wt = need_dx ? c.take<f16_t>(d.D * w.ld_wt) : nullptr;
+    w.pdx = need_dx && w.sdx > 1 ? c.take<float>((i64)w.sdx * d.T * d.D) : nullptr;
+    w.pdw = need_dw && w.sdw > 1 ? c.take<float>((i64)w.sdw * d.V * d.D) : nullptr;
+    w.bytes = c.at;
+    return w;
+  }
   const int bm = CE_BM[ce_logits_tile(d)];
   w.db = need_db ? c.take<float>((d.T + bm - 1) / bm * d.V) : nullptr;
   w.xc = c.take<f16_t>(d.T * s.ldx);
@@ -977,6 +1248,22 @@ CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need
   w.pdw = need_dw && w.dw.part ? c.take<float>(w.pdw_piece * (w.Tc < d.T ? (d.V + w.Vc - 1) / w.Vc : 1)) : nullptr;
   w.bytes = c.at;
   return w;
+}
+
+template <typename T, int KD, bool DW>
+int ce_launch_fused(const CeFused& a, hipStream_t st) {
+  constexpr int lds = 2 * (KD * 8192 + 1024);
+  static const bool ok = nt_allow_lds((const void*)ce_fused_kernel<T, KD, DW>);
+  if (!ok) return FI_ERR_UNSUPPORTED;
+  const i64 n = (i64)((a.out.M + 255) / 256) * a.out.splits;
+  hipLaunchKernelGGL((ce_fused_kernel<T, KD, DW>), dim3((unsigned)ce_up(n, 8)), dim3(512), lds, st, a);
+  FI_CHECK_LAUNCH();
+  return 0;
+}
+template <bool DW>
+int ce_fused(const CeFused& a, const FiLinearCe& d, int kp, hipStream_t st) {
+  if (d.dtype == FI_BF16) return kp <= 64 ? ce_launch_fused<bf16_t, 2, DW>(a, st) : ce_launch_fused<bf16_t, 4, DW>(a, st);
+  return kp <= 64 ? ce_launch_fused<f16_t, 2, DW>(a, st) : ce_launch_fused<f16_t, 4, DW>(a, st);
 }
 
 template <class Core, bool PAIR>
@@ -1087,7 +1374,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
     FI_CHECK_LAUNCH();
   }
   const i64 ng = (d->T + 255) / 256;
-  hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)ng), dim3(256), 0, st, gloss, d->reduction, ws.parts, sv, (int)s.pair, ws.scal, ws.g, labels,
+  hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)ng), dim3(256), 0, st, gloss, d->reduction, ws.parts, sv, (int)s.pair, ws.scal, ws.g, ws.meta, bias, d->V, ws.bias_pad, labels,
                      d->ltype, (i64)d->T, (i64)d->ignore_index, (char*)dx, (i64)d->D * (s.pair ? 4 : 2));
   FI_CHECK_LAUNCH();
   const int f = s.pair ? 2 : 1;
@@ -1096,6 +1383,30 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   gx.splits = ws.dx.splits, gx.out = dx, gx.out_dtype = d->dtype, gx.ldo = d->D, gx.idx = sv.idx, gx.scal = ws.scal, gx.rscale = s.scaled ? SC_RW : -1;
   gw.a = ws.dlt, gw.lda = ws.ld_dlt, gw.ldb = ws.ld_xt, gw.N = d->D, gw.count = sv.count;
   gw.splits = ws.dw.splits, gw.out_dtype = d->wdtype, gw.accumulate = dw_accumulate, gw.ldo = d->D, gw.scal = ws.scal, gw.rscale = s.scaled ? SC_RX : -1;
+  if (ws.fused) {
+    const void* const wop = s.w_direct ? w : (const void*)ws.wc;
+    CeFused a = {};
+    a.s = sv, a.meta = ws.meta, a.bias = ws.bias_pad, a.V = d->V;
+    if (dx) {
+      gx.vec = d->D % 4 == 0 && ((uintptr_t)dx & 15) == 0, gx.splits = ws.sdx, gx.part = ws.pdx, gx.M = (int)d->T, gx.Tc = d->T;
+      a.out = gx, a.own = ws.xc, a.ld_own = s.ldx, a.tile = wop, a.ld_tile = s.ldw, a.turned = ws.wt, a.ld_turned = ws.ld_wt;
+      if ((rc = ce_fused<false>(a, *d, s.kp, st))) return rc;
+      gx.vec = d->D % 8 == 0 && ((uintptr_t)dx & 15) == 0;              // (the join stores 8 at a time)
+      if (gx.part && (rc = ce_join(gx, st))) return rc;
+    }
+    if (dw || db) {
+      gw.vec = d->D % 4 == 0 && ((uintptr_t)dw & 15) == 0, gw.splits = ws.sdw, gw.part = ws.pdw, gw.M = d->V, gw.Tc = d->T, gw.out = dw;
+      a.out = gw, a.own = wop, a.ld_own = s.ldw, a.tile = ws.xc, a.ld_tile = s.ldx, a.turned = ws.xt, a.ld_turned = ws.ld_xt, a.db = ws.db;
+      if ((rc = ce_fused<true>(a, *d, s.kp, st))) return rc;
+      gw.vec = d->D % 8 == 0 && ((uintptr_t)dw & 15) == 0;
+      if (gw.part && (rc = ce_join(gw, st))) return rc;
+    }
+    if (db) {
+      hipLaunchKernelGGL(ce_dbias_kernel, dim3((unsigned)((d->V + 15) / 16)), dim3(1024), 0, st, ws.db, 1, ws.sdw, d->V, sv.count, ws.scal, db, db_accumulate);
+      FI_CHECK_LAUNCH();
+    }
+    return 0;
+  }
   gx.vec = d->D % 8 == 0 && ((uintptr_t)dx & 15) == 0, gw.vec = d->D % 8 == 0 && ((uintptr_t)dw & 15) == 0;
   CeLogits a = {};
   a.x = ws.xc, a.ldx = s.ldx, a.w = s.w_direct ? w : ws.wc, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
@@ -1128,7 +1439,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
     }
   }
   if (db) {
-    hipLaunchKernelGGL(ce_dbias_kernel, dim3((unsigned)((d->V + 15) / 16)), dim3(1024), 0, st, ws.db, CE_BM[ce_logits_tile(*d)], d->V, sv.count, ws.scal, db, db_accumulate);
+    hipLaunchKernelGGL(ce_dbias_kernel, dim3((unsigned)((d->V + 15) / 16)), dim3(1024), 0, st, ws.db, CE_BM[ce_logits_tile(*d)], 0, d->V, sv.count, ws.scal, db, db_accumulate);
     FI_CHECK_LAUNCH();
   }
   return 0;

@@ -421,3 +421,19 @@ def test_refusals_on_the_device():
     (g,) = torch.autograd.grad(ops.linear_ce_loss(xr, w, b, lab), xr, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,classes,width", [(5, 3, 4), (64, 64, 64), (65, 129, 65), (1000, 63, 12), (130, 4000, 128), (20000, 70, 24), (900, 20000, 100)])
+def test_linear_ce_narrow_features_keep_the_gradient_in_registers(dtype, rows, classes, width):
+    """Up to 128 features: either side streamed in tiles of 64, split or whole, tails on both sides, four or eight values to a vector or none."""
+    x, w, b, lab = _head(rows * 3 + classes, rows, classes, width, dtype, 0.1 if rows > 5 else 0.0)
+    lab[-1] = classes - 1
+    up = torch.full((), 64.0 if dtype == F16 else 1.0, device="cuda")
+    _, full = _ce_check(x, w, b, lab, above=up)
+    b2 = b.clone()
+    b2[0] = 90.0                                                      # a class whose exponential overflows without its row's maximum
+    _ce_check(x, w, b2, lab, above=up)
+    w32 = w.float().requires_grad_(True)                              # fp32 parameter: the gradient is added to, not rounded
+    ops.linear_ce_loss(x, w32, b, lab).backward()
+    assert w32.grad.dtype == F32 and torch.isfinite(w32.grad).all()
