@@ -73,9 +73,11 @@ __global__ __launch_bounds__(256) void ce_count_kernel(const void* labels, int l
 
 // each thread owns 8 consecutive rows; the workgroups before this one are summed again by every workgroup
 __global__ __launch_bounds__(256) void ce_gather_kernel(const void* labels, int ltype, i64 T, i64 ignore, int V, const int* cnt, CeSaved s,
-                                                        float* zt, float* rows_out) {
+                                                        float* zt, float* rows_out, const float* bias, float* bias_pad) {
   __shared__ int sm[256], base_sm[4];
   const int tid = threadIdx.x;
+  if (bias_pad)                                                         // (the streamed form reads it in whole tiles of 64 classes)
+    for (i64 v = (i64)blockIdx.x * 256 + tid; v < ((V + 63) & ~63); v += (i64)gridDim.x * 256) bias_pad[v] = bias && v < V ? bias[v] : 0.f;
   int before = 0;
   for (int k = tid; k < (int)blockIdx.x; k += 256) before += cnt[k];
 #pragma unroll
@@ -725,30 +727,40 @@ __global__ __launch_bounds__(Core::THREADS) void ce_grad_kernel(CeGrad a) {
     }
 }
 
-// joins the split parts of an output in their order
+// joins the split parts of an output: SUB lanes per 8 values, each over its share of the parts, then over the lanes -- a fixed order
+template <int SUB>
 __global__ __launch_bounds__(256) void ce_join_kernel(CeGrad a) {
   const i64 left = (i64)a.count[0] - a.t0;
   const i64 M = a.rows_are_tokens ? (left < 0 ? 0 : left < a.Tc ? left : a.Tc) : a.M;
   const i64 nv = (a.N + 7) / 8, total = M * nv;
   const float rg = a.scal[SC_RG], rb = ce_rscale(a);
-  for (i64 e = (i64)blockIdx.x * 256 + threadIdx.x; e < total; e += (i64)gridDim.x * 256) {
-    const i64 r = e / nv;
+  const int sub = threadIdx.x % SUB;
+  for (i64 e0 = (i64)blockIdx.x * (256 / SUB); e0 < total; e0 += (i64)gridDim.x * (256 / SUB)) {
+    const i64 e = e0 + threadIdx.x / SUB, r = e / nv;
     const int k = (int)(e - r * nv) * 8, n = a.N - k < 8 ? a.N - k : 8;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-      const float* p = a.part + ((i64)s * a.M + r) * a.N + k;
-      if ((a.N & 7) == 0) {
-        const float4 x = ((const float4*)p)[0], y = ((const float4*)p)[1];
-        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
-      } else {
+    if (e < total) {
+      for (int s = sub; s < a.splits; s += SUB) {
+        const float* p = a.part + ((i64)s * a.M + r) * a.N + k;
+        if ((a.N & 7) == 0) {
+          const float4 x = ((const float4*)p)[0], y = ((const float4*)p)[1];
+          v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+        } else {
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
-          if (t < n) v[t] += p[t];
+          for (int t = 0; t < 8; ++t)
+            if (t < n) v[t] += p[t];
+        }
       }
     }
 #pragma unroll
-    for (int t = 0; t < 8; ++t) v[t] = v[t] * rg * rb;
-    ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : r, k, v, n);
+    for (int o = SUB / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] += __shfl_xor(v[t], o, 64);
+    if (e < total && sub == 0) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] = v[t] * rg * rb;
+      ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : r, k, v, n);
+    }
   }
 }
 
@@ -772,14 +784,14 @@ __global__ __launch_bounds__(1024) void ce_dbias_kernel(const float* part, int t
   }
 }
 
-// ---- the backward pass of narrow operands: G stays in registers ------------------------------------------------------------------------
+// ---- narrow operands: logits and G stay in registers -------------------------------------------------------------------------------------
 // With up to 128 features the two gradient products do less work per value of G than writing and reading it costs (2 x 4 bytes against 4 D
 // operations), so each makes its own G.  A wave owns 32 rows -- tokens for dx, classes for dW (DW) -- whose operand fragments stay in registers; the
 // other side is streamed through LDS in tiles of 64, once as rows [64][K] for the logits and once turned, [D][64], for the product with G.
 // G never leaves the lane that made it: the matrix instruction returns 4 consecutive rows of its first operand per lane, so if fragment row i of
 // tile j is taken from streamed row 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4, a lane's results of two tiles are 8 consecutive streamed rows
 // -- exactly the fragment that the next product wants from it.  (Pieces of a row are swizzled by (row & 3) | (row / 8 & 1) * 4, which is free of
-// bank conflicts under that order.)
+// bank conflicts under that order.)  The forward pass of such operands streams the classes the same way and keeps each row's running maximum and sum.
 struct CeFused {
   CeGrad out;
   CeSaved s;
@@ -790,6 +802,8 @@ struct CeFused {
   const float4* meta;      // per token: maximum * log2 e, factor / sum, factor, label
   const float* bias;       // padded to 64 classes (zeros without a bias)
   float* db;               // DW: [split][V] partial sums, or NULL
+  float2* part;            // FWD: [row][split] maximum and sum
+  float* zt;               // FWD: the label's logit
   int V;
 };
 
@@ -816,14 +830,16 @@ __device__ __forceinline__ void ce_put4(const CeGrad& a, i64 row, int col, const
   }
 }
 
-template <typename T, int KD, bool DW>                                  // KD: 32 features each
+enum { CE_DX, CE_DW, CE_FWD };
+template <typename T, int KD, int MODE>                                 // KD: 32 features each
 __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
-  constexpr int S_BYTES = KD * 4096, T_BYTES = KD * 4096, X_BYTES = 1024, SLOT = S_BYTES + T_BYTES + X_BYTES;   // rows, turned, table or bias
+  constexpr bool DW = MODE == CE_DW, FWD = MODE == CE_FWD;
+  constexpr int S_BYTES = KD * 4096, T_BYTES = FWD ? 0 : KD * 4096, X_BYTES = 1024, SLOT = S_BYTES + T_BYTES + X_BYTES;   // rows, turned, table or bias
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef __attribute__((address_space(3))) char* lds_ptr_t;
   typedef typename DT<T>::frag_t frag_t;
   const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr_t)smem;
-  const int n = a.s.count[0], M = DW ? a.V : n, S = DW ? n : a.V, D = a.out.N;
+  const int n = a.s.count[0], M = DW ? a.V : n, S = DW ? n : a.V, D = FWD ? 1 : a.out.N;
   int ti, sp;
   if (!ce_tile((M + 255) / 256, a.out.splits, ti, sp)) return;
   const int tiles = (S + 63) / 64, per = (tiles + a.out.splits - 1) / a.out.splits, t0 = sp * per < tiles ? sp * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
@@ -831,11 +847,14 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
   const int o0 = ti * 256 + w * 32;
 
   // DMA: waves 0 .. 3 fetch the rows (8 rows of 128 bytes per instruction), 4 .. 7 the turned ones, wave 0 also the table's 1 KB (the bias' 256 bytes)
-  const bool isT = w >= 4;
-  unsigned voff[KD];
+  // (forward: all eight the rows)
+  constexpr int Q = FWD ? KD / 2 : KD;
+  const bool isT = !FWD && w >= 4;
+  const int wq = FWD ? w : w & 3;
+  unsigned voff[Q];
 #pragma unroll
-  for (int q = 0; q < KD; ++q) {
-    const int id = (w & 3) * KD + q;
+  for (int q = 0; q < Q; ++q) {
+    const int id = wq * Q + q;
     if (isT) {
       const int r = id * 8 + (l >> 3);
       voff[q] = (unsigned)(r < D ? r : D - 1) * (unsigned)(a.ld_turned * 2) + (unsigned)(((l & 7) ^ (l >> 3)) * 16);
@@ -849,12 +868,12 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
     if (isT) {
       const nt_v4i rs = nt_rsrc(a.turned + (i64)t * 64, ((unsigned long long)(D - 1) * a.ld_turned + 64) * 2);
 #pragma unroll
-      for (int q = 0; q < KD; ++q) nt_dma16(rs, base + (unsigned)(S_BYTES + ((w & 3) * KD + q) * 1024), voff[q], 0u);
+      for (int q = 0; q < Q; ++q) nt_dma16(rs, base + (unsigned)(S_BYTES + (wq * Q + q) * 1024), voff[q], 0u);
     } else {
       // (rows behind the last one lie beyond the resource: zeros)
       const nt_v4i rs = nt_rsrc((const T*)a.tile + (i64)t * 64 * a.ld_tile, ((unsigned long long)(S - t * 64 - 1) * a.ld_tile + KD * 32) * 2);
 #pragma unroll
-      for (int q = 0; q < KD; ++q) nt_dma16(rs, base + (unsigned)(((w & 3) * KD + q) * 1024), voff[q], 0u);
+      for (int q = 0; q < Q; ++q) nt_dma16(rs, base + (unsigned)((wq * Q + q) * 1024), voff[q], 0u);
       if (w == 0) {
         const nt_v4i rx = DW ? nt_rsrc(a.meta + (i64)t * 64, 1024) : nt_rsrc(a.bias + (i64)t * 64, 256);
         nt_dma16(rx, base + (unsigned)(S_BYTES + T_BYTES), (unsigned)(l * 16), 0u);
@@ -875,6 +894,9 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
     m2[i] = y[i] = gg[i] = b[i] = 0.f, lab[i] = -1;
     if constexpr (DW) {
       b[i] = a.bias[oc];
+    } else if constexpr (FWD) {
+      lab[i] = o < M ? a.s.lab[oc] : -1;
+      m2[i] = -INFINITY;                                                // the running maximum; y: the running sum
     } else {
       const float4 m = a.meta[oc];
       m2[i] = m.x, y[i] = m.y, gg[i] = m.z, lab[i] = __float_as_int(m.w);
@@ -913,7 +935,37 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) z[i][j] = mfma16(f, own[i][k], z[i][j]);
       }
-    if constexpr (DW) {
+    if constexpr (FWD) {
+      if (t * 64 + 64 > S) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (t * 64 + 32 * (j >> 1) + 8 * g + 4 * (j & 1) + r >= S) z[0][j][r] = z[1][j][r] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = lab[i] - t * 64;
+        if ((unsigned)c < 64u) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (c == 32 * (j >> 1) + 8 * g + 4 * (j & 1) + r) a.zt[o0 + i * 16 + lr] = z[i][j][r];
+        }
+        float top = m2[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(fmaxf(top, fmaxf(z[i][j][0], z[i][j][1])), fmaxf(z[i][j][2], z[i][j][3]));
+        const float safe = (top == -INFINITY ? 0.f : top) * CE_LOG2E;
+        float sum = y[i] * __builtin_amdgcn_exp2f(__builtin_fmaf(m2[i], CE_LOG2E, -safe));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j][r], CE_LOG2E, -safe));
+        m2[i] = top, y[i] = sum;
+      }
+      continue;
+    } else if constexpr (DW) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -968,6 +1020,20 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
     }
   }
 
+  if constexpr (FWD) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float m = fmaxf(m2[i], __shfl_xor(m2[i], 16, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float safe = m == -INFINITY ? 0.f : m;
+      float sum = y[i] * __builtin_amdgcn_exp2f((m2[i] - safe) * CE_LOG2E);
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      const int o = o0 + i * 16 + lr;
+      if (g == 0 && o < M) a.part[(i64)o * a.out.splits + sp] = make_float2(m, sum);
+    }
+    return;
+  }
   const float rg = a.out.scal[SC_RG], rb = ce_rscale(a.out);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -1121,9 +1187,38 @@ int ce_amax(const FiLinearCe& d, const void* x, const void* w, const CeSaved& s,
   return 0;
 }
 
+// Logits and G stay in registers (ce_fused_kernel) for 16-bit operands of up to 128 features; rows up to where a turned operand's offsets fit 32 bits
+bool ce_fused_ok(const FiLinearCe& d, const CeShape& s) { return !s.pair && s.kp <= 128 && d.T <= (1 << 23); }
+// (up to 64 rows the 64 x 256 tiles of the general product read the classes with more workgroups)
+bool ce_fused_fwd_ok(const FiLinearCe& d, const CeShape& s) { return ce_fused_ok(d, s) && d.T > 64; }
+// parts of the streamed side: enough workgroups (of 256 own rows) to fill the chip twice, no fewer than 8 tiles of 64 each
+int ce_fused_splits(i64 own, i64 streamed) {
+  const i64 wgs = (own + 255) / 256, tiles = (streamed + 63) / 64;
+  i64 s = 512 / wgs;
+  if (s > tiles / 8) s = tiles / 8;
+  if (s > 256) s = 256;
+  return s < 1 ? 1 : (int)s;
+}
+template <typename T, int KD, int MODE>
+int ce_launch_fused(const CeFused& a, hipStream_t st) {
+  constexpr int lds = 2 * (KD * (MODE == CE_FWD ? 4096 : 8192) + 1024);
+  static const bool ok = nt_allow_lds((const void*)ce_fused_kernel<T, KD, MODE>);
+  if (!ok) return FI_ERR_UNSUPPORTED;
+  const i64 n = (i64)((a.out.M + 255) / 256) * a.out.splits;
+  hipLaunchKernelGGL((ce_fused_kernel<T, KD, MODE>), dim3((unsigned)ce_up(n, 8)), dim3(512), lds, st, a);
+  FI_CHECK_LAUNCH();
+  return 0;
+}
+template <int MODE>
+int ce_fused(const CeFused& a, const FiLinearCe& d, int kp, hipStream_t st) {
+  if (d.dtype == FI_BF16) return kp <= 64 ? ce_launch_fused<bf16_t, 2, MODE>(a, st) : ce_launch_fused<bf16_t, 4, MODE>(a, st);
+  return kp <= 64 ? ce_launch_fused<f16_t, 2, MODE>(a, st) : ce_launch_fused<f16_t, 4, MODE>(a, st);
+}
+
 struct CeFwdWs {
   int* cnt;
-  float *parts, *zt;
+  float *parts, *zt, *bias_pad;
+  int nparts;              // of a row's statistics
   f16_t *xc, *wc;
   float2* part;
   double* sums;
@@ -1138,7 +1233,11 @@ CeFwdWs ce_fwd_ws(const FiLinearCe& d, const CeShape& s, void* p) {
   w.sums = c.take<double>(CE_LOSS_WGS);
   w.xc = c.take<f16_t>(d.T * s.ldx);
   w.wc = s.w_direct ? nullptr : c.take<f16_t>((i64)d.V * s.ldx);
-  w.part = c.take<float2>(d.T * ((d.V + CE_BN[ce_logits_tile(d)] - 1) / CE_BN[ce_logits_tile(d)]));
+  const bool fused = ce_fused_fwd_ok(d, s);
+  const int bn = CE_BN[ce_logits_tile(d)];
+  w.nparts = fused ? ce_fused_splits(d.T, d.V) : (d.V + bn - 1) / bn;
+  w.bias_pad = fused ? c.take<float>(ce_up(d.V, 64)) : nullptr;
+  w.part = c.take<float2>(d.T * w.nparts);
   w.bytes = c.at;
   return w;
 }
@@ -1191,16 +1290,6 @@ struct CeBwdWs {
   CeGradPlan dx, dw;
   i64 pdw_piece, bytes;
 };
-// G stays in registers (ce_fused_kernel) for 16-bit operands of up to 128 features; rows up to where a turned operand's offsets fit 32 bits
-bool ce_fused_ok(const FiLinearCe& d, const CeShape& s) { return !s.pair && s.kp <= 128 && d.T <= (1 << 23); }
-// parts of the streamed side: enough workgroups (of 256 own rows) to fill the chip twice, no fewer than 8 tiles of 64 each
-int ce_fused_splits(i64 own, i64 streamed) {
-  const i64 wgs = (own + 255) / 256, tiles = (streamed + 63) / 64;
-  i64 s = 512 / wgs;
-  if (s > tiles / 8) s = tiles / 8;
-  if (s > 256) s = 256;
-  return s < 1 ? 1 : (int)s;
-}
 constexpr i64 CE_PIECE = 1LL << 27;              // values of G held at a time (two orientations: 512 MiB; twice that for pairs)
 CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need_dw, bool need_db, void* p) {
   Carve c{(char*)p};
@@ -1250,21 +1339,6 @@ CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need
   return w;
 }
 
-template <typename T, int KD, bool DW>
-int ce_launch_fused(const CeFused& a, hipStream_t st) {
-  constexpr int lds = 2 * (KD * 8192 + 1024);
-  static const bool ok = nt_allow_lds((const void*)ce_fused_kernel<T, KD, DW>);
-  if (!ok) return FI_ERR_UNSUPPORTED;
-  const i64 n = (i64)((a.out.M + 255) / 256) * a.out.splits;
-  hipLaunchKernelGGL((ce_fused_kernel<T, KD, DW>), dim3((unsigned)ce_up(n, 8)), dim3(512), lds, st, a);
-  FI_CHECK_LAUNCH();
-  return 0;
-}
-template <bool DW>
-int ce_fused(const CeFused& a, const FiLinearCe& d, int kp, hipStream_t st) {
-  if (d.dtype == FI_BF16) return kp <= 64 ? ce_launch_fused<bf16_t, 2, DW>(a, st) : ce_launch_fused<bf16_t, 4, DW>(a, st);
-  return kp <= 64 ? ce_launch_fused<f16_t, 2, DW>(a, st) : ce_launch_fused<f16_t, 4, DW>(a, st);
-}
 
 template <class Core, bool PAIR>
 int ce_launch_grad(const CeGrad& a, hipStream_t st) {
@@ -1282,8 +1356,13 @@ int ce_grad(const CeGrad& a, int tile, hipStream_t st) {
                      : ce_launch_grad<NtCore<f16_t, PAIR, 64, 64, 32, 32, 3>, PAIR>(a, st);
 }
 int ce_join(const CeGrad& a, hipStream_t st) {
-  const i64 n = ((i64)a.M * ((a.N + 7) / 8) + 255) / 256;
-  hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)(n < 4096 ? n : 4096)), dim3(256), 0, st, a);
+  const int sub = a.splits >= 32 ? 16 : 1;
+  const i64 n = ((i64)a.M * ((a.N + 7) / 8) * sub + 255) / 256;
+  const unsigned grid = (unsigned)(n < 4096 ? n : 4096);
+  if (sub == 16)
+    hipLaunchKernelGGL(ce_join_kernel<16>, dim3(grid), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL(ce_join_kernel<1>, dim3(grid), dim3(256), 0, st, a);
   FI_CHECK_LAUNCH();
   return 0;
 }
@@ -1313,28 +1392,35 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
     hipLaunchKernelGGL(ce_count_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, ws.cnt);
     FI_CHECK_LAUNCH();
   }
-  hipLaunchKernelGGL(ce_gather_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, d->V, ws.cnt, sv, ws.zt, rows_out);
+  hipLaunchKernelGGL(ce_gather_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, d->V, ws.cnt, sv, ws.zt, rows_out, bias, ws.bias_pad);
   FI_CHECK_LAUNCH();
   if (s.pair && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
   float* const scal = s.pair ? sv.scal : nullptr;
   if ((rc = ce_pack(ce_pack_x(*d, s, x, sv, ws.parts, scal, ws.xc), s.w_direct ? CePack{} : ce_pack_w(*d, s, w, ws.parts, scal, ws.wc), st))) return rc;
-  CeLogits a = {};
-  const int bn = CE_BN[ce_logits_tile(*d)];
-  a.x = ws.xc, a.ldx = s.ldx, a.w = s.w_direct ? w : ws.wc, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
-  a.scal = scal, a.s = sv, a.part = ws.part, a.zt = ws.zt, a.ntj = (d->V + bn - 1) / bn;
-  if ((rc = ce_logits_any(a, *d, true, st))) return rc;
-  const int lanes = a.ntj > 32 ? 64 : a.ntj > 4 ? 8 : 1;
+  const void* const wop = s.w_direct ? w : (const void*)ws.wc;
+  if (ce_fused_fwd_ok(*d, s)) {
+    CeFused a = {};
+    a.out.M = (int)d->T, a.out.splits = ws.nparts, a.s = sv, a.own = ws.xc, a.ld_own = s.ldx, a.tile = wop, a.ld_tile = s.ldw;
+    a.bias = ws.bias_pad, a.V = d->V, a.part = ws.part, a.zt = ws.zt;
+    if ((rc = ce_fused<CE_FWD>(a, *d, s.kp, st))) return rc;
+  } else {
+    CeLogits a = {};
+    a.x = ws.xc, a.ldx = s.ldx, a.w = wop, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
+    a.scal = scal, a.s = sv, a.part = ws.part, a.zt = ws.zt, a.ntj = ws.nparts;
+    if ((rc = ce_logits_any(a, *d, true, st))) return rc;
+  }
+  const int lanes = ws.nparts > 32 ? 64 : ws.nparts > 4 ? 8 : 1;
   i64 g = (d->T * lanes + 255) / 256;
   if (g > CE_LOSS_WGS) g = CE_LOSS_WGS;
   if (g <= (lanes == 1 ? 16 : 2)) g = 1;                                // (short: one workgroup also writes the loss)
   float* const alone = g == 1 && d->reduction != 0 ? loss : nullptr;
   const int mean = d->reduction == 1;
   if (lanes == 64)
-    hipLaunchKernelGGL(ce_rows_kernel<64>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums, mean, alone);
+    hipLaunchKernelGGL(ce_rows_kernel<64>, dim3((unsigned)g), dim3(256), 0, st, ws.part, ws.nparts, ws.zt, sv, rows_out, ws.sums, mean, alone);
   else if (lanes == 8)
-    hipLaunchKernelGGL(ce_rows_kernel<8>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums, mean, alone);
+    hipLaunchKernelGGL(ce_rows_kernel<8>, dim3((unsigned)g), dim3(256), 0, st, ws.part, ws.nparts, ws.zt, sv, rows_out, ws.sums, mean, alone);
   else
-    hipLaunchKernelGGL(ce_rows_kernel<1>, dim3((unsigned)g), dim3(256), 0, st, ws.part, a.ntj, ws.zt, sv, rows_out, ws.sums, mean, alone);
+    hipLaunchKernelGGL(ce_rows_kernel<1>, dim3((unsigned)g), dim3(256), 0, st, ws.part, ws.nparts, ws.zt, sv, rows_out, ws.sums, mean, alone);
   FI_CHECK_LAUNCH();
   if (d->reduction != 0 && !alone) {
     hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(256), 0, st, ws.sums, (int)g, sv.count, mean, loss);
@@ -1390,14 +1476,14 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
     if (dx) {
       gx.vec = d->D % 4 == 0 && ((uintptr_t)dx & 15) == 0, gx.splits = ws.sdx, gx.part = ws.pdx, gx.M = (int)d->T, gx.Tc = d->T;
       a.out = gx, a.own = ws.xc, a.ld_own = s.ldx, a.tile = wop, a.ld_tile = s.ldw, a.turned = ws.wt, a.ld_turned = ws.ld_wt;
-      if ((rc = ce_fused<false>(a, *d, s.kp, st))) return rc;
+      if ((rc = ce_fused<CE_DX>(a, *d, s.kp, st))) return rc;
       gx.vec = d->D % 8 == 0 && ((uintptr_t)dx & 15) == 0;              // (the join stores 8 at a time)
       if (gx.part && (rc = ce_join(gx, st))) return rc;
     }
     if (dw || db) {
       gw.vec = d->D % 4 == 0 && ((uintptr_t)dw & 15) == 0, gw.splits = ws.sdw, gw.part = ws.pdw, gw.M = d->V, gw.Tc = d->T, gw.out = dw;
       a.out = gw, a.own = wop, a.ld_own = s.ldw, a.tile = ws.xc, a.ld_tile = s.ldx, a.turned = ws.xt, a.ld_turned = ws.ld_xt, a.db = ws.db;
-      if ((rc = ce_fused<true>(a, *d, s.kp, st))) return rc;
+      if ((rc = ce_fused<CE_DW>(a, *d, s.kp, st))) return rc;
       gw.vec = d->D % 8 == 0 && ((uintptr_t)dw & 15) == 0;
       if (gw.part && (rc = ce_join(gw, st))) return rc;
     }
