@@ -108,8 +108,9 @@ __device__ __host__ __forceinline__ long ns_items(const NsItem& q, int kind, int
   return kind == NS_SUMS ? ns_sums(q) : kind == NS_A ? tri * q.split : kind == NS_JOIN ? (q.split > 1 ? tri : 0)
          : kind == NS_S ? tri : kind == NS_NARROW ? ns_chunks(q.n) : mt * nt;
 }
-__device__ __host__ __forceinline__ int ns_tile_of(const NsArgs& g, int kind) {
-  return kind == NS_A || kind == NS_JOIN ? g.tile[0] : kind == NS_S ? g.tile[1] : kind == NS_X ? g.tile[2] : 64;
+__device__ __host__ __forceinline__ int ns_side(int tile) { return tile < 64 ? 64 : tile; }
+__device__ __host__ __forceinline__ int ns_side_of(const NsArgs& g, int kind) {
+  return ns_side(kind == NS_A || kind == NS_JOIN ? g.tile[0] : kind == NS_S ? g.tile[1] : kind == NS_X ? g.tile[2] : 64);
 }
 __device__ __forceinline__ const NsTable* ns_table(const char* ws) { return (const NsTable*)ws; }
 // the last matrix that starts at or before work item w: a lane each (64 matrices at most)
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
     const int l = threadIdx.x;
     if (l < g.count) t->it[l] = g.it[l];
     for (int kind = 0; kind < NS_KINDS; ++kind) {
-      int n = l < g.count ? (int)ns_items(g.it[l], kind, ns_tile_of(g, kind)) : 0, sum = n;
+      int n = l < g.count ? (int)ns_items(g.it[l], kind, ns_side_of(g, kind)) : 0, sum = n;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const int up = __shfl_up(sum, o, 64);
@@ -221,8 +222,10 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsCtl g) {
   }
 }
 
+// (32 stands for tiles of 64 whose sums are kept apart)
 template <int TILE>
 struct NsTile;
+template <> struct NsTile<32> { typedef NtCore<f16_t, true, 64, 64, 32, 32, 3, true> Core; };
 template <> struct NsTile<64> { typedef NtCore<f16_t, true, 64, 64, 32, 32, 3> Core; };
 template <> struct NsTile<128> { typedef NtCore<f16_t, true, 128, 128, 64, 32, 2> Core; };
 template <> struct NsTile<256> { typedef NtCore<f16_t, true, 256, 256, 64, 64> Core; };
@@ -308,7 +311,8 @@ __global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_product_kernel
   const int k = ns_find(g, PHASE == 0 ? NS_A : PHASE == 1 ? NS_S : NS_X, w, first);
   const NsItem q = ns_table(g.ws)->it[k];
   const NsMem mem = ns_mem(g, q);
-  const int mt = (q.m + TILE - 1) / TILE, mpad = ns_pad(q.m), npad = ns_pad(q.n);
+  constexpr int SIDE = Core::BM;
+  const int mt = (q.m + SIDE - 1) / SIDE, mpad = ns_pad(q.m), npad = ns_pad(q.n);
   int t = w - first, sp = 0, ti, tj;
   if (PHASE == 0) {                               // (workgroups that run together share a part of the contraction)
     const int tri = mt * (mt + 1) / 2;
@@ -327,9 +331,9 @@ __global__ __launch_bounds__(NsTile<TILE>::Core::THREADS) void ns_product_kernel
   const int s0 = sp * per, s1 = s0 + per < stages ? s0 + per : stages;
   Core c;
   c.clear();
-  c.run(a + (long)ti * TILE * ld, ld, q.m - ti * TILE, b + (long)tj * TILE * ld, ld, (PHASE == 2 ? q.n : q.m) - tj * TILE, s0, s1, smem);
+  c.run(a + (long)ti * SIDE * ld, ld, q.m - ti * SIDE, b + (long)tj * SIDE * ld, ld, (PHASE == 2 ? q.n : q.m) - tj * SIDE, s0, s1, smem);
   if (PHASE == 0 && q.split > 1) {
-    f32x4* p = (f32x4*)(mem.part + ((long)t * q.split + sp) * TILE * TILE) + (long)Core::wave() * Core::TI * Core::TJ * 64 + Core::lane();
+    f32x4* p = (f32x4*)(mem.part + ((long)t * q.split + sp) * Core::BM * Core::BM) + (long)Core::wave() * Core::TI * Core::TJ * 64 + Core::lane();
 #pragma unroll
     for (int i = 0; i < Core::TI; ++i)
 #pragma unroll
@@ -355,8 +359,8 @@ __global__ __launch_bounds__(64) void ns_join_kernel(NsCtl g) {
   ns_tri(t, ti, tj);
   Core c;
   c.clear();
-  const f32x4* p = (const f32x4*)(mem.part + (long)t * q.split * TILE * TILE) + (long)wave * Core::TI * Core::TJ * 64 + Core::lane();
-  for (int s = 0; s < q.split; ++s, p += TILE * TILE / 4) {
+  const f32x4* p = (const f32x4*)(mem.part + (long)t * q.split * Core::BM * Core::BM) + (long)wave * Core::TI * Core::TJ * 64 + Core::lane();
+  for (int s = 0; s < q.split; ++s, p += Core::BM * Core::BM / 4) {
 #pragma unroll
     for (int i = 0; i < Core::TI; ++i)
 #pragma unroll
@@ -384,9 +388,10 @@ struct NsPair64 {
     *(uint4*)at(row, k, 1) = lo;
   }
 };
-// wave w's 32 x 32 quarter of a b^T, added to acc (coordinates as NtCore's)
+// wave w's 32 x 32 quarter of a b^T, added to acc (coordinates as NtCore's; hi * lo + lo * hi summed apart, as there)
 __device__ __forceinline__ void ns_mul64(const NsPair64& a, const NsPair64& b, f32x4 (&acc)[2][2]) {
   const int w = (int)(threadIdx.x >> 6), l = threadIdx.x & 63, r0 = (w >> 1) * 32 + (l & 15), c0 = (w & 1) * 32 + (l & 15), g = (l >> 4) * 8;
+  f32x4 low[2][2] = {};
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     f16x8 bh[2], bl[2];
@@ -397,12 +402,15 @@ __device__ __forceinline__ void ns_mul64(const NsPair64& a, const NsPair64& b, f
       const f16x8 ah = *(const f16x8*)a.at(r0 + i * 16, s * 32 + g, 0), al = *(const f16x8*)a.at(r0 + i * 16, s * 32 + g, 1);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        acc[i][j] = mfma16(bh[j], al, acc[i][j]);
-        acc[i][j] = mfma16(bl[j], ah, acc[i][j]);
+        low[i][j] = mfma16(bl[j], al, low[i][j]);
+        low[i][j] = mfma16(bh[j], al, low[i][j]);
+        low[i][j] = mfma16(bl[j], ah, low[i][j]);
         acc[i][j] = mfma16(bh[j], ah, acc[i][j]);
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] += low[i >> 1][i & 1];
 }
 // fp32 64 x 64 in LDS, in NtBlock's arrangement, for the whole workgroup
 typedef NtBlock<64, 64> NsF64;
@@ -508,8 +516,12 @@ __global__ __launch_bounds__(256) void ns_narrow_step_kernel(NsCtl g) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r) {
+          // (A as its square saw it: b and c then act on the same eigenvalues, and their roundings' effects largely cancel)
+          const f16_t hi = (f16_t)a[i][j][r], lo = (f16_t)(a[i][j][r] - (float)hi);
+          a[i][j][r] = (float)hi + (float)lo;
           acc[i][j][r] = g.cc * (acc[i][j][r] * (1.f / NS_SCALE)) + g.cb * a[i][j][r] + (r0 + i * 16 == c0 + j * 16 + r ? g.ca * NS_SCALE : 0.f);
+        }
   }
   ns_f64_put(f, acc);                                                   // (every wave has read A's copy: the barrier above)
   __syncthreads();
@@ -599,6 +611,14 @@ NsPlan ns_plan(const FiNsMat* const* mats, int count) {
       }
     }
   }
+  // small matrices are held to an fp32 iteration's error: their tiles keep the low parts' sums apart
+  int most = 0;
+  for (int i = 0; i < count; ++i) {
+    const int m = mats[i]->rows < mats[i]->cols ? mats[i]->rows : mats[i]->cols;
+    if (m > most) most = m;
+  }
+  for (int phase = 0; phase < 3 && most <= 256; ++phase)
+    if (p.tile[phase] == 64) p.tile[phase] = 32;
   return p;
 }
 
@@ -620,9 +640,9 @@ long ns_layout(const FiNsMat* const* mats, int count, const NsPlan& plan, NsArgs
       at += ns_narrow_mem(nullptr, q).bytes;
       continue;
     }
-    const long mt = (q.m + plan.tile[0] - 1) / plan.tile[0];
+    const long side = ns_side(plan.tile[0]), mt = (q.m + side - 1) / side;
     at += ns_mem(nullptr, q).bytes;
-    if (q.split > 1) at += 4L * (mt * (mt + 1) / 2) * q.split * plan.tile[0] * plan.tile[0];
+    if (q.split > 1) at += 4L * (mt * (mt + 1) / 2) * q.split * side * side;
   }
   return at;
 }
@@ -652,7 +672,7 @@ int ns_check(const FiNsMat* mats, int count, int steps, const float* coeffs) {
 
 int ns_total(const NsArgs& g, int kind) {
   long n = 0;
-  for (int i = 0; i < g.count; ++i) n += ns_items(g.it[i], kind, ns_tile_of(g, kind));
+  for (int i = 0; i < g.count; ++i) n += ns_items(g.it[i], kind, ns_side_of(g, kind));
   return n < (1L << 30) ? (int)n : -1;
 }
 template <int PHASE, int TILE>
@@ -670,7 +690,7 @@ int ns_product(const NsCtl& c, int items, int joins, hipStream_t st) {
 }
 template <int PHASE>
 int ns_product(const NsCtl& c, int tile, int items, int joins, hipStream_t st) {
-  return tile == 64 ? ns_product<PHASE, 64>(c, items, joins, st) : tile == 128 ? ns_product<PHASE, 128>(c, items, joins, st)
+  return tile == 32 ? ns_product<PHASE, 32>(c, items, joins, st) : tile == 64 ? ns_product<PHASE, 64>(c, items, joins, st) : tile == 128 ? ns_product<PHASE, 128>(c, items, joins, st)
                                                                                : ns_product<PHASE, 256>(c, items, joins, st);
 }
 

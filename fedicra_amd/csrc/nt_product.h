@@ -39,7 +39,10 @@ static inline bool nt_allow_lds(const void* kernel) {
 __device__ __forceinline__ void nt_wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // SLOTS: two where two stages fill the LDS or several workgroups share a CU; more where a lone workgroup would wait for each stage's latency.
-template <typename T, bool PAIR, int BM_, int BN_, int WM_, int WN_, int SLOTS_ = 2>
+// APART: pairs also take lo * lo, and what has a low part is summed in accumulators of its own: the matrix pipe rounds an accumulator at every
+// instruction, and small matrices are held to an fp32 sum's few roundings (in an orthogonalised 2 x 50 matrix 8.0e-7 of the result becomes 5.4e-7,
+// where fp32 products leave 6.9e-7).  A third more matrix instructions; long sums have no need of it.
+template <typename T, bool PAIR, int BM_, int BN_, int WM_, int WN_, int SLOTS_ = 2, bool APART_ = false>
 struct NtCore {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, SLOTS = SLOTS_;
   static constexpr int NWN = BN / WN, NW = (BM / WM) * NWN, THREADS = NW * 64;
@@ -50,6 +53,7 @@ struct NtCore {
   static_assert(WM % BLOCK == 0 && WN % BLOCK == 0 && NW * BLOCK * BLOCK * 4 <= LDS, "scratch");
   static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;       // DMA instructions of a wave per stage: 8 rows of A, of B
   static_assert(PA * NW * 8 == BM && PB * NW * 8 == BN, "whole DMA instructions for every wave");
+  static constexpr bool APART = PAIR && APART_;
   typedef typename DT<T>::frag_t frag_t;
 
   f32x4 acc[TI][TJ];
@@ -112,6 +116,12 @@ struct NtCore {
 #pragma unroll
       for (int k = 0; k < SLOTS - 1; ++k) fetch(s0 + k, k);
     }
+    constexpr int LI = APART ? TI : 1, LJ = APART ? TJ : 1;
+    f32x4 low[LI][LJ];
+#pragma unroll
+    for (int i = 0; i < LI; ++i)
+#pragma unroll
+      for (int j = 0; j < LJ; ++j) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     int cur = 0, free = SLOTS - 1;                                      // slots of stage s and of the one before it
     for (int s = s0; s < s1; ++s) {
       // stage s is there for every wave, and every wave has read the one before it
@@ -138,10 +148,14 @@ struct NtCore {
             al[u ^ 1] = *(const frag_t*)(sa + (i + 1) * 2048 + p1);
           }
           __builtin_amdgcn_sched_barrier(0);
+          if constexpr (APART) {
 #pragma unroll
-          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bh[j], al[u], acc[i][j]);
+            for (int j = 0; j < TJ; ++j) low[i][j] = mfma16(bl[j], al[u], low[i][j]);
+          }
 #pragma unroll
-          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bl[j], ah[u], acc[i][j]);
+          for (int j = 0; j < TJ; ++j) (APART ? low[i % LI][j % LJ] : acc[i][j]) = mfma16(bh[j], al[u], APART ? low[i % LI][j % LJ] : acc[i][j]);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) (APART ? low[i % LI][j % LJ] : acc[i][j]) = mfma16(bl[j], ah[u], APART ? low[i % LI][j % LJ] : acc[i][j]);
 #pragma unroll
           for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(bh[j], ah[u], acc[i][j]);
           __builtin_amdgcn_sched_barrier(0);
@@ -163,6 +177,12 @@ struct NtCore {
       }
       free = cur;
       cur = cur + 1 < SLOTS ? cur + 1 : 0;
+    }
+    if constexpr (APART) {
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) acc[i][j] += low[i][j];
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // the ring is free: epilogues use it as scratch
   }
