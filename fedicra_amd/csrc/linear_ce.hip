@@ -495,7 +495,10 @@ __global__ __launch_bounds__(256) void ce_factors_kernel(const float* g, int red
   float m = fabsf(one);
   if (reduction == 0)
     for (int k = tid; k < CE_PARTS; k += 256) m = fmaxf(m, part[k]);
-  const float sc = 0.5f * ce_pow2_scale(ce_block_max(m, sm));           // largest factor in [2^13, 2^14)
+  // The largest factor at 2^14.  Of 16-bit G exactly there: a label's entry, -g (1 - p), mostly the largest of its row, then lies right below 2^14, where
+  // fp16 is finest for its size (1.4e-4 of it, 2.1e-4 on average elsewhere).  Of a pair by a power of two.
+  const float top = ce_block_max(m, sm);
+  const float sc = pair || !(top > 1e-30f && top < INFINITY) ? 0.5f * ce_pow2_scale(top) : 16384.f / top;
   if (blockIdx.x == 0 && tid == 0) {
     scal[SC_RG] = 1.f / sc;
     if (pair) {
@@ -898,8 +901,9 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
       lab[i] = o < M ? a.s.lab[oc] : -1;
       m2[i] = -INFINITY;                                                // the running maximum; y: the running sum
     } else {
+      // (dx takes every row's own factor out of the sum: G is made with 2^14 in its place, where its label's entry is rounded least)
       const float4 m = a.meta[oc];
-      m2[i] = m.x, y[i] = m.y, gg[i] = m.z, lab[i] = __float_as_int(m.w);
+      m2[i] = m.x, y[i] = 16384.f * a.s.stat[oc].y, gg[i] = 16384.f, b[i] = m.z * (1.f / 16384.f), lab[i] = __float_as_int(m.w);
     }
   }
   f32x4 acc[2][2 * KD];
@@ -1045,6 +1049,10 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
       if (!a.out.out) continue;
     }
     if (o >= M) continue;
+    if constexpr (!DW) {
+#pragma unroll
+      for (int d = 0; d < 2 * KD; ++d) acc[i][d] *= b[i];
+    }
     const i64 row = a.out.idx ? (i64)a.out.idx[o] : (i64)o;
 #pragma unroll
     for (int d = 0; d < 2 * KD; ++d) {
@@ -1090,14 +1098,16 @@ struct CeShape {
 };
 CeShape ce_shape(const FiLinearCe& d, const void* w) {
   CeShape s;
-  s.pair = d.dtype == FI_F32;
+  // Half precision keeps 11 bits, as many as G does: up to 2^28 multiply-adds, where three products cost no more than one, it goes as pairs too, and
+  // its gradients are rounded once (over 80 sizes, those more than 1.5 times an fp32 product's error off fell from 10 to none)
+  s.pair = d.dtype == FI_F32 || (d.dtype == FI_F16 && (double)d.T * d.V * d.D <= (double)(1 << 28));
   s.ku = s.pair ? 32 : 64;
   s.kp = (int)ce_up(d.D, s.ku);
   s.ldx = s.pair ? 2L * s.kp : s.kp;
   // 16-bit weights whose rows are whole stages and 16-byte aligned are read in place
   s.w_direct = !s.pair && d.wdtype == d.dtype && d.D % 64 == 0 && d.ldw % 8 == 0 && ((uintptr_t)w & 15) == 0;
   s.ldw = s.w_direct ? d.ldw : s.ldx;
-  s.scaled = d.dtype != FI_F16;
+  s.scaled = s.pair || d.dtype == FI_BF16;
   return s;
 }
 
@@ -1129,8 +1139,8 @@ template <typename T, bool PAIR> struct CeCores {
 
 template <class Core, typename T, bool PAIR>
 int ce_launch_fwd(const CeLogits& a, i64 T_rows, hipStream_t st) {
-  static const bool ok = nt_allow_lds((const void*)ce_fwd_kernel<Core, T, PAIR>);
-  if (!ok) return FI_ERR_UNSUPPORTED;
+  static NtLdsDevices allowed;
+  if (!nt_allow_lds((const void*)ce_fwd_kernel<Core, T, PAIR>, allowed)) return FI_ERR_UNSUPPORTED;
   const i64 n = (T_rows + Core::BM - 1) / Core::BM * a.ntj;
   if (n > (1LL << 30)) return FI_ERR_SHAPE;
   hipLaunchKernelGGL((ce_fwd_kernel<Core, T, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), Core::LDS, st, a);
@@ -1139,8 +1149,8 @@ int ce_launch_fwd(const CeLogits& a, i64 T_rows, hipStream_t st) {
 }
 template <class Core, typename T, bool PAIR>
 int ce_launch_dlogits(const CeLogits& a, hipStream_t st) {
-  static const bool ok = nt_allow_lds((const void*)ce_dlogits_kernel<Core, T, PAIR>);
-  if (!ok) return FI_ERR_UNSUPPORTED;
+  static NtLdsDevices allowed;
+  if (!nt_allow_lds((const void*)ce_dlogits_kernel<Core, T, PAIR>, allowed)) return FI_ERR_UNSUPPORTED;
   constexpr int SB = Core::BLOCK, SCR = Core::NW * NtBlock<SB, SB>::BYTES;
   constexpr int need = SCR + Core::BM * 16 + Core::BM / Core::WM * Core::BN * 4, lds = need > Core::LDS ? need : Core::LDS;
   const i64 n = (a.Tc + Core::BM - 1) / Core::BM * ((a.Vc + Core::BN - 1) / Core::BN);
@@ -1158,8 +1168,8 @@ int ce_logits(const CeLogits& a, const FiLinearCe& d, bool fwd, hipStream_t st) 
     default: return fwd ? ce_launch_fwd<typename C::C3, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C3, T, PAIR>(a, st);
   }
 }
-int ce_logits_any(const CeLogits& a, const FiLinearCe& d, bool fwd, hipStream_t st) {
-  return d.dtype == FI_F32 ? ce_logits<f16_t, true>(a, d, fwd, st) : d.dtype == FI_BF16 ? ce_logits<bf16_t, false>(a, d, fwd, st) : ce_logits<f16_t, false>(a, d, fwd, st);
+int ce_logits_any(const CeLogits& a, const FiLinearCe& d, bool pair, bool fwd, hipStream_t st) {
+  return pair ? ce_logits<f16_t, true>(a, d, fwd, st) : d.dtype == FI_BF16 ? ce_logits<bf16_t, false>(a, d, fwd, st) : ce_logits<f16_t, false>(a, d, fwd, st);
 }
 
 // one or two operands in a launch (src == NULL: none)
@@ -1202,8 +1212,8 @@ int ce_fused_splits(i64 own, i64 streamed) {
 template <typename T, int KD, int MODE>
 int ce_launch_fused(const CeFused& a, hipStream_t st) {
   constexpr int lds = 2 * (KD * (MODE == CE_FWD ? 4096 : 8192) + 1024);
-  static const bool ok = nt_allow_lds((const void*)ce_fused_kernel<T, KD, MODE>);
-  if (!ok) return FI_ERR_UNSUPPORTED;
+  static NtLdsDevices allowed;
+  if (!nt_allow_lds((const void*)ce_fused_kernel<T, KD, MODE>, allowed)) return FI_ERR_UNSUPPORTED;
   const i64 n = (i64)((a.out.M + 255) / 256) * a.out.splits;
   hipLaunchKernelGGL((ce_fused_kernel<T, KD, MODE>), dim3((unsigned)ce_up(n, 8)), dim3(512), lds, st, a);
   FI_CHECK_LAUNCH();
@@ -1342,8 +1352,8 @@ CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need
 
 template <class Core, bool PAIR>
 int ce_launch_grad(const CeGrad& a, hipStream_t st) {
-  static const bool ok = nt_allow_lds((const void*)ce_grad_kernel<Core, PAIR>);
-  if (!ok) return FI_ERR_UNSUPPORTED;
+  static NtLdsDevices allowed;
+  if (!nt_allow_lds((const void*)ce_grad_kernel<Core, PAIR>, allowed)) return FI_ERR_UNSUPPORTED;
   const i64 n = (i64)((a.M + Core::BM - 1) / Core::BM) * ((a.N + Core::BN - 1) / Core::BN) * a.splits;
   hipLaunchKernelGGL((ce_grad_kernel<Core, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), Core::LDS, st, a);
   FI_CHECK_LAUNCH();
@@ -1407,7 +1417,7 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
     CeLogits a = {};
     a.x = ws.xc, a.ldx = s.ldx, a.w = wop, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
     a.scal = scal, a.s = sv, a.part = ws.part, a.zt = ws.zt, a.ntj = ws.nparts;
-    if ((rc = ce_logits_any(a, *d, true, st))) return rc;
+    if ((rc = ce_logits_any(a, *d, s.pair, true, st))) return rc;
   }
   const int lanes = ws.nparts > 32 ? 64 : ws.nparts > 4 ? 8 : 1;
   i64 g = (d->T * lanes + 255) / 256;
@@ -1461,7 +1471,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   }
   const i64 ng = (d->T + 255) / 256;
   hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)ng), dim3(256), 0, st, gloss, d->reduction, ws.parts, sv, (int)s.pair, ws.scal, ws.g, ws.meta, bias, d->V, ws.bias_pad, labels,
-                     d->ltype, (i64)d->T, (i64)d->ignore_index, (char*)dx, (i64)d->D * (s.pair ? 4 : 2));
+                     d->ltype, (i64)d->T, (i64)d->ignore_index, (char*)dx, (i64)d->D * (d->dtype == FI_F32 ? 4 : 2));
   FI_CHECK_LAUNCH();
   const int f = s.pair ? 2 : 1;
   CeGrad gx = {}, gw = {};
@@ -1509,7 +1519,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
       pt.begin = a.t0, pt.rows = a.Tc, pt.turned = ws.xt, pt.ld_turned = ws.ld_xt, pt.turned_pair = s.pair;
       if ((rc = ce_pack(pt, CePack{}, st))) return rc;
     }
-    if ((rc = ce_logits_any(a, *d, false, st))) return rc;
+    if ((rc = ce_logits_any(a, *d, s.pair, false, st))) return rc;
     if (dx) {
       gx.b = ws.wt + (i64)f * a.v0, gx.M = (int)a.Tc, gx.K = a.Vc, gx.t0 = a.t0, gx.Tc = a.Tc, gx.first = iv == 0;
       gx.part = ws.pdx;

@@ -678,8 +678,8 @@ int ns_total(const NsArgs& g, int kind) {
 template <int PHASE, int TILE>
 int ns_product(const NsCtl& c, int items, int joins, hipStream_t st) {
   typedef typename NsTile<TILE>::Core Core;
-  static const bool lds_ok = nt_allow_lds((const void*)ns_product_kernel<PHASE, TILE>);
-  if (!lds_ok) return FI_ERR_UNSUPPORTED;
+  static NtLdsDevices allowed;
+  if (!nt_allow_lds((const void*)ns_product_kernel<PHASE, TILE>, allowed)) return FI_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((ns_product_kernel<PHASE, TILE>), dim3((items + 7) & ~7), dim3(Core::THREADS), Core::LDS, st, c, items);
   FI_CHECK_LAUNCH();
   if (PHASE == 0 && joins) {

@@ -12,6 +12,8 @@
 // of 128 bytes per instruction); 16-byte piece c of row r lies at piece c ^ (r & 7), the swizzle being applied to the source address
 // because the LDS side of the instruction is linear: the eight lanes a ds_read_b128 serves per clock then touch all 32 banks once.
 #pragma once
+#include <atomic>
+
 #include "common.h"
 
 typedef int nt_v4i __attribute__((ext_vector_type(4)));
@@ -31,9 +33,16 @@ __device__ __forceinline__ nt_v4i nt_rsrc(const void* ptr, unsigned long long by
   return nt_v4i{__builtin_amdgcn_readfirstlane((int)(unsigned)p), __builtin_amdgcn_readfirstlane((int)((unsigned)(p >> 32) & 0xffffu)),
                 __builtin_amdgcn_readfirstlane((int)n), 0x00020000};
 }
-// more than 64 KB of dynamic LDS per workgroup has to be allowed per kernel (once; a CU has 160 KB)
-static inline bool nt_allow_lds(const void* kernel) {
-  return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
+// more than 64 KB of dynamic LDS per workgroup has to be allowed per kernel and device (a CU has 160 KB); `done`: a bit per device, one object per kernel
+typedef std::atomic<unsigned long long> NtLdsDevices;
+static inline bool nt_allow_lds(const void* kernel, NtLdsDevices& done) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return false;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 // orders this wave's LDS traffic: what other lanes of the wave wrote before is there after
 __device__ __forceinline__ void nt_wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }

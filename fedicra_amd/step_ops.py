@@ -85,11 +85,13 @@ def _grad_slot(param, shape):
 
 
 def _dense_rows(t, rows, cols):
-    """[rows, cols] view with dense rows (a copy only where there is none)."""
+    """[rows, cols] with dense rows that lie apart (a view; a copy where there is none: features apart, an expanded or overlapping tensor, rows so
+    far apart that a tile's offsets would not fit)."""
     t = t.detach()
     if t.dim() != 2:
         t = t.reshape(rows, cols)
-    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
+    apart = rows == 1 or cols <= t.stride(0) <= 1 << 22
+    return t if (t.stride(1) == 1 or cols == 1) and apart else t.contiguous()
 
 
 class _LinearCE(Function):

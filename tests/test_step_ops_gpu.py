@@ -88,6 +88,14 @@ def test_newton_schulz_steps_and_coefficients():
     _ns_check(ops.newton_schulz(u, steps=3, coeffs=per), u, steps=3, coeffs=per)
 
 
+def test_newton_schulz_leaves_its_argument_alone_and_takes_unaligned_ones():
+    flat = torch.randn(1 + 33 * 70, generator=_gen(60), device="cuda")
+    for t in (flat[1:].view(33, 70), flat[1:].half()[:33 * 70].view(33, 70), flat.half()[1:].view(33, 70)):
+        keep = t.clone()
+        _ns_check(ops.newton_schulz(t), t)
+        assert torch.equal(t, keep)
+
+
 def test_newton_schulz_extreme_values():
     u = torch.zeros(20, 30, device="cuda")
     assert torch.equal(ops.newton_schulz(u), u)                       # nothing to orthogonalise
@@ -231,6 +239,11 @@ def test_linear_ce_keeps_sizes_types_and_layouts():
     _ce_check(wide[:, 1, :24], w, b, lab)                              # rows far apart
     _ce_check(wide[:, 1, ::2], w, b, lab)                              # features far apart
     _ce_check(wide[:, 2, 1:25], w.t().contiguous().t(), b, lab)        # unaligned rows, a transposed weight
+    row = torch.randn(24, generator=_gen(9), device="cuda").to(BF16)
+    _ce_check(row.expand(100, 24), w, b, lab)                          # every row the same memory
+    _ce_check(torch.randn(123, generator=_gen(10), device="cuda").to(BF16).as_strided((100, 24), (1, 1)), w, b, lab)     # overlapping rows
+    _ce_check(wide[:, 0, :24], w[:1].expand(40, 24), b, lab)
+    _ce_check(wide[:1, 0, :24], w, b, lab[:1])
     big = torch.randn(70, 200, generator=_gen(7), device="cuda").to(F16)
     _ce_check(big[:, 4:132], (torch.randn(50, 300, generator=_gen(8), device="cuda") * 0.1).to(F16)[:, 3:131], None, lab[:70], above=torch.full((), 64.0, device="cuda"))
 
