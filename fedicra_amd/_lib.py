@@ -1197,18 +1197,28 @@ def linear_ce_desc(x, w, labels, ignore_index, reduction):
                       max(x.stride(0), x.shape[1]), max(w.stride(0), w.shape[1]), int(ignore_index))
 
 
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
 def linear_ce_fwd(d, x, w, bias, labels, loss):
     """Returns the buffer the backward pass needs."""
-    dev = _dev(x).device
-    saved = _scratch(lib().fi_linear_ce_saved(C.byref(d)), "fi_linear_ce_saved", dev)
-    ws = _scratch(lib().fi_linear_ce_fwd_workspace(C.byref(d), ptr(w)), "fi_linear_ce_fwd_workspace", dev)
-    _chk(lib().fi_linear_ce_fwd(C.byref(d), ptr(x), ptr(w), ptr(bias), ptr(labels), ptr(loss), ptr(saved), ptr(ws), stream()),
+    dev, so, ref = _dev(x).device, lib(), C.byref(d)
+    pw = C.c_void_p(w.data_ptr())
+    saved = _scratch(so.fi_linear_ce_saved(ref), "fi_linear_ce_saved", dev)
+    ws = _scratch(so.fi_linear_ce_fwd_workspace(ref, pw), "fi_linear_ce_fwd_workspace", dev)
+    _chk(so.fi_linear_ce_fwd(ref, C.c_void_p(x.data_ptr()), pw, C.c_void_p(_address(bias)), C.c_void_p(labels.data_ptr()),
+                             C.c_void_p(loss.data_ptr()), C.c_void_p(saved.data_ptr()), C.c_void_p(ws.data_ptr()), stream()),
          "fi_linear_ce_fwd")
     return saved
 
 
 def linear_ce_bwd(d, x, w, bias, labels, saved, gloss, dx, dw, dw_accumulate, db, db_accumulate):
-    size = lib().fi_linear_ce_bwd_workspace(C.byref(d), ptr(w), int(dx is not None), int(dw is not None), int(db is not None))
+    so, ref = lib(), C.byref(d)
+    pw = C.c_void_p(w.data_ptr())
+    size = so.fi_linear_ce_bwd_workspace(ref, pw, int(dx is not None), int(dw is not None), int(db is not None))
     ws = _scratch(size, "fi_linear_ce_bwd_workspace", _dev(x).device)
-    _chk(lib().fi_linear_ce_bwd(C.byref(d), ptr(x), ptr(w), ptr(bias), ptr(labels), ptr(saved), ptr(gloss), ptr(dx), ptr(dw),
-                                int(dw_accumulate), ptr(db), int(db_accumulate), ptr(ws), stream()), "fi_linear_ce_bwd")
+    _chk(so.fi_linear_ce_bwd(ref, C.c_void_p(x.data_ptr()), pw, C.c_void_p(_address(bias)), C.c_void_p(labels.data_ptr()),
+                             C.c_void_p(saved.data_ptr()), C.c_void_p(gloss.data_ptr()), C.c_void_p(_address(dx)), C.c_void_p(_address(dw)),
+                             int(dw_accumulate), C.c_void_p(_address(db)), int(db_accumulate), C.c_void_p(ws.data_ptr()), stream()),
+         "fi_linear_ce_bwd")

@@ -160,6 +160,96 @@ __global__ __launch_bounds__(256) void ce_amax_kernel(CeAmax x, CeAmax w) {
   if (threadIdx.x == 0) a.part[blockIdx.x] = m;
 }
 
+// ---- the backward pass's rows --------------------------------------------------------------------------------------------------------------
+// dx of the rows that take no part: a lane looks at a label, the wave clears the rows it finds
+__device__ __forceinline__ void ce_zero_rows(const void* labels, int ltype, i64 T, i64 ignore, char* dx, i64 row_bytes) {
+  const int l = threadIdx.x & 63;
+  const i64 r0 = ((i64)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
+  const bool mine = r0 + l < T && ce_label(labels, ltype, r0 + l) == ignore;
+  unsigned long long todo = __ballot(mine);
+  const bool vec = row_bytes % 16 == 0 && ((uintptr_t)dx & 15) == 0;
+  if (vec && row_bytes <= 512) {                                        // several rows at a time
+    const int per = (int)(row_bytes / 16), rows = 64 / per;
+    if (todo)
+      for (int i = 0; i < 64; i += rows) {
+        const int r = i + l / per;
+        if (l / per < rows && r < 64 && (todo >> r & 1)) ((uint4*)(dx + (r0 + r) * row_bytes))[l % per] = make_uint4(0, 0, 0, 0);
+      }
+    return;
+  }
+  while (todo) {
+    const int r = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    char* p = dx + (r0 + r) * row_bytes;
+    if (vec)
+      for (i64 c = l; c < row_bytes / 16; c += 64) ((uint4*)p)[c] = make_uint4(0, 0, 0, 0);
+    else
+      for (i64 c = l; c < row_bytes / 2; c += 64) ((uint16_t*)p)[c] = 0;
+  }
+}
+
+// rows' factors g_t * scale (reduction 0: one upstream gradient per row; 1 mean, 2 sum: one for all); zeros for dx's other rows
+struct CeFactors {
+  const float* g;          // upstream gradient
+  int reduction;
+  const float* part;       // reduction 0: maxima of |g|
+  CeSaved s;
+  int pair;
+  float *scal, *out;
+  float4* meta;
+  const float* bias;
+  float* bias_pad;
+  const void* labels;
+  int ltype, V;
+  i64 T, ignore;
+  char* dx;
+  i64 row_bytes;
+};
+__device__ __forceinline__ void ce_factors(const CeFactors& a, float* sm) {
+  const CeSaved& s = a.s;
+  const float* const g = a.g;
+  const int reduction = a.reduction, pair = a.pair, V = a.V, n = s.count[0], tid = threadIdx.x;
+  const float *const part = a.part, *const bias = a.bias;
+  float *const scal = a.scal, *const out = a.out, *const bias_pad = a.bias_pad;
+  float4* const meta = a.meta;
+  if (a.dx) ce_zero_rows(a.labels, a.ltype, a.T, a.ignore, a.dx, a.row_bytes);
+  const float one = reduction == 1 ? (float)((double)g[0] / (double)n) : reduction == 2 ? g[0] : 0.f;
+  float m = fabsf(one);
+  if (reduction == 0)
+    for (int k = tid; k < CE_PARTS; k += 256) m = fmaxf(m, part[k]);
+  // The largest factor at 2^14.  Of 16-bit G exactly there: a label's entry, -g (1 - p), mostly the largest of its row, then lies right below 2^14, where
+  // fp16 is finest for its size (1.4e-4 of it, 2.1e-4 on average elsewhere).  Of a pair by a power of two.
+  const float top = ce_block_max(m, sm);
+  const float sc = pair || !(top > 1e-30f && top < INFINITY) ? 0.5f * ce_pow2_scale(top) : 16384.f / top;
+  if (blockIdx.x == 0 && tid == 0) {
+    scal[SC_RG] = 1.f / sc;
+    if (pair) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) scal[k] = s.scal[k];
+    }
+  }
+  for (i64 r = (i64)blockIdx.x * 256 + tid; r < n; r += (i64)gridDim.x * 256) {
+    const float f = reduction == 0 ? g[s.idx[r]] : one;
+    out[r] = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : f * sc;
+  }
+  if (!meta) return;
+  // the fused form's row table, whole tiles of 64 rows long (a row behind the last one: exp2(-inf) * 0), and its bias likewise
+  for (i64 r = (i64)blockIdx.x * 256 + tid; r < ((n + 63) & ~63); r += (i64)gridDim.x * 256) {
+    float4 m = make_float4(INFINITY, 0.f, 0.f, __int_as_float(-1));
+    if (r < n) {
+      const float2 st = s.stat[r];
+      const float f = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : (reduction == 0 ? g[s.idx[r]] : one) * sc;
+      m = make_float4(st.x * CE_LOG2E, f * st.y, f, __int_as_float(s.lab[r]));
+    }
+    meta[r] = m;
+  }
+  for (i64 v = (i64)blockIdx.x * 256 + tid; v < ((V + 63) & ~63); v += (i64)gridDim.x * 256) bias_pad[v] = bias && v < V ? bias[v] : 0.f;
+}
+__global__ __launch_bounds__(256) void ce_factors_kernel(CeFactors a) {
+  __shared__ float sm[4];
+  ce_factors(a, sm);
+}
+
 // ---- packing an operand ---------------------------------------------------------------------------------------------------------------
 struct CePack {
   const void* src;         // [rows][D], leading dimension ld, storage `dtype`
@@ -193,9 +283,14 @@ __device__ __forceinline__ void ce_load8(const T* q, int left, int vec, float (&
   for (int t = 0; t < 8; ++t) v[t] = t < left ? to_f32(q[t]) : 0.f;
 }
 // one 64 x 64 block of the source per workgroup (blockIdx.x: rows, .y: columns, .z: which operand); pads are written as zeros
-__global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw) {
+// (the last slice of a launch with f.g: the rows' factors, which need nothing of the operands)
+__global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw, CeFactors f) {
   __shared__ float tile[64][65];
   __shared__ float sm[4];
+  if (f.g && blockIdx.z == gridDim.z - 1) {
+    if (blockIdx.y == 0) ce_factors(f, sm);
+    return;
+  }
   const CePack& a = blockIdx.z ? pw : px;
   const i64 have = a.count ? (i64)a.count[0] - a.begin : a.rows, rows = have < a.rows ? have : a.rows;
   const i64 r0 = (i64)blockIdx.x * 64;
@@ -275,6 +370,9 @@ struct CeLogits {
   f16_t *dl, *dlt;
   i64 ld_dl, ld_dlt;
   float* db;               // [row tile][V] partial column sums, or NULL
+  float* db_out;           // or, where one row tile holds every row, the sums themselves
+  int db_add;
+  const float* rg;
 };
 
 // item -> tile, groups of 8 row tiles walking the classes together so that an XCD's workgroups share both operands in its L2
@@ -313,7 +411,7 @@ __device__ __forceinline__ void ce_begin(Core& c, const CeLogits& a, int c0) {
 template <bool PAIR, class Core>
 __device__ __forceinline__ void ce_finish(Core& c, const CeLogits& a, int c0) {
   if constexpr (PAIR) {
-    const float rx = a.scal[SC_RX], rw = a.scal[SC_RW];
+    const float rx = a.scal ? a.scal[SC_RX] : 1.f, rw = a.scal ? a.scal[SC_RW] : 1.f;
     const int j0 = c0 + Core::col0() + 4 * (Core::lane() >> 4);
 #pragma unroll
     for (int j = 0; j < Core::TJ; ++j)
@@ -458,72 +556,6 @@ __global__ __launch_bounds__(256) void ce_gmax_kernel(const float* g, const int*
   __syncthreads();
   if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
 }
-// dx of the rows that take no part: a lane looks at a label, the wave clears the rows it finds
-__device__ __forceinline__ void ce_zero_rows(const void* labels, int ltype, i64 T, i64 ignore, char* dx, i64 row_bytes) {
-  const int l = threadIdx.x & 63;
-  const i64 r0 = ((i64)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
-  const bool mine = r0 + l < T && ce_label(labels, ltype, r0 + l) == ignore;
-  unsigned long long todo = __ballot(mine);
-  const bool vec = row_bytes % 16 == 0 && ((uintptr_t)dx & 15) == 0;
-  if (vec && row_bytes <= 512) {                                        // several rows at a time
-    const int per = (int)(row_bytes / 16), rows = 64 / per;
-    if (todo)
-      for (int i = 0; i < 64; i += rows) {
-        const int r = i + l / per;
-        if (l / per < rows && r < 64 && (todo >> r & 1)) ((uint4*)(dx + (r0 + r) * row_bytes))[l % per] = make_uint4(0, 0, 0, 0);
-      }
-    return;
-  }
-  while (todo) {
-    const int r = __builtin_ctzll(todo);
-    todo &= todo - 1;
-    char* p = dx + (r0 + r) * row_bytes;
-    if (vec)
-      for (i64 c = l; c < row_bytes / 16; c += 64) ((uint4*)p)[c] = make_uint4(0, 0, 0, 0);
-    else
-      for (i64 c = l; c < row_bytes / 2; c += 64) ((uint16_t*)p)[c] = 0;
-  }
-}
-
-// rows' factors g_t * scale (reduction 0: one upstream gradient per row; 1 mean, 2 sum: one for all); zeros for dx's other rows
-__global__ __launch_bounds__(256) void ce_factors_kernel(const float* g, int reduction, const float* part, CeSaved s, int pair, float* scal, float* out, float4* meta,
-                                                         const float* bias, int V, float* bias_pad, const void* labels, int ltype, i64 T, i64 ignore, char* dx, i64 row_bytes) {
-  __shared__ float sm[4];
-  const int n = s.count[0], tid = threadIdx.x;
-  if (dx) ce_zero_rows(labels, ltype, T, ignore, dx, row_bytes);
-  const float one = reduction == 1 ? (float)((double)g[0] / (double)n) : reduction == 2 ? g[0] : 0.f;
-  float m = fabsf(one);
-  if (reduction == 0)
-    for (int k = tid; k < CE_PARTS; k += 256) m = fmaxf(m, part[k]);
-  // The largest factor at 2^14.  Of 16-bit G exactly there: a label's entry, -g (1 - p), mostly the largest of its row, then lies right below 2^14, where
-  // fp16 is finest for its size (1.4e-4 of it, 2.1e-4 on average elsewhere).  Of a pair by a power of two.
-  const float top = ce_block_max(m, sm);
-  const float sc = pair || !(top > 1e-30f && top < INFINITY) ? 0.5f * ce_pow2_scale(top) : 16384.f / top;
-  if (blockIdx.x == 0 && tid == 0) {
-    scal[SC_RG] = 1.f / sc;
-    if (pair) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) scal[k] = s.scal[k];
-    }
-  }
-  for (i64 r = (i64)blockIdx.x * 256 + tid; r < n; r += (i64)gridDim.x * 256) {
-    const float f = reduction == 0 ? g[s.idx[r]] : one;
-    out[r] = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : f * sc;
-  }
-  if (!meta) return;
-  // the fused form's row table, whole tiles of 64 rows long (a row behind the last one: exp2(-inf) * 0), and its bias likewise
-  for (i64 r = (i64)blockIdx.x * 256 + tid; r < ((n + 63) & ~63); r += (i64)gridDim.x * 256) {
-    float4 m = make_float4(INFINITY, 0.f, 0.f, __int_as_float(-1));
-    if (r < n) {
-      const float2 st = s.stat[r];
-      const float f = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : (reduction == 0 ? g[s.idx[r]] : one) * sc;
-      m = make_float4(st.x * CE_LOG2E, f * st.y, f, __int_as_float(s.lab[r]));
-    }
-    meta[r] = m;
-  }
-  for (i64 v = (i64)blockIdx.x * 256 + tid; v < ((V + 63) & ~63); v += (i64)gridDim.x * 256) bias_pad[v] = bias && v < V ? bias[v] : 0.f;
-}
-
 template <bool PAIR>
 __device__ __forceinline__ int ce_kpad(int n) { return PAIR ? (n + 31) & ~31 : (n + 63) & ~63; }
 
@@ -535,7 +567,11 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
   const i64 left = (i64)a.s.count[0] - a.t0;
   const int n = (int)(left < 0 ? 0 : left < a.Tc ? left : a.Tc);       // rows of this piece
   int ti, tj;
-  if (!ce_tile((n + Core::BM - 1) / Core::BM, (a.Vc + Core::BN - 1) / Core::BN, ti, tj)) return;
+  if (!ce_tile((n + Core::BM - 1) / Core::BM, (a.Vc + Core::BN - 1) / Core::BN, ti, tj)) {
+    if (n == 0 && a.db_out && !a.db_add)
+      for (i64 v = (i64)blockIdx.x * Core::THREADS + threadIdx.x; v < a.V; v += (i64)gridDim.x * Core::THREADS) a.db_out[v] = 0.f;
+    return;
+  }
   const int r0 = ti * Core::BM, c0 = tj * Core::BN;
   const i64 rg = a.t0 + r0;
   const int cg = a.v0 + c0;
@@ -581,7 +617,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
           for (int i = 0; i < Core::TI; ++i) c.acc[i][j][r] = 0.f;
         }
   }
-  if (a.db) {
+  if (a.db || a.db_out) {
 #pragma unroll
     for (int j = 0; j < Core::TJ; ++j)
 #pragma unroll
@@ -597,7 +633,12 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
       float v = 0.f;
 #pragma unroll
       for (int q = 0; q < Core::BM / Core::WM; ++q) v += colsum[q * Core::BN + j];
-      if (cg + j < a.V) a.db[(rg / Core::BM) * a.V + cg + j] = v;
+      if (cg + j < a.V) {
+        if (a.db_out)
+          a.db_out[cg + j] = (a.db_add ? a.db_out[cg + j] : 0.f) + v * a.rg[0];
+        else
+          a.db[(rg / Core::BM) * a.V + cg + j] = v;
+      }
     }
   }
   const NtBlock<SB, SB> blk{(float*)(smem + Core::wave() * NtBlock<SB, SB>::BYTES)};
@@ -1107,7 +1148,7 @@ CeShape ce_shape(const FiLinearCe& d, const void* w) {
   // 16-bit weights whose rows are whole stages and 16-byte aligned are read in place
   s.w_direct = !s.pair && d.wdtype == d.dtype && d.D % 64 == 0 && d.ldw % 8 == 0 && ((uintptr_t)w & 15) == 0;
   s.ldw = s.w_direct ? d.ldw : s.ldx;
-  s.scaled = s.pair || d.dtype == FI_BF16;
+  s.scaled = d.dtype != FI_F16 || (s.pair && d.wdtype != FI_F16);       // (fp16 values are their own high parts)
   return s;
 }
 
@@ -1173,7 +1214,7 @@ int ce_logits_any(const CeLogits& a, const FiLinearCe& d, bool pair, bool fwd, h
 }
 
 // one or two operands in a launch (src == NULL: none)
-int ce_pack(const CePack& x, const CePack& w, hipStream_t st) {
+int ce_pack(const CePack& x, const CePack& w, hipStream_t st, const CeFactors& f = CeFactors{}) {
   i64 gx = 0;
   int gy = 0;
   for (const CePack* p : {&x, &w}) {
@@ -1183,7 +1224,7 @@ int ce_pack(const CePack& x, const CePack& w, hipStream_t st) {
     if ((cols + 63) / 64 > gy) gy = (cols + 63) / 64;
   }
   if (!x.src && !w.src) return 0;
-  hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)gx, (unsigned)gy, x.src && w.src ? 2 : 1), dim3(256), 0, st, x.src ? x : w, w);
+  hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)gx, (unsigned)gy, (x.src && w.src ? 2 : 1) + (f.g ? 1 : 0)), dim3(256), 0, st, x.src ? x : w, w, f);
   FI_CHECK_LAUNCH();
   return 0;
 }
@@ -1284,6 +1325,7 @@ CeGradPlan ce_grad_plan(i64 M, i64 N, i64 K, int ku, bool pieces) {
   i64 s = 512 / tiles;
   if (s > stages / 8) s = stages / 8;
   if (s > 64) s = 64;
+  if (stages < 64) s = 1;                        // (the join costs as much)
   if (s < 1) s = 1;
   p.splits = (int)s;
   p.part = p.splits > 1 || pieces;
@@ -1313,7 +1355,7 @@ CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need
   const i64 vc = CE_PIECE / w.Tc / 256 * 256;
   w.Vc = (int)(vc < Vp ? vc : Vp);
   w.ld_xt = f * w.Tc, w.ld_wt = f * Vp, w.ld_dl = (i64)f * w.Vc, w.ld_dlt = f * w.Tc;
-  w.parts = c.take<float>(2 * CE_PARTS);
+  w.parts = c.take<float>(3 * CE_PARTS);
   w.scal = c.take<float>(SC_N);
   w.g = c.take<float>(d.T);
   w.meta = nullptr, w.bias_pad = nullptr;
@@ -1406,8 +1448,8 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
   }
   hipLaunchKernelGGL(ce_gather_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, d->V, ws.cnt, sv, ws.zt, rows_out, bias, ws.bias_pad);
   FI_CHECK_LAUNCH();
-  if (s.pair && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
-  float* const scal = s.pair ? sv.scal : nullptr;
+  float* const scal = s.pair && s.scaled ? sv.scal : nullptr;
+  if (scal && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
   if ((rc = ce_pack(ce_pack_x(*d, s, x, sv, ws.parts, scal, ws.xc), s.w_direct ? CePack{} : ce_pack_w(*d, s, w, ws.parts, scal, ws.wc), st))) return rc;
   const void* const wop = s.w_direct ? w : (const void*)ws.wc;
   if (ce_fused_fwd_ok(*d, s)) {
@@ -1459,22 +1501,25 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   const CeSaved sv = ce_saved((void*)saved, d->T);
   // (the pair form's scales were made by the forward pass)
   const float* const parts = s.scaled && !s.pair ? ws.parts : nullptr;
-  float* const scal = s.pair ? sv.scal : s.scaled ? ws.scal : nullptr;
+  float* const scal = !s.scaled ? nullptr : s.pair ? sv.scal : ws.scal;
   if (parts && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
   CePack px = ce_pack_x(*d, s, x, sv, parts, scal, ws.xc), pw = ce_pack_w(*d, s, w, parts, scal, ws.wc);
   const bool rows_pieces = ws.Tc < d->T;
   if (!rows_pieces) px.turned = ws.xt, px.ld_turned = ws.ld_xt, px.turned_pair = s.pair;
   pw.turned = ws.wt, pw.ld_turned = ws.ld_wt, pw.turned_pair = s.pair;
   if (s.w_direct && !ws.wt) pw.src = nullptr;                           // (its scale is dx's alone)
-  if ((rc = ce_pack(px, pw, st))) return rc;
   if (d->reduction == 0) {
-    hipLaunchKernelGGL(ce_gmax_kernel, dim3(CE_PARTS), dim3(256), 0, st, gloss, sv.idx, sv.count, ws.parts);
+    hipLaunchKernelGGL(ce_gmax_kernel, dim3(CE_PARTS), dim3(256), 0, st, gloss, sv.idx, sv.count, ws.parts + 2 * CE_PARTS);
     FI_CHECK_LAUNCH();
   }
-  const i64 ng = (d->T + 255) / 256;
-  hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)ng), dim3(256), 0, st, gloss, d->reduction, ws.parts, sv, (int)s.pair, ws.scal, ws.g, ws.meta, bias, d->V, ws.bias_pad, labels,
-                     d->ltype, (i64)d->T, (i64)d->ignore_index, (char*)dx, (i64)d->D * (d->dtype == FI_F32 ? 4 : 2));
-  FI_CHECK_LAUNCH();
+  const CeFactors fac = {gloss, d->reduction, ws.parts + 2 * CE_PARTS, sv, (int)s.pair, ws.scal, ws.g, ws.meta, bias, ws.bias_pad, labels,
+                         d->ltype, d->V, d->T, d->ignore_index, (char*)dx, (i64)d->D * (d->dtype == FI_F32 ? 4 : 2)};
+  const bool few = d->T <= 4096;                                        // (a launch less; its workgroups cover every row: 64 of them to a workgroup's 256)
+  if ((rc = ce_pack(px, pw, st, few ? fac : CeFactors{}))) return rc;
+  if (!few) {
+    hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)((d->T + 255) / 256)), dim3(256), 0, st, fac);
+    FI_CHECK_LAUNCH();
+  }
   const int f = s.pair ? 2 : 1;
   CeGrad gx = {}, gw = {};
   gx.a = ws.dl, gx.lda = ws.ld_dl, gx.ldb = ws.ld_wt, gx.N = d->D, gx.count = sv.count, gx.rows_are_tokens = 1;
@@ -1508,7 +1553,8 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   gx.vec = d->D % 8 == 0 && ((uintptr_t)dx & 15) == 0, gw.vec = d->D % 8 == 0 && ((uintptr_t)dw & 15) == 0;
   CeLogits a = {};
   a.x = ws.xc, a.ldx = s.ldx, a.w = s.w_direct ? w : ws.wc, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
-  a.scal = s.pair ? ws.scal : nullptr, a.s = sv, a.g = ws.g, a.dl = ws.dl, a.dlt = ws.dlt, a.ld_dl = ws.ld_dl, a.ld_dlt = ws.ld_dlt, a.db = ws.db;
+  a.scal = s.pair && s.scaled ? ws.scal : nullptr, a.s = sv, a.g = ws.g, a.dl = ws.dl, a.dlt = ws.dlt, a.ld_dl = ws.ld_dl, a.ld_dlt = ws.ld_dlt, a.db = ws.db;
+  if (db && d->T <= CE_BM[ce_logits_tile(*d)]) a.db = nullptr, a.db_out = db, a.db_add = db_accumulate, a.rg = ws.scal + SC_RG;
   const int wsize = d->wdtype == FI_F32 ? 4 : 2;
   // the classes innermost: dx of a row piece is complete with its last class piece, dW's parts are joined behind the last row piece
   const i64 nt = (d->T + ws.Tc - 1) / ws.Tc, nv = (d->V + ws.Vc - 1) / ws.Vc;
@@ -1536,7 +1582,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
       if (gw.part && it == nt - 1 && (rc = ce_join(gw, st))) return rc;
     }
   }
-  if (db) {
+  if (db && !a.db_out) {
     hipLaunchKernelGGL(ce_dbias_kernel, dim3((unsigned)((d->V + 15) / 16)), dim3(1024), 0, st, ws.db, CE_BM[ce_logits_tile(*d)], 0, d->V, sv.count, ws.scal, db, db_accumulate);
     FI_CHECK_LAUNCH();
   }
