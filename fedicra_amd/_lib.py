@@ -146,7 +146,8 @@ def ptr(t):
 
 
 def stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current stream's handle (by way of a torch.cuda.Stream object it costs several launches' worth of host time)."""
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _dev(t):
@@ -1201,24 +1202,25 @@ def _address(t):
     return None if t is None else t.data_ptr()
 
 
+_P = C.c_void_p
+
+
 def linear_ce_fwd(d, x, w, bias, labels, loss):
     """Returns the buffer the backward pass needs."""
     dev, so, ref = _dev(x).device, lib(), C.byref(d)
-    pw = C.c_void_p(w.data_ptr())
+    pw = _P(w.data_ptr())
     saved = _scratch(so.fi_linear_ce_saved(ref), "fi_linear_ce_saved", dev)
     ws = _scratch(so.fi_linear_ce_fwd_workspace(ref, pw), "fi_linear_ce_fwd_workspace", dev)
-    _chk(so.fi_linear_ce_fwd(ref, C.c_void_p(x.data_ptr()), pw, C.c_void_p(_address(bias)), C.c_void_p(labels.data_ptr()),
-                             C.c_void_p(loss.data_ptr()), C.c_void_p(saved.data_ptr()), C.c_void_p(ws.data_ptr()), stream()),
-         "fi_linear_ce_fwd")
+    _chk(so.fi_linear_ce_fwd(ref, _P(x.data_ptr()), pw, _P(_address(bias)), _P(labels.data_ptr()), _P(loss.data_ptr()),
+                             _P(saved.data_ptr()), _P(ws.data_ptr()), stream()), "fi_linear_ce_fwd")
     return saved
 
 
 def linear_ce_bwd(d, x, w, bias, labels, saved, gloss, dx, dw, dw_accumulate, db, db_accumulate):
     so, ref = lib(), C.byref(d)
-    pw = C.c_void_p(w.data_ptr())
+    pw = _P(w.data_ptr())
     size = so.fi_linear_ce_bwd_workspace(ref, pw, int(dx is not None), int(dw is not None), int(db is not None))
     ws = _scratch(size, "fi_linear_ce_bwd_workspace", _dev(x).device)
-    _chk(so.fi_linear_ce_bwd(ref, C.c_void_p(x.data_ptr()), pw, C.c_void_p(_address(bias)), C.c_void_p(labels.data_ptr()),
-                             C.c_void_p(saved.data_ptr()), C.c_void_p(gloss.data_ptr()), C.c_void_p(_address(dx)), C.c_void_p(_address(dw)),
-                             int(dw_accumulate), C.c_void_p(_address(db)), int(db_accumulate), C.c_void_p(ws.data_ptr()), stream()),
-         "fi_linear_ce_bwd")
+    _chk(so.fi_linear_ce_bwd(ref, _P(x.data_ptr()), pw, _P(_address(bias)), _P(labels.data_ptr()), _P(saved.data_ptr()),
+                             _P(gloss.data_ptr()), _P(_address(dx)), _P(_address(dw)), int(dw_accumulate), _P(_address(db)),
+                             int(db_accumulate), _P(ws.data_ptr()), stream()), "fi_linear_ce_bwd")

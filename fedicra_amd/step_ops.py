@@ -94,14 +94,17 @@ def _dense_rows(t, rows, cols):
     return t if (t.stride(1) == 1 or cols == 1) and apart else t.contiguous()
 
 
+def _fp32_row(t):
+    return t if t is None or t.dtype == torch.float32 and t.is_contiguous() else t.detach().float().contiguous()
+
+
 class _LinearCE(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, labels, ignore_index, reduction):
         V, D = weight.shape[:2]
         T = labels.numel()
         x2, w2 = _dense_rows(x, T, D), _dense_rows(weight, V, D)
-        b2 = None if bias is None else bias.detach().float().contiguous()
-        l2 = labels.contiguous()
+        b2, l2 = _fp32_row(bias), labels.contiguous()
         loss = torch.empty(labels.shape if reduction == "none" else (), dtype=torch.float32, device=x.device)
         with _on(x.device):
             desc = L.linear_ce_desc(x2, w2, l2, ignore_index, reduction)
@@ -116,8 +119,7 @@ class _LinearCE(Function):
         x, weight, bias, labels, saved = ctx.saved_tensors
         V, D = weight.shape[:2]
         x2, w2 = _dense_rows(x, labels.numel(), D), _dense_rows(weight, V, D)
-        b2 = None if bias is None else bias.detach().float().contiguous()
-        l2 = labels.contiguous()
+        b2, l2 = _fp32_row(bias), labels.contiguous()
         gl = g.to(torch.float32).contiguous()
         dx = dw = db = gw = gb = None
         dw_add = db_add = False
@@ -131,7 +133,7 @@ class _LinearCE(Function):
             else:
                 db = torch.empty(V, dtype=torch.float32, device=x.device)
         with _on(x.device):
-            desc = L.linear_ce_desc(x2, w2, l2, ctx.ignore_index, ctx.reduction)
+            desc = L.linear_ce_desc(x2, w2, l2, ctx.ignore_index, ctx.reduction)    # (a hook on saved tensors may have moved the rows together)
             L.linear_ce_bwd(desc, x2, w2, b2, l2, saved, gl, dx, dw, dw_add, db, db_add)
         if db is not None and bias.dtype != torch.float32:
             gb = db.to(bias.dtype)
@@ -164,8 +166,8 @@ def linear_ce_loss(x, weight, bias, labels, ignore_index=-100, reduction="mean")
         raise L.FiError(f"linear_ce_loss: labels are int64, int32 or uint8, not {labels.dtype}")
     if L.dt(weight.dtype) != L.dt(x.dtype) and weight.dtype != torch.float32:
         raise L.FiError(f"linear_ce_loss: weight is of x's type or fp32, not {weight.dtype} for {x.dtype}")
-    for t in (x, weight, labels) + (() if bias is None else (bias,)):
-        L._dev(t)
-        if t.device != x.device:
+    dev = L._dev(x).device
+    for t in (weight, labels) if bias is None else (weight, labels, bias):
+        if L._dev(t).device != dev:
             raise ValueError("linear_ce_loss: x, weight, bias and labels live on one device")
     return _LinearCE.apply(x, weight, bias, labels, int(ignore_index), reduction)
