@@ -303,9 +303,12 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw, CeFa
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) a.put[0] = sc, a.rput[0] = 1.f / sc;
   }
   if (r0 >= rows || c0 >= (a.same && a.same_k > a.D ? a.same_k : a.D)) return;
-  for (int e = tid; e < 64 * 8; e += 256) {
-    const i64 r = r0 + (e >> 3);
-    const int c = c0 + (e & 7) * 8, left = r < rows ? a.D - c : 0;
+  // 8 columns a lane, as many lanes a row as the block has columns for (a power of two)
+  const int cols = (a.same && a.same_k > a.D ? a.same_k : a.D) - c0, sh = cols > 32 ? 3 : cols > 16 ? 2 : cols > 8 ? 1 : 0;
+  for (int e = tid; e < 64 << sh; e += 256) {
+    const int er = e >> sh, ec = (e & ((1 << sh) - 1)) * 8;
+    const i64 r = r0 + er;
+    const int c = c0 + ec, left = r < rows ? a.D - c : 0;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (left > 0) {
       const i64 at = (a.idx ? (i64)a.idx[a.begin + r] : r) * a.ld + c;
@@ -331,14 +334,14 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw, CeFa
     }
     if (a.turned) {
 #pragma unroll
-      for (int t = 0; t < 8; ++t) tile[e >> 3][(e & 7) * 8 + t] = v[t] * sc;
+      for (int t = 0; t < 8; ++t) tile[er][ec + t] = v[t] * sc;
     }
   }
   if (!a.turned) return;
   __syncthreads();
   for (int e = tid; e < 64 * 8; e += 256) {
     const int r = e >> 3, c = (e & 7) * 8;
-    if (c0 + r >= a.D) continue;
+    if (c0 + r >= a.D) break;
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = tile[c + i][r];
@@ -883,7 +886,7 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
   typedef __attribute__((address_space(3))) char* lds_ptr_t;
   typedef typename DT<T>::frag_t frag_t;
   const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr_t)smem;
-  const int n = a.s.count[0], M = DW ? a.V : n, S = DW ? n : a.V, D = FWD ? 1 : a.out.N;
+  const int n = a.s.count[0], M = DW ? a.V : n, S = DW ? n : a.V, D = a.out.N, width = (D + 7) & ~7;
   int ti, sp;
   if (!ce_tile((M + 255) / 256, a.out.splits, ti, sp)) return;
   const int tiles = (S + 63) / 64, per = (tiles + a.out.splits - 1) / a.out.splits, t0 = sp * per < tiles ? sp * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
@@ -904,7 +907,8 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
       voff[q] = (unsigned)(r < D ? r : D - 1) * (unsigned)(a.ld_turned * 2) + (unsigned)(((l & 7) ^ (l >> 3)) * 16);
     } else {
       const int r = (id & 7) * 8 + (l >> 3);
-      voff[q] = (unsigned)r * (unsigned)(a.ld_tile * 2) + (unsigned)((id >> 3) * 128 + (((l & 7) ^ (((l >> 3) & 3) | ((id & 1) << 2))) * 16));
+      const int c = (id >> 3) * 64 + ((l & 7) ^ (((l >> 3) & 3) | ((id & 1) << 2))) * 8;
+      voff[q] = c < width ? (unsigned)r * (unsigned)(a.ld_tile * 2) + (unsigned)(c * 2) : 0x80000000u;       // (behind a row's end: beyond the resource)
     }
   }
   auto fetch = [&](int t, int slot) {
@@ -914,8 +918,9 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
 #pragma unroll
       for (int q = 0; q < Q; ++q) nt_dma16(rs, base + (unsigned)(S_BYTES + (wq * Q + q) * 1024), voff[q], 0u);
     } else {
-      // (rows behind the last one lie beyond the resource: zeros)
-      const nt_v4i rs = nt_rsrc((const T*)a.tile + (i64)t * 64 * a.ld_tile, ((unsigned long long)(S - t * 64 - 1) * a.ld_tile + KD * 32) * 2);
+      // (rows behind the last one lie beyond the resource, which stays below 2^31 bytes: zeros)
+      const int rows = S - t * 64 < 64 ? S - t * 64 : 64;
+      const nt_v4i rs = nt_rsrc((const T*)a.tile + (i64)t * 64 * a.ld_tile, ((unsigned long long)(rows - 1) * a.ld_tile + width) * 2);
 #pragma unroll
       for (int q = 0; q < Q; ++q) nt_dma16(rs, base + (unsigned)((wq * Q + q) * 1024), voff[q], 0u);
       if (w == 0) {
@@ -934,7 +939,7 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
   for (int i = 0; i < 2; ++i) {
     const int o = o0 + i * 16 + lr, oc = o < M ? o : M - 1;
 #pragma unroll
-    for (int k = 0; k < KD; ++k) own[i][k] = *(const frag_t*)((const T*)a.own + (i64)oc * a.ld_own + k * 32 + g * 8);
+    for (int k = 0; k < KD; ++k) own[i][k] = k * 32 + g * 8 < width ? *(const frag_t*)((const T*)a.own + (i64)oc * a.ld_own + k * 32 + g * 8) : frag_t{};
     m2[i] = y[i] = gg[i] = b[i] = 0.f, lab[i] = -1;
     if constexpr (DW) {
       b[i] = a.bias[oc];
@@ -957,6 +962,7 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
     const int slot = (t - t0) & 1;
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (t + 1 < t1) fetch(t + 1, slot ^ 1);
+    if (o0 >= M) continue;                                              // (a wave without rows only fetches)
     const char* const sm = smem + slot * SLOT;
     const float4* const xm = (const float4*)(sm + S_BYTES + T_BYTES);
     f32x4 z[2][4];
@@ -972,7 +978,8 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
       }
     }
 #pragma unroll
-    for (int k = 0; k < KD; ++k)
+    for (int k = 0; k < KD; ++k) {
+      if (KD == 2 && k == 1 && width <= 32) break;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 32 * (j >> 1) + 8 * (lr >> 2) + 4 * (j & 1) + (lr & 3), c = (k & 1) * 4 + g;
@@ -980,6 +987,7 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) z[i][j] = mfma16(f, own[i][k], z[i][j]);
       }
+    }
     if constexpr (FWD) {
       if (t * 64 + 64 > S) {
 #pragma unroll
@@ -1057,6 +1065,7 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
         for (int e = 0; e < 4; ++e) gf[i][e] = (f16_t)z[i][2 * q][e], gf[i][4 + e] = (f16_t)z[i][2 * q + 1][e];
 #pragma unroll
       for (int d = 0; d < 2 * KD; ++d) {
+        if (KD == 2 && d * 16 >= D) break;
         const int r = d * 16 + lr;
         const f16x8 f = *(const f16x8*)(sm + S_BYTES + r * 128 + (((q * 4 + g) ^ (r & 7)) * 16));
 #pragma unroll
@@ -1129,24 +1138,29 @@ struct Carve {
 };
 
 struct CeShape {
-  bool pair;
+  bool pair, fused;
   int ku;                  // values per stage
   int kp;                  // D padded to stages
+  int kw;                  // packed rows' width: kp; in the fused form, which masks the rest of a stage, a multiple of 8
   i64 ldx;                 // packed operand rows, elements
   bool w_direct;           // W is used where it lies
   i64 ldw;
   bool scaled;             // scales are computed (pair forms, or fp16 made of bf16)
 };
-CeShape ce_shape(const FiLinearCe& d, const void* w) {
+// Logits and G stay in registers (ce_fused_kernel) for 16-bit operands of up to 128 features; rows up to where a turned operand's offsets fit 32 bits
+// (forward pass of up to 64 rows: the 64 x 256 tiles of the general product read the classes with more workgroups)
+CeShape ce_shape(const FiLinearCe& d, const void* w, bool fwd) {
   CeShape s;
   // Half precision keeps 11 bits, as many as G does: up to 2^28 multiply-adds, where three products cost no more than one, it goes as pairs too, and
   // its gradients are rounded once (over 80 sizes, those more than 1.5 times an fp32 product's error off fell from 10 to none)
   s.pair = d.dtype == FI_F32 || (d.dtype == FI_F16 && (double)d.T * d.V * d.D <= (double)(1 << 28));
   s.ku = s.pair ? 32 : 64;
   s.kp = (int)ce_up(d.D, s.ku);
-  s.ldx = s.pair ? 2L * s.kp : s.kp;
-  // 16-bit weights whose rows are whole stages and 16-byte aligned are read in place
-  s.w_direct = !s.pair && d.wdtype == d.dtype && d.D % 64 == 0 && d.ldw % 8 == 0 && ((uintptr_t)w & 15) == 0;
+  s.fused = !s.pair && s.kp <= 128 && d.T <= (1 << 23) && !(fwd && d.T <= 64);
+  s.kw = s.fused ? (int)ce_up(d.D, 8) : s.kp;
+  s.ldx = s.pair ? 2L * s.kw : s.kw;
+  // 16-bit weights whose rows need no padding and are 16-byte aligned are read in place
+  s.w_direct = !s.pair && d.wdtype == d.dtype && d.D == s.kw && d.ldw % 8 == 0 && ((uintptr_t)w & 15) == 0;
   s.ldw = s.w_direct ? d.ldw : s.ldx;
   s.scaled = d.dtype != FI_F16 || (s.pair && d.wdtype != FI_F16);       // (fp16 values are their own high parts)
   return s;
@@ -1238,10 +1252,6 @@ int ce_amax(const FiLinearCe& d, const void* x, const void* w, const CeSaved& s,
   return 0;
 }
 
-// Logits and G stay in registers (ce_fused_kernel) for 16-bit operands of up to 128 features; rows up to where a turned operand's offsets fit 32 bits
-bool ce_fused_ok(const FiLinearCe& d, const CeShape& s) { return !s.pair && s.kp <= 128 && d.T <= (1 << 23); }
-// (up to 64 rows the 64 x 256 tiles of the general product read the classes with more workgroups)
-bool ce_fused_fwd_ok(const FiLinearCe& d, const CeShape& s) { return ce_fused_ok(d, s) && d.T > 64; }
 // parts of the streamed side: enough workgroups (of 256 own rows) to fill the chip twice, no fewer than 8 tiles of 64 each
 int ce_fused_splits(i64 own, i64 streamed) {
   const i64 wgs = (own + 255) / 256, tiles = (streamed + 63) / 64;
@@ -1284,10 +1294,9 @@ CeFwdWs ce_fwd_ws(const FiLinearCe& d, const CeShape& s, void* p) {
   w.sums = c.take<double>(CE_LOSS_WGS);
   w.xc = c.take<f16_t>(d.T * s.ldx);
   w.wc = s.w_direct ? nullptr : c.take<f16_t>((i64)d.V * s.ldx);
-  const bool fused = ce_fused_fwd_ok(d, s);
   const int bn = CE_BN[ce_logits_tile(d)];
-  w.nparts = fused ? ce_fused_splits(d.T, d.V) : (d.V + bn - 1) / bn;
-  w.bias_pad = fused ? c.take<float>(ce_up(d.V, 64)) : nullptr;
+  w.nparts = s.fused ? ce_fused_splits(d.T, d.V) : (d.V + bn - 1) / bn;
+  w.bias_pad = s.fused ? c.take<float>(ce_up(d.V, 64)) : nullptr;
   w.part = c.take<float2>(d.T * w.nparts);
   w.bytes = c.at;
   return w;
@@ -1298,14 +1307,14 @@ CePack ce_pack_x(const FiLinearCe& d, const CeShape& s, const void* x, const CeS
   CePack k = {};
   k.src = x, k.dtype = d.dtype, k.D = d.D, k.vec = ce_vec(x, d.dtype, d.ldx), k.ld = d.ldx, k.rows = d.T, k.idx = sv.idx, k.count = sv.count;
   if (scal) k.part = parts, k.scale = parts ? nullptr : scal + SC_X, k.put = scal + SC_X, k.rput = scal + SC_RX;
-  k.same = xc, k.ld_same = s.ldx, k.same_k = s.kp, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
+  k.same = xc, k.ld_same = s.ldx, k.same_k = s.kw, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
   return k;
 }
 CePack ce_pack_w(const FiLinearCe& d, const CeShape& s, const void* w, const float* parts, float* scal, f16_t* wc) {
   CePack k = {};
   k.src = w, k.dtype = d.wdtype, k.D = d.D, k.vec = ce_vec(w, d.wdtype, d.ldw), k.ld = d.ldw, k.rows = d.V;
   if (scal) k.part = parts ? parts + CE_PARTS : nullptr, k.scale = parts ? nullptr : scal + SC_W, k.put = scal + SC_W, k.rput = scal + SC_RW;
-  k.same = wc, k.ld_same = s.ldx, k.same_k = s.kp, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
+  k.same = wc, k.ld_same = s.ldx, k.same_k = s.kw, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
   return k;
 }
 
@@ -1334,7 +1343,6 @@ CeGradPlan ce_grad_plan(i64 M, i64 N, i64 K, int ku, bool pieces) {
 struct CeBwdWs {
   float *parts, *scal, *g, *db, *pdx, *pdw, *bias_pad;
   float4* meta;
-  bool fused;
   int sdx, sdw;
   f16_t *xc, *wc, *xt, *wt, *dl, *dlt;
   i64 ld_xt, ld_wt, ld_dl, ld_dlt, Tc;
@@ -1359,8 +1367,7 @@ CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need
   w.scal = c.take<float>(SC_N);
   w.g = c.take<float>(d.T);
   w.meta = nullptr, w.bias_pad = nullptr;
-  w.fused = ce_fused_ok(d, s);
-  if (w.fused) {
+  if (s.fused) {
     w.sdx = ce_fused_splits(d.T, d.V), w.sdw = ce_fused_splits(d.V, d.T);
     w.ld_xt = Tp, w.ld_wt = Vp, w.Tc = Tp;
     w.meta = c.take<float4>(ce_up(d.T, 64));
@@ -1429,7 +1436,7 @@ extern "C" long fi_linear_ce_saved(const FiLinearCe* d) {
 }
 extern "C" long fi_linear_ce_fwd_workspace(const FiLinearCe* d, const void* w) {
   const int rc = ce_check(d);
-  return rc ? rc : ce_fwd_ws(*d, ce_shape(*d, w), nullptr).bytes;
+  return rc ? rc : ce_fwd_ws(*d, ce_shape(*d, w, true), nullptr).bytes;
 }
 extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* w, const float* bias, const void* labels, float* loss,
                                 void* saved, void* workspace, void* stream) {
@@ -1437,7 +1444,7 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
   if (rc) return rc;
   if (!x || !w || !labels || !loss || !saved || !workspace) return FI_ERR_NULL;
   hipStream_t st = (hipStream_t)stream;
-  const CeShape s = ce_shape(*d, w);
+  const CeShape s = ce_shape(*d, w, true);
   const CeFwdWs ws = ce_fwd_ws(*d, s, workspace);
   const CeSaved sv = ce_saved(saved, d->T);
   float* const rows_out = d->reduction == 0 ? loss : nullptr;
@@ -1452,9 +1459,9 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
   if (scal && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
   if ((rc = ce_pack(ce_pack_x(*d, s, x, sv, ws.parts, scal, ws.xc), s.w_direct ? CePack{} : ce_pack_w(*d, s, w, ws.parts, scal, ws.wc), st))) return rc;
   const void* const wop = s.w_direct ? w : (const void*)ws.wc;
-  if (ce_fused_fwd_ok(*d, s)) {
+  if (s.fused) {
     CeFused a = {};
-    a.out.M = (int)d->T, a.out.splits = ws.nparts, a.s = sv, a.own = ws.xc, a.ld_own = s.ldx, a.tile = wop, a.ld_tile = s.ldw;
+    a.out.M = (int)d->T, a.out.N = d->D, a.out.splits = ws.nparts, a.s = sv, a.own = ws.xc, a.ld_own = s.ldx, a.tile = wop, a.ld_tile = s.ldw;
     a.bias = ws.bias_pad, a.V = d->V, a.part = ws.part, a.zt = ws.zt;
     if ((rc = ce_fused<CE_FWD>(a, *d, s.kp, st))) return rc;
   } else {
@@ -1485,7 +1492,7 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
 
 extern "C" long fi_linear_ce_bwd_workspace(const FiLinearCe* d, const void* w, int need_dx, int need_dw, int need_db) {
   const int rc = ce_check(d);
-  return rc ? rc : ce_bwd_ws(*d, ce_shape(*d, w), need_dx != 0, need_dw != 0, need_db != 0, nullptr).bytes;
+  return rc ? rc : ce_bwd_ws(*d, ce_shape(*d, w, false), need_dx != 0, need_dw != 0, need_db != 0, nullptr).bytes;
 }
 extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* w, const float* bias, const void* labels, const void* saved,
                                 const float* gloss, void* dx, void* dw, int dw_accumulate, float* db, int db_accumulate, void* workspace,
@@ -1496,7 +1503,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   if (dw_accumulate && d->wdtype != FI_F32) return FI_ERR_DTYPE;
   if (!dx && !dw && !db) return 0;
   hipStream_t st = (hipStream_t)stream;
-  const CeShape s = ce_shape(*d, w);
+  const CeShape s = ce_shape(*d, w, false);
   const CeBwdWs ws = ce_bwd_ws(*d, s, dx != nullptr, dw != nullptr, db != nullptr, workspace);
   const CeSaved sv = ce_saved((void*)saved, d->T);
   // (the pair form's scales were made by the forward pass)
@@ -1526,7 +1533,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   gx.splits = ws.dx.splits, gx.out = dx, gx.out_dtype = d->dtype, gx.ldo = d->D, gx.idx = sv.idx, gx.scal = ws.scal, gx.rscale = s.scaled ? SC_RW : -1;
   gw.a = ws.dlt, gw.lda = ws.ld_dlt, gw.ldb = ws.ld_xt, gw.N = d->D, gw.count = sv.count;
   gw.splits = ws.dw.splits, gw.out_dtype = d->wdtype, gw.accumulate = dw_accumulate, gw.ldo = d->D, gw.scal = ws.scal, gw.rscale = s.scaled ? SC_RX : -1;
-  if (ws.fused) {
+  if (s.fused) {
     const void* const wop = s.w_direct ? w : (const void*)ws.wc;
     CeFused a = {};
     a.s = sv, a.meta = ws.meta, a.bias = ws.bias_pad, a.V = d->V;
