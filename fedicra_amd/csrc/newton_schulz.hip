@@ -10,7 +10,12 @@
 // Work per step: m^2 n + m^3 multiply-adds halved by symmetry + m^2 n: A and S are computed on and below the diagonal and stored twice.  Every
 // product's second operand is wanted with its contraction index contiguous, so X is kept in both orientations (X for A, X^T for S X); the
 // product that makes the next X stores both.  All matrices of a call (one model's filters) share each launch: 2, and 3 (4 where A's contraction is
-// split) per step, whatever their number; where none has more than 64 rows, one per step (ns_narrow_step_kernel).
+// split) per step, whatever their number; where none has more than 64 rows, one per step (ns_narrow_step_kernel).  Matrices of up to 16 rows are done
+// with the first two (ns_short_apply).
+//
+// Measured (five steps): 2048 x 8192 bf16 1.73 ms, 968 TFLOP/s of matrix instructions where a large library product reaches 1430 -- per step S X 180 us
+// (1145 TFLOP/s), A 106, its join 26, S 46 (560: 528 tiles of 64); 4096 x 1024 fp32 413 us; 1000 x 1537 bf16 276 us (tiles for 1.6 rounds of
+// the chip and 15 us a product: latency); a U-Net's 23 filters fp32 188 us (22 launches of 6 .. 15 us); 64 x 576 fp32 70 us (7 of 8 .. 11 us).
 #include <math.h>
 
 #include "nt_product.h"
@@ -25,10 +30,10 @@ struct NsItem {
   const void* u;
   void* out;
   unsigned base;                                 // its place in the workspace, in 256 bytes
-  int m, n, tall, dtype, split;
+  int m, n, tall, dtype, split;                  // split: parts of A's contraction; 0: the short form
 };
 // Work items of a launch, by kind
-enum { NS_SUMS, NS_PREP, NS_A, NS_JOIN, NS_S, NS_X, NS_NARROW, NS_KINDS };
+enum { NS_SUMS, NS_PREP, NS_A, NS_JOIN, NS_S, NS_X, NS_NARROW, NS_SHORT, NS_KINDS };
 // The call's matrices on the device, at the head of the workspace.  They travel once, as the first kernel's arguments; that kernel leaves them here
 // and the others get a pointer: arguments of kilobytes cost the host some microseconds per launch.
 struct NsTable {
@@ -40,12 +45,19 @@ struct NsArgs {
   NsItem it[NS_MAX];
   int count, narrow, tile[3];
   float eps;
+  int first[NS_MAX];                             // each matrix's first work item of the first launch
 };
 static_assert(sizeof(NsArgs) <= 4096, "kernel arguments");
 struct NsCtl {
   char* ws;
   int count, cur, last;
   float ca, cb, cc, eps;
+};
+// the short form takes all steps in one launch, whose first `items` workgroups are the other matrices'
+constexpr int NS_STEPS = 32;
+struct NsAll {
+  int items, steps;
+  float c[3 * NS_STEPS];
 };
 
 __device__ __host__ __forceinline__ int ns_pad(int v) { return (v + 31) & ~31; }
@@ -102,8 +114,16 @@ __device__ __host__ __forceinline__ NsNarrow ns_narrow_mem(char* p, const NsItem
   return r;
 }
 
+// matrices of at most 16 rows, see further down: columns per workgroup -- whole tiles of 64, at most 128 workgroups
+__device__ __host__ __forceinline__ int ns_short_cols(int n) {
+  const int per = ((n + 127) / 128 + 63) & ~63;
+  return per < 256 ? 256 : per;
+}
+
 // how many work items of a kind a matrix has (T: the launch's tile)
 __device__ __host__ __forceinline__ long ns_items(const NsItem& q, int kind, int T) {
+  if (!q.split) return kind == NS_SUMS || kind == NS_SHORT ? (q.n + ns_short_cols(q.n) - 1) / ns_short_cols(q.n) : 0;
+  if (kind == NS_SHORT) return 0;
   const long mt = (q.m + T - 1) / T, nt = (q.n + T - 1) / T, tri = mt * (mt + 1) / 2;
   return kind == NS_SUMS ? ns_sums(q) : kind == NS_A ? tri * q.split : kind == NS_JOIN ? (q.split > 1 ? tri : 0)
          : kind == NS_S ? tri : kind == NS_NARROW ? ns_chunks(q.n) : mt * nt;
@@ -148,11 +168,116 @@ __device__ __forceinline__ double ns_squares(const T* p, long n) {
   }
   return acc;
 }
-// the sums of squares; the first workgroup also leaves the table for the kernels behind
+// ---- matrices of at most 16 rows -------------------------------------------------------------------------------------------------------
+// The steps' matrices are all polynomials of G = U U^T and commute, so X after the last step is P X0 with a 16 x 16 matrix P:
+//     A <- G / (sqrt(trace G) + eps)^2,  P <- I;   per step  S = a I + b A + c A A,  P <- S P,  A <- S A S.
+// Squaring U loses half its digits and P's entries reach 3.4^steps, so all of it is fp64, for which 16 rows are little work: the result is off by its
+// rounding to fp32, where pairs are off by their 22 bits (and short sums show every rounding).  Two launches for any number of steps, both shared
+// with the other matrices of the call: G in parts of 256 columns or more, and P -- by every workgroup for itself, some 4 us for five steps -- with its
+// product with the workgroup's columns.
+constexpr int NS_SHORT_ROWS = 16, NS_SHORT_LDS = 4 * 16 * 18 * 8;
+constexpr int NS_GRAM_LD = 260;
+__device__ __forceinline__ void ns_short_gram(char* ws, const NsItem& q, int chunk, float* xs) {       // xs: [16][NS_GRAM_LD]
+  const int per = ns_short_cols(q.n), lo = chunk * per, hi = lo + per < q.n ? lo + per : q.n, tid = threadIdx.x, i = tid >> 4, j = tid & 15;
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int t = lo; t < hi; t += 256) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int e = k * 256 + tid, r = q.tall ? e & 15 : k, c = q.tall ? e >> 4 : tid;
+      xs[r * NS_GRAM_LD + c] = r < q.m && t + c < hi ? ns_load(q.u, q.dtype, q.tall ? (long)(t + c) * q.m + r : (long)r * q.n + t + c) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int c = 0; c < 256; c += 4) {
+      const float4 x = *(const float4*)(xs + i * NS_GRAM_LD + c), y = *(const float4*)(xs + j * NS_GRAM_LD + c);
+      acc[0] += (double)x.x * (double)y.x;
+      acc[1] += (double)x.y * (double)y.y;
+      acc[2] += (double)x.z * (double)y.z;
+      acc[3] += (double)x.w * (double)y.w;
+    }
+  }
+  ((double*)(ws + (long)q.base * 256))[chunk * 256 + tid] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+}
+// (the matrices are symmetric: a product's element is that of two rows, which are read in vectors)
+typedef double NsRow[18];
+__device__ __forceinline__ void ns_row16(const NsRow& a, double (&v)[16]) {
+#pragma unroll
+  for (int d = 0; d < 16; d += 2) {
+    const double2 x = *(const double2*)(a + d);
+    v[d] = x.x, v[d + 1] = x.y;
+  }
+}
+__device__ __forceinline__ double ns_dot16(const double (&a)[16], const double (&b)[16]) {
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+  for (int d = 0; d < 16; ++d) v[d & 3] += a[d] * b[d];
+  return (v[0] + v[1]) + (v[2] + v[3]);
+}
+template <typename T>
+__device__ __forceinline__ void ns_short_columns(const NsItem& q, int lo, int hi, const NsRow* P) {
+  const T* const u = (const T*)q.u;
+  T* const out = (T*)q.out;
+  const long sr = q.tall ? 1 : q.n, sc = q.tall ? q.m : 1;              // strides of X's rows and columns
+  for (int c = lo + (int)threadIdx.x; c < hi; c += 256) {               // (a column is read whole before it is written: out may be u)
+    double x[16];
+#pragma unroll
+    for (int d = 0; d < 16; ++d) x[d] = d < q.m ? (double)to_f32(u[d * sr + c * sc]) : 0.0;
+    for (int r = 0; r < q.m; ++r) {
+      double v = 0.0;
+#pragma unroll
+      for (int d = 0; d < 16; ++d) v += P[r][d] * x[d];
+      out[r * sr + c * sc] = (T)(float)v;
+    }
+  }
+}
+__device__ __forceinline__ void ns_short_apply(const NsCtl& g, const NsAll& all, int w, char* lds) {
+  NsRow *const A = (NsRow*)lds, *const S = A + 16, *const P = A + 32, *const B = A + 48;
+  int first;
+  const int k = ns_find(g, NS_SHORT, w, first), tid = threadIdx.x, i = tid >> 4, j = tid & 15;
+  const NsItem q = ns_table(g.ws)->it[k];
+  const int per = ns_short_cols(q.n), parts = (q.n + per - 1) / per, lo = (w - first) * per, hi = lo + per < q.n ? lo + per : q.n;
+  const double* const part = (const double*)(g.ws + (long)q.base * 256) + tid;
+  double v = 0.0, trace = 0.0;
+  for (int p = 0; p < parts; ++p) v += part[p * 256];
+  A[i][j] = v;
+  __syncthreads();
+#pragma unroll
+  for (int d = 0; d < 16; ++d) trace += A[d][d];
+  const double norm = sqrt(trace) + (double)g.eps, inv = norm == 0.0 ? 0.0 : 1.0 / norm;
+  __syncthreads();
+  A[i][j] = v * inv * inv;
+  P[i][j] = i == j ? inv : 0.0;
+  double a[16], f[16], x[16];
+  for (int s = 0; s < all.steps; ++s) {
+    __syncthreads();
+    ns_row16(A[i], a), ns_row16(A[j], x);
+    S[i][j] = (i == j ? (double)all.c[3 * s] : 0.0) + (double)all.c[3 * s + 1] * A[i][j] + (double)all.c[3 * s + 2] * ns_dot16(a, x);
+    __syncthreads();
+    ns_row16(S[j], x);
+    B[i][j] = ns_dot16(a, x);
+    ns_row16(S[i], f), ns_row16(P[j], x);
+    const double p = ns_dot16(f, x);
+    __syncthreads();
+    ns_row16(B[j], x);
+    P[i][j] = p;
+    A[i][j] = ns_dot16(f, x);
+  }
+  __syncthreads();
+  if (q.dtype == FI_F32)
+    ns_short_columns<float>(q, lo, hi, P);
+  else if (q.dtype == FI_BF16)
+    ns_short_columns<bf16_t>(q, lo, hi, P);
+  else
+    ns_short_columns<f16_t>(q, lo, hi, P);
+}
+
+// the sums of squares (the short form's G); the first workgroup also leaves the table for the kernels behind
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
   __shared__ double sm[4];
-  int k = 0, w = (int)blockIdx.x;
-  while (k + 1 < g.count && w >= ns_sums(g.it[k])) w -= ns_sums(g.it[k++]);
+  __shared__ __attribute__((aligned(16))) float xs[16 * NS_GRAM_LD];
+  const int at = (int)(threadIdx.x & 63) < g.count ? g.first[threadIdx.x & 63] : 0x7fffffff;
+  const int k = 63 - __builtin_clzll(__ballot(at <= (int)blockIdx.x)), w = (int)blockIdx.x - __builtin_amdgcn_readlane(at, k);
   const NsItem& q = g.it[k];
   if (blockIdx.x == 0 && threadIdx.x < 64) {
     NsTable* const t = (NsTable*)g.ws;
@@ -168,6 +293,10 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
       t->start[kind][l] = sum - n;
     }
   }
+  if (!q.split) {
+    ns_short_gram(g.ws, q, w, xs);
+    return;
+  }
   const long total = (long)q.m * q.n, lo = (long)w * NS_CHUNK, n = total - lo < NS_CHUNK ? total - lo : NS_CHUNK;
   double acc = q.dtype == FI_F32 ? ns_squares((const float*)q.u + lo, n) : q.dtype == FI_BF16 ? ns_squares((const bf16_t*)q.u + lo, n)
                                                                                            : ns_squares((const f16_t*)q.u + lo, n);
@@ -180,10 +309,15 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
 }
 
 // U, normalised, as pair rows in both orientations: one 64 x 64 block of U per workgroup
-__global__ __launch_bounds__(256) void ns_prep_kernel(NsCtl g) {
-  __shared__ float tile[64][65];
+__global__ __launch_bounds__(256) void ns_prep_kernel(NsCtl g, NsAll all) {
+  __shared__ __attribute__((aligned(16))) float tile[64][65];
   __shared__ double sm[4];
   __shared__ float s_inv;
+  static_assert(sizeof(tile) >= NS_SHORT_LDS, "LDS");
+  if ((int)blockIdx.x >= all.items) {
+    ns_short_apply(g, all, (int)blockIdx.x - all.items, (char*)tile);
+    return;
+  }
   int first;
   const int w = (int)blockIdx.x, k = ns_find(g, NS_PREP, w, first), tid = threadIdx.x;
   const NsItem q = ns_table(g.ws)->it[k];
@@ -434,10 +568,15 @@ __device__ __forceinline__ void ns_part_put(float* part, const f32x4 (&acc)[2][2
 }
 
 // normalises U into xt and makes the first partial A
-__global__ __launch_bounds__(256) void ns_narrow_prep_kernel(NsCtl g) {
+__global__ __launch_bounds__(256) void ns_narrow_prep_kernel(NsCtl g, NsAll all) {
   __shared__ __attribute__((aligned(16))) char pool[64 * 65 * 4 + NsPair64::BYTES];
   __shared__ double sm[4];
   __shared__ float s_inv;
+  static_assert(sizeof(pool) >= NS_SHORT_LDS, "LDS");
+  if ((int)blockIdx.x >= all.items) {
+    ns_short_apply(g, all, (int)blockIdx.x - all.items, pool);
+    return;
+  }
   float* const tile = (float*)pool;                                     // [row of X][65]
   const NsPair64 xa{pool + ((64 * 65 * 4 + 127) & ~127)};
   int first;
@@ -623,7 +762,7 @@ NsPlan ns_plan(const FiNsMat* const* mats, int count) {
 }
 
 // Fills in the matrices of a launch group; returns their workspace's size.
-long ns_layout(const FiNsMat* const* mats, int count, const NsPlan& plan, NsArgs& g) {
+long ns_layout(const FiNsMat* const* mats, int count, const NsPlan& plan, bool shorts, NsArgs& g) {
   long at = (sizeof(NsTable) + 255) & ~255L;
   g.count = count, g.narrow = plan.narrow;
   for (int k = 0; k < 3; ++k) g.tile[k] = plan.narrow ? 64 : plan.tile[k];
@@ -636,13 +775,11 @@ long ns_layout(const FiNsMat* const* mats, int count, const NsPlan& plan, NsArgs
     const int stages = ns_pad(q.n) / 32, per = (stages + plan.split - 1) / plan.split;
     q.split = (stages + per - 1) / per;          // (no part is empty)
     q.base = (unsigned)(at >> 8);
-    if (plan.narrow) {
-      at += ns_narrow_mem(nullptr, q).bytes;
-      continue;
-    }
-    const long side = ns_side(plan.tile[0]), mt = (q.m + side - 1) / side;
-    at += ns_mem(nullptr, q).bytes;
-    if (q.split > 1) at += 4L * (mt * (mt + 1) / 2) * q.split * side * side;
+    const long side = ns_side(plan.tile[0]), mt = (q.m + side - 1) / side, own = plan.narrow ? ns_narrow_mem(nullptr, q).bytes : ns_mem(nullptr, q).bytes;
+    const long few = q.m <= NS_SHORT_ROWS ? 2048L * ((q.n + ns_short_cols(q.n) - 1) / ns_short_cols(q.n)) : 0;      // (whichever form the steps' number allows)
+    at += own > few ? own : few;
+    if (!plan.narrow && q.split > 1) at += 4L * (mt * (mt + 1) / 2) * q.split * side * side;
+    if (shorts && q.m <= NS_SHORT_ROWS) q.split = 0;
   }
   return at;
 }
@@ -699,15 +836,18 @@ int ns_run(NsArgs& g, int steps, const float* coeffs, float eps, hipStream_t st)
   for (int k = 0; k < NS_KINDS; ++k)
     if ((n[k] = ns_total(g, k)) < 0) return FI_ERR_SHAPE;
   g.eps = eps;
+  for (int i = 0, at = 0; i < g.count; ++i) g.first[i] = at, at += (int)ns_items(g.it[i], NS_SUMS, 64);
   NsCtl c = {g.ws, g.count, 0, 0, 0.f, 0.f, 0.f, eps};
+  NsAll all = {n[g.narrow ? NS_NARROW : NS_PREP], steps, {}};
+  for (int k = 0; k < 3 * steps && k < 3 * NS_STEPS; ++k) all.c[k] = coeffs[k];
   hipLaunchKernelGGL(ns_norm_kernel, dim3(n[NS_SUMS]), dim3(256), 0, st, g);
   FI_CHECK_LAUNCH();
   if (g.narrow)
-    hipLaunchKernelGGL(ns_narrow_prep_kernel, dim3(n[NS_NARROW]), dim3(256), 0, st, c);
+    hipLaunchKernelGGL(ns_narrow_prep_kernel, dim3(all.items + n[NS_SHORT]), dim3(256), 0, st, c, all);
   else
-    hipLaunchKernelGGL(ns_prep_kernel, dim3(n[NS_PREP]), dim3(256), 0, st, c);
+    hipLaunchKernelGGL(ns_prep_kernel, dim3(all.items + n[NS_SHORT]), dim3(256), 0, st, c, all);
   FI_CHECK_LAUNCH();
-  for (int k = 0; k < steps; ++k) {
+  for (int k = 0; k < steps && all.items; ++k) {
     c.ca = coeffs[3 * k], c.cb = coeffs[3 * k + 1], c.cc = coeffs[3 * k + 2];
     c.cur = k & 1, c.last = k + 1 == steps;
     if (g.narrow) {
@@ -725,7 +865,7 @@ int ns_run(NsArgs& g, int steps, const float* coeffs, float eps, hipStream_t st)
 
 // f(arguments) for every launch group; the workspace is used again by each.  Returns its size, or an error (positive ones as -1000 - error).
 template <class F>
-long ns_groups(const FiNsMat* mats, int count, char* ws, F f) {
+long ns_groups(const FiNsMat* mats, int count, int steps, char* ws, F f) {
   long most = 0;
   for (int lo = 0; lo < count; lo += NS_MAX) {
     const FiNsMat* pick[NS_MAX];
@@ -734,7 +874,7 @@ long ns_groups(const FiNsMat* mats, int count, char* ws, F f) {
     const NsPlan plan = ns_plan(pick, n);
     NsArgs g = {};
     g.ws = ws;
-    const long bytes = ns_layout(pick, n, plan, g);
+    const long bytes = ns_layout(pick, n, plan, steps <= NS_STEPS, g);
     if (bytes >> 40) return FI_ERR_SHAPE;
     if (bytes > most) most = bytes;
     const int rc = f(g);
@@ -749,7 +889,7 @@ extern "C" long fi_newton_schulz_workspace(const FiNsMat* mats, int count) {
   const float c[3] = {0.f, 0.f, 0.f};
   const int rc = ns_check(mats, count, 1, c);
   if (rc) return rc;
-  return ns_groups(mats, count, nullptr, [](NsArgs&) { return 0; });
+  return ns_groups(mats, count, 1, nullptr, [](NsArgs&) { return 0; });
 }
 
 extern "C" int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const float* coeffs, float eps, void* workspace, void* stream) {
@@ -759,7 +899,7 @@ extern "C" int fi_newton_schulz(const FiNsMat* mats, int count, int steps, const
   for (int i = 0; i < count; ++i)
     if (!mats[i].u || !mats[i].out) return FI_ERR_NULL;
   hipStream_t st = (hipStream_t)stream;
-  const long got = ns_groups(mats, count, (char*)workspace, [&](NsArgs& g) { return ns_run(g, steps, coeffs, eps, st); });
+  const long got = ns_groups(mats, count, steps, (char*)workspace, [&](NsArgs& g) { return ns_run(g, steps, coeffs, eps, st); });
   return got >= 0 ? 0 : got > -1000 ? (int)got : (int)(-1000 - got);
 }
 

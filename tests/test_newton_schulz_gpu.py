@@ -67,6 +67,29 @@ def test_newton_schulz_of_many_matrices_in_one_call_equals_each_alone():
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+def test_newton_schulz_short_matrices_keep_their_accuracy_beside_large_ones():
+    """A matrix of up to 16 rows is taken through all its steps in 64 bits, whatever it is called with."""
+    short = [_update(3, 4, 7), _update(4, 2, 50), _update(5, 900, 16), _update(6, 1, 1)]
+    alone = ops.newton_schulz(short)
+    large = _update(7, 300, 520)
+    mixed = ops.newton_schulz([short[0], large, *short[1:], large])
+    for a, b in zip(alone, [mixed[0], *mixed[2:5]]):
+        assert torch.equal(a, b)
+    assert torch.equal(mixed[1], mixed[5])
+    _ns_check(mixed[1], large)
+    for u, got in zip(short, alone):
+        # X0 and the coefficients as the definition has them up to fp32's half step, 2^-24, each (5 steps of 3 coefficients, eps, the result's own
+        # rounding), every one of which moves a value of at most 1.2 by no more than its growth, 3.4445, times itself
+        assert (got.double() - _ns64(u)).abs().max().item() <= 17 * 1.2 * 3.4445 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("shape,dtype", [((5, 70000), F32), ((40000, 16), BF16), ((16, 257), F16), ((255, 3), F32), ((1, 33000), F32)])
+def test_newton_schulz_few_rows_over_long_ones(shape, dtype):
+    u = _update(70, *shape, dtype, 1.0)
+    _ns_check(ops.newton_schulz(u), u)
+    _ns_check(ops.newton_schulz(u, steps=33, coeffs=(1.0, 0.0, 0.0)), u, steps=33, coeffs=(1.0, 0.0, 0.0))      # more steps than one launch takes
+
+
 def test_newton_schulz_batch_strides_and_mixed_types():
     b = torch.stack([_update(i, 24, 50) for i in range(3)])
     for u, o in zip(b, ops.newton_schulz(b)):
