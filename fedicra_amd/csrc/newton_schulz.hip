@@ -308,11 +308,17 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
   if (threadIdx.x == 0) sums[w] = sm[0] + sm[1] + sm[2] + sm[3];
 }
 
+// storage's scale / (|U| + eps); a zero matrix stays one where eps is zero too
+__device__ __forceinline__ double ns_inverse(double squares, float eps) {
+  const double norm = sqrt(squares) + (double)eps;
+  return norm == 0.0 ? 0.0 : (double)NS_SCALE / norm;
+}
+
 // U, normalised, as pair rows in both orientations: one 64 x 64 block of U per workgroup
 __global__ __launch_bounds__(256) void ns_prep_kernel(NsCtl g, NsAll all) {
   __shared__ __attribute__((aligned(16))) float tile[64][65];
   __shared__ double sm[4];
-  __shared__ float s_inv;
+  __shared__ double s_inv;
   static_assert(sizeof(tile) >= NS_SHORT_LDS, "LDS");
   if ((int)blockIdx.x >= all.items) {
     ns_short_apply(g, all, (int)blockIdx.x - all.items, (char*)tile);
@@ -327,14 +333,14 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsCtl g, NsAll all) {
   acc = wave_sum(acc);
   if ((tid & 63) == 0) sm[tid >> 6] = acc;
   __syncthreads();
-  if (tid == 0) s_inv = (float)((double)NS_SCALE / (sqrt(sm[0] + sm[1] + sm[2] + sm[3]) + (double)g.eps));
+  if (tid == 0) s_inv = ns_inverse(sm[0] + sm[1] + sm[2] + sm[3], g.eps);
   __syncthreads();
-  const float inv = s_inv;
+  const double inv = s_inv;                                             // (past fp32's range where eps is zero and |U| next to it)
   const int rows = q.tall ? q.n : q.m, cols = q.tall ? q.m : q.n;
   const int nb = (cols + 63) / 64, t = w - first, r0 = (t / nb) * 64, c0 = (t % nb) * 64;
   for (int e = tid; e < 64 * 64; e += 256) {
     const int r = r0 + (e >> 6), c = c0 + (e & 63);
-    tile[e >> 6][e & 63] = r < rows && c < cols ? ns_load(q.u, q.dtype, (long)r * cols + c) * inv : 0.f;
+    tile[e >> 6][e & 63] = r < rows && c < cols ? (float)(ns_load(q.u, q.dtype, (long)r * cols + c) * inv) : 0.f;
   }
   __syncthreads();
   f16_t* const same = q.tall ? mem.xt[0] : mem.x;          // U's own orientation
@@ -571,7 +577,7 @@ __device__ __forceinline__ void ns_part_put(float* part, const f32x4 (&acc)[2][2
 __global__ __launch_bounds__(256) void ns_narrow_prep_kernel(NsCtl g, NsAll all) {
   __shared__ __attribute__((aligned(16))) char pool[64 * 65 * 4 + NsPair64::BYTES];
   __shared__ double sm[4];
-  __shared__ float s_inv;
+  __shared__ double s_inv;
   static_assert(sizeof(pool) >= NS_SHORT_LDS, "LDS");
   if ((int)blockIdx.x >= all.items) {
     ns_short_apply(g, all, (int)blockIdx.x - all.items, pool);
@@ -588,9 +594,9 @@ __global__ __launch_bounds__(256) void ns_narrow_prep_kernel(NsCtl g, NsAll all)
   sum = wave_sum(sum);
   if ((tid & 63) == 0) sm[tid >> 6] = sum;
   __syncthreads();
-  if (tid == 0) s_inv = (float)((double)NS_SCALE / (sqrt(sm[0] + sm[1] + sm[2] + sm[3]) + (double)g.eps));
+  if (tid == 0) s_inv = ns_inverse(sm[0] + sm[1] + sm[2] + sm[3], g.eps);
   __syncthreads();
-  const float inv = s_inv;
+  const double inv = s_inv;                                             // (past fp32's range where eps is zero and |U| next to it)
   const int tiles = (q.n + 63) / 64, P = ns_chunks(q.n), ch = (tiles + P - 1) / P;
   f32x4 acc[2][2] = {};
   for (int t = chunk * ch; t < tiles && t < chunk * ch + ch; ++t) {
@@ -598,7 +604,7 @@ __global__ __launch_bounds__(256) void ns_narrow_prep_kernel(NsCtl g, NsAll all)
     __syncthreads();
     for (int e = tid; e < 64 * 64; e += 256) {
       const int i = q.tall ? e & 63 : e >> 6, j = q.tall ? e >> 6 : e & 63;                    // X's row and column; along U's rows either way
-      tile[i * 65 + j] = i < q.m && c0 + j < q.n ? ns_load(q.u, q.dtype, q.tall ? (long)(c0 + j) * q.m + i : (long)i * q.n + c0 + j) * inv : 0.f;
+      tile[i * 65 + j] = i < q.m && c0 + j < q.n ? (float)(ns_load(q.u, q.dtype, q.tall ? (long)(c0 + j) * q.m + i : (long)i * q.n + c0 + j) * inv) : 0.f;
     }
     __syncthreads();
     for (int e = tid; e < 64 * 8; e += 256) {

@@ -136,6 +136,18 @@ def test_newton_schulz_extreme_values():
         _ns_check(got[1], good)                                       # its neighbour in the launch is not touched
 
 
+@pytest.mark.parametrize("shape", [(1, 1), (4, 5), (20, 30), (70, 90), (300, 270)])
+def test_newton_schulz_of_zeros_without_eps(shape):
+    u = torch.zeros(shape, device="cuda")
+    assert torch.equal(ops.newton_schulz(u, eps=0.0), u)
+    tiny = torch.full(shape, 2.0 ** -130, device="cuda")              # rank one: every entry 1 / sqrt(m n) of the polynomial of 1
+    s = 1.0
+    for _ in range(5):
+        s = COEFFS[0] * s + COEFFS[1] * s ** 3 + COEFFS[2] * s ** 5
+    want = s / math.sqrt(u.numel())
+    assert (ops.newton_schulz(tiny, eps=0.0).double() - want).norm().item() <= 4 * COEFFS[0] ** 5 * 2.0 ** -22
+
+
 def test_newton_schulz_graph_replays():
     us = [_update(i, 40 + i, 300, BF16) for i in range(3)]
     eager = ops.newton_schulz(us)
