@@ -273,9 +273,12 @@ __device__ __forceinline__ void ns_short_apply(const NsCtl& g, const NsAll& all,
 }
 
 // the sums of squares (the short form's G); the first workgroup also leaves the table for the kernels behind
+// (SHORT, here and below: with matrices of few rows among the others, whose form needs registers that would halve the others' waves: the next kernel
+// takes 54 us instead of 39 at 2048 x 8192)
+template <bool SHORT>
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
   __shared__ double sm[4];
-  __shared__ __attribute__((aligned(16))) float xs[16 * NS_GRAM_LD];
+  __shared__ __attribute__((aligned(16))) float xs[SHORT ? 16 * NS_GRAM_LD : 1];
   const int at = (int)(threadIdx.x & 63) < g.count ? g.first[threadIdx.x & 63] : 0x7fffffff;
   const int k = 63 - __builtin_clzll(__ballot(at <= (int)blockIdx.x)), w = (int)blockIdx.x - __builtin_amdgcn_readlane(at, k);
   const NsItem& q = g.it[k];
@@ -293,7 +296,7 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
       t->start[kind][l] = sum - n;
     }
   }
-  if (!q.split) {
+  if (SHORT && !q.split) {
     ns_short_gram(g.ws, q, w, xs);
     return;
   }
@@ -308,19 +311,20 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs g) {
   if (threadIdx.x == 0) sums[w] = sm[0] + sm[1] + sm[2] + sm[3];
 }
 
-// storage's scale / (|U| + eps); a zero matrix stays one where eps is zero too
-__device__ __forceinline__ double ns_inverse(double squares, float eps) {
-  const double norm = sqrt(squares) + (double)eps;
-  return norm == 0.0 ? 0.0 : (double)NS_SCALE / norm;
+// storage's scale / (|U| + eps) as x * y (y = 1 but past fp32's range, where eps is zero and |U| next to it); a zero matrix stays one where eps is zero too
+__device__ __forceinline__ float2 ns_inverse(double squares, float eps) {
+  const double norm = sqrt(squares) + (double)eps, inv = norm == 0.0 ? 0.0 : (double)NS_SCALE / norm;
+  return inv > 0x1p100 ? make_float2((float)(inv * 0x1p-80), 0x1p80f) : make_float2((float)inv, 1.f);
 }
 
 // U, normalised, as pair rows in both orientations: one 64 x 64 block of U per workgroup
+template <bool SHORT>
 __global__ __launch_bounds__(256) void ns_prep_kernel(NsCtl g, NsAll all) {
   __shared__ __attribute__((aligned(16))) float tile[64][65];
   __shared__ double sm[4];
-  __shared__ double s_inv;
+  __shared__ float2 s_inv;
   static_assert(sizeof(tile) >= NS_SHORT_LDS, "LDS");
-  if ((int)blockIdx.x >= all.items) {
+  if (SHORT && (int)blockIdx.x >= all.items) {
     ns_short_apply(g, all, (int)blockIdx.x - all.items, (char*)tile);
     return;
   }
@@ -335,12 +339,12 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsCtl g, NsAll all) {
   __syncthreads();
   if (tid == 0) s_inv = ns_inverse(sm[0] + sm[1] + sm[2] + sm[3], g.eps);
   __syncthreads();
-  const double inv = s_inv;                                             // (past fp32's range where eps is zero and |U| next to it)
+  const float2 inv = s_inv;
   const int rows = q.tall ? q.n : q.m, cols = q.tall ? q.m : q.n;
   const int nb = (cols + 63) / 64, t = w - first, r0 = (t / nb) * 64, c0 = (t % nb) * 64;
   for (int e = tid; e < 64 * 64; e += 256) {
     const int r = r0 + (e >> 6), c = c0 + (e & 63);
-    tile[e >> 6][e & 63] = r < rows && c < cols ? (float)(ns_load(q.u, q.dtype, (long)r * cols + c) * inv) : 0.f;
+    tile[e >> 6][e & 63] = r < rows && c < cols ? ns_load(q.u, q.dtype, (long)r * cols + c) * inv.y * inv.x : 0.f;
   }
   __syncthreads();
   f16_t* const same = q.tall ? mem.xt[0] : mem.x;          // U's own orientation
@@ -574,12 +578,13 @@ __device__ __forceinline__ void ns_part_put(float* part, const f32x4 (&acc)[2][2
 }
 
 // normalises U into xt and makes the first partial A
+template <bool SHORT>
 __global__ __launch_bounds__(256) void ns_narrow_prep_kernel(NsCtl g, NsAll all) {
   __shared__ __attribute__((aligned(16))) char pool[64 * 65 * 4 + NsPair64::BYTES];
   __shared__ double sm[4];
-  __shared__ double s_inv;
+  __shared__ float2 s_inv;
   static_assert(sizeof(pool) >= NS_SHORT_LDS, "LDS");
-  if ((int)blockIdx.x >= all.items) {
+  if (SHORT && (int)blockIdx.x >= all.items) {
     ns_short_apply(g, all, (int)blockIdx.x - all.items, pool);
     return;
   }
@@ -596,7 +601,7 @@ __global__ __launch_bounds__(256) void ns_narrow_prep_kernel(NsCtl g, NsAll all)
   __syncthreads();
   if (tid == 0) s_inv = ns_inverse(sm[0] + sm[1] + sm[2] + sm[3], g.eps);
   __syncthreads();
-  const double inv = s_inv;                                             // (past fp32's range where eps is zero and |U| next to it)
+  const float2 inv = s_inv;
   const int tiles = (q.n + 63) / 64, P = ns_chunks(q.n), ch = (tiles + P - 1) / P;
   f32x4 acc[2][2] = {};
   for (int t = chunk * ch; t < tiles && t < chunk * ch + ch; ++t) {
@@ -604,7 +609,7 @@ __global__ __launch_bounds__(256) void ns_narrow_prep_kernel(NsCtl g, NsAll all)
     __syncthreads();
     for (int e = tid; e < 64 * 64; e += 256) {
       const int i = q.tall ? e & 63 : e >> 6, j = q.tall ? e >> 6 : e & 63;                    // X's row and column; along U's rows either way
-      tile[i * 65 + j] = i < q.m && c0 + j < q.n ? (float)(ns_load(q.u, q.dtype, q.tall ? (long)(c0 + j) * q.m + i : (long)i * q.n + c0 + j) * inv) : 0.f;
+      tile[i * 65 + j] = i < q.m && c0 + j < q.n ? ns_load(q.u, q.dtype, q.tall ? (long)(c0 + j) * q.m + i : (long)i * q.n + c0 + j) * inv.y * inv.x : 0.f;
     }
     __syncthreads();
     for (int e = tid; e < 64 * 8; e += 256) {
@@ -846,12 +851,10 @@ int ns_run(NsArgs& g, int steps, const float* coeffs, float eps, hipStream_t st)
   NsCtl c = {g.ws, g.count, 0, 0, 0.f, 0.f, 0.f, eps};
   NsAll all = {n[g.narrow ? NS_NARROW : NS_PREP], steps, {}};
   for (int k = 0; k < 3 * steps && k < 3 * NS_STEPS; ++k) all.c[k] = coeffs[k];
-  hipLaunchKernelGGL(ns_norm_kernel, dim3(n[NS_SUMS]), dim3(256), 0, st, g);
+  hipLaunchKernelGGL(n[NS_SHORT] ? ns_norm_kernel<true> : ns_norm_kernel<false>, dim3(n[NS_SUMS]), dim3(256), 0, st, g);
   FI_CHECK_LAUNCH();
-  if (g.narrow)
-    hipLaunchKernelGGL(ns_narrow_prep_kernel, dim3(all.items + n[NS_SHORT]), dim3(256), 0, st, c, all);
-  else
-    hipLaunchKernelGGL(ns_prep_kernel, dim3(all.items + n[NS_SHORT]), dim3(256), 0, st, c, all);
+  auto* const prep = n[NS_SHORT] ? (g.narrow ? ns_narrow_prep_kernel<true> : ns_prep_kernel<true>) : g.narrow ? ns_narrow_prep_kernel<false> : ns_prep_kernel<false>;
+  hipLaunchKernelGGL(prep, dim3(all.items + n[NS_SHORT]), dim3(256), 0, st, c, all);
   FI_CHECK_LAUNCH();
   for (int k = 0; k < steps && all.items; ++k) {
     c.ca = coeffs[3 * k], c.cb = coeffs[3 * k + 1], c.cc = coeffs[3 * k + 2];
