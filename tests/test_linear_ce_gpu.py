@@ -140,6 +140,19 @@ def test_linear_ce_parameter_in_fp32_under_16_bit_features():
     _within(w32.grad, want[2], tol[2], ("dw", F32))
 
 
+@pytest.mark.parametrize("dtype,rows,classes,width", [(F16, 300, 200, 72), (F16, 4000, 700, 100), (BF16, 300, 200, 72), (BF16, 300, 200, 200)])
+def test_linear_ce_fp32_weights_meet_16_bit_features_rounded(dtype, rows, classes, width):
+    """fp32 weights are the 16-bit type's in the product and in dx, whatever form the sizes choose."""
+    x, w, b, lab = _head(31, rows, classes, width, dtype, 0.1, F32)
+    w = w + 1e-4 * torch.randn(w.shape, generator=_gen(32), device="cuda")          # (no longer the type's own values)
+    got = []
+    for v in (w, w.to(dtype).float()):
+        leaves = [x.detach().requires_grad_(True), v.detach().requires_grad_(True)]
+        loss = ops.linear_ce_loss(*leaves, b, lab)
+        got.append([loss.detach(), *torch.autograd.grad(loss, leaves)])
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
 def test_linear_ce_everything_ignored_and_nothing_ignored():
     x, w, b, lab = _head(10, 300, 20, 16, BF16)
     none = torch.full_like(lab, -100)
