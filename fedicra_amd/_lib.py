@@ -123,6 +123,13 @@ def lib():
         for name in ("fi_newton_schulz_workspace", "fi_linear_ce_saved", "fi_linear_ce_fwd_workspace", "fi_linear_ce_bwd_workspace",
                      "fi_muon_step_workspace"):
             getattr(_lib, name).restype = C.c_long
+        # (given their types, these take addresses as plain integers: a third of the host time of wrapping each)
+        p, i = C.c_void_p, C.c_int
+        _lib.fi_linear_ce_saved.argtypes = [p]
+        _lib.fi_linear_ce_fwd_workspace.argtypes = [p, p]
+        _lib.fi_linear_ce_bwd_workspace.argtypes = [p, p, i, i, i]
+        _lib.fi_linear_ce_fwd.argtypes = [p] * 9
+        _lib.fi_linear_ce_bwd.argtypes = [p] * 9 + [i, p, i, p, p]
     return _lib
 
 
@@ -1202,25 +1209,19 @@ def _address(t):
     return None if t is None else t.data_ptr()
 
 
-_P = C.c_void_p
-
-
 def linear_ce_fwd(d, x, w, bias, labels, loss):
     """Returns the buffer the backward pass needs."""
-    dev, so, ref = _dev(x).device, lib(), C.byref(d)
-    pw = _P(w.data_ptr())
+    dev, so, ref, pw = _dev(x).device, lib(), C.addressof(d), w.data_ptr()
     saved = _scratch(so.fi_linear_ce_saved(ref), "fi_linear_ce_saved", dev)
     ws = _scratch(so.fi_linear_ce_fwd_workspace(ref, pw), "fi_linear_ce_fwd_workspace", dev)
-    _chk(so.fi_linear_ce_fwd(ref, _P(x.data_ptr()), pw, _P(_address(bias)), _P(labels.data_ptr()), _P(loss.data_ptr()),
-                             _P(saved.data_ptr()), _P(ws.data_ptr()), stream()), "fi_linear_ce_fwd")
+    _chk(so.fi_linear_ce_fwd(ref, x.data_ptr(), pw, _address(bias), labels.data_ptr(), loss.data_ptr(), saved.data_ptr(), ws.data_ptr(),
+                             stream()), "fi_linear_ce_fwd")
     return saved
 
 
 def linear_ce_bwd(d, x, w, bias, labels, saved, gloss, dx, dw, dw_accumulate, db, db_accumulate):
-    so, ref = lib(), C.byref(d)
-    pw = _P(w.data_ptr())
-    size = so.fi_linear_ce_bwd_workspace(ref, pw, int(dx is not None), int(dw is not None), int(db is not None))
+    so, ref, pw = lib(), C.addressof(d), w.data_ptr()
+    size = so.fi_linear_ce_bwd_workspace(ref, pw, dx is not None, dw is not None, db is not None)
     ws = _scratch(size, "fi_linear_ce_bwd_workspace", _dev(x).device)
-    _chk(so.fi_linear_ce_bwd(ref, _P(x.data_ptr()), pw, _P(_address(bias)), _P(labels.data_ptr()), _P(saved.data_ptr()),
-                             _P(gloss.data_ptr()), _P(_address(dx)), _P(_address(dw)), int(dw_accumulate), _P(_address(db)),
-                             int(db_accumulate), _P(ws.data_ptr()), stream()), "fi_linear_ce_bwd")
+    _chk(so.fi_linear_ce_bwd(ref, x.data_ptr(), pw, _address(bias), labels.data_ptr(), saved.data_ptr(), gloss.data_ptr(), _address(dx),
+                             _address(dw), dw_accumulate, _address(db), db_accumulate, ws.data_ptr(), stream()), "fi_linear_ce_bwd")

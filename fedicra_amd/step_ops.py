@@ -16,9 +16,12 @@ from . import _lib as L
 NS_COEFFS = (3.4445, -4.7750, 2.0315)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """The device's context where it is not the current one (entering it costs as much as a launch)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def newton_schulz(updates, steps=5, coeffs=NS_COEFFS, eps=1e-7):
@@ -72,26 +75,25 @@ def _newton_schulz_into(updates, outs, steps, coeffs, eps):
 def _grad_slot(param, shape):
     """Where a gradient of `param` goes: (tensor to write, add to it?, what autograd gets).  A dense fp32 slice of the flat gradient buffer
     is added to in place (ops._grad_target), anything else gets a fresh tensor."""
-    from . import ops
     sink = getattr(param, "_fi_gview", None)
     if sink is not None:
+        from . import ops
         tgt, _, ret = ops._grad_target(param)
         if ret is None and tgt.reshape(shape).data_ptr() == tgt.data_ptr():
             return tgt.reshape(shape), True, None
         if ret is not None and ret.reshape(shape).data_ptr() == ret.data_ptr():
             return ret.reshape(shape), True, ret
-    g = torch.empty(shape, dtype=param.dtype, device=param.device)
-    return g, False, g.reshape(param.shape)
+    g = param.new_empty(shape)
+    return g, False, g if param.dim() == len(shape) else g.reshape(param.shape)
 
 
 def _dense_rows(t, rows, cols):
     """[rows, cols] with dense rows that lie apart (a view; a copy where there is none: features apart, an expanded or overlapping tensor, rows so
     far apart that a tile's offsets would not fit)."""
-    t = t.detach()
     if t.dim() != 2:
         t = t.reshape(rows, cols)
-    apart = rows == 1 or cols <= t.stride(0) <= 1 << 22
-    return t if (t.stride(1) == 1 or cols == 1) and apart else t.contiguous()
+    step, along = t.stride()
+    return t if (along == 1 or cols == 1) and (rows == 1 or cols <= step <= 1 << 22) else t.contiguous()
 
 
 def _fp32_row(t):
@@ -120,11 +122,11 @@ class _LinearCE(Function):
         V, D = weight.shape[:2]
         x2, w2 = _dense_rows(x, labels.numel(), D), _dense_rows(weight, V, D)
         b2, l2 = _fp32_row(bias), labels.contiguous()
-        gl = g.to(torch.float32).contiguous()
+        gl = _fp32_row(g)
         dx = dw = db = gw = gb = None
         dw_add = db_add = False
         if ctx.needs_input_grad[0]:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            dx = x.new_empty(x.shape)
         if ctx.needs_input_grad[1]:
             dw, dw_add, gw = _grad_slot(weight, (V, D))
         if bias is not None and ctx.needs_input_grad[2]:
@@ -156,9 +158,9 @@ def linear_ce_loss(x, weight, bias, labels, ignore_index=-100, reduction="mean")
         raise ValueError(f"linear_ce_loss: reduction is 'mean', 'sum' or 'none', not {reduction!r}")
     if x.dim() < 1 or weight.dim() < 2 or x.shape[-1] != weight.shape[1] or weight.numel() != weight.shape[0] * weight.shape[1]:
         raise ValueError(f"linear_ce_loss: x [..., D] and weight [V, D] do not go together: {tuple(x.shape)}, {tuple(weight.shape)}")
-    if tuple(labels.shape) != tuple(x.shape[:-1]):
+    if labels.shape != x.shape[:-1]:
         raise ValueError(f"linear_ce_loss: labels {tuple(labels.shape)} for rows {tuple(x.shape[:-1])}")
-    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+    if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"linear_ce_loss: bias {tuple(bias.shape)} for {weight.shape[0]} classes")
     if x.numel() == 0 or weight.numel() == 0:
         raise ValueError("linear_ce_loss: no rows, no classes or no features")
