@@ -125,6 +125,7 @@ struct CeAmax {
   i64 ld, rows;
   const int *idx, *count;  // row list and its length, or NULL
   float* part;             // [CE_PARTS]
+  i64 tail;                // values behind the last row
 };
 template <typename T>
 __device__ __forceinline__ float ce_amax_rows(const CeAmax& a, i64 rows) {
@@ -146,6 +147,10 @@ __device__ __forceinline__ float ce_amax_rows(const CeAmax& a, i64 rows) {
       const float v = fabsf(to_f32(q[c]));
       if (v < INFINITY) m = fmaxf(m, v);
     }
+  }
+  for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x; c < a.tail; c += (i64)gridDim.x * 256) {
+    const float v = fabsf(to_f32(((const T*)a.p)[rows * a.ld + c]));
+    if (v < INFINITY) m = fmaxf(m, v);
   }
   return m;
 }
@@ -310,23 +315,36 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw, CeFa
   if (r0 >= rows || c0 >= (a.same && a.same_k > a.D ? a.same_k : a.D)) return;
   // 8 columns a lane, as many lanes a row as the block has columns for (a power of two)
   const int cols = (a.same && a.same_k > a.D ? a.same_k : a.D) - c0, sh = cols > 32 ? 3 : cols > 16 ? 2 : cols > 8 ? 1 : 0;
+  // rows that vectors do not fit come by a value per lane, through the tile (122 x 72099 x 1730 fp32: 380 -> ## us a launch)
+  const bool by_one = !a.vec && a.D - c0 >= 16;
+  if (by_one) {
+    for (int e = tid; e < 64 * 64; e += 256) {
+      const i64 r = r0 + (e >> 6);
+      const int c = c0 + (e & 63);
+      tile[e >> 6][e & 63] = r < rows && c < a.D ? ce_load(a.src, a.dtype, (a.idx ? (i64)a.idx[a.begin + r] : r) * a.ld + c) : 0.f;
+    }
+    __syncthreads();
+  }
   for (int e = tid; e < 64 << sh; e += 256) {
     const int er = e >> sh, ec = (e & ((1 << sh) - 1)) * 8;
     const i64 r = r0 + er;
     const int c = c0 + ec, left = r < rows ? a.D - c : 0;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (left > 0) {
-      const i64 at = (a.idx ? (i64)a.idx[a.begin + r] : r) * a.ld + c;
-      if (a.dtype == FI_F32) {
-        ce_load8((const float*)a.src + at, left, a.vec, v);
-        if (a.round != FI_F32) {
+    if (by_one) {
 #pragma unroll
-          for (int t = 0; t < 8; ++t) v[t] = a.round == FI_BF16 ? (float)(bf16_t)v[t] : (float)(f16_t)v[t];
-        }
-      } else if (a.dtype == FI_BF16)
+      for (int t = 0; t < 8; ++t) v[t] = tile[er][ec + t];
+    } else if (left > 0) {
+      const i64 at = (a.idx ? (i64)a.idx[a.begin + r] : r) * a.ld + c;
+      if (a.dtype == FI_F32)
+        ce_load8((const float*)a.src + at, left, a.vec, v);
+      else if (a.dtype == FI_BF16)
         ce_load8((const bf16_t*)a.src + at, left, a.vec, v);
       else
         ce_load8((const f16_t*)a.src + at, left, a.vec, v);
+    }
+    if (a.round != a.dtype) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] = a.round == FI_BF16 ? (float)(bf16_t)v[t] : (float)(f16_t)v[t];
     }
     if (a.same && r < rows && c < a.same_k) {
       char* row = (char*)a.same + r * a.ld_same * 2;
@@ -756,28 +774,35 @@ __global__ __launch_bounds__(Core::THREADS) void ce_grad_kernel(CeGrad a) {
     for (int bj = 0; bj < Core::WN / SB; ++bj) {
       const int gi = ti * Core::BM + Core::row0() + bi * SB, gj = tj * Core::BN + Core::col0() + bj * SB;
       blk.put(c, bi, bj, 1.f);
+      if (a.part ? (a.N & 7) != 0 : !a.vec || a.accumulate) {
+        blk.each([&](int i, int j, float v) {
+          const int r = gi + i, k = gj + j;
+          if (r >= M || k >= a.N) return;
+          if (a.part) {
+            float* p = a.part + ((i64)sp * a.M + r) * a.N + k;
+            *p = a.first ? v : *p + v;
+          } else {
+            const float one[8] = {v * rg * rb};
+            ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : (i64)r, k, one, 1);
+          }
+        });
+        continue;
+      }
       blk.template rows<false>([&](int i, int j0, float (&v)[8]) {
         const int r = gi + i, k = gj + j0;
         if (r >= M || k >= a.N) return;
-        const int nv = a.N - k < 8 ? a.N - k : 8;
         if (a.part) {
           float* p = a.part + ((i64)sp * a.M + r) * a.N + k;
-          if ((a.N & 7) == 0) {
-            float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
-            if (!a.first) {
-              const float4 x = ((const float4*)p)[0], y = ((const float4*)p)[1];
-              lo.x += x.x, lo.y += x.y, lo.z += x.z, lo.w += x.w, hi.x += y.x, hi.y += y.y, hi.z += y.z, hi.w += y.w;
-            }
-            ((float4*)p)[0] = lo, ((float4*)p)[1] = hi;
-            return;
+          float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
+          if (!a.first) {
+            const float4 x = ((const float4*)p)[0], y = ((const float4*)p)[1];
+            lo.x += x.x, lo.y += x.y, lo.z += x.z, lo.w += x.w, hi.x += y.x, hi.y += y.y, hi.z += y.z, hi.w += y.w;
           }
-#pragma unroll
-          for (int t = 0; t < 8; ++t)
-            if (t < nv) p[t] = a.first ? v[t] : p[t] + v[t];
+          ((float4*)p)[0] = lo, ((float4*)p)[1] = hi;
         } else {
 #pragma unroll
           for (int t = 0; t < 8; ++t) v[t] = v[t] * rg * rb;
-          ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : (i64)r, k, v, nv);
+          ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : (i64)r, k, v, 8);
         }
       });
     }
@@ -1191,8 +1216,8 @@ int ce_check(const FiLinearCe* d) {
 
 // tiles of the logits' product: 256 x 256; 64 rows where there are no more (the classes are then streamed once, and three quarters of a
 // tall tile would repeat the last row); 64 or 128 classes likewise
-int ce_logits_tile(const FiLinearCe& d) { return d.T <= 64 ? 1 : d.V <= 64 ? 2 : d.V <= 128 ? 3 : 0; }
-constexpr int CE_BM[4] = {256, 64, 256, 256}, CE_BN[4] = {256, 256, 64, 128};
+int ce_logits_tile(const FiLinearCe& d) { return d.T <= 64 ? 1 : d.V <= 64 ? 2 : d.V <= 128 ? 3 : d.T <= 128 ? 4 : 0; }
+constexpr int CE_BM[5] = {256, 64, 256, 256, 128}, CE_BN[5] = {256, 256, 64, 128, 256};
 
 // (the same tile by 16 waves of 64 x 64 in the forward pass -- four per SIMD hide LDS and DMA latency: 845 -> 757 us at 7370 x 50000 x 1024 -- and by
 // 8 of 128 x 64 for G, whose epilogue wants 64 x 64 blocks of scratch: 267 against 290 us a piece of 7370 x 16384)
@@ -1202,6 +1227,7 @@ template <typename T, bool PAIR> struct CeCores {
   typedef NtCore<T, PAIR, 64, 256, 64, 32> C1;
   typedef NtCore<T, PAIR, 256, 64, 32, 64> C2;
   typedef NtCore<T, PAIR, 256, 128, 64, 64> C3;
+  typedef NtCore<T, PAIR, 128, 256, 64, 64> C4;
 };
 
 template <class Core, typename T, bool PAIR>
@@ -1232,7 +1258,8 @@ int ce_logits(const CeLogits& a, const FiLinearCe& d, bool fwd, hipStream_t st) 
     case 0: return fwd ? ce_launch_fwd<typename C::F0, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C0, T, PAIR>(a, st);
     case 1: return fwd ? ce_launch_fwd<typename C::C1, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C1, T, PAIR>(a, st);
     case 2: return fwd ? ce_launch_fwd<typename C::C2, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C2, T, PAIR>(a, st);
-    default: return fwd ? ce_launch_fwd<typename C::C3, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C3, T, PAIR>(a, st);
+    case 3: return fwd ? ce_launch_fwd<typename C::C3, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C3, T, PAIR>(a, st);
+    default: return fwd ? ce_launch_fwd<typename C::C4, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C4, T, PAIR>(a, st);
   }
 }
 int ce_logits_any(const CeLogits& a, const FiLinearCe& d, bool pair, bool fwd, hipStream_t st) {
@@ -1257,8 +1284,12 @@ int ce_pack(const CePack& x, const CePack& w, hipStream_t st, const CeFactors& f
 int ce_vec(const void* p, int dtype, i64 ld) { return ((uintptr_t)p & 15) == 0 && ld % (dtype == FI_F32 ? 4 : 8) == 0; }
 
 int ce_amax(const FiLinearCe& d, const void* x, const void* w, const CeSaved& s, float* parts, hipStream_t st) {
-  const CeAmax ax = {x, d.dtype, d.D, ce_vec(x, d.dtype, d.ldx), d.ldx, d.T, s.idx, s.count, parts};
-  const CeAmax aw = {w, d.wdtype, d.D, ce_vec(w, d.wdtype, d.ldw), d.ldw, d.V, nullptr, nullptr, parts + CE_PARTS};
+  const CeAmax ax = {x, d.dtype, d.D, ce_vec(x, d.dtype, d.ldx), d.ldx, d.T, s.idx, s.count, parts, 0};
+  CeAmax aw = {w, d.wdtype, d.D, ce_vec(w, d.wdtype, d.ldw), d.ldw, d.V, nullptr, nullptr, parts + CE_PARTS, 0};
+  if (!aw.vec && d.ldw == d.D && ((uintptr_t)w & 15) == 0) {            // rows of any width that follow one another are as good as rows of 4096
+    const i64 total = (i64)d.V * d.D;
+    aw.vec = 1, aw.D = 4096, aw.ld = 4096, aw.rows = total / 4096, aw.tail = total % 4096;
+  }
   hipLaunchKernelGGL(ce_amax_kernel, dim3(CE_PARTS, 2), dim3(256), 0, st, ax, aw);
   FI_CHECK_LAUNCH();
   return 0;

@@ -240,6 +240,13 @@ struct NtBlock {
       }
     }
   }
+  // f(i, j, v): a value per lane, along the rows: for rows that vectors do not fit
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    const int l = threadIdx.x & 63;
+#pragma unroll 8
+    for (int e = l; e < SI * SJ; e += 64) f(e / SJ, e % SJ, *at(e / SJ, e % SJ));
+  }
   // f(j, i0, v): 8 values of column j from row i0 on
   template <class F>
   __device__ __forceinline__ void cols(F f) const {

@@ -90,7 +90,7 @@ def _head(seed, rows, classes, width, dtype, ignored=0.0, wdtype=None):
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("rows,classes,width", [(1, 1, 1), (1, 2, 8), (3, 7, 9), (16, 1000, 256), (64, 65, 64), (65, 64, 96), (63, 300, 33), (257, 257, 129),
-                                                (300, 513, 64), (513, 105, 16), (2049, 33, 40), (4500, 700, 200)])
+                                                (300, 513, 64), (513, 105, 16), (2049, 33, 40), (4500, 700, 200), (100, 300, 130), (128, 1000, 190), (129, 1000, 190)])
 def test_linear_ce_sizes_and_types(rows, classes, width, dtype):
     x, w, b, lab = _head(rows + classes, rows, classes, width, dtype, 0.2 if rows > 3 else 0.0)
     lab[0] = classes - 1
