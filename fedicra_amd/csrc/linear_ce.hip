@@ -294,6 +294,9 @@ __device__ __forceinline__ void ce_load8(const T* q, int left, int vec, float (&
 }
 // one 64 x 64 block of the source per workgroup (blockIdx.x: rows, .y: columns, .z: which operand); pads are written as zeros
 // (the last slice of a launch with f.g: the rows' factors, which need nothing of the operands)
+// LOOSE: some rows are not aligned for vectors; they come by a value per lane, through the tile (122 x 72099 x 1730 fp32: 380 -> 315 us a launch, whose
+// registers cost aligned operands a third: 15 -> 20 us at 524288 x 16)
+template <bool LOOSE>
 __global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw, CeFactors f) {
   __shared__ float tile[64][65];
   __shared__ float sm[4];
@@ -315,14 +318,25 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw, CeFa
   if (r0 >= rows || c0 >= (a.same && a.same_k > a.D ? a.same_k : a.D)) return;
   // 8 columns a lane, as many lanes a row as the block has columns for (a power of two)
   const int cols = (a.same && a.same_k > a.D ? a.same_k : a.D) - c0, sh = cols > 32 ? 3 : cols > 16 ? 2 : cols > 8 ? 1 : 0;
-  // rows that vectors do not fit come by a value per lane, through the tile (122 x 72099 x 1730 fp32: 380 -> ## us a launch)
-  const bool by_one = !a.vec && a.D - c0 >= 16;
+  const bool by_one = LOOSE && !a.vec && a.D - c0 >= 16;
   if (by_one) {
-    for (int e = tid; e < 64 * 64; e += 256) {
-      const i64 r = r0 + (e >> 6);
-      const int c = c0 + (e & 63);
-      tile[e >> 6][e & 63] = r < rows && c < a.D ? ce_load(a.src, a.dtype, (a.idx ? (i64)a.idx[a.begin + r] : r) * a.ld + c) : 0.f;
-    }
+    const auto stage = [&](const auto* src) {
+      const int c = c0 + (tid & 63);
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const i64 r = r0 + k * 4 + (tid >> 6);
+        v[k] = r < rows && c < a.D ? to_f32(src[(a.idx ? (i64)a.idx[a.begin + r] : r) * a.ld + c]) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) tile[k * 4 + (tid >> 6)][tid & 63] = v[k];
+    };
+    if (a.dtype == FI_F32)
+      stage((const float*)a.src);
+    else if (a.dtype == FI_BF16)
+      stage((const bf16_t*)a.src);
+    else
+      stage((const f16_t*)a.src);
     __syncthreads();
   }
   for (int e = tid; e < 64 << sh; e += 256) {
@@ -1215,7 +1229,7 @@ int ce_check(const FiLinearCe* d) {
 }
 
 // tiles of the logits' product: 256 x 256; 64 rows where there are no more (the classes are then streamed once, and three quarters of a
-// tall tile would repeat the last row); 64 or 128 classes likewise
+// tall tile would repeat the last row), 128 likewise (122 x 72099 x 1730 fp32: G 264 -> 221 us, forward 223 -> 190); 64 or 128 classes too
 int ce_logits_tile(const FiLinearCe& d) { return d.T <= 64 ? 1 : d.V <= 64 ? 2 : d.V <= 128 ? 3 : d.T <= 128 ? 4 : 0; }
 constexpr int CE_BM[5] = {256, 64, 256, 256, 128}, CE_BN[5] = {256, 256, 64, 128, 256};
 
@@ -1277,7 +1291,8 @@ int ce_pack(const CePack& x, const CePack& w, hipStream_t st, const CeFactors& f
     if ((cols + 63) / 64 > gy) gy = (cols + 63) / 64;
   }
   if (!x.src && !w.src) return 0;
-  hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)gx, (unsigned)gy, (x.src && w.src ? 2 : 1) + (f.g ? 1 : 0)), dim3(256), 0, st, x.src ? x : w, w, f);
+  const bool loose = (x.src && !x.vec) || (w.src && !w.vec);
+  hipLaunchKernelGGL(loose ? ce_pack_kernel<true> : ce_pack_kernel<false>, dim3((unsigned)gx, (unsigned)gy, (x.src && w.src ? 2 : 1) + (f.g ? 1 : 0)), dim3(256), 0, st, x.src ? x : w, w, f);
   FI_CHECK_LAUNCH();
   return 0;
 }
