@@ -1060,13 +1060,15 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
         float top = m2[i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) top = fmaxf(fmaxf(top, fmaxf(z[i][j][0], z[i][j][1])), fmaxf(z[i][j][2], z[i][j][3]));
-        const float safe = (top == -INFINITY ? 0.f : top) * CE_LOG2E;
-        float sum = y[i] * __builtin_amdgcn_exp2f(__builtin_fmaf(m2[i], CE_LOG2E, -safe));
+        // (the sum so far is multiplied by exactly one where the maximum stays, however many tiles there are; a tile's own sum first, so that the
+        // running one is rounded once per tile)
+        const float safe = top == -INFINITY ? 0.f : top, m = safe * CE_LOG2E, keep = __builtin_amdgcn_exp2f((m2[i] - safe) * CE_LOG2E);
+        float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j][r], CE_LOG2E, -safe));
-        m2[i] = top, y[i] = sum;
+          for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j][r], CE_LOG2E, -m));
+        m2[i] = top, y[i] = __builtin_fmaf(y[i], keep, sum);
       }
       continue;
     } else if constexpr (DW) {
