@@ -248,7 +248,7 @@ __device__ __forceinline__ void ce_factors(const CeFactors& a, float* sm) {
     if (r < n) {
       const float2 st = s.stat[r];
       const float f = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : (reduction == 0 ? g[s.idx[r]] : one) * sc;
-      m = make_float4(st.x * CE_LOG2E, f * st.y, f, __int_as_float(s.lab[r]));
+      m = make_float4(st.x, f * st.y, f, __int_as_float(s.lab[r]));
     }
     meta[r] = m;
   }
@@ -431,11 +431,9 @@ __device__ __forceinline__ bool ce_tile(int nti, int ntj, int& ti, int& tj) {
   return true;
 }
 
-// exp(z - m) with m2 = m log2 e: one rounding more is spent on the parity type, whose row sums are held to fp32's error
-template <bool PAIR>
-__device__ __forceinline__ float ce_exp(float z, float m, float m2) {
-  return __builtin_amdgcn_exp2f(PAIR ? (z - m) * CE_LOG2E : __builtin_fmaf(z, CE_LOG2E, -m2));
-}
+// exp(z - m).  The difference comes first: one fma of z, log2 e and -m log2 e would save an operation, but is not zero at z = m -- it is the
+// rounding of m log2 e, which overflows the exponential where every class of a lane is ruled out by a bias of -1e10 or less.
+__device__ __forceinline__ float ce_exp(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * CE_LOG2E); }
 
 // The bias of a lane's columns: 16-bit operands start from it, pairs get it behind their scales.
 template <bool PAIR, class Core>
@@ -508,12 +506,12 @@ __global__ __launch_bounds__(Core::THREADS) void ce_fwd_kernel(CeLogits a) {
 #pragma unroll
     for (int j = 0; j < Core::TJ; ++j)
       m = fmaxf(fmaxf(m, fmaxf(c.acc[i][j][0], c.acc[i][j][1])), fmaxf(c.acc[i][j][2], c.acc[i][j][3]));
-    const float safe = m == -INFINITY ? 0.f : m, m2 = safe * CE_LOG2E;
+    const float safe = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < Core::TJ; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum += ce_exp<PAIR>(c.acc[i][j][r], safe, m2);
+      for (int r = 0; r < 4; ++r) sum += ce_exp(c.acc[i][j][r], safe);
     red[q0 * Core::BM + row] = make_float2(m, sum);
   }
   __syncthreads();
@@ -526,7 +524,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_fwd_kernel(CeLogits a) {
 #pragma unroll
     for (int q = 0; q < 4 * Core::NWN; ++q) {
       const float2 o = red[q * Core::BM + row];
-      sum += o.y * __builtin_amdgcn_exp2f((o.x - safe) * CE_LOG2E);
+      sum += o.y * ce_exp(o.x, safe);
     }
     a.part[(i64)(r0 + row) * a.ntj + tj] = make_float2(m, sum);
   }
@@ -551,7 +549,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int nt
     if (r < n) {
       for (int k = sub; k < ntj; k += LANES) {
         const float2 p = part[r * ntj + k];
-        sum += (double)(p.y * __builtin_amdgcn_exp2f((p.x - safe) * CE_LOG2E));
+        sum += (double)(p.y * ce_exp(p.x, safe));
       }
     }
 #pragma unroll
@@ -623,14 +621,14 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
   ce_begin<PAIR>(c, a, cg);
   c.run((const T*)a.x + rg * a.ldx, a.ldx, n - r0, (const T*)a.w + (i64)cg * a.ldw, a.ldw, a.V - cg, 0, a.stages, smem);
   ce_finish<PAIR>(c, a, cg);
-  float4* meta = (float4*)(smem + EXTRA);                               // [BM]: maximum (* log2 e unless PAIR), factor / sum, factor, label
+  float4* meta = (float4*)(smem + EXTRA);                               // [BM]: maximum, factor / sum, factor, label
   float* colsum = (float*)(smem + EXTRA + Core::BM * 16);              // [BM / WM][BN]
   for (int row = threadIdx.x; row < Core::BM; row += Core::THREADS) {
     float4 m = make_float4(INFINITY, 0.f, 0.f, __int_as_float(-1));    // (rows behind the last one: exp2(-inf) = 0)
     if (r0 + row < n) {
       const float2 st = a.s.stat[rg + row];
       const float g = a.g[rg + row];
-      m = make_float4(PAIR ? st.x : st.x * CE_LOG2E, g * st.y, g, __int_as_float(a.s.lab[rg + row]));
+      m = make_float4(st.x, g * st.y, g, __int_as_float(a.s.lab[rg + row]));
     }
     meta[row] = m;
   }
@@ -642,7 +640,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
 #pragma unroll
     for (int j = 0; j < Core::TJ; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) c.acc[i][j][r] = ce_exp<PAIR>(c.acc[i][j][r], m.x, m.x) * m.y;
+      for (int r = 0; r < 4; ++r) c.acc[i][j][r] = ce_exp(c.acc[i][j][r], m.x) * m.y;
     const int lab = __float_as_int(m.w) - (cg + Core::col0());
     if ((unsigned)lab < (unsigned)Core::WN) {
 #pragma unroll
@@ -897,7 +895,7 @@ struct CeFused {
   i64 ld_own, ld_tile;
   const f16_t* turned;     // the streamed side turned, [D][..]
   i64 ld_turned;
-  const float4* meta;      // per token: maximum * log2 e, factor / sum, factor, label
+  const float4* meta;      // per token: maximum, factor / sum, factor, label
   const float* bias;       // padded to 64 classes (zeros without a bias)
   float* db;               // DW: [split][V] partial sums, or NULL
   float2* part;            // FWD: [row][split] maximum and sum
@@ -984,23 +982,23 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
 
   // own rows
   frag_t own[2][KD];
-  float m2[2], y[2], gg[2], b[2], cs[2] = {0.f, 0.f};
+  float mx[2], y[2], gg[2], b[2], cs[2] = {0.f, 0.f};
   int lab[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int o = o0 + i * 16 + lr, oc = o < M ? o : M - 1;
 #pragma unroll
     for (int k = 0; k < KD; ++k) own[i][k] = k * 32 + g * 8 < width ? *(const frag_t*)((const T*)a.own + (i64)oc * a.ld_own + k * 32 + g * 8) : frag_t{};
-    m2[i] = y[i] = gg[i] = b[i] = 0.f, lab[i] = -1;
+    mx[i] = y[i] = gg[i] = b[i] = 0.f, lab[i] = -1;
     if constexpr (DW) {
       b[i] = a.bias[oc];
     } else if constexpr (FWD) {
       lab[i] = o < M ? a.s.lab[oc] : -1;
-      m2[i] = -INFINITY;                                                // the running maximum; y: the running sum
+      mx[i] = -INFINITY;                                                // the running maximum; y: the running sum
     } else {
       // (dx takes every row's own factor out of the sum: G is made with 2^14 in its place, where its label's entry is rounded least)
       const float4 m = a.meta[oc];
-      m2[i] = m.x, y[i] = 16384.f * a.s.stat[oc].y, gg[i] = 16384.f, b[i] = m.z * (1.f / 16384.f), lab[i] = __float_as_int(m.w);
+      mx[i] = m.x, y[i] = 16384.f * a.s.stat[oc].y, gg[i] = 16384.f, b[i] = m.z * (1.f / 16384.f), lab[i] = __float_as_int(m.w);
     }
   }
   f32x4 acc[2][2 * KD];
@@ -1057,18 +1055,18 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
             for (int r = 0; r < 4; ++r)
               if (c == 32 * (j >> 1) + 8 * g + 4 * (j & 1) + r) a.zt[o0 + i * 16 + lr] = z[i][j][r];
         }
-        float top = m2[i];
+        float top = mx[i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) top = fmaxf(fmaxf(top, fmaxf(z[i][j][0], z[i][j][1])), fmaxf(z[i][j][2], z[i][j][3]));
         // (the sum so far is multiplied by exactly one where the maximum stays, however many tiles there are; a tile's own sum first, so that the
         // running one is rounded once per tile)
-        const float safe = top == -INFINITY ? 0.f : top, m = safe * CE_LOG2E, keep = __builtin_amdgcn_exp2f((m2[i] - safe) * CE_LOG2E);
+        const float safe = top == -INFINITY ? 0.f : top, keep = ce_exp(mx[i], safe);
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j][r], CE_LOG2E, -m));
-        m2[i] = top, y[i] = __builtin_fmaf(y[i], keep, sum);
+          for (int r = 0; r < 4; ++r) sum += ce_exp(z[i][j][r], safe);
+        mx[i] = top, y[i] = __builtin_fmaf(y[i], keep, sum);
       }
       continue;
     } else if constexpr (DW) {
@@ -1080,7 +1078,7 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
           const int cls = __float_as_int(m.w) - o0 - lr;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float v = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j][r], CE_LOG2E, -m.x)) * m.y;
+            float v = ce_exp(z[i][j][r], m.x) * m.y;
             v -= cls == i * 16 ? m.z : 0.f;
             cs[i] += v;
             z[i][j][r] = v;
@@ -1092,7 +1090,7 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) z[i][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j][r], CE_LOG2E, -m2[i])) * y[i];
+          for (int r = 0; r < 4; ++r) z[i][j][r] = ce_exp(z[i][j][r], mx[i]) * y[i];
         const int c = lab[i] - t * 64;
         if ((unsigned)c < 64u) {
 #pragma unroll
@@ -1130,10 +1128,10 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
   if constexpr (FWD) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      float m = fmaxf(m2[i], __shfl_xor(m2[i], 16, 64));
+      float m = fmaxf(mx[i], __shfl_xor(mx[i], 16, 64));
       m = fmaxf(m, __shfl_xor(m, 32, 64));
       const float safe = m == -INFINITY ? 0.f : m;
-      float sum = y[i] * __builtin_amdgcn_exp2f((m2[i] - safe) * CE_LOG2E);
+      float sum = y[i] * ce_exp(mx[i], safe);
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
       const int o = o0 + i * 16 + lr;
