@@ -263,14 +263,21 @@ struct NtBlock {
   }
 };
 
+// the value as it is: where it is a product, its parts must all come of one rounded number.  (The compiler otherwise takes a high part from the rounded
+// product to be stored and from the exact one, by v_fma_mixlo_f16, to be subtracted: at a tie these differ by a step of fp16, and the low part is lost.)
+__device__ __forceinline__ float nt_fixed(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
 // 8 values -> high and low fp16 parts (value = hi + lo up to 2^-22 of it)
 __device__ __forceinline__ void nt_split8(const float (&v)[8], uint4& hi, uint4& lo) {
   unsigned h[4], q[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
+    const float x = nt_fixed(v[2 * t]), y = nt_fixed(v[2 * t + 1]);
     f16x2_t a, b;
-    a[0] = (f16_t)v[2 * t], a[1] = (f16_t)v[2 * t + 1];
-    b[0] = (f16_t)(v[2 * t] - (float)a[0]), b[1] = (f16_t)(v[2 * t + 1] - (float)a[1]);
+    a[0] = (f16_t)x, a[1] = (f16_t)y;
+    b[0] = (f16_t)(x - (float)a[0]), b[1] = (f16_t)(y - (float)a[1]);
     h[t] = __builtin_bit_cast(unsigned, a), q[t] = __builtin_bit_cast(unsigned, b);
   }
   hi = make_uint4(h[0], h[1], h[2], h[3]);
