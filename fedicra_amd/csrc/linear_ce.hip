@@ -601,7 +601,9 @@ __global__ __launch_bounds__(256) void ce_gmax_kernel(const float* g, const int*
 template <bool PAIR>
 __device__ __forceinline__ int ce_kpad(int n) { return PAIR ? (n + 31) & ~31 : (n + 63) & ~63; }
 
-// G of a piece, in both orientations
+// G of a piece, in both orientations.  A row of dx is its own factor times what it would be with a factor of one: the rows that dx's product reads are made
+// with CE_UNIT in the factor's place, which its epilogue puts right, and only the columns that dW's sum over rows reads carry the factors.
+constexpr float CE_UNIT = 16384.f;
 template <class Core, typename T, bool PAIR>
 __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -621,22 +623,25 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
   ce_begin<PAIR>(c, a, cg);
   c.run((const T*)a.x + rg * a.ldx, a.ldx, n - r0, (const T*)a.w + (i64)cg * a.ldw, a.ldw, a.V - cg, 0, a.stages, smem);
   ce_finish<PAIR>(c, a, cg);
-  float4* meta = (float4*)(smem + EXTRA);                               // [BM]: maximum, factor / sum, factor, label
-  float* colsum = (float*)(smem + EXTRA + Core::BM * 16);              // [BM / WM][BN]
+  float4* meta = (float4*)(smem + EXTRA);                               // [BM]: maximum, CE_UNIT / sum, factor / CE_UNIT, label
+  float* fac = (float*)(smem + EXTRA + Core::BM * 16);                  // [BM]: the factors alone, for vectors of rows
+  float* colsum = fac + Core::BM;                                      // [BM / WM][BN]
   for (int row = threadIdx.x; row < Core::BM; row += Core::THREADS) {
     float4 m = make_float4(INFINITY, 0.f, 0.f, __int_as_float(-1));    // (rows behind the last one: exp2(-inf) = 0)
     if (r0 + row < n) {
       const float2 st = a.s.stat[rg + row];
-      const float g = a.g[rg + row];
-      m = make_float4(st.x, g * st.y, g, __int_as_float(a.s.lab[rg + row]));
+      m = make_float4(st.x, CE_UNIT * st.y, a.g[rg + row] * (1.f / CE_UNIT), __int_as_float(a.s.lab[rg + row]));
     }
     meta[row] = m;
+    fac[row] = m.z;
   }
   __syncthreads();
   const int l = Core::lane(), j0 = cg + Core::col0() + 4 * (l >> 4);
+  float mine[Core::TI];
 #pragma unroll
   for (int i = 0; i < Core::TI; ++i) {
     const float4 m = meta[Core::row0() + i * 16 + (l & 15)];
+    mine[i] = m.z;
 #pragma unroll
     for (int j = 0; j < Core::TJ; ++j)
 #pragma unroll
@@ -646,7 +651,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
 #pragma unroll
       for (int j = 0; j < Core::TJ; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) c.acc[i][j][r] -= lab == j * 16 + 4 * (l >> 4) + r ? m.z : 0.f;
+        for (int r = 0; r < 4; ++r) c.acc[i][j][r] -= lab == j * 16 + 4 * (l >> 4) + r ? CE_UNIT : 0.f;
     }
   }
   if (cg + Core::BN > a.V) {
@@ -666,7 +671,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
       for (int r = 0; r < 4; ++r) {
         float v = 0.f;
 #pragma unroll
-        for (int i = 0; i < Core::TI; ++i) v += c.acc[i][j][r];
+        for (int i = 0; i < Core::TI; ++i) v += c.acc[i][j][r] * mine[i];
         v = fi_row16_sum(v);
         if ((l & 15) == 0) colsum[(Core::wave() / Core::NWN) * Core::BN + Core::col0() + j * 16 + 4 * (l >> 4) + r] = v;
       }
@@ -704,6 +709,8 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
       if (a.dlt) {
         blk.cols([&](int j, int i0, float (&v)[8]) {
           if (gj + j >= vcols || gi + i0 >= npad) return;
+          const float4 lo = *(const float4*)(fac + gi - r0 + i0), hi = *(const float4*)(fac + gi - r0 + i0 + 4);
+          v[0] *= lo.x, v[1] *= lo.y, v[2] *= lo.z, v[3] *= lo.w, v[4] *= hi.x, v[5] *= hi.y, v[6] *= hi.z, v[7] *= hi.w;
           f16_t* row = a.dlt + (i64)(gj + j) * a.ld_dlt;
           if constexpr (PAIR)
             nt_store_pair(row, gi + i0, v);
@@ -730,6 +737,7 @@ struct CeGrad {
   int out_dtype, accumulate, vec;
   i64 ldo;
   const int* idx;          // dx: where a row belongs, else NULL
+  const float* rowf;       // dx of G made with CE_UNIT: the rows' factors, else NULL
   const float* scal;
   int rscale;              // index of the reciprocal of b's scale, -1: none
 };
@@ -758,6 +766,7 @@ __device__ __forceinline__ void ce_put(const CeGrad& a, i64 row, int col, const 
     }
   }
 }
+__device__ __forceinline__ float ce_row_factor(const CeGrad& a, i64 r) { return a.rowf ? a.rowf[a.t0 + r] * (1.f / CE_UNIT) : 1.f; }
 __device__ __forceinline__ float ce_rscale(const CeGrad& a) { return a.rscale >= 0 ? a.scal[a.rscale] : 1.f; }
 
 template <class Core, bool PAIR>
@@ -794,7 +803,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_grad_kernel(CeGrad a) {
             float* p = a.part + ((i64)sp * a.M + r) * a.N + k;
             *p = a.first ? v : *p + v;
           } else {
-            const float one[8] = {v * rg * rb};
+            const float one[8] = {v * rg * rb * ce_row_factor(a, r)};
             ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : (i64)r, k, one, 1);
           }
         });
@@ -812,8 +821,9 @@ __global__ __launch_bounds__(Core::THREADS) void ce_grad_kernel(CeGrad a) {
           }
           ((float4*)p)[0] = lo, ((float4*)p)[1] = hi;
         } else {
+          const float f = ce_row_factor(a, r);
 #pragma unroll
-          for (int t = 0; t < 8; ++t) v[t] = v[t] * rg * rb;
+          for (int t = 0; t < 8; ++t) v[t] = v[t] * rg * rb * f;
           ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : (i64)r, k, v, 8);
         }
       });
@@ -850,8 +860,9 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeGrad a) {
 #pragma unroll
       for (int t = 0; t < 8; ++t) v[t] += __shfl_xor(v[t], o, 64);
     if (e < total && sub == 0) {
+      const float f = ce_row_factor(a, r);
 #pragma unroll
-      for (int t = 0; t < 8; ++t) v[t] = v[t] * rg * rb;
+      for (int t = 0; t < 8; ++t) v[t] = v[t] * rg * rb * f;
       ce_put(a, a.idx ? (i64)a.idx[a.t0 + r] : r, k, v, n);
     }
   }
@@ -996,9 +1007,9 @@ __global__ __launch_bounds__(512) void ce_fused_kernel(CeFused a) {
       lab[i] = o < M ? a.s.lab[oc] : -1;
       mx[i] = -INFINITY;                                                // the running maximum; y: the running sum
     } else {
-      // (dx takes every row's own factor out of the sum: G is made with 2^14 in its place, where its label's entry is rounded least)
+      // (dx takes every row's own factor out of the sum: G is made with CE_UNIT in its place, where its label's entry is rounded least)
       const float4 m = a.meta[oc];
-      mx[i] = m.x, y[i] = 16384.f * a.s.stat[oc].y, gg[i] = 16384.f, b[i] = m.z * (1.f / 16384.f), lab[i] = __float_as_int(m.w);
+      mx[i] = m.x, y[i] = CE_UNIT * a.s.stat[oc].y, gg[i] = CE_UNIT, b[i] = m.z * (1.f / CE_UNIT), lab[i] = __float_as_int(m.w);
     }
   }
   f32x4 acc[2][2 * KD];
@@ -1259,7 +1270,7 @@ int ce_launch_dlogits(const CeLogits& a, hipStream_t st) {
   static NtLdsDevices allowed;
   if (!nt_allow_lds((const void*)ce_dlogits_kernel<Core, T, PAIR>, allowed)) return FI_ERR_UNSUPPORTED;
   constexpr int SB = Core::BLOCK, SCR = Core::NW * NtBlock<SB, SB>::BYTES;
-  constexpr int need = SCR + Core::BM * 16 + Core::BM / Core::WM * Core::BN * 4, lds = need > Core::LDS ? need : Core::LDS;
+  constexpr int need = SCR + Core::BM * 20 + Core::BM / Core::WM * Core::BN * 4, lds = need > Core::LDS ? need : Core::LDS;
   const i64 n = (a.Tc + Core::BM - 1) / Core::BM * ((a.Vc + Core::BN - 1) / Core::BN);
   hipLaunchKernelGGL((ce_dlogits_kernel<Core, T, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), lds, st, a);
   FI_CHECK_LAUNCH();
@@ -1615,6 +1626,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
     }
     return 0;
   }
+  gx.rowf = ws.g;
   gx.vec = d->D % 8 == 0 && ((uintptr_t)dx & 15) == 0, gw.vec = d->D % 8 == 0 && ((uintptr_t)dw & 15) == 0;
   CeLogits a = {};
   a.x = ws.xc, a.ldx = s.ldx, a.w = s.w_direct ? w : ws.wc, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
