@@ -10,10 +10,11 @@
 // Only labelled rows take part: their numbers are gathered first (stable, no atomics), x is packed through that list, and every
 // kernel takes the number of rows from the device -- nine pixels of ten unlabelled cost a tenth.
 //
-// Types: 16-bit x and W go to the matrix pipe as they are; fp32 as pairs of fp16 (nt_product.h) under one power-of-two scale per tensor, which
-// keeps 22 bits of everything within 2^-17 of the tensor's largest value; short products of fp16 as pairs too, for G's sake (ce_shape).  In the backward products x and W are always fp16 (bf16 ones
-// converted exactly, under such a scale), because G in fp16 keeps 11 bits where bf16 would keep 8; G is scaled so that the largest |g_t| is at
-// 2^14.  Row statistics, sums and db are fp32 (joins in fp64).
+// Types: fp32 operands and their G go to the matrix pipe as triples of bf16 (nt_product.h): exactly, whatever their sizes, so that no row, class or feature costs
+// another its bits; short products of fp16 as triples too, for G's sake (ce_shape).  Other 16-bit x and W go as they are.  Their G is fp16, which keeps 11 bits
+// where bf16 would keep 8, and so are x and W in its products: bf16 ones under a power-of-two scale per tensor, exact down to 2^-31 of the tensor's largest value and
+// lost below 2^-39.  For dx a row of G is made with a factor of one, at 2^14, for dW with its own, the largest |g_t| at 2^14; what lies below 2^-39 of that is
+// lost.  Row statistics, sums and db are fp32 (joins in fp64).
 //
 // Measured at 7370 labelled rows x 50000 x 1024 bf16: forward 684 us (1103 TFLOP/s), and per half of the classes G 494 (764: its stores) and each
 // gradient 393 (960), where a large library product reaches 1430 and one of a gradient's size 1068.  Bound by the fill of LDS from L2 and by its
@@ -29,22 +30,21 @@ constexpr int CE_PARTS = 1024;                  // partial results of the max pa
 constexpr int CE_LOSS_WGS = 512;
 
 // kept from the forward to the backward pass, at the head of the caller's `saved` buffer; T = rows
-//   int count (labelled rows), float scales[4] at byte 16 (pair form) | ... 64 bytes | int idx[T] | int label[T] | float2 stat[T] (row maximum, 1 / sum)
+//   int count (labelled rows) | ... 64 bytes | int idx[T] | int label[T] | float2 stat[T] (row maximum, 1 / sum)
 struct CeSaved {
   int* count;
   int* idx;
   int* lab;
   float2* stat;
-  float* scal;
 };
 __host__ __device__ __forceinline__ i64 ce_up(i64 v, i64 a) { return (v + a - 1) / a * a; }
 CeSaved ce_saved(void* p, i64 T) {
   char* c = (char*)p;
   const i64 n = ce_up(4 * T, 64);
-  return CeSaved{(int*)c, (int*)(c + 64), (int*)(c + 64 + n), (float2*)(c + 64 + 2 * n), (float*)(c + 16)};
+  return CeSaved{(int*)c, (int*)(c + 64), (int*)(c + 64 + n), (float2*)(c + 64 + 2 * n)};
 }
 
-// scalars on the device: [0] / [1] the scale of x / W in pair or converted form, [2] / [3] their reciprocals, [4] 1 / (scale of G)
+// the backward pass's scalars on the device: [0] / [1] the scale of bf16 x / W as fp16, [2] / [3] their reciprocals, [4] 1 / (scale of G)
 enum { SC_X = 0, SC_W = 1, SC_RX = 2, SC_RW = 3, SC_RG = 4, SC_N = 8 };
 
 __device__ __forceinline__ float ce_load(const void* p, int dtype, i64 i) {
@@ -197,13 +197,15 @@ __device__ __forceinline__ void ce_zero_rows(const void* labels, int ltype, i64 
   }
 }
 
-// rows' factors g_t * scale (reduction 0: one upstream gradient per row; 1 mean, 2 sum: one for all); zeros for dx's other rows
+// G is made with CE_UNIT in the factors' place (triples: with one).  These are the rows' factors g_t * scale over that (reduction 0: one upstream gradient per row;
+// 1 mean, 2 sum: one for all); zeros for dx's other rows
+constexpr float CE_UNIT = 16384.f;
 struct CeFactors {
   const float* g;          // upstream gradient
   int reduction;
   const float* part;       // reduction 0: maxima of |g|
   CeSaved s;
-  int pair;
+  int triple;
   float *scal, *out;
   float4* meta;
   const float* bias;
@@ -217,29 +219,23 @@ struct CeFactors {
 __device__ __forceinline__ void ce_factors(const CeFactors& a, float* sm) {
   const CeSaved& s = a.s;
   const float* const g = a.g;
-  const int reduction = a.reduction, pair = a.pair, V = a.V, n = s.count[0], tid = threadIdx.x;
+  const int reduction = a.reduction, triple = a.triple, V = a.V, n = s.count[0], tid = threadIdx.x;
   const float *const part = a.part, *const bias = a.bias;
   float *const scal = a.scal, *const out = a.out, *const bias_pad = a.bias_pad;
   float4* const meta = a.meta;
   if (a.dx) ce_zero_rows(a.labels, a.ltype, a.T, a.ignore, a.dx, a.row_bytes);
   const float one = reduction == 1 ? (float)((double)g[0] / (double)n) : reduction == 2 ? g[0] : 0.f;
   float m = fabsf(one);
-  if (reduction == 0)
+  if (reduction == 0 && !triple)
     for (int k = tid; k < CE_PARTS; k += 256) m = fmaxf(m, part[k]);
-  // The largest factor at 2^14.  Of 16-bit G exactly there: a label's entry, -g (1 - p), mostly the largest of its row, then lies right below 2^14, where
-  // fp16 is finest for its size (1.4e-4 of it, 2.1e-4 on average elsewhere).  Of a pair by a power of two.
-  const float top = ce_block_max(m, sm);
-  const float sc = pair || !(top > 1e-30f && top < INFINITY) ? 0.5f * ce_pow2_scale(top) : 16384.f / top;
-  if (blockIdx.x == 0 && tid == 0) {
-    scal[SC_RG] = 1.f / sc;
-    if (pair) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) scal[k] = s.scal[k];
-    }
-  }
+  // The largest factor of 16-bit G is at 2^14 exactly: a label's entry, -g (1 - p), mostly the largest of its row, then lies right below 2^14, where
+  // fp16 is finest for its size (1.4e-4 of it, 2.1e-4 on average elsewhere).  Triples need no scale.
+  const float top = triple ? 1.f : ce_block_max(m, sm);
+  const float sc = triple ? 1.f : !(top > 1e-30f && top < INFINITY) ? 0.5f * ce_pow2_scale(top) : CE_UNIT / top;
+  if (blockIdx.x == 0 && tid == 0) scal[SC_RG] = 1.f / sc;
   for (i64 r = (i64)blockIdx.x * 256 + tid; r < n; r += (i64)gridDim.x * 256) {
     const float f = reduction == 0 ? g[s.idx[r]] : one;
-    out[r] = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : f * sc;
+    out[r] = s.lab[r] < 0 ? __uint_as_float(0x7fc00000u) : f * (sc / (triple ? 1.f : CE_UNIT));
   }
   if (!meta) return;
   // the fused form's row table, whole tiles of 64 rows long (a row behind the last one: exp2(-inf) * 0), and its bias likewise
@@ -267,16 +263,16 @@ struct CePack {
   i64 ld, rows, begin;     // rows [begin, begin + rows) of the source (of the list); same and turned start there
   const int* idx;          // row list (x) or NULL
   const int* count;        // rows from the device, or NULL
-  const float* part;       // CE_PARTS maxima the scale comes from, or NULL
-  const float* scale;      // or the scale itself, or NULL: 1.  Applied to the pair form and to fp16 made of bf16
+  const float* part;       // CE_PARTS maxima that the scale of fp16 made of bf16 comes from
+  const float* scale;      // or the scale itself; neither: 1
   float *put, *rput;       // where the scale and its reciprocal go (with part)
   void* same;              // [rows][K] operand rows, or NULL
   i64 ld_same;
   int same_k;              // its padded width: whole stages, a multiple of 8
-  int same_kind;           // 0 bf16, 1 fp16, 2 pair
-  void* turned;            // [D][rows] operand rows (fp16 or pair), or NULL
+  int same_kind;           // 0 bf16, 1 fp16, 2 triples
+  void* turned;            // [D][rows] operand rows (fp16, scaled, or triples), or NULL
   i64 ld_turned;
-  int turned_pair;
+  int turned_triple;
 };
 template <typename T>
 __device__ __forceinline__ void ce_load8(const T* q, int left, int vec, float (&v)[8]) {
@@ -294,7 +290,7 @@ __device__ __forceinline__ void ce_load8(const T* q, int left, int vec, float (&
 }
 // one 64 x 64 block of the source per workgroup (blockIdx.x: rows, .y: columns, .z: which operand); pads are written as zeros
 // (the last slice of a launch with f.g: the rows' factors, which need nothing of the operands)
-// LOOSE: some rows are not aligned for vectors; they come by a value per lane, through the tile (122 x 72099 x 1730 fp32: 380 -> 315 us a launch, whose
+// LOOSE: some rows are not aligned for vectors; they come by a value per lane, through the tile (122 x 72099 x 1730 fp32: 528 -> 427 us a launch, whose
 // registers cost aligned operands a third: 15 -> 20 us at 524288 x 16)
 template <bool LOOSE>
 __global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw, CeFactors f) {
@@ -363,10 +359,7 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw, CeFa
     if (a.same && r < rows && c < a.same_k) {
       char* row = (char*)a.same + r * a.ld_same * 2;
       if (a.same_kind == 2) {
-        float q[8];
-#pragma unroll
-        for (int t = 0; t < 8; ++t) q[t] = v[t] * sc;
-        nt_store_pair((f16_t*)row, c, q);
+        nt_store_triple((bf16_t*)row, c, v);
       } else if (a.same_kind == 1) {
         *(uint4*)((f16_t*)row + c) = VecWords<f16_t>::pack(v);
       } else {
@@ -386,9 +379,9 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CePack px, CePack pw, CeFa
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = tile[c + i][r];
-    f16_t* row = (f16_t*)a.turned + (i64)(c0 + r) * a.ld_turned;
-    if (a.turned_pair)
-      nt_store_pair(row, r0 + c, v);
+    uint16_t* row = (uint16_t*)a.turned + (i64)(c0 + r) * a.ld_turned;
+    if (a.turned_triple)
+      nt_store_triple((bf16_t*)row, r0 + c, v);
     else
       *(uint4*)(row + r0 + c) = VecWords<f16_t>::pack(v);
   }
@@ -401,7 +394,6 @@ struct CeLogits {
   i64 ldx, ldw;
   int stages, V;
   const float* bias;
-  const float* scal;       // NULL, or the pair form's scales
   CeSaved s;
   // forward
   float2* part;            // [row][ntj]
@@ -410,8 +402,8 @@ struct CeLogits {
   // backward: rows [t0, t0 + Tc), classes [v0, v0 + Vc)
   i64 t0, Tc;
   int v0, Vc;
-  const float* g;          // row factors, scaled
-  f16_t *dl, *dlt;
+  const float* g;          // row factors
+  uint16_t *dl, *dlt;
   i64 ld_dl, ld_dlt;
   float* db;               // [row tile][V] partial column sums, or NULL
   float* db_out;           // or, where one row tile holds every row, the sums themselves
@@ -435,11 +427,11 @@ __device__ __forceinline__ bool ce_tile(int nti, int ntj, int& ti, int& tj) {
 // rounding of m log2 e, which overflows the exponential where every class of a lane is ruled out by a bias of -1e10 or less.
 __device__ __forceinline__ float ce_exp(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * CE_LOG2E); }
 
-// The bias of a lane's columns: 16-bit operands start from it, pairs get it behind their scales.
-template <bool PAIR, class Core>
+// The bias of a lane's columns: 16-bit operands start from it, triples get it behind their sum (a rounding instead of one per instruction).
+template <class Core>
 __device__ __forceinline__ void ce_begin(Core& c, const CeLogits& a, int c0) {
   c.clear();
-  if (PAIR || !a.bias) return;
+  if (Core::PARTS == 3 || !a.bias) return;
   const int j0 = c0 + Core::col0() + 4 * (Core::lane() >> 4);
 #pragma unroll
   for (int j = 0; j < Core::TJ; ++j)
@@ -450,23 +442,22 @@ __device__ __forceinline__ void ce_begin(Core& c, const CeLogits& a, int c0) {
       for (int i = 0; i < Core::TI; ++i) c.acc[i][j][r] = b;
     }
 }
-template <bool PAIR, class Core>
+template <class Core>
 __device__ __forceinline__ void ce_finish(Core& c, const CeLogits& a, int c0) {
-  if constexpr (PAIR) {
-    const float rx = a.scal ? a.scal[SC_RX] : 1.f, rw = a.scal ? a.scal[SC_RW] : 1.f;
+  if (Core::PARTS == 3 && a.bias) {
     const int j0 = c0 + Core::col0() + 4 * (Core::lane() >> 4);
 #pragma unroll
     for (int j = 0; j < Core::TJ; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float b = a.bias && j0 + j * 16 + r < a.V ? a.bias[j0 + j * 16 + r] : 0.f;
+        const float b = j0 + j * 16 + r < a.V ? a.bias[j0 + j * 16 + r] : 0.f;
 #pragma unroll
-        for (int i = 0; i < Core::TI; ++i) c.acc[i][j][r] = c.acc[i][j][r] * rx * rw + b;
+        for (int i = 0; i < Core::TI; ++i) c.acc[i][j][r] += b;
       }
   }
 }
 
-template <class Core, typename T, bool PAIR>
+template <class Core, typename T>
 __global__ __launch_bounds__(Core::THREADS) void ce_fwd_kernel(CeLogits a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int n = a.s.count[0];
@@ -474,9 +465,9 @@ __global__ __launch_bounds__(Core::THREADS) void ce_fwd_kernel(CeLogits a) {
   if (!ce_tile((n + Core::BM - 1) / Core::BM, a.ntj, ti, tj)) return;
   const int r0 = ti * Core::BM, c0 = tj * Core::BN;
   Core c;
-  ce_begin<PAIR>(c, a, c0);
+  ce_begin(c, a, c0);
   c.run((const T*)a.x + (i64)r0 * a.ldx, a.ldx, n - r0, (const T*)a.w + (i64)c0 * a.ldw, a.ldw, a.V - c0, 0, a.stages, smem);
-  ce_finish<PAIR>(c, a, c0);
+  ce_finish(c, a, c0);
   const int l = Core::lane(), j0 = c0 + Core::col0() + 4 * (l >> 4);
   if (c0 + Core::BN > a.V) {
 #pragma unroll
@@ -598,15 +589,22 @@ __global__ __launch_bounds__(256) void ce_gmax_kernel(const float* g, const int*
   __syncthreads();
   if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
 }
-template <bool PAIR>
-__device__ __forceinline__ int ce_kpad(int n) { return PAIR ? (n + 31) & ~31 : (n + 63) & ~63; }
+template <class Core>
+__device__ __forceinline__ int ce_kpad(int n) { return Core::PARTS == 3 ? (n + 31) & ~31 : (n + 63) & ~63; }
+template <class Core>
+__device__ __forceinline__ void ce_store_g(uint16_t* row, long k, const float (&v)[8]) {
+  if constexpr (Core::PARTS == 3)
+    nt_store_triple((bf16_t*)row, k, v);
+  else
+    *(uint4*)(row + k) = VecWords<f16_t>::pack(v);
+}
 
 // G of a piece, in both orientations.  A row of dx is its own factor times what it would be with a factor of one: the rows that dx's product reads are made
 // with CE_UNIT in the factor's place, which its epilogue puts right, and only the columns that dW's sum over rows reads carry the factors.
-constexpr float CE_UNIT = 16384.f;
-template <class Core, typename T, bool PAIR>
+template <class Core, typename T>
 __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr float UNIT = Core::PARTS == 3 ? 1.f : CE_UNIT;
   constexpr int SB = Core::BLOCK, EXTRA = Core::NW * NtBlock<SB, SB>::BYTES;
   const i64 left = (i64)a.s.count[0] - a.t0;
   const int n = (int)(left < 0 ? 0 : left < a.Tc ? left : a.Tc);       // rows of this piece
@@ -620,17 +618,17 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
   const i64 rg = a.t0 + r0;
   const int cg = a.v0 + c0;
   Core c;
-  ce_begin<PAIR>(c, a, cg);
+  ce_begin(c, a, cg);
   c.run((const T*)a.x + rg * a.ldx, a.ldx, n - r0, (const T*)a.w + (i64)cg * a.ldw, a.ldw, a.V - cg, 0, a.stages, smem);
-  ce_finish<PAIR>(c, a, cg);
-  float4* meta = (float4*)(smem + EXTRA);                               // [BM]: maximum, CE_UNIT / sum, factor / CE_UNIT, label
+  ce_finish(c, a, cg);
+  float4* meta = (float4*)(smem + EXTRA);                               // [BM]: maximum, UNIT / sum, factor, label
   float* fac = (float*)(smem + EXTRA + Core::BM * 16);                  // [BM]: the factors alone, for vectors of rows
   float* colsum = fac + Core::BM;                                      // [BM / WM][BN]
   for (int row = threadIdx.x; row < Core::BM; row += Core::THREADS) {
     float4 m = make_float4(INFINITY, 0.f, 0.f, __int_as_float(-1));    // (rows behind the last one: exp2(-inf) = 0)
     if (r0 + row < n) {
       const float2 st = a.s.stat[rg + row];
-      m = make_float4(st.x, CE_UNIT * st.y, a.g[rg + row] * (1.f / CE_UNIT), __int_as_float(a.s.lab[rg + row]));
+      m = make_float4(st.x, UNIT * st.y, a.g[rg + row], __int_as_float(a.s.lab[rg + row]));
     }
     meta[row] = m;
     fac[row] = m.z;
@@ -651,7 +649,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
 #pragma unroll
       for (int j = 0; j < Core::TJ; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) c.acc[i][j][r] -= lab == j * 16 + 4 * (l >> 4) + r ? CE_UNIT : 0.f;
+        for (int r = 0; r < 4; ++r) c.acc[i][j][r] -= lab == j * 16 + 4 * (l >> 4) + r ? UNIT : 0.f;
     }
   }
   if (cg + Core::BN > a.V) {
@@ -689,7 +687,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
     }
   }
   const NtBlock<SB, SB> blk{(float*)(smem + Core::wave() * NtBlock<SB, SB>::BYTES)};
-  const int vcols = a.V - a.v0 < a.Vc ? a.V - a.v0 : a.Vc, vpad = ce_kpad<PAIR>(vcols), npad = ce_kpad<PAIR>(n);
+  const int vcols = a.V - a.v0 < a.Vc ? a.V - a.v0 : a.Vc, vpad = ce_kpad<Core>(vcols), npad = ce_kpad<Core>(n);
 #pragma unroll
   for (int bi = 0; bi < Core::WM / SB; ++bi)
 #pragma unroll
@@ -699,11 +697,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
       if (a.dl) {
         blk.template rows<false>([&](int i, int j0, float (&v)[8]) {
           if (gi + i >= n || gj + j0 >= vpad) return;
-          f16_t* row = a.dl + (i64)(gi + i) * a.ld_dl;
-          if constexpr (PAIR)
-            nt_store_pair(row, gj + j0, v);
-          else
-            *(uint4*)(row + gj + j0) = VecWords<f16_t>::pack(v);
+          ce_store_g<Core>(a.dl + (i64)(gi + i) * a.ld_dl, gj + j0, v);
         });
       }
       if (a.dlt) {
@@ -711,11 +705,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
           if (gj + j >= vcols || gi + i0 >= npad) return;
           const float4 lo = *(const float4*)(fac + gi - r0 + i0), hi = *(const float4*)(fac + gi - r0 + i0 + 4);
           v[0] *= lo.x, v[1] *= lo.y, v[2] *= lo.z, v[3] *= lo.w, v[4] *= hi.x, v[5] *= hi.y, v[6] *= hi.z, v[7] *= hi.w;
-          f16_t* row = a.dlt + (i64)(gj + j) * a.ld_dlt;
-          if constexpr (PAIR)
-            nt_store_pair(row, gi + i0, v);
-          else
-            *(uint4*)(row + gi + i0) = VecWords<f16_t>::pack(v);
+          ce_store_g<Core>(a.dlt + (i64)(gj + j) * a.ld_dlt, gi + i0, v);
         });
       }
     }
@@ -723,7 +713,7 @@ __global__ __launch_bounds__(Core::THREADS) void ce_dlogits_kernel(CeLogits a) {
 
 // dx (A = G rows, B = W^T rows) or dW (A = G^T rows, B = x^T rows)
 struct CeGrad {
-  const f16_t *a, *b;
+  const uint16_t *a, *b;
   i64 lda, ldb;
   int M, N;                // upper bound of the output's rows; columns (D)
   i64 K;                   // upper bound of the contraction (values)
@@ -737,7 +727,7 @@ struct CeGrad {
   int out_dtype, accumulate, vec;
   i64 ldo;
   const int* idx;          // dx: where a row belongs, else NULL
-  const float* rowf;       // dx of G made with CE_UNIT: the rows' factors, else NULL
+  const float* rowf;       // dx: the rows' factors, where G was made without them, else NULL
   const float* scal;
   int rscale;              // index of the reciprocal of b's scale, -1: none
 };
@@ -766,10 +756,10 @@ __device__ __forceinline__ void ce_put(const CeGrad& a, i64 row, int col, const 
     }
   }
 }
-__device__ __forceinline__ float ce_row_factor(const CeGrad& a, i64 r) { return a.rowf ? a.rowf[a.t0 + r] * (1.f / CE_UNIT) : 1.f; }
+__device__ __forceinline__ float ce_row_factor(const CeGrad& a, i64 r) { return a.rowf ? a.rowf[a.t0 + r] : 1.f; }
 __device__ __forceinline__ float ce_rscale(const CeGrad& a) { return a.rscale >= 0 ? a.scal[a.rscale] : 1.f; }
 
-template <class Core, bool PAIR>
+template <class Core, typename T>
 __global__ __launch_bounds__(Core::THREADS) void ce_grad_kernel(CeGrad a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const i64 left = (i64)a.count[0] - a.t0;
@@ -781,11 +771,11 @@ __global__ __launch_bounds__(Core::THREADS) void ce_grad_kernel(CeGrad a) {
   if (!ce_tile(nti, ntj * a.splits, ti, tj)) return;
   const int sp = tj / ntj;                                              // (workgroups that run together share a part of the contraction)
   tj -= sp * ntj;
-  const int stages = (int)((K + (PAIR ? 31 : 63)) / (PAIR ? 32 : 64)), per = (stages + a.splits - 1) / a.splits;
+  const int stages = (int)((K + (Core::PARTS == 3 ? 31 : 63)) / (Core::PARTS == 3 ? 32 : 64)), per = (stages + a.splits - 1) / a.splits;
   const int s0 = sp * per < stages ? sp * per : stages, s1 = s0 + per < stages ? s0 + per : stages;
   Core c;
   c.clear();
-  c.run(a.a + (i64)ti * Core::BM * a.lda, a.lda, M - ti * Core::BM, a.b + (i64)tj * Core::BN * a.ldb, a.ldb, a.N - tj * Core::BN, s0, s1, smem);
+  c.run((const T*)a.a + (i64)ti * Core::BM * a.lda, a.lda, M - ti * Core::BM, (const T*)a.b + (i64)tj * Core::BN * a.ldb, a.ldb, a.N - tj * Core::BN, s0, s1, smem);
   constexpr int SB = Core::BLOCK;
   const NtBlock<SB, SB> blk{(float*)(smem + Core::wave() * NtBlock<SB, SB>::BYTES)};
   const float rg = a.scal[SC_RG], rb = ce_rscale(a);
@@ -904,7 +894,7 @@ struct CeFused {
   CeSaved s;
   const void *own, *tile;  // rows in registers, streamed rows: packed operands
   i64 ld_own, ld_tile;
-  const f16_t* turned;     // the streamed side turned, [D][..]
+  const uint16_t* turned;  // the streamed side turned, [D][..]
   i64 ld_turned;
   const float4* meta;      // per token: maximum, factor / sum, factor, label
   const float* bias;       // padded to 64 classes (zeros without a bias)
@@ -1200,31 +1190,39 @@ struct Carve {
 };
 
 struct CeShape {
-  bool pair, fused;
+  bool triple, fused;
+  int tile;                // of the logits' product, see CE_BM
   int ku;                  // values per stage
   int kp;                  // D padded to stages
   int kw;                  // packed rows' width: kp; in the fused form, which masks the rest of a stage, a multiple of 8
   i64 ldx;                 // packed operand rows, elements
   bool w_direct;           // W is used where it lies
   i64 ldw;
-  bool scaled;             // scales are computed (pair forms, or fp16 made of bf16)
+  bool scaled;             // scales are computed (fp16 made of bf16)
 };
+// tiles of the logits' product: 256 x 256, of triples, whose two stages would not fit the LDS, 128 x 256; 64 rows where there are no more (the classes are then
+// streamed once, and three quarters of a tall tile would repeat the last row), 128 likewise (122 x 72099 x 1730 bf16: G 126 -> 116 us, forward 105 -> 100); 64
+// or 128 classes too
+int ce_logits_tile(const FiLinearCe& d, bool triple) { return d.T <= 64 ? 1 : d.V <= 64 ? 2 : d.V <= 128 ? 3 : d.T <= 128 || triple ? 4 : 0; }
+constexpr int CE_BM[5] = {256, 64, 256, 256, 128}, CE_BN[5] = {256, 256, 64, 128, 256};
+
 // Logits and G stay in registers (ce_fused_kernel) for 16-bit operands of up to 128 features; rows up to where a turned operand's offsets fit 32 bits
 // (forward pass of up to 64 rows: the 64 x 256 tiles of the general product read the classes with more workgroups)
 CeShape ce_shape(const FiLinearCe& d, const void* w, bool fwd) {
   CeShape s;
-  // Half precision keeps 11 bits, as many as G does: up to 2^28 multiply-adds, where three products cost no more than one, it goes as pairs too, and
+  // Half precision keeps 11 bits, as many as G does: up to 2^28 multiply-adds, where six products cost little more than one, it goes as triples too, and
   // its gradients are rounded once (over 80 sizes, those more than 1.5 times an fp32 product's error off fell from 10 to none)
-  s.pair = d.dtype == FI_F32 || (d.dtype == FI_F16 && (double)d.T * d.V * d.D <= (double)(1 << 28));
-  s.ku = s.pair ? 32 : 64;
+  s.triple = d.dtype == FI_F32 || (d.dtype == FI_F16 && (double)d.T * d.V * d.D <= (double)(1 << 28));
+  s.ku = s.triple ? 32 : 64;
   s.kp = (int)ce_up(d.D, s.ku);
-  s.fused = !s.pair && s.kp <= 128 && d.T <= (1 << 23) && !(fwd && d.T <= 64);
+  s.fused = !s.triple && s.kp <= 128 && d.T <= (1 << 23) && !(fwd && d.T <= 64);
+  s.tile = ce_logits_tile(d, s.triple);
   s.kw = s.fused ? (int)ce_up(d.D, 8) : s.kp;
-  s.ldx = s.pair ? 2L * s.kw : s.kw;
+  s.ldx = s.triple ? 3L * s.kw : s.kw;
   // 16-bit weights whose rows need no padding and are 16-byte aligned are read in place
-  s.w_direct = !s.pair && d.wdtype == d.dtype && d.D == s.kw && d.ldw % 8 == 0 && ((uintptr_t)w & 15) == 0;
+  s.w_direct = !s.triple && d.wdtype == d.dtype && d.D == s.kw && d.ldw % 8 == 0 && ((uintptr_t)w & 15) == 0;
   s.ldw = s.w_direct ? d.ldw : s.ldx;
-  s.scaled = d.dtype != FI_F16;                  // (fp16 values are their own high parts)
+  s.scaled = d.dtype == FI_BF16;
   return s;
 }
 
@@ -1239,56 +1237,50 @@ int ce_check(const FiLinearCe* d) {
   return 0;
 }
 
-// tiles of the logits' product: 256 x 256; 64 rows where there are no more (the classes are then streamed once, and three quarters of a
-// tall tile would repeat the last row), 128 likewise (122 x 72099 x 1730 fp32: G 264 -> 221 us, forward 223 -> 190); 64 or 128 classes too
-int ce_logits_tile(const FiLinearCe& d) { return d.T <= 64 ? 1 : d.V <= 64 ? 2 : d.V <= 128 ? 3 : d.T <= 128 ? 4 : 0; }
-constexpr int CE_BM[5] = {256, 64, 256, 256, 128}, CE_BN[5] = {256, 256, 64, 128, 256};
-
 // (the same tile by 16 waves of 64 x 64 in the forward pass -- four per SIMD hide LDS and DMA latency: 845 -> 757 us at 7370 x 50000 x 1024 -- and by
 // 8 of 128 x 64 for G, whose epilogue wants 64 x 64 blocks of scratch: 267 against 290 us a piece of 7370 x 16384)
-template <typename T, bool PAIR> struct CeCores {
-  typedef NtCore<T, PAIR, 256, 256, 64, 64> F0;
-  typedef NtCore<T, PAIR, 256, 256, 128, 64> C0;
-  typedef NtCore<T, PAIR, 64, 256, 64, 32> C1;
-  typedef NtCore<T, PAIR, 256, 64, 32, 64> C2;
-  typedef NtCore<T, PAIR, 256, 128, 64, 64> C3;
-  typedef NtCore<T, PAIR, 128, 256, 64, 64> C4;
+template <typename T, int PARTS> struct CeCores {
+  typedef NtCore<T, PARTS, 64, 256, 64, 32> C1;
+  typedef NtCore<T, PARTS, 256, 64, 32, 64> C2;
+  typedef NtCore<T, PARTS, 256, 128, 64, 64> C3;
+  typedef NtCore<T, PARTS, 128, 256, 64, 64> C4;
 };
 
-template <class Core, typename T, bool PAIR>
+template <class Core, typename T>
 int ce_launch_fwd(const CeLogits& a, i64 T_rows, hipStream_t st) {
   static NtLdsDevices allowed;
-  if (!nt_allow_lds((const void*)ce_fwd_kernel<Core, T, PAIR>, allowed)) return FI_ERR_UNSUPPORTED;
+  if (!nt_allow_lds((const void*)ce_fwd_kernel<Core, T>, allowed)) return FI_ERR_UNSUPPORTED;
   const i64 n = (T_rows + Core::BM - 1) / Core::BM * a.ntj;
   if (n > (1LL << 30)) return FI_ERR_SHAPE;
-  hipLaunchKernelGGL((ce_fwd_kernel<Core, T, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), Core::LDS, st, a);
+  hipLaunchKernelGGL((ce_fwd_kernel<Core, T>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), Core::LDS, st, a);
   FI_CHECK_LAUNCH();
   return 0;
 }
-template <class Core, typename T, bool PAIR>
+template <class Core, typename T>
 int ce_launch_dlogits(const CeLogits& a, hipStream_t st) {
   static NtLdsDevices allowed;
-  if (!nt_allow_lds((const void*)ce_dlogits_kernel<Core, T, PAIR>, allowed)) return FI_ERR_UNSUPPORTED;
+  if (!nt_allow_lds((const void*)ce_dlogits_kernel<Core, T>, allowed)) return FI_ERR_UNSUPPORTED;
   constexpr int SB = Core::BLOCK, SCR = Core::NW * NtBlock<SB, SB>::BYTES;
   constexpr int need = SCR + Core::BM * 20 + Core::BM / Core::WM * Core::BN * 4, lds = need > Core::LDS ? need : Core::LDS;
   const i64 n = (a.Tc + Core::BM - 1) / Core::BM * ((a.Vc + Core::BN - 1) / Core::BN);
-  hipLaunchKernelGGL((ce_dlogits_kernel<Core, T, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), lds, st, a);
+  hipLaunchKernelGGL((ce_dlogits_kernel<Core, T>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), lds, st, a);
   FI_CHECK_LAUNCH();
   return 0;
 }
-template <typename T, bool PAIR>
-int ce_logits(const CeLogits& a, const FiLinearCe& d, bool fwd, hipStream_t st) {
-  typedef CeCores<T, PAIR> C;
-  switch (ce_logits_tile(d)) {
-    case 0: return fwd ? ce_launch_fwd<typename C::F0, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C0, T, PAIR>(a, st);
-    case 1: return fwd ? ce_launch_fwd<typename C::C1, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C1, T, PAIR>(a, st);
-    case 2: return fwd ? ce_launch_fwd<typename C::C2, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C2, T, PAIR>(a, st);
-    case 3: return fwd ? ce_launch_fwd<typename C::C3, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C3, T, PAIR>(a, st);
-    default: return fwd ? ce_launch_fwd<typename C::C4, T, PAIR>(a, d.T, st) : ce_launch_dlogits<typename C::C4, T, PAIR>(a, st);
+template <typename T, int PARTS>
+int ce_logits(const CeLogits& a, i64 T_rows, int tile, bool fwd, hipStream_t st) {
+  typedef CeCores<T, PARTS> C;
+  switch (tile) {
+    case 1: return fwd ? ce_launch_fwd<typename C::C1, T>(a, T_rows, st) : ce_launch_dlogits<typename C::C1, T>(a, st);
+    case 2: return fwd ? ce_launch_fwd<typename C::C2, T>(a, T_rows, st) : ce_launch_dlogits<typename C::C2, T>(a, st);
+    case 3: return fwd ? ce_launch_fwd<typename C::C3, T>(a, T_rows, st) : ce_launch_dlogits<typename C::C3, T>(a, st);
+    case 4: return fwd ? ce_launch_fwd<typename C::C4, T>(a, T_rows, st) : ce_launch_dlogits<typename C::C4, T>(a, st);
   }
+  if constexpr (PARTS == 1) return fwd ? ce_launch_fwd<NtCore<T, 1, 256, 256, 64, 64>, T>(a, T_rows, st) : ce_launch_dlogits<NtCore<T, 1, 256, 256, 128, 64>, T>(a, st);
+  return FI_ERR_UNSUPPORTED;
 }
-int ce_logits_any(const CeLogits& a, const FiLinearCe& d, bool pair, bool fwd, hipStream_t st) {
-  return pair ? ce_logits<f16_t, true>(a, d, fwd, st) : d.dtype == FI_BF16 ? ce_logits<bf16_t, false>(a, d, fwd, st) : ce_logits<f16_t, false>(a, d, fwd, st);
+int ce_logits_any(const CeLogits& a, const FiLinearCe& d, const CeShape& s, bool fwd, hipStream_t st) {
+  return s.triple ? ce_logits<bf16_t, 3>(a, d.T, s.tile, fwd, st) : d.dtype == FI_BF16 ? ce_logits<bf16_t, 1>(a, d.T, s.tile, fwd, st) : ce_logits<f16_t, 1>(a, d.T, s.tile, fwd, st);
 }
 
 // one or two operands in a launch (src == NULL: none)
@@ -1347,9 +1339,9 @@ int ce_fused(const CeFused& a, const FiLinearCe& d, int kp, hipStream_t st) {
 
 struct CeFwdWs {
   int* cnt;
-  float *parts, *zt, *bias_pad;
+  float *zt, *bias_pad;
   int nparts;              // of a row's statistics
-  f16_t *xc, *wc;
+  uint16_t *xc, *wc;
   float2* part;
   double* sums;
   i64 bytes;
@@ -1358,12 +1350,11 @@ CeFwdWs ce_fwd_ws(const FiLinearCe& d, const CeShape& s, void* p) {
   Carve c{(char*)p};
   CeFwdWs w;
   w.cnt = c.take<int>((d.T + CE_ROWS - 1) / CE_ROWS);
-  w.parts = c.take<float>(2 * CE_PARTS);
   w.zt = c.take<float>(d.T);
   w.sums = c.take<double>(CE_LOSS_WGS);
-  w.xc = c.take<f16_t>(d.T * s.ldx);
-  w.wc = s.w_direct ? nullptr : c.take<f16_t>((i64)d.V * s.ldx);
-  const int bn = CE_BN[ce_logits_tile(d)];
+  w.xc = c.take<uint16_t>(d.T * s.ldx);
+  w.wc = s.w_direct ? nullptr : c.take<uint16_t>((i64)d.V * s.ldx);
+  const int bn = CE_BN[s.tile];
   w.nparts = s.fused ? ce_fused_splits(d.T, d.V) : (d.V + bn - 1) / bn;
   w.bias_pad = s.fused ? c.take<float>(ce_up(d.V, 64)) : nullptr;
   w.part = c.take<float2>(d.T * w.nparts);
@@ -1371,19 +1362,19 @@ CeFwdWs ce_fwd_ws(const FiLinearCe& d, const CeShape& s, void* p) {
   return w;
 }
 
-// scal: where the scales are (parts == NULL) or go
-CePack ce_pack_x(const FiLinearCe& d, const CeShape& s, const void* x, const CeSaved& sv, const float* parts, float* scal, f16_t* xc) {
+// scal: NULL, or where the scales are (parts == NULL) or go
+CePack ce_pack_x(const FiLinearCe& d, const CeShape& s, const void* x, const CeSaved& sv, const float* parts, float* scal, uint16_t* xc) {
   CePack k = {};
   k.src = x, k.dtype = k.round = d.dtype, k.D = d.D, k.vec = ce_vec(x, d.dtype, d.ldx), k.ld = d.ldx, k.rows = d.T, k.idx = sv.idx, k.count = sv.count;
   if (scal) k.part = parts, k.scale = parts ? nullptr : scal + SC_X, k.put = scal + SC_X, k.rput = scal + SC_RX;
-  k.same = xc, k.ld_same = s.ldx, k.same_k = s.kw, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
+  k.same = xc, k.ld_same = s.ldx, k.same_k = s.kw, k.same_kind = s.triple ? 2 : d.dtype == FI_F16 ? 1 : 0;
   return k;
 }
-CePack ce_pack_w(const FiLinearCe& d, const CeShape& s, const void* w, const float* parts, float* scal, f16_t* wc) {
+CePack ce_pack_w(const FiLinearCe& d, const CeShape& s, const void* w, const float* parts, float* scal, uint16_t* wc) {
   CePack k = {};
   k.src = w, k.dtype = d.wdtype, k.round = d.dtype, k.D = d.D, k.vec = ce_vec(w, d.wdtype, d.ldw), k.ld = d.ldw, k.rows = d.V;
-  if (scal) k.part = parts ? parts + CE_PARTS : nullptr, k.scale = parts ? nullptr : scal + SC_W, k.put = scal + SC_W, k.rput = scal + SC_RW;
-  k.same = wc, k.ld_same = s.ldx, k.same_k = s.kw, k.same_kind = s.pair ? 2 : d.dtype == FI_F16 ? 1 : 0;
+  if (scal) k.part = parts + CE_PARTS, k.put = scal + SC_W, k.rput = scal + SC_RW;
+  k.same = wc, k.ld_same = s.ldx, k.same_k = s.kw, k.same_kind = s.triple ? 2 : d.dtype == FI_F16 ? 1 : 0;
   return k;
 }
 
@@ -1392,14 +1383,13 @@ struct CeGradPlan {
   int tile, splits;
   bool part;
 };
-// Output tiles of 256 x 256, 128 x 128 or 64 x 64 (columns or rows that few); a contraction is split where the tiles do not fill the chip.
-constexpr int CE_GT[3] = {256, 128, 64};
-CeGradPlan ce_grad_plan(i64 M, i64 N, i64 K, int ku, bool pieces) {
+// Output tiles of 256 x 256 (of triples 128 x 256), 128 x 128 or 64 x 64 (columns or rows that few); a contraction is split where the tiles do not fill the chip.
+CeGradPlan ce_grad_plan(i64 M, i64 N, i64 K, bool triple, bool pieces) {
   CeGradPlan p;
-  const i64 least = M < N ? M : N;
-  p.tile = least > 128 && (M + 255) / 256 * ((N + 255) / 256) >= 128 ? 0 : least > 64 ? 1 : 2;
-  const int t = CE_GT[p.tile];
-  const i64 tiles = (M + t - 1) / t * ((N + t - 1) / t), stages = (K + ku - 1) / ku;
+  const i64 least = M < N ? M : N, bm = triple ? 128 : 256, ku = triple ? 32 : 64;
+  p.tile = least > 128 && (M + bm - 1) / bm * ((N + 255) / 256) >= 128 ? 0 : least > 64 ? 1 : 2;
+  const i64 tm = p.tile == 0 ? bm : p.tile == 1 ? 128 : 64, tn = p.tile == 0 ? 256 : tm;
+  const i64 tiles = (M + tm - 1) / tm * ((N + tn - 1) / tn), stages = (K + ku - 1) / ku;
   i64 s = 512 / tiles;
   if (s > stages / 8) s = stages / 8;
   if (s > 64) s = 64;
@@ -1413,19 +1403,19 @@ struct CeBwdWs {
   float *parts, *scal, *g, *db, *pdx, *pdw, *bias_pad;
   float4* meta;
   int sdx, sdw;
-  f16_t *xc, *wc, *xt, *wt, *dl, *dlt;
+  uint16_t *xc, *wc, *xt, *wt, *dl, *dlt;
   i64 ld_xt, ld_wt, ld_dl, ld_dlt, Tc;
   int Vc;
   CeGradPlan dx, dw;
   i64 pdw_piece, bytes;
 };
-// values of G held at a time: two orientations of 16 bits, 1 GiB (2 GiB of pairs).  Smaller pieces write dx's sums more often: 7370 x 50000 x 1024 takes 3486 us
+// values of G held at a time: two orientations of 16 bits, 1 GiB (3 GiB of triples).  Smaller pieces write dx's sums more often: 7370 x 50000 x 1024 takes 3486 us
 // with 2^27, 3291 with 2^28, 3235 with 2^29
 constexpr i64 CE_PIECE = 1LL << 28;
 CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need_dw, bool need_db, void* p) {
   Carve c{(char*)p};
   CeBwdWs w;
-  const int f = s.pair ? 2 : 1;
+  const int f = s.triple ? 3 : 1;
   const i64 Tp = ce_up(d.T, 256), Vp = ce_up(d.V, 256);
   // a piece: all rows, if 256 classes of them fit, and as many classes as do
   w.Tc = Tp < CE_PIECE / 256 ? Tp : CE_PIECE / 256;
@@ -1442,25 +1432,25 @@ CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need
     w.meta = c.take<float4>(ce_up(d.T, 64));
     w.bias_pad = c.take<float>(ce_up(d.V, 64));
     w.db = need_db ? c.take<float>((i64)w.sdw * d.V) : nullptr;
-    w.xc = c.take<f16_t>(d.T * s.ldx);
-    w.wc = s.w_direct ? nullptr : c.take<f16_t>((i64)d.V * s.ldx);
-    w.xt = need_dw || need_db ? c.take<f16_t>(d.D * w.ld_xt) : nullptr;
-    w.wt = need_dx ? c.take<f16_t>(d.D * w.ld_wt) : nullptr;
+    w.xc = c.take<uint16_t>(d.T * s.ldx);
+    w.wc = s.w_direct ? nullptr : c.take<uint16_t>((i64)d.V * s.ldx);
+    w.xt = need_dw || need_db ? c.take<uint16_t>(d.D * w.ld_xt) : nullptr;
+    w.wt = need_dx ? c.take<uint16_t>(d.D * w.ld_wt) : nullptr;
     w.pdx = need_dx && w.sdx > 1 ? c.take<float>((i64)w.sdx * d.T * d.D) : nullptr;
     w.pdw = need_dw && w.sdw > 1 ? c.take<float>((i64)w.sdw * d.V * d.D) : nullptr;
     w.bytes = c.at;
     return w;
   }
-  const int bm = CE_BM[ce_logits_tile(d)];
+  const int bm = CE_BM[s.tile];
   w.db = need_db ? c.take<float>((d.T + bm - 1) / bm * d.V) : nullptr;
-  w.xc = c.take<f16_t>(d.T * s.ldx);
-  w.wc = s.w_direct ? nullptr : c.take<f16_t>((i64)d.V * s.ldx);
-  w.xt = need_dw ? c.take<f16_t>(d.D * w.ld_xt) : nullptr;
-  w.wt = need_dx ? c.take<f16_t>(d.D * w.ld_wt) : nullptr;
-  w.dl = need_dx ? c.take<f16_t>(w.Tc * w.ld_dl) : nullptr;
-  w.dlt = need_dw ? c.take<f16_t>((i64)w.Vc * w.ld_dlt) : nullptr;
-  w.dx = ce_grad_plan(d.T < w.Tc ? d.T : w.Tc, d.D, d.V < w.Vc ? d.V : w.Vc, s.ku, w.Vc < d.V);
-  w.dw = ce_grad_plan(d.V < w.Vc ? d.V : w.Vc, d.D, d.T < w.Tc ? d.T : w.Tc, s.ku, w.Tc < d.T);
+  w.xc = c.take<uint16_t>(d.T * s.ldx);
+  w.wc = s.w_direct ? nullptr : c.take<uint16_t>((i64)d.V * s.ldx);
+  w.xt = need_dw ? c.take<uint16_t>(d.D * w.ld_xt) : nullptr;
+  w.wt = need_dx ? c.take<uint16_t>(d.D * w.ld_wt) : nullptr;
+  w.dl = need_dx ? c.take<uint16_t>(w.Tc * w.ld_dl) : nullptr;
+  w.dlt = need_dw ? c.take<uint16_t>((i64)w.Vc * w.ld_dlt) : nullptr;
+  w.dx = ce_grad_plan(d.T < w.Tc ? d.T : w.Tc, d.D, d.V < w.Vc ? d.V : w.Vc, s.triple, w.Vc < d.V);
+  w.dw = ce_grad_plan(d.V < w.Vc ? d.V : w.Vc, d.D, d.T < w.Tc ? d.T : w.Tc, s.triple, w.Tc < d.T);
   w.pdx = need_dx && w.dx.part ? c.take<float>((i64)w.dx.splits * w.Tc * d.D) : nullptr;
   // (dW's sum over several row pieces is kept for every class piece)
   w.pdw_piece = (i64)w.dw.splits * w.Vc * d.D;
@@ -1470,20 +1460,23 @@ CeBwdWs ce_bwd_ws(const FiLinearCe& d, const CeShape& s, bool need_dx, bool need
 }
 
 
-template <class Core, bool PAIR>
+template <class Core, typename T>
 int ce_launch_grad(const CeGrad& a, hipStream_t st) {
   static NtLdsDevices allowed;
-  if (!nt_allow_lds((const void*)ce_grad_kernel<Core, PAIR>, allowed)) return FI_ERR_UNSUPPORTED;
+  if (!nt_allow_lds((const void*)ce_grad_kernel<Core, T>, allowed)) return FI_ERR_UNSUPPORTED;
   const i64 n = (i64)((a.M + Core::BM - 1) / Core::BM) * ((a.N + Core::BN - 1) / Core::BN) * a.splits;
-  hipLaunchKernelGGL((ce_grad_kernel<Core, PAIR>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), Core::LDS, st, a);
+  hipLaunchKernelGGL((ce_grad_kernel<Core, T>), dim3((unsigned)ce_up(n, 8)), dim3(Core::THREADS), Core::LDS, st, a);
   FI_CHECK_LAUNCH();
   return 0;
 }
-template <bool PAIR>
-int ce_grad(const CeGrad& a, int tile, hipStream_t st) {
-  return tile == 0 ? ce_launch_grad<NtCore<f16_t, PAIR, 256, 256, 64, 64>, PAIR>(a, st)
-         : tile == 1 ? ce_launch_grad<NtCore<f16_t, PAIR, 128, 128, 64, PAIR ? 32 : 64>, PAIR>(a, st)
-                     : ce_launch_grad<NtCore<f16_t, PAIR, 64, 64, 32, 32, 3>, PAIR>(a, st);
+int ce_grad(const CeGrad& a, bool triple, int tile, hipStream_t st) {
+  if (triple)
+    return tile == 0 ? ce_launch_grad<NtCore<bf16_t, 3, 128, 256, 64, 64>, bf16_t>(a, st)
+           : tile == 1 ? ce_launch_grad<NtCore<bf16_t, 3, 128, 128, 64, 32, 3>, bf16_t>(a, st)
+                       : ce_launch_grad<NtCore<bf16_t, 3, 64, 64, 32, 32, 3>, bf16_t>(a, st);
+  return tile == 0 ? ce_launch_grad<NtCore<f16_t, 1, 256, 256, 64, 64>, f16_t>(a, st)
+         : tile == 1 ? ce_launch_grad<NtCore<f16_t, 1, 128, 128, 64, 64>, f16_t>(a, st)
+                     : ce_launch_grad<NtCore<f16_t, 1, 64, 64, 32, 32, 3>, f16_t>(a, st);
 }
 int ce_join(const CeGrad& a, hipStream_t st) {
   const int sub = a.splits >= 32 ? 16 : 1;
@@ -1524,9 +1517,7 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
   }
   hipLaunchKernelGGL(ce_gather_kernel, dim3(nb), dim3(256), 0, st, labels, d->ltype, (i64)d->T, (i64)d->ignore_index, d->V, ws.cnt, sv, ws.zt, rows_out, bias, ws.bias_pad);
   FI_CHECK_LAUNCH();
-  float* const scal = s.pair && s.scaled ? sv.scal : nullptr;
-  if (scal && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
-  if ((rc = ce_pack(ce_pack_x(*d, s, x, sv, ws.parts, scal, ws.xc), s.w_direct ? CePack{} : ce_pack_w(*d, s, w, ws.parts, scal, ws.wc), st))) return rc;
+  if ((rc = ce_pack(ce_pack_x(*d, s, x, sv, nullptr, nullptr, ws.xc), s.w_direct ? CePack{} : ce_pack_w(*d, s, w, nullptr, nullptr, ws.wc), st))) return rc;
   const void* const wop = s.w_direct ? w : (const void*)ws.wc;
   if (s.fused) {
     CeFused a = {};
@@ -1536,8 +1527,8 @@ extern "C" int fi_linear_ce_fwd(const FiLinearCe* d, const void* x, const void* 
   } else {
     CeLogits a = {};
     a.x = ws.xc, a.ldx = s.ldx, a.w = wop, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
-    a.scal = scal, a.s = sv, a.part = ws.part, a.zt = ws.zt, a.ntj = ws.nparts;
-    if ((rc = ce_logits_any(a, *d, s.pair, true, st))) return rc;
+    a.s = sv, a.part = ws.part, a.zt = ws.zt, a.ntj = ws.nparts;
+    if ((rc = ce_logits_any(a, *d, s, true, st))) return rc;
   }
   const int lanes = ws.nparts > 32 ? 64 : ws.nparts > 4 ? 8 : 1;
   i64 g = (d->T * lanes + 255) / 256;
@@ -1575,20 +1566,18 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   const CeShape s = ce_shape(*d, w, false);
   const CeBwdWs ws = ce_bwd_ws(*d, s, dx != nullptr, dw != nullptr, db != nullptr, workspace);
   const CeSaved sv = ce_saved((void*)saved, d->T);
-  // (the pair form's scales were made by the forward pass)
-  const float* const parts = s.scaled && !s.pair ? ws.parts : nullptr;
-  float* const scal = !s.scaled ? nullptr : s.pair ? sv.scal : ws.scal;
-  if (parts && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
-  CePack px = ce_pack_x(*d, s, x, sv, parts, scal, ws.xc), pw = ce_pack_w(*d, s, w, parts, scal, ws.wc);
+  float* const scal = s.scaled ? ws.scal : nullptr;
+  if (scal && (rc = ce_amax(*d, x, w, sv, ws.parts, st))) return rc;
+  CePack px = ce_pack_x(*d, s, x, sv, ws.parts, scal, ws.xc), pw = ce_pack_w(*d, s, w, ws.parts, scal, ws.wc);
   const bool rows_pieces = ws.Tc < d->T;
-  if (!rows_pieces) px.turned = ws.xt, px.ld_turned = ws.ld_xt, px.turned_pair = s.pair;
-  pw.turned = ws.wt, pw.ld_turned = ws.ld_wt, pw.turned_pair = s.pair;
+  if (!rows_pieces) px.turned = ws.xt, px.ld_turned = ws.ld_xt, px.turned_triple = s.triple;
+  pw.turned = ws.wt, pw.ld_turned = ws.ld_wt, pw.turned_triple = s.triple;
   if (s.w_direct && !ws.wt) pw.src = nullptr;                           // (its scale is dx's alone)
-  if (d->reduction == 0) {
+  if (d->reduction == 0 && !s.triple) {
     hipLaunchKernelGGL(ce_gmax_kernel, dim3(CE_PARTS), dim3(256), 0, st, gloss, sv.idx, sv.count, ws.parts + 2 * CE_PARTS);
     FI_CHECK_LAUNCH();
   }
-  const CeFactors fac = {gloss, d->reduction, ws.parts + 2 * CE_PARTS, sv, (int)s.pair, ws.scal, ws.g, ws.meta, bias, ws.bias_pad, labels,
+  const CeFactors fac = {gloss, d->reduction, ws.parts + 2 * CE_PARTS, sv, (int)s.triple, ws.scal, ws.g, ws.meta, bias, ws.bias_pad, labels,
                          d->ltype, d->V, d->T, d->ignore_index, (char*)dx, (i64)d->D * (d->dtype == FI_F32 ? 4 : 2)};
   const bool few = d->T <= 4096;                                        // (a launch less; its workgroups cover every row: 64 of them to a workgroup's 256)
   if ((rc = ce_pack(px, pw, st, few ? fac : CeFactors{}))) return rc;
@@ -1596,7 +1585,7 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
     hipLaunchKernelGGL(ce_factors_kernel, dim3((unsigned)((d->T + 255) / 256)), dim3(256), 0, st, fac);
     FI_CHECK_LAUNCH();
   }
-  const int f = s.pair ? 2 : 1;
+  const int f = s.triple ? 3 : 1;
   CeGrad gx = {}, gw = {};
   gx.a = ws.dl, gx.lda = ws.ld_dl, gx.ldb = ws.ld_wt, gx.N = d->D, gx.count = sv.count, gx.rows_are_tokens = 1;
   gx.splits = ws.dx.splits, gx.out = dx, gx.out_dtype = d->dtype, gx.ldo = d->D, gx.idx = sv.idx, gx.scal = ws.scal, gx.rscale = s.scaled ? SC_RW : -1;
@@ -1630,8 +1619,8 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
   gx.vec = d->D % 8 == 0 && ((uintptr_t)dx & 15) == 0, gw.vec = d->D % 8 == 0 && ((uintptr_t)dw & 15) == 0;
   CeLogits a = {};
   a.x = ws.xc, a.ldx = s.ldx, a.w = s.w_direct ? w : ws.wc, a.ldw = s.ldw, a.stages = s.kp / s.ku, a.V = d->V, a.bias = bias;
-  a.scal = s.pair && s.scaled ? ws.scal : nullptr, a.s = sv, a.g = ws.g, a.dl = ws.dl, a.dlt = ws.dlt, a.ld_dl = ws.ld_dl, a.ld_dlt = ws.ld_dlt, a.db = ws.db;
-  if (db && d->T <= CE_BM[ce_logits_tile(*d)]) a.db = nullptr, a.db_out = db, a.db_add = db_accumulate, a.rg = ws.scal + SC_RG;
+  a.s = sv, a.g = ws.g, a.dl = ws.dl, a.dlt = ws.dlt, a.ld_dl = ws.ld_dl, a.ld_dlt = ws.ld_dlt, a.db = ws.db;
+  if (db && d->T <= CE_BM[s.tile]) a.db = nullptr, a.db_out = db, a.db_add = db_accumulate, a.rg = ws.scal + SC_RG;
   const int wsize = d->wdtype == FI_F32 ? 4 : 2;
   // the classes innermost: dx of a row piece is complete with its last class piece, dW's parts are joined behind the last row piece
   const i64 nt = (d->T + ws.Tc - 1) / ws.Tc, nv = (d->V + ws.Vc - 1) / ws.Vc;
@@ -1641,26 +1630,26 @@ extern "C" int fi_linear_ce_bwd(const FiLinearCe* d, const void* x, const void* 
     a.v0 = (int)(iv * ws.Vc), a.Vc = ws.Vc < d->V - a.v0 ? ws.Vc : d->V - a.v0;
     if (rows_pieces && dw && iv == 0) {
       CePack pt = ce_pack_x(*d, s, x, sv, nullptr, scal, nullptr);
-      pt.begin = a.t0, pt.rows = a.Tc, pt.turned = ws.xt, pt.ld_turned = ws.ld_xt, pt.turned_pair = s.pair;
+      pt.begin = a.t0, pt.rows = a.Tc, pt.turned = ws.xt, pt.ld_turned = ws.ld_xt, pt.turned_triple = s.triple;
       if ((rc = ce_pack(pt, CePack{}, st))) return rc;
     }
-    if ((rc = ce_logits_any(a, *d, s.pair, false, st))) return rc;
+    if ((rc = ce_logits_any(a, *d, s, false, st))) return rc;
     if (dx) {
       gx.b = ws.wt + (i64)f * a.v0, gx.M = (int)a.Tc, gx.K = a.Vc, gx.t0 = a.t0, gx.Tc = a.Tc, gx.first = iv == 0;
       gx.part = ws.pdx;
-      if ((rc = s.pair ? ce_grad<true>(gx, ws.dx.tile, st) : ce_grad<false>(gx, ws.dx.tile, st))) return rc;
+      if ((rc = ce_grad(gx, s.triple, ws.dx.tile, st))) return rc;
       if (gx.part && iv == nv - 1 && (rc = ce_join(gx, st))) return rc;
     }
     if (dw) {
       gw.b = ws.xt, gw.M = a.Vc, gw.K = a.Tc, gw.t0 = a.t0, gw.Tc = a.Tc, gw.first = it == 0;
       gw.out = (char*)dw + (i64)a.v0 * d->D * wsize;
       gw.part = ws.pdw ? ws.pdw + (rows_pieces ? iv * ws.pdw_piece : 0) : nullptr;
-      if ((rc = s.pair ? ce_grad<true>(gw, ws.dw.tile, st) : ce_grad<false>(gw, ws.dw.tile, st))) return rc;
+      if ((rc = ce_grad(gw, s.triple, ws.dw.tile, st))) return rc;
       if (gw.part && it == nt - 1 && (rc = ce_join(gw, st))) return rc;
     }
   }
   if (db && !a.db_out) {
-    hipLaunchKernelGGL(ce_dbias_kernel, dim3((unsigned)((d->V + 15) / 16)), dim3(1024), 0, st, ws.db, CE_BM[ce_logits_tile(*d)], 0, d->V, sv.count, ws.scal, db, db_accumulate);
+    hipLaunchKernelGGL(ce_dbias_kernel, dim3((unsigned)((d->V + 15) / 16)), dim3(1024), 0, st, ws.db, CE_BM[s.tile], 0, d->V, sv.count, ws.scal, db, db_accumulate);
     FI_CHECK_LAUNCH();
   }
   return 0;

@@ -369,10 +369,10 @@ __global__ __launch_bounds__(256) void ns_prep_kernel(NsCtl g, NsAll all) {
 // (32 stands for tiles of 64 whose sums are kept apart)
 template <int TILE>
 struct NsTile;
-template <> struct NsTile<32> { typedef NtCore<f16_t, true, 64, 64, 32, 32, 3, true> Core; };
-template <> struct NsTile<64> { typedef NtCore<f16_t, true, 64, 64, 32, 32, 3> Core; };
-template <> struct NsTile<128> { typedef NtCore<f16_t, true, 128, 128, 64, 32, 2> Core; };
-template <> struct NsTile<256> { typedef NtCore<f16_t, true, 256, 256, 64, 64> Core; };
+template <> struct NsTile<32> { typedef NtCore<f16_t, 2, 64, 64, 32, 32, 3, true> Core; };
+template <> struct NsTile<64> { typedef NtCore<f16_t, 2, 64, 64, 32, 32, 3> Core; };
+template <> struct NsTile<128> { typedef NtCore<f16_t, 2, 128, 128, 64, 32, 2> Core; };
+template <> struct NsTile<256> { typedef NtCore<f16_t, 2, 256, 256, 64, 64> Core; };
 
 __device__ __forceinline__ void ns_put(void* out, int dtype, long at, const float (&v)[8], int n) {
 #pragma unroll

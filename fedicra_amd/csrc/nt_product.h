@@ -1,16 +1,20 @@
 // The matrix-pipe product core behind newton_schulz.hip and linear_ce.hip:  C[i][j] = sum_k A[i][k] * B[j][k], both operands with
 // their contraction index contiguous ("NT"), 16-bit storage, fp32 accumulation (v_mfma_f32_16x16x32).
 //
-// Operands come in one of two forms:
-//   plain  rows of 16-bit values, a multiple of 64 per row (the tail is zero);
-//   pair   every value as the sum of two fp16 (22 significant bits): per 32 values of a row 64 bytes of high parts, then 64 bytes of
-//          low parts.  Three products hi*hi + hi*lo + lo*hi give what an fp32 product gives up to 2^-22 per term, at a third of the
-//          16-bit matrix rate -- three times what fp32 products reach (1430 / 3 against 154 TFLOP/s at 8192 cubed) -- and one LDS fragment serves two products.
-// Either way 128 bytes of a row are one STAGE of the contraction, so that loading, LDS layout and addressing are the same.
+// Operands come in one of three forms, by the number of 16-bit PARTS of a value:
+//   1  rows of 16-bit values, a multiple of 64 per row (the tail is zero);
+//   2  (pairs) every value as the sum of two fp16 (22 significant bits): per 32 values of a row 64 bytes of high parts, then 64 bytes of
+//      low parts.  Three products hi*hi + hi*lo + lo*hi give what an fp32 product gives up to 2^-22 per term, at a third of the
+//      16-bit matrix rate -- three times what fp32 products reach (1430 / 3 against 154 TFLOP/s at 8192 cubed) -- and one LDS fragment serves two products.
+//      For values of one size: fp16 has no exponents below 2^-24, so what is 2^-17 of the largest has lost bits;
+//   3  (triples) every fp32 value exactly, as the sum of three bf16, which have fp32's exponents: 64 bytes each of first, second and third parts.  Six products
+//      leave out what is below 2^-23 of a term, at a sixth of the 16-bit matrix rate.
+// 128 bytes of a row are one STAGE of the contraction, of triples 192 (64 values, 32, 32).
 //
 // A workgroup owns a BM x BN tile, a wave WM x WN of it.  Stages are brought into an LDS ring of SLOTS by LDS-DMA (16 bytes per lane, 8 rows
 // of 128 bytes per instruction); 16-byte piece c of row r lies at piece c ^ (r & 7), the swizzle being applied to the source address
-// because the LDS side of the instruction is linear: the eight lanes a ds_read_b128 serves per clock then touch all 32 banks once.
+// because the LDS side of the instruction is linear: the eight lanes a ds_read_b128 serves per clock then touch all 32 banks once.  Triples' third parts
+// lie behind, 16 rows of 64 bytes per instruction, piece c of row r at c ^ (r / 2 & 3).
 #pragma once
 #include <atomic>
 
@@ -48,21 +52,26 @@ static inline bool nt_allow_lds(const void* kernel, NtLdsDevices& done) {
 __device__ __forceinline__ void nt_wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // SLOTS: two where two stages fill the LDS or several workgroups share a CU; more where a lone workgroup would wait for each stage's latency.
-// APART: pairs also take lo * lo, and what has a low part is summed in accumulators of its own: the matrix pipe rounds an accumulator at every
+// APART (pairs): they also take lo * lo, and what has a low part is summed in accumulators of its own: the matrix pipe rounds an accumulator at every
 // instruction, and small matrices are held to an fp32 sum's few roundings (orthogonalised matrices of 17 .. 31 rows are 1.1e-6 of the result off without,
-// 8.5e-7 with, 1.2e-6 by fp32 products).  A third more matrix instructions; long sums have no need of it.
-template <typename T, bool PAIR, int BM_, int BN_, int WM_, int WN_, int SLOTS_ = 2, bool APART_ = false>
+// 8.5e-7 with, 1.2e-6 by fp32 products).  A third more matrix instructions; long sums have no need of it.  Triples always keep theirs apart, for no more
+// instructions: a loss's fp32 gradients are 2e-7 off on average, 3.5e-7 in one accumulator, 6e-7 by fp32 products (4001 x 8003 x 384: 156 us, 144 in one).
+template <typename T, int PARTS_, int BM_, int BN_, int WM_, int WN_, int SLOTS_ = 2, bool APART_ = false>
 struct NtCore {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, SLOTS = SLOTS_;
+  static constexpr int PARTS = PARTS_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, SLOTS = SLOTS_;
   static constexpr int NWN = BN / WN, NW = (BM / WM) * NWN, THREADS = NW * 64;
   static constexpr int TI = WM / 16, TJ = WN / 16;
-  static constexpr int STAGE = (BM + BN) * 128, LDS = SLOTS * STAGE;
+  static constexpr int ROW = PARTS == 3 ? 192 : 128;              // bytes of a row per stage
+  static constexpr int STAGE = (BM + BN) * ROW, LDS = SLOTS * STAGE;
+  static_assert(LDS <= 160 * 1024, "LDS");
   // side of the blocks a wave stores its results by (NtBlock): its scratch lies in the ring
   static constexpr int BLOCK = WM >= 64 && WN >= 64 && NW * 64 * 64 * 4 <= LDS ? 64 : 32;
   static_assert(WM % BLOCK == 0 && WN % BLOCK == 0 && NW * BLOCK * BLOCK * 4 <= LDS, "scratch");
   static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;       // DMA instructions of a wave per stage: 8 rows of A, of B
   static_assert(PA * NW * 8 == BM && PB * NW * 8 == BN, "whole DMA instructions for every wave");
-  static constexpr bool APART = PAIR && APART_;
+  static constexpr int P3 = PARTS == 3 ? ((BM + BN) / 16 + NW - 1) / NW : 0;     // and for 16 rows' third parts, A's before B's
+  static_assert(SLOTS == 2 || P3 * NW * 16 == (PARTS == 3 ? BM + BN : 0), "the waits count the same loads in every wave");
+  static constexpr bool APART = PARTS == 3 || PARTS == 2 && APART_;
   typedef typename DT<T>::frag_t frag_t;
 
   f32x4 acc[TI][TJ];
@@ -91,8 +100,8 @@ struct NtCore {
     const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr_t)smem;
     const int w = wave(), l = lane();
     // (the resources end with the operands' last byte in use: nothing behind them is ever fetched)
-    const nt_v4i ra = nt_rsrc(a, ((unsigned long long)(rowsA - 1) * lda + (unsigned long long)s1 * 64) * 2);
-    const nt_v4i rb = nt_rsrc(b, ((unsigned long long)(rowsB - 1) * ldb + (unsigned long long)s1 * 64) * 2);
+    const nt_v4i ra = nt_rsrc(a, (unsigned long long)(rowsA - 1) * lda * 2 + (unsigned long long)s1 * ROW);
+    const nt_v4i rb = nt_rsrc(b, (unsigned long long)(rowsB - 1) * ldb * 2 + (unsigned long long)s1 * ROW);
     const unsigned piece = (unsigned)(((l & 7) ^ (l >> 3)) * 16);
     unsigned va[PA], vb[PB];
 #pragma unroll
@@ -106,6 +115,12 @@ struct NtCore {
       vb[q] = (unsigned)(r < rowsB ? r : rowsB - 1) * (unsigned)(ldb * 2) + piece;
     }
     const unsigned la = lds0 + (unsigned)(w * PA * 1024), lb = lds0 + (unsigned)(BM * 128 + w * PB * 1024);
+    unsigned vc[P3 ? P3 : 1];
+#pragma unroll
+    for (int q = 0; q < P3; ++q) {
+      const int r = (w * P3 + q) * 16 + (l >> 2), piece3 = 128 + ((l & 3) ^ ((r >> 1) & 3)) * 16;
+      vc[q] = r < BM ? (unsigned)(r < rowsA ? r : rowsA - 1) * (unsigned)(lda * 2) + piece3 : (unsigned)(r - BM < rowsB ? r - BM : rowsB - 1) * (unsigned)(ldb * 2) + piece3;
+    }
     // (a stage behind the last one is asked for through an empty resource: zeros, no traffic, and every step counts the same loads)
     const int endA = ra[2], endB = rb[2];
     auto fetch = [&](int s, int slot) {
@@ -113,13 +128,23 @@ struct NtCore {
       xa[2] = s < s1 ? endA : 0;
       xb[2] = s < s1 ? endB : 0;
 #pragma unroll
-      for (int q = 0; q < PA; ++q) nt_dma16(xa, la + (unsigned)(slot * STAGE + q * 1024), va[q], (unsigned)s * 128u);
+      for (int q = 0; q < PA; ++q) nt_dma16(xa, la + (unsigned)(slot * STAGE + q * 1024), va[q], (unsigned)s * ROW);
 #pragma unroll
-      for (int q = 0; q < PB; ++q) nt_dma16(xb, lb + (unsigned)(slot * STAGE + q * 1024), vb[q], (unsigned)s * 128u);
+      for (int q = 0; q < PB; ++q) nt_dma16(xb, lb + (unsigned)(slot * STAGE + q * 1024), vb[q], (unsigned)s * ROW);
+#pragma unroll
+      for (int q = 0; q < P3; ++q) {
+        const int r = (w * P3 + q) * 16;                                // (the same in all lanes)
+        if (r < BM)
+          nt_dma16(xa, lds0 + (unsigned)(slot * STAGE + (BM + BN) * 128 + r * 64), vc[q], (unsigned)s * ROW);
+        else if (r < BM + BN)
+          nt_dma16(xb, lds0 + (unsigned)(slot * STAGE + (BM + BN) * 128 + r * 64), vc[q], (unsigned)s * ROW);
+      }
     };
     const int sw = l & 7, g = l >> 4, lr = l & 15;
     const int oa = (row0() + lr) * 128, ob = BM * 128 + (col0() + lr) * 128;
     const int p0 = ((g) ^ sw) * 16, p1 = ((4 + g) ^ sw) * 16;
+    // (from oa / ob to the third parts of the same row: 64 bytes a row there)
+    const int p2 = (g ^ ((l >> 1) & 3)) * 16, oa3 = (BM + BN) * 128 + (row0() + lr) * 64 + p2, ob3 = (BM + BN) * 128 + (BM + col0() + lr) * 64 + p2;
 
     if (s0 < s1) {
 #pragma unroll
@@ -134,11 +159,49 @@ struct NtCore {
     int cur = 0, free = SLOTS - 1;                                      // slots of stage s and of the one before it
     for (int s = s0; s < s1; ++s) {
       // stage s is there for every wave, and every wave has read the one before it
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((SLOTS - 2) * (PA + PB)) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((SLOTS - 2) * (PA + PB + P3)) : "memory");
       fetch(s + SLOTS - 1, free);
       const char* sa = smem + cur * STAGE + oa;
       const char* sb = smem + cur * STAGE + ob;
-      if constexpr (PAIR) {
+      if constexpr (PARTS == 3) {
+        const char* sa3 = smem + cur * STAGE + oa3;
+        const char* sb3 = smem + cur * STAGE + ob3;
+        frag_t b0[TJ], b1[TJ], b2[TJ];
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+          b0[j] = *(const frag_t*)(sb + j * 2048 + p0);
+          b1[j] = *(const frag_t*)(sb + j * 2048 + p1);
+          b2[j] = *(const frag_t*)(sb3 + j * 1024);
+        }
+        frag_t a0[2], a1[2], a2[2];
+        a0[0] = *(const frag_t*)(sa + p0);
+        a1[0] = *(const frag_t*)(sa + p1);
+        a2[0] = *(const frag_t*)sa3;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+          const int u = i & 1;
+          if (i + 1 < TI) {
+            a0[u ^ 1] = *(const frag_t*)(sa + (i + 1) * 2048 + p0);
+            a1[u ^ 1] = *(const frag_t*)(sa + (i + 1) * 2048 + p1);
+            a2[u ^ 1] = *(const frag_t*)(sa3 + (i + 1) * 1024);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          // (the smallest first)
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) low[i % LI][j % LJ] = mfma16(b0[j], a2[u], low[i % LI][j % LJ]);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) low[i % LI][j % LJ] = mfma16(b2[j], a0[u], low[i % LI][j % LJ]);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) low[i % LI][j % LJ] = mfma16(b1[j], a1[u], low[i % LI][j % LJ]);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) low[i % LI][j % LJ] = mfma16(b0[j], a1[u], low[i % LI][j % LJ]);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) low[i % LI][j % LJ] = mfma16(b1[j], a0[u], low[i % LI][j % LJ]);
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) acc[i][j] = mfma16(b0[j], a0[u], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else if constexpr (PARTS == 2) {
         frag_t bh[TJ], bl[TJ];
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
@@ -300,6 +363,24 @@ __device__ __forceinline__ void nt_load_pair(const f16_t* row, long k, float (&v
   VecWords<f16_t>::unpack(lo, b);
 #pragma unroll
   for (int t = 0; t < 8; ++t) v[t] = a[t] + b[t];
+}
+
+// 8 fp32 values -> three bf16 parts, exactly: the first within half its step of 2^-8, so that 16 bits are left for the others.  (Next to fp32's largest
+// bf16 would round up to infinity: the first part ends at its own largest.  NaN and infinities come out as NaN.)
+__device__ __forceinline__ void nt_store_triple(bf16_t* row, long k, const float (&v)[8]) {           // k: a multiple of 8
+  float a[8], b[8], c[8];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const float x = nt_fixed(v[t]);
+    a[t] = (float)(bf16_t)__builtin_amdgcn_fmed3f(x, -0x1.fep127f, 0x1.fep127f);
+    const float r = x - a[t];
+    b[t] = (float)(bf16_t)r;
+    c[t] = r - b[t];
+  }
+  bf16_t* p = row + (k >> 5) * 96 + (k & 31);
+  *(uint4*)p = VecWords<bf16_t>::pack(a);
+  *(uint4*)(p + 32) = VecWords<bf16_t>::pack(b);
+  *(uint4*)(p + 64) = VecWords<bf16_t>::pack(c);
 }
 
 // Workgroups are handed to the eight XCDs in turn (id % 8): this maps a launch of `n` work items (grid rounded up to a multiple of 8) so that each

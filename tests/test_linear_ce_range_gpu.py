@@ -1,4 +1,4 @@
-"""ops.linear_ce_loss where sizes differ by many orders: rows' own factors."""
+"""ops.linear_ce_loss where sizes differ by many orders: rows' own factors, rows, classes and features of fp32 operands."""
 import pytest
 import torch
 
@@ -34,3 +34,58 @@ def test_a_row_of_dx_knows_its_own_factor_alone(dtype, rows, classes, width):
         want, tol = _ce64(x, w, b, lab, -100, "none", above)
         _within(dw, want[2], tol[2], ("dw", dtype))
         _within(db, want[3], tol[3], ("db", F32))
+
+
+SIZES = [(300, 400, 200), (64, 2000, 40), (600, 50, 33), (100, 700, 72), (300, 100, 72)]
+
+
+@pytest.mark.parametrize("big", [1e6, 1e10, 1e30, torch.finfo(F32).max])
+@pytest.mark.parametrize("rows,classes,width", SIZES)
+def test_a_large_value_in_one_row_leaves_the_others_alone(rows, classes, width, big):
+    """A labelled row whose one feature is far larger than all else.  It is its own class for certain (no gradient): losses and dx of the other rows, dw and db
+    are those of the other rows alone."""
+    x, w, b, lab = _head(rows, rows, classes, width, F32, 0.1)
+    x[0, 3] = big
+    w[:, 3] *= 0.2
+    w[7, 3] = 0.9
+    lab[0], lab[1] = 7, 5
+    loss, dx, dw, db = _none(x, w, b, lab)
+    assert float(loss[0]) == 0.0 and not dx[0].any()
+    want, tol = _ce64(x[1:], w, b, lab[1:], -100, "none", torch.ones(rows - 1, device="cuda"))
+    _within(loss[1:], want[0], tol[0], ("loss", F32))
+    _within(dx[1:], want[1], tol[1], ("dx", F32))
+    _within(dw, want[2], tol[2], ("dw", F32))
+    _within(db, want[3], tol[3], ("db", F32))
+
+
+@pytest.mark.parametrize("big", [1e6, 1e10, 1e30, torch.finfo(F32).max])
+@pytest.mark.parametrize("rows,classes,width", SIZES)
+def test_a_large_weight_of_one_class_leaves_the_others_alone(rows, classes, width, big):
+    """A class that one huge weight rules out for every row: everything else is as without it."""
+    x, w, b, lab = _head(rows, rows, classes, width, F32, 0.1)
+    x[:, 3] = -0.5 - 0.4 * torch.rand(rows, generator=_gen(1), device="cuda")
+    lab = torch.where(lab == 7, torch.full_like(lab, 8), lab)
+    w[7, 3] = big
+    loss, dx, dw, db = _none(x, w, b, lab)
+    kept = torch.arange(classes, device="cuda") != 7
+    want, tol = _ce64(x, w[kept], b[kept], torch.where(lab > 7, lab - 1, lab), -100, "none", torch.ones(rows, device="cuda"))
+    _within(loss, want[0], tol[0], ("loss", F32))
+    _within(dx, want[1], tol[1], ("dx", F32))
+    _within(dw[kept], want[2], tol[2], ("dw", F32))
+    _within(db[kept], want[3], tol[3], ("db", F32))
+    assert not dw[7].any() and float(db[7]) == 0.0
+
+
+@pytest.mark.parametrize("rows,classes,width", SIZES)
+def test_features_of_unlike_size(rows, classes, width):
+    """Features from 1e-8 to 1e8 whose weights make up for it."""
+    x, w, b, lab = _head(rows, rows, classes, width, F32, 0.1)
+    s = 10.0 ** (torch.rand(width, generator=_gen(2), device="cuda") * 16 - 8)
+    x, w = x * s, w / s
+    above = torch.ones(rows, device="cuda")
+    loss, dx, dw, db = _none(x, w, b, lab)
+    want, tol = _ce64(x, w, b, lab, -100, "none", above)
+    _within(loss, want[0], tol[0], ("loss", F32))
+    _within(dx, want[1], tol[1], ("dx", F32))
+    _within(dw, want[2], tol[2], ("dw", F32))
+    _within(db, want[3], tol[3], ("db", F32))
