@@ -89,3 +89,25 @@ def test_features_of_unlike_size(rows, classes, width):
     _within(dx, want[1], tol[1], ("dx", F32))
     _within(dw, want[2], tol[2], ("dw", F32))
     _within(db, want[3], tol[3], ("db", F32))
+
+
+def test_tens_of_millions_of_rows():
+    """So many that the labelled ones before a workgroup's are counted by a scan; few are labelled."""
+    rows, classes, width = 36_000_000, 5, 2
+    g = _gen(7)
+    x = torch.randn(rows, width, generator=g, device="cuda").to(BF16)
+    w, b = torch.randn(classes, width, generator=g, device="cuda").to(BF16), torch.randn(classes, generator=g, device="cuda")
+    lab = torch.full((rows,), 255, dtype=torch.uint8, device="cuda")
+    at = torch.unique(torch.randint(0, rows, (40000,), generator=g, device="cuda"))
+    at[0], at[-1] = 0, rows - 1
+    lab[at] = torch.randint(0, classes, at.shape, generator=g, device="cuda").to(torch.uint8)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    loss = ops.linear_ce_loss(*leaves, lab, 255)
+    dx, dw, db = torch.autograd.grad(loss, leaves)
+    want, tol = _ce64(x[at], w, b, lab[at], 255, "mean", torch.ones((), device="cuda"))
+    _within(loss.detach().reshape(1), want[0].reshape(1), tol[0], ("loss", F32))
+    _within(dx[at], want[1], tol[1], ("dx", BF16))
+    _within(dw, want[2], tol[2], ("dw", BF16))
+    _within(db, want[3], tol[3], ("db", F32))
+    dx[at] = 0
+    assert not dx.any()
