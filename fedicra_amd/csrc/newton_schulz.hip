@@ -795,16 +795,7 @@ long ns_layout(const FiNsMat* const* mats, int count, const NsPlan& plan, bool s
   return at;
 }
 
-int ns_check(const FiNsMat* mats, int count, int steps, const float* coeffs) {
-  if (!mats || !coeffs) return FI_ERR_NULL;
-  if (count < 1 || steps < 1) return FI_ERR_SHAPE;
-  for (int i = 0; i < count; ++i) {
-    const FiNsMat& q = mats[i];
-    if (q.dtype != FI_F32 && q.dtype != FI_BF16 && q.dtype != FI_F16) return FI_ERR_DTYPE;
-    if (q.rows < 1 || q.cols < 1 || q.rows > (1 << 20) || q.cols > (1 << 20)) return FI_ERR_SHAPE;
-    const int m = q.rows < q.cols ? q.rows : q.cols;
-    if (m > 32768) return FI_ERR_SHAPE;
-  }
+int ns_check_polynomial(int steps, const float* coeffs) {
   // every singular value starts in [0, 1]: the polynomial must keep X, A and S inside the storage's range (16 / 2^-12)
   for (int i = 0; i <= 1024; ++i) {
     double s = i / 1024.0;
@@ -816,6 +807,19 @@ int ns_check(const FiNsMat* mats, int count, int steps, const float* coeffs) {
     }
   }
   return 0;
+}
+
+int ns_check(const FiNsMat* mats, int count, int steps, const float* coeffs) {
+  if (!mats || !coeffs) return FI_ERR_NULL;
+  if (count < 1 || steps < 1) return FI_ERR_SHAPE;
+  for (int i = 0; i < count; ++i) {
+    const FiNsMat& q = mats[i];
+    if (q.dtype != FI_F32 && q.dtype != FI_BF16 && q.dtype != FI_F16) return FI_ERR_DTYPE;
+    if (q.rows < 1 || q.cols < 1 || q.rows > (1 << 20) || q.cols > (1 << 20)) return FI_ERR_SHAPE;
+    const int m = q.rows < q.cols ? q.rows : q.cols;
+    if (m > 32768) return FI_ERR_SHAPE;
+  }
+  return ns_check_polynomial(steps, coeffs);
 }
 
 int ns_total(const NsArgs& g, int kind) {
@@ -1010,6 +1014,9 @@ extern "C" int fi_muon_step(const FiMuonMat* mats, int count, const double* lr, 
   const long total = fi_muon_step_workspace(mats, count);
   if (total < 0) return (int)total;
   if (!lr || !coeffs || !workspace) return FI_ERR_NULL;
+  if (steps < 1) return FI_ERR_SHAPE;
+  const int rc0 = ns_check_polynomial(steps, coeffs);                   // (before the momentum moves: an error leaves everything as it was)
+  if (rc0) return rc0;
   for (int i = 0; i < count; ++i)
     if (!mats[i].param || !mats[i].grad || !mats[i].buf) return FI_ERR_NULL;
   hipStream_t st = (hipStream_t)stream;

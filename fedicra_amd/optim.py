@@ -238,13 +238,7 @@ class FusedMuon(FusedAdamW):
             for s, e in self.model.param_ranges(active):
                 L.amp_unscale(G[s:e], scale, found_inf)
         rest = [n for n in active if n not in self._matrices]
-        if rest:
-            gi, ranges = self._group_for(rest)
-            L.adamw_hyper(self.steps[gi:gi + 1], self.hyper[gi], self.lr_state, self.betas[0], self.betas[1], self.wd)
-            if scale is not None:
-                L.amp_guard(self.steps[gi:gi + 1], self.hyper[gi], found_inf)
-            for s, e in ranges:
-                L.adamw_step(P[s:e], G[s:e], self.m[s:e], self.v[s:e], self.hyper[gi], self.betas[0], self.betas[1], self.eps)
+        group = self._group_for(rest) if rest else None
         items = []
         for n in active:
             if n in self._matrices:
@@ -252,9 +246,16 @@ class FusedMuon(FusedAdamW):
                 s, e = p._fi_off, p._fi_off + p.numel()
                 rows, cols = p.shape[0], p.numel() // p.shape[0]          # (the order of a row's values does not matter to the iteration)
                 items.append((P[s:e], G[s:e], self.m[s:e], rows, cols, max(1.0, rows / cols) ** 0.5))
-        if items:
+        if items:                             # (first: an iteration that the library refuses leaves everything as it was)
             L.muon_step(items, self.lr_state, self.momentum, self.nesterov, self.wd, len(self.ns_coeffs), self.ns_coeffs, 1e-7,
                         None if scale is None else found_inf)
+        if group:
+            gi, ranges = group
+            L.adamw_hyper(self.steps[gi:gi + 1], self.hyper[gi], self.lr_state, self.betas[0], self.betas[1], self.wd)
+            if scale is not None:
+                L.amp_guard(self.steps[gi:gi + 1], self.hyper[gi], found_inf)
+            for s, e in ranges:
+                L.adamw_step(P[s:e], G[s:e], self.m[s:e], self.v[s:e], self.hyper[gi], self.betas[0], self.betas[1], self.eps)
         ops.bump_weights_epoch()
 
 
