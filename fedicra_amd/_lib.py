@@ -1200,9 +1200,10 @@ def _scratch(size, what, device):
 
 
 def linear_ce_desc(x, w, labels, ignore_index, reduction):
-    """x [T, D], w [V, D], both with dense rows; labels [T] dense."""
-    return FiLinearCe(dt(x.dtype), dt(w.dtype), LABEL_TYPES[labels.dtype], REDUCTIONS[reduction], w.shape[0], w.shape[1], x.shape[0],
-                      max(x.stride(0), x.shape[1]), max(w.stride(0), w.shape[1]), int(ignore_index))
+    """x [T, D], w [V, D], both with dense rows; labels [T] dense.  (A lone row's stride means nothing.)"""
+    (T, D), V = x.shape, w.shape[0]
+    return FiLinearCe(dt(x.dtype), dt(w.dtype), LABEL_TYPES[labels.dtype], REDUCTIONS[reduction], V, D, T, x.stride(0) if T > 1 else D,
+                      w.stride(0) if V > 1 else D, int(ignore_index))
 
 
 def _address(t):

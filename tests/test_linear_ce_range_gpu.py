@@ -111,3 +111,25 @@ def test_tens_of_millions_of_rows():
     _within(db, want[3], tol[3], ("db", F32))
     dx[at] = 0
     assert not dx.any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_lone_row_or_class_of_any_stride(dtype):
+    """What a slice of a large tensor leaves: one row, its stride far beyond what several rows may have."""
+    store = torch.randn(1 << 10, generator=_gen(8), device="cuda").to(dtype)
+    x = store.as_strided((1, 24), (1 << 40, 1))
+    w = store.as_strided((1, 24), (1 << 23, 1), 512)
+    b = torch.zeros(1, device="cuda")
+    loss, dx, dw, db = _none(x, w, b, torch.zeros(1, dtype=torch.int64, device="cuda"))
+    assert float(loss[0]) == 0.0 and not dx.any() and not dw.any() and not db.any()
+    lab = torch.zeros(50, dtype=torch.int64, device="cuda")
+    loss, dx, dw, db = _none(torch.randn(50, 24, generator=_gen(9), device="cuda").to(dtype), w, b, lab)
+    assert not loss.any() and not dx.any() and not dw.any() and not db.any()
+    w = torch.randn(30, 24, generator=_gen(10), device="cuda").to(dtype)
+    b = torch.randn(30, generator=_gen(11), device="cuda")
+    loss, dx, dw, db = _none(x, w, b, lab[:1])
+    want, tol = _ce64(x, w, b, lab[:1], -100, "none", torch.ones(1, device="cuda"))
+    _within(loss, want[0], tol[0], ("loss", F32))
+    _within(dx, want[1], tol[1], ("dx", dtype))
+    _within(dw, want[2], tol[2], ("dw", dtype))
+    _within(db, want[3], tol[3], ("db", F32))
