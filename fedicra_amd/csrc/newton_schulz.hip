@@ -761,7 +761,8 @@ NsPlan ns_plan(const FiNsMat* const* mats, int count) {
       }
     }
   }
-  // small matrices are held to an fp32 iteration's error: their tiles keep the low parts' sums apart
+  // small matrices are held to an fp32 iteration's error: where no larger one shares their launches, their tiles keep the low parts' sums apart (17 .. 64 rows: 6.2e-7 ..
+  // 9.0e-7 of the result off by themselves, 7.7e-7 .. 1.04e-6 beside a matrix of 300 or 1000 rows, 7.9e-7 .. 1.2e-6 by fp32 products)
   int most = 0;
   for (int i = 0; i < count; ++i) {
     const int m = mats[i]->rows < mats[i]->cols ? mats[i]->rows : mats[i]->cols;
