@@ -16,9 +16,10 @@
 // lost below 2^-39.  For dx a row of G is made with a factor of one, at 2^14, for dW with its own, the largest |g_t| at 2^14; what lies below 2^-39 of that is
 // lost.  Row statistics, sums and db are fp32 (joins in fp64).
 //
-// Measured at 7370 labelled rows x 50000 x 1024 bf16: forward 684 us (1103 TFLOP/s), and per half of the classes G 494 (764: its stores) and each
-// gradient 393 (960), where a large library product reaches 1430 and one of a gradient's size 1068.  Bound by the fill of LDS from L2 and by its
-// reads: without any fill the product of 7370 x 1024 x 16384 takes 158 us where it takes 221.
+// Measured at 7370 labelled rows x 50000 x 1024 bf16: forward 691 us (1092 TFLOP/s), and per half of the classes G 503 (750: its stores) and each
+// gradient 392 (963), where a large library product reaches 1430 and one of a gradient's size 1068.  Bound by the fill of LDS from L2 and by its
+// reads: without any fill the product of 7370 x 1024 x 16384 takes 158 us where it takes 221.  4001 x 8003 x 384 fp32 (triples): forward 144 us (1020 TFLOP/s of
+// matrix instructions), G 197, each gradient 173.
 #include "nt_product.h"
 
 namespace {
@@ -911,8 +912,8 @@ __global__ __launch_bounds__(1024) void ce_dbias_kernel(const float* part, int t
 // -- exactly the fragment that the next product wants from it.  (Pieces of a row are swizzled by (row & 3) | (row / 8 & 1) * 4, which is free of
 // bank conflicts under that order.)  The forward pass of such operands streams the classes the same way and keeps each row's running maximum and sum.
 // Rows are packed to a multiple of 8 features only; the rest of a stage is masked in the load (its offset lies beyond the resource: zeros).
-// Measured: 16384 x 65536 x 128 bf16 dx 548 us, dW 586, forward 322: half the matrix rate, the exponential, scaling and conversion of every value of
-// G sharing the issue port with the products; 524288 x 105 x 16 bf16 32, 36 and 27 us.
+// Measured: 16384 x 65536 x 128 bf16 dx 584 us, dW 625, forward 351: half the matrix rate, the exponential, scaling and conversion of every value of
+// G sharing the issue port with the products; 524288 x 105 x 16 bf16 33, 38 and 29 us.
 struct CeFused {
   CeGrad out;
   CeSaved s;

@@ -13,9 +13,9 @@
 // split) per step, whatever their number; where none has more than 64 rows, one per step (ns_narrow_step_kernel).  Matrices of up to 16 rows are done
 // with the first two (ns_short_apply).
 //
-// Measured (five steps): 2048 x 8192 bf16 1.73 ms, 968 TFLOP/s of matrix instructions where a large library product reaches 1430 -- per step S X 180 us
-// (1145 TFLOP/s), A 106, its join 26, S 46 (560: 528 tiles of 64); 4096 x 1024 fp32 413 us; 1000 x 1537 bf16 276 us (tiles for 1.6 rounds of
-// the chip and 15 us a product: latency); a U-Net's 23 filters fp32 188 us (22 launches of 6 .. 15 us); 64 x 576 fp32 70 us (7 of 8 .. 11 us).
+// Measured (five steps): 2048 x 8192 bf16 1.70 .. 1.78 ms, 970 TFLOP/s of matrix instructions where a large library product reaches 1430 -- per step S X 180 us
+// (1145 TFLOP/s), A 106, its join 26, S 46 (560: 528 tiles of 64); 4096 x 1024 fp32 400 .. 425 us; 1000 x 1537 bf16 264 .. 285 us (tiles for 1.6 rounds of
+// the chip and 15 us a product: latency); a U-Net's 23 filters fp32 186 us (22 launches of 6 .. 15 us); 64 x 576 fp32 71 us (7 of 9 .. 11 us).
 #include <math.h>
 
 #include "nt_product.h"

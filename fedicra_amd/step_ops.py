@@ -144,13 +144,18 @@ class _LinearCE(Function):
 
 def linear_ce_loss(x, weight, bias, labels, ignore_index=-100, reduction="mean"):
     """Softmax cross entropy of a linear head, ``CrossEntropyLoss(ignore_index)(x @ weight.T + bias, labels)``, without its logits: the
-    product runs a tile at a time and its gradient a piece of rows x classes at a time, so that memory does not grow with rows x classes.
+    product runs a tile at a time and its gradient a piece of rows x classes at a time.  Of rows x classes there are in memory pieces of at most 3 GiB and, above 128
+    features or in fp32, 1/32 byte each (a row's statistics per 256 classes, the bias gradient's per 128 or 256 rows).
 
     x [..., D] fp32, bf16 or fp16 (any leading sizes; the labels' sizes); weight [V, D], or a 1x1 convolution's [V, D, 1, 1(, 1)], in x's type or
     fp32 (a 16-bit x then meets it rounded to x's type, like every operator here); bias [V] or None; labels int64, int32 or uint8.
     Rows whose label is ``ignore_index`` take no part, whatever x holds there, and cost (next to) nothing.  ``reduction``: "mean" over the
     labelled rows (NaN when there are none, as ``ce_loss``), "sum", or "none" -- a loss per row, 0 where ignored.  A label that is neither a class
-    nor ``ignore_index`` makes the loss and the gradients NaN.
+    nor ``ignore_index`` makes the loss and the gradients NaN.  Classes may be ruled out by a bias of -inf or any large negative value.
+
+    fp32: what fp32 products and sums give, whatever the sizes of rows, classes and features.  16-bit x: logits and sums in fp32, the logits' gradient rounded
+    once to fp16 (not at all up to 2^28 multiply-adds of fp16) relative to the row's own upstream gradient for dx, to the largest of all for the weight's: what
+    lies below 2^-39 of that is lost, and so are bf16 values below 2^-39 of their tensor's largest.
 
     The gradients have the types of x, weight and bias (a parameter of a flat-store model: added to its slice of the flat buffer).  Twice
     differentiating is refused."""

@@ -757,7 +757,9 @@ int fi_muon_step(const FiMuonMat* mats, int count, const double* lr, float momen
  *        (fi_linear_ce_saved bytes) is what bwd needs besides x, w and bias.
  *   bwd: gloss = upstream gradient, fp32 [T] or [1]; dx in x's type, dense [T][D]; dw in w's type, dense [V][D] (dw_accumulate: fp32, +=); db fp32
  *        [V] (db_accumulate: +=); any of the three may be NULL.
- * Deterministic: no atomics.  T < 2^30, V <= 2^20, D <= 65536. */
+ * Numerics: fp32 operands enter the products exactly (three bf16 parts of each value); for 16-bit ones the logits' gradient is rounded once to fp16, for dx relative to
+ * its row's own gloss, for dw to the largest of all (what is below 2^-39 of it is lost).
+ * Deterministic: no atomics.  T < 2^30, V <= 2^20, D <= 65536, and tiles of 256 rows x 256 classes (fp32: 128 x 256) < 2^30. */
 #define FI_LABEL_U8 0
 #define FI_LABEL_I32 1
 #define FI_LABEL_I64 2

@@ -80,3 +80,15 @@ def test_small_matrices_beside_a_larger_one(m, n):
         err = (got.double() - want).norm().item()
         print(m, n, len(others) and tuple(others[0].shape), "%.2e of %.2e" % (err / want.norm().item(), bound / 2 / want.norm().item()))
         assert err <= bound, (err, bound)
+
+
+@pytest.mark.parametrize("dtype,rows,classes,width", [(F32, 300, 20, 16), (F32, 100, 700, 72), (F32, 20, 300, 40), (F32, 600, 300, 200), (BF16, 300, 400, 200), (BF16, 40, 300, 200),
+                                                      (F16, 300, 400, 200), (F16, 3000, 1000, 100), (F16, 1500, 1000, 200)])
+def test_no_labelled_row(dtype, rows, classes, width):
+    x, w, b, lab = _head(rows, rows, classes, width, dtype)
+    lab.fill_(-100)
+    for red in ("mean", "sum", "none"):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        loss = ops.linear_ce_loss(*leaves, lab, -100, red)
+        assert torch.isnan(loss) if red == "mean" else (loss == 0).all()
+        assert all((g == 0).all() for g in torch.autograd.grad(loss, leaves, torch.ones_like(loss)))
