@@ -10,7 +10,7 @@
 // Only labelled rows take part: their numbers are gathered first (stable, no atomics), x is packed through that list, and every
 // kernel takes the number of rows from the device -- nine pixels of ten unlabelled cost a tenth.
 //
-// Types: fp32 operands and their G go to the matrix pipe as triples of bf16 (nt_product.h): exactly, whatever their sizes, so that no row, class or feature costs
+// Types: fp32 operands and their G go to the matrix pipe as triples of bf16 (nt_product.h): exactly, whatever their sizes (from 8e-34 on), so that no row, class or feature costs
 // another its bits; short products of fp16 as triples too, for G's sake (ce_shape).  Other 16-bit x and W go as they are.  Their G is fp16, which keeps 11 bits
 // where bf16 would keep 8, and so are x and W in its products: bf16 ones under a power-of-two scale per tensor, exact down to 2^-31 of the tensor's largest value and
 // lost below 2^-39.  For dx a row of G is made with a factor of one, at 2^14, for dW with its own, the largest |g_t| at 2^14; what lies below 2^-39 of that is

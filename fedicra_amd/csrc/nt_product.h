@@ -8,7 +8,8 @@
 //      16-bit matrix rate -- three times what fp32 products reach (1430 / 3 against 154 TFLOP/s at 8192 cubed) -- and one LDS fragment serves two products.
 //      For values of one size: fp16 has no exponents below 2^-24, so what is 2^-17 of the largest has lost bits;
 //   3  (triples) every fp32 value exactly, as the sum of three bf16, which have fp32's exponents: 64 bytes each of first, second and third parts.  Six products
-//      leave out what is below 2^-23 of a term, at a sixth of the 16-bit matrix rate.
+//      leave out what is below 2^-23 of a term, at a sixth of the 16-bit matrix rate.  (The matrix pipe takes a part below 2^-126 as zero: values below 2^-110, 8e-34, lose
+//      their last bits.)
 // 128 bytes of a row are one STAGE of the contraction, of triples 192 (64 values, 32, 32).
 //
 // A workgroup owns a BM x BN tile, a wave WM x WN of it.  Stages are brought into an LDS ring of SLOTS by LDS-DMA (16 bytes per lane, 8 rows

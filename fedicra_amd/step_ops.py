@@ -153,7 +153,7 @@ def linear_ce_loss(x, weight, bias, labels, ignore_index=-100, reduction="mean")
     labelled rows (NaN when there are none, as ``ce_loss``), "sum", or "none" -- a loss per row, 0 where ignored.  A label that is neither a class
     nor ``ignore_index`` makes the loss and the gradients NaN.  Classes may be ruled out by a bias of -inf or any large negative value.
 
-    fp32: what fp32 products and sums give, whatever the sizes of rows, classes and features.  16-bit x: logits and sums in fp32, the logits' gradient rounded
+    fp32: what fp32 products and sums give, whatever the sizes of rows, classes and features (from 1e-33 on).  16-bit x: logits and sums in fp32, the logits' gradient rounded
     once to fp16 (not at all up to 2^28 multiply-adds of fp16) relative to the row's own upstream gradient for dx, to the largest of all for the weight's: what
     lies below 2^-39 of that is lost, and so are bf16 values below 2^-39 of their tensor's largest.
 

@@ -133,3 +133,15 @@ def test_a_lone_row_or_class_of_any_stride(dtype):
     _within(dx, want[1], tol[1], ("dx", dtype))
     _within(dw, want[2], tol[2], ("dw", dtype))
     _within(db, want[3], tol[3], ("db", F32))
+
+
+@pytest.mark.parametrize("size", [1e-32, 1e30])
+def test_features_next_to_the_ends_of_the_range(size):
+    x, w, b, lab = _head(12, 300, 400, 72, F32, 0.1)
+    x, w = (x.double() * size).float(), (w.double() / size).float()
+    loss, dx, dw, db = _none(x, w, b, lab)
+    want, tol = _ce64(x, w, b, lab, -100, "none", torch.ones(300, device="cuda"))
+    _within(loss, want[0], tol[0], ("loss", F32))
+    _within(dx, want[1], tol[1], ("dx", F32))
+    _within(dw, want[2], tol[2], ("dw", F32))
+    _within(db, want[3], tol[3], ("db", F32))
